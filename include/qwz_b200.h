@@ -34,12 +34,14 @@ extern "C" {
 
 #define QWZ_DTYPE_F16 0
 #define QWZ_DTYPE_BF16 1
+#define QWZ_DTYPE_F32 2 /* logits of qwz_token_logprobs only */
 
 /* Bits of the device error word. */
 #define QWZ_DEVERR_TABLE_RANGE 1
 #define QWZ_DEVERR_PAGE_RANGE 2
 #define QWZ_DEVERR_SLOT_RANGE 4
 #define QWZ_DEVERR_TIMEOUT 8 /* a bounded in-kernel wait gave up */
+#define QWZ_DEVERR_POOL_EMPTY 16 /* qwz_batch_tables: not enough free pages (or ring places) */
 
 /* Library version string. */
 const char* qwz_version(void);
@@ -393,6 +395,87 @@ int qwz_k8v4_combine(const float* partial_o, const float* partial_ml, void* out,
                      int32_t num_splits, const void* sinks, int32_t q_len, int32_t dtype, void* stream);
 int qwz_k8v4_gather(const void* words, const void* scales, const int32_t* block_table, int32_t table_width,
                     int32_t num_pages, int32_t length, int32_t bits, void* out, void* stream);
+
+/*
+ * Many requests over one NVFP4 pool (no reference counterpart: its engine
+ * serves one session).  The pool is the NVFP4 layout with any number of KV
+ * heads and head_dim 64, 128 or 256: codes uint8 [P, 256, kv_heads, dim / 2],
+ * scales E4M3 [P, 256, kv_heads, dim / 16].  A slot is page * 256 + offset.
+ * A step of R requests is described by
+ *   cu_rows [R + 1]  request b's new rows are rows cu_rows[b] .. cu_rows[b + 1]
+ *   kv_lens [R]      its tokens including the new rows
+ *   block_table [R, table_width]  its logical page -> physical page
+ * all int32 device arrays, never read on the host.
+ *
+ * qwz_batch_tables builds that description from the requests' lengths:
+ *   lengths [R]   tokens held; new_rows [R] rows to add (0: idle, < 0: the
+ *                 request ends); held [R] pages held (its first table entries)
+ *   ring [ring_size], ring_state [2] = (first, count): free page ids, at
+ *                 places first .. first + count - 1 modulo ring_size
+ * Pages are taken from the ring in request order and entered in block_table
+ * (in place); those of requests that end are put back behind the free ones.
+ * Outputs (no storage shared with the inputs, so a step may be built again
+ * from the same state): cu_rows, kv_lens, held_out [R], ring_out [2], and for
+ * row r < rows slots[r], positions[r] (token position), request_of[r].  Rows
+ * past cu_rows[R] get slot -1, position 0, request -1.  A request that does
+ * not fit its table row (QWZ_DEVERR_TABLE_RANGE), or, from the first one that
+ * the free pages do not cover on, any request that needs a page
+ * (QWZ_DEVERR_POOL_EMPTY), is denied: it takes no page, its rows get slot -1
+ * and its kv_lens is 0.  A request that ends has kv_lens 0 and held_out 0.
+ */
+int qwz_batch_tables(const int32_t* lengths, const int32_t* new_rows, const int32_t* held, int32_t* ring,
+                     const int32_t* ring_state, int32_t* block_table, int32_t* cu_rows, int32_t* kv_lens,
+                     int32_t* held_out, int32_t* ring_out, int32_t* slots, int32_t* positions, int32_t* request_of,
+                     int32_t requests, int32_t table_width, int32_t ring_size, int64_t rows, void* stream);
+
+/*
+ * Quantises rows k, v [rows, kv_heads, dim] (FP16/BF16, row strides in
+ * elements, multiples of 8, 16-byte aligned) into their slots, with the
+ * rounding of qwz_nvfp4_append.  A negative slot is not stored; one outside
+ * the pool sets QWZ_DEVERR_SLOT_RANGE.  k_held, v_held (NULL: not wanted):
+ * [rows, kv_heads, dim] contiguous, same type, the values that the cache holds
+ * for the rows (written for rows without a slot too).
+ */
+int qwz_batch_append(const void* k, const void* v, void* k_cache, void* v_cache, void* k_scales, void* v_scales,
+                     const int32_t* slots, void* k_held, void* v_held, int64_t rows, int64_t k_stride,
+                     int64_t v_stride, int32_t num_kv_heads, int32_t head_dim, int32_t num_pages, int32_t dtype,
+                     void* stream);
+
+/*
+ * Attention of every request's rows over its pages: row s of the n rows of a
+ * request with kv tokens sees tokens j < kv - n + s + 1 (none: the row is 0).
+ *   q, out  [rows, q_heads, dim] FP16/BF16, row strides in elements (multiples
+ *           of 8); q_heads is 1 to 64 times kv_heads
+ *   max_rows  host bound of a request's rows; a larger request is cut there
+ *   workspace qwz_batch_attend_workspace_bytes(head_dim) bytes (0: bad
+ *           head_dim), 16-byte aligned, for one call at a time
+ * Rows outside every request are not written.  A length beyond the table or a
+ * row range outside [0, rows] sets QWZ_DEVERR_TABLE_RANGE (clipped, or the
+ * request skipped); a table entry outside the pool sets QWZ_DEVERR_PAGE_RANGE
+ * and its tokens count as absent.
+ */
+int64_t qwz_batch_attend_workspace_bytes(int32_t head_dim);
+int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+                     const void* v_scales, const int32_t* block_table, const int32_t* cu_rows,
+                     const int32_t* kv_lens, void* out, void* workspace, int64_t workspace_bytes, int32_t rows,
+                     int32_t requests, int32_t max_rows, int32_t table_width, int32_t num_pages,
+                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t q_stride,
+                     int64_t out_stride, float sm_scale, int32_t dtype, void* stream);
+
+/*
+ * Of each row of logits [rows, vocab] (FP16/BF16/FP32, any row stride): the
+ * log probability of ids[row] (int32, or int64 when ids64 != 0), the entropy
+ * in nats, and the `top` (0..32) most likely tokens with their log
+ * probabilities, equal logits by lowest index.  ids < 0: log probability 0;
+ * ids >= vocab: NaN and QWZ_DEVERR_SLOT_RANGE.  -inf logits are impossible
+ * tokens; a row of nothing else gives log probabilities -inf and entropy 0.  A
+ * NaN or +inf logit makes the row's numbers NaN (NaN ranks last).  workspace:
+ * qwz_token_logprobs_workspace_bytes (0: bad sizes), 16-byte aligned.
+ */
+int64_t qwz_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top, int32_t dtype);
+int qwz_token_logprobs(const void* logits, const void* ids, int32_t ids64, float* logprob, float* entropy,
+                       float* top_logprobs, int32_t* top_ids, void* workspace, int64_t workspace_bytes, int32_t rows,
+                       int32_t vocab, int32_t top, int64_t stride, int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

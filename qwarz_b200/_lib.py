@@ -17,6 +17,7 @@ QWZ_EINVAL = -1
 QWZ_ELAUNCH = -2
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
+DTYPE_F32 = 2  # logits only
 NODE_SPLIT = 0
 NODE_COMBINE = 1
 
@@ -60,8 +61,16 @@ SIGNATURES = {
     "qwz_shard_exchange_combine_emulated": [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p,
                                             c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32,
                                             c_void_p],
+    "qwz_batch_tables": [c_void_p] * 13 + [c_int32] * 3 + [c_int64, c_void_p],
+    "qwz_batch_append": [c_void_p] * 9 + [c_int64] * 3 + [c_int32] * 4 + [c_void_p],
+    "qwz_batch_attend_workspace_bytes": [c_int32],
+    "qwz_batch_attend": [c_void_p] * 10 + [c_int64] + [c_int32] * 8 + [c_int64] * 2 + [c_float, c_int32, c_void_p],
+    "qwz_token_logprobs_workspace_bytes": [c_int32] * 4,
+    "qwz_token_logprobs": [c_void_p, c_void_p, c_int32] + [c_void_p] * 5 + [c_int64] + [c_int32] * 3
+                          + [c_int64, c_int32, c_void_p],
 }
-_RESTYPE = {"qwz_version": c_char_p, "qwz_last_error": c_char_p, "qwz_peer_buffer_bytes": c_int64}
+_RESTYPE = {"qwz_version": c_char_p, "qwz_last_error": c_char_p, "qwz_peer_buffer_bytes": c_int64,
+            "qwz_batch_attend_workspace_bytes": c_int64, "qwz_token_logprobs_workspace_bytes": c_int64}
 
 _LIB = None
 

@@ -1,0 +1,72 @@
+// Device helpers shared by the kernels that serve many requests from one
+// NVFP4 pool: the split of all requests' work over the CTAs of a launch, and
+// the records through which CTAs that share an item hand over their partials.
+//
+// The work of a launch is the concatenation, over requests, heads and groups
+// of query rows, of the KV tiles each of them has to visit.  CTA i of N takes
+// units [i * total / N, (i + 1) * total / N), so the CTAs' shares differ by at
+// most one tile whatever the lengths are, and only the first and the last item
+// of a CTA can be shared with other CTAs: two records a CTA hold every partial,
+// independent of the number of requests.  Every CTA finds its share from the
+// lengths alone (one scan), so a call needs no schedule made beforehand.
+#pragma once
+
+#include "qwz_common.cuh"
+#include "qwz_kernels.h"
+
+#include <math_constants.h>
+
+namespace qwz {
+namespace batch {
+
+// Rows and tokens of request b, clipped to what the buffers hold.
+struct Req {
+  int row0;  // first row in q / out
+  int n;     // rows
+  int kv;    // tokens after the step
+};
+
+QWZ_DEVINL Req load_req(const BatchAttnParams& p, int b) {
+  Req r;
+  const int lo = __ldg(p.cu_rows + b), hi = __ldg(p.cu_rows + b + 1);
+  r.row0 = lo;
+  r.n = hi - lo;
+  r.kv = __ldg(p.kv_lens + b);
+  if (lo < 0 || hi < lo || hi > p.rows) {  // never address rows that do not exist
+    flag_error(kErrTableRange);
+    r.row0 = 0;
+    r.n = 0;
+  }
+  if (r.kv > p.table_width * kPage) {
+    flag_error(kErrTableRange);
+    r.kv = p.table_width * kPage;
+  }
+  if (r.kv < 0) r.kv = 0;
+  return r;
+}
+
+// Exclusive scan of one value a thread over the CTA (blockDim.x <= 1024, a
+// multiple of 32); returns the thread's prefix, the CTA's total in `total`.
+QWZ_DEVINL long long block_scan(long long v, long long* warp_sums, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  long long before = 0;
+  total = 0;
+  for (int w = 0; w < warps; ++w) {
+    const long long s = warp_sums[w];
+    if (w < warp) before += s;
+    total += s;
+  }
+  __syncthreads();
+  return before + x - v;
+}
+
+}  // namespace batch
+}  // namespace qwz

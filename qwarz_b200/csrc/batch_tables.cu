@@ -1,0 +1,257 @@
+// Paging of many requests on the device: page allocation, block tables, slot
+// map and row offsets of one step from the requests' lengths; and the writer
+// that quantises the step's K/V rows into their slots (sm_100a).
+//
+// Tables.  Request b holds held[b] pages and lengths[b] tokens and adds
+// new[b] rows, or ends (new[b] < 0).  With
+//   grow[b] = max(0, ceil((lengths[b] + new[b]) / 256) - held[b])  (new[b] > 0)
+// pages are taken from a ring of free ids in request order (exclusive scan of
+// grow), those of requests that end go behind the free ones.  Row r of request
+// b, position p = lengths[b] + r, gets slot table[b][p / 256] * 256 + p % 256.
+// All of it is a few bytes a request and 12 bytes a row: the launch and the
+// latency of one scan bound it, so every CTA scans all requests by itself (two
+// packed 64-bit scans) instead of waiting for another CTA, and then fills its
+// part of the rows and of the tables.
+#include "batch_common.cuh"
+#include "nvfp4_quant.cuh"
+
+namespace qwz {
+
+namespace {
+
+constexpr int kTabThreads = 1024;
+
+struct TabReq {
+  int len, n, held, grow;  // n: rows; grow before the pool's limit
+  bool ends, wide;         // wide: does not fit the table
+};
+
+QWZ_DEVINL TabReq tab_req(const BatchTablesParams& p, int b) {
+  TabReq t;
+  t.len = max(__ldg(p.lengths + b), 0);
+  t.n = __ldg(p.new_rows + b);
+  t.held = min(max(__ldg(p.held + b), 0), p.table_width);
+  t.ends = t.n < 0;
+  t.n = max(t.n, 0);
+  const long long end = (long long)t.len + t.n;
+  t.wide = t.n > 0 && end > (long long)p.table_width * kPage;
+  t.grow = (t.n > 0 && !t.wide) ? max((int)((end + kPage - 1) / kPage) - t.held, 0) : 0;
+  return t;
+}
+
+QWZ_DEVINL long long pack(int lo, int hi) { return ((long long)hi << 32) | (unsigned)lo; }
+QWZ_DEVINL int lo32(long long v) { return (int)(unsigned)v; }
+QWZ_DEVINL int hi32(long long v) { return (int)(v >> 32); }
+
+}  // namespace
+
+__global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_constant__ BatchTablesParams p) {
+  __shared__ long long starts[kTabThreads];  // (rows, grown pages) before each thread's requests
+  __shared__ long long sums[32];
+  const int tid = threadIdx.x;
+  griddep_wait();
+  const int head = __ldg(p.ring_state), count = __ldg(p.ring_state + 1);
+  const int per = (p.requests + kTabThreads - 1) / kTabThreads;
+  const int b_lo = min(tid * per, p.requests), b_hi = min(b_lo + per, p.requests);
+
+  long long v = 0, total;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const TabReq t = tab_req(p, b);
+    v += pack(t.n, t.grow);
+  }
+  const long long before = batch::block_scan(v, sums, total);
+  starts[tid] = before;
+  // granted and freed pages: a request is granted while the pool lasts
+  auto denied = [&](const TabReq& t, int first) { return t.n > 0 && (t.wide || (t.grow > 0 && first + t.grow > count)); };
+  v = 0;
+  int first = hi32(before);
+  for (int b = b_lo; b < b_hi; ++b) {
+    const TabReq t = tab_req(p, b);
+    v += pack(t.ends ? t.held : 0, denied(t, first) ? 0 : t.grow);
+    first += t.grow;
+  }
+  long long pages;
+  int freed = lo32(batch::block_scan(v, sums, pages));
+  const int rows = lo32(total);
+
+  // the requests: CTA 0 writes the per-request words, the table entries and
+  // the ring are shared out by request
+  const int F = p.ring_size;
+  auto ring_at = [&](long long i) { return (int)((head + i) % F); };
+  const bool state_ok = head >= 0 && head < F && count >= 0 && count <= F;
+  int row = lo32(before);
+  first = hi32(before);
+  for (int b = b_lo; b < b_hi; ++b) {
+    const TabReq t = tab_req(p, b);
+    const bool no = denied(t, first);
+    if (blockIdx.x == 0) {
+      p.cu_rows[b] = row;
+      p.kv_lens[b] = (t.ends || no) ? 0 : t.len + t.n;
+      p.held_out[b] = t.ends ? 0 : t.held + (no ? 0 : t.grow);
+      if (no) flag_error(t.wide ? kErrTableRange : kErrPoolEmpty);
+    }
+    if ((unsigned)b % gridDim.x == blockIdx.x && state_ok) {
+      int32_t* table = p.block_table + (size_t)b * p.table_width;
+      if (!no)
+        for (int j = 0; j < t.grow; ++j) table[t.held + j] = __ldg(p.ring + ring_at((long long)first + j));
+      if (t.ends)
+        for (int j = 0; j < t.held; ++j) {
+          const long long at = (long long)count + freed + j;
+          if (at < F) p.ring[ring_at(at)] = table[j];
+          else flag_error(kErrPoolEmpty);  // more pages than the ring has places
+        }
+    }
+    row += t.n;
+    first += t.grow;
+    freed += t.ends ? t.held : 0;
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    p.cu_rows[p.requests] = rows;
+    p.ring_out[0] = state_ok ? ring_at(hi32(pages)) : head;
+    p.ring_out[1] = (int)min((long long)count - hi32(pages) + lo32(pages), (long long)F);
+    if (!state_ok) flag_error(kErrPageRange);
+    if (rows > p.rows) flag_error(kErrSlotRange);  // rows past the slot map's end get no slot
+  }
+
+  // the rows: find the thread whose requests hold the row, walk to the request
+  for (long long r = (long long)blockIdx.x * kTabThreads + tid; r < p.rows; r += (long long)gridDim.x * kTabThreads) {
+    int slot = -1, pos = 0, req = -1;
+    if (r < rows) {
+      int at = 0;
+      for (int step = kTabThreads / 2; step > 0; step >>= 1)
+        if (lo32(starts[at + step]) <= r) at += step;
+      int off = (int)r - lo32(starts[at]);
+      first = hi32(starts[at]);
+      int b = at * per;
+      TabReq t = tab_req(p, b);
+      while (off >= t.n && b + 1 < p.requests) {
+        off -= t.n;
+        first += t.grow;
+        t = tab_req(p, ++b);
+      }
+      req = b;
+      pos = t.len + off;
+      if (!denied(t, first) && state_ok) {
+        const int j = pos / kPage;
+        int page;
+        if (j < t.held) page = p.block_table[(size_t)b * p.table_width + j];
+        else page = __ldg(p.ring + ring_at((long long)first + j - t.held));
+        if (page >= 0 && page <= 0x7fffffff / kPage - 1) slot = page * kPage + pos % kPage;
+        else flag_error(kErrPageRange);
+      }
+    }
+    p.slots[r] = slot;
+    p.positions[r] = pos;
+    p.request_of[r] = req;
+  }
+  griddep_launch_dependents();
+}
+
+// One thread quantises one 16-element block of K or V: 32 bytes in, 8 code
+// bytes, one scale byte and (optionally) the 32 bytes the cache now stands for
+// out; bound by HBM.  The rounding is that of nvfp4_quant.cuh: s = E4M3(amax /
+// 6), code = E2M1 of the correctly rounded x / s.  The quotient is made from
+// the correctly rounded reciprocal by one residual step (Markstein: correctly
+// rounded when the reciprocal is), 3 operations instead of a division, and
+// converted two at a time; |x| is first cut at 8 s (E2M1 ends at 6), which also
+// keeps infinities out of the residual and sends NaN to +6, as there.
+template <typename T>
+__global__ void __launch_bounds__(256) batch_append_kernel(const __grid_constant__ BatchAppendParams p) {
+  griddep_wait();
+  const int blocks = p.dim / 16;
+  const long long per_row = (long long)p.kv_heads * blocks;
+  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+  const bool is_v = blockIdx.y != 0;
+  if (idx >= p.rows * per_row) return;
+  const long long row = idx / per_row;
+  const int in = (int)(idx % per_row);  // head * blocks + block
+  const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + row * (is_v ? p.v_stride : p.k_stride) + in * 16;
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
+  const uint4 b = __ldg(reinterpret_cast<const uint4*>(src) + 1);
+  const int slot = __ldg(p.slots + row);
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  float x[16], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = InTraits<T>::to_float2(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+    amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+  }
+  const uint32_t sbits = quant::e4m3_encode_nonneg(__fdiv_rn(amax, 6.0f));
+  const float s = quant::e4m3_decode(sbits);
+  uint32_t code[2] = {0u, 0u};
+  if (s > 0.f) {
+    const float r = __frcp_rn(s), cut = 8.f * s;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float y[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float c = fmaxf(fminf(x[i + e], cut), -cut);
+        const float q = __fmul_rn(c, r);
+        y[e] = __fmaf_rn(__fmaf_rn(-q, s, c), r, q);
+      }
+      uint32_t pair;
+      asm("{\n .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n cvt.u32.u8 %0, t;\n}\n"
+          : "=r"(pair)
+          : "f"(y[0]), "f"(y[1]));
+      code[i >> 3] |= pair << (4 * (i & 7));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // a zero magnitude carries no sign
+      const uint32_t m = code[i] & 0x77777777u;
+      const uint32_t some = (m | (m >> 1) | (m >> 2)) & 0x11111111u;
+      code[i] = m | (code[i] & (some << 3));
+    }
+  }
+  if (slot >= 0 && (slot >> 8) < p.num_pages) {
+    const size_t at = (size_t)slot * per_row + in;
+    *reinterpret_cast<uint2*>((is_v ? p.v_cache : p.k_cache) + at * 8) = make_uint2(code[0], code[1]);
+    (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)sbits;
+  } else if (slot >= 0) {
+    flag_error(kErrSlotRange);
+  }
+  void* held = is_v ? p.v_held : p.k_held;
+  if (held != nullptr) {  // code x scale: at most 6 significant bits, exact in FP16 and BF16
+    uint32_t h[8], s0, s1;
+    {
+      uint32_t t[4];
+      e2m1x8_to_f16x2x4(code[0], t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = t[i];
+      e2m1x8_to_f16x2x4(code[1], t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[4 + i] = t[i];
+    }
+    e4m3x4_to_f16x2x2(sbits * 0x0101u, s0, s1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[i] = hmul2_u32(h[i], s0);
+      if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+        const float2 f = InTraits<__half>::to_float2(h[i]);
+        const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
+        h[i] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(held) + (row * per_row + in) * 16);
+    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+  }
+}
+
+cudaError_t launch_batch_tables(const BatchTablesParams& p, int sms, cudaStream_t stream) {
+  const long long want = (p.rows + kTabThreads - 1) / kTabThreads;
+  const int grid = (int)max(1LL, min(want, (long long)sms));
+  return launch_pdl(batch_tables_kernel, dim3(grid), dim3(kTabThreads), 0, stream, p);
+}
+
+cudaError_t launch_batch_append(const BatchAppendParams& p, int dtype, cudaStream_t stream) {
+  if (p.rows <= 0) return cudaSuccess;
+  const long long n = p.rows * (long long)p.kv_heads * (p.dim / 16);
+  const dim3 grid((unsigned)((n + 255) / 256), 2);
+  if (dtype == kDtypeBF16) return launch_pdl(batch_append_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
+  return launch_pdl(batch_append_kernel<__half>, grid, dim3(256), 0, stream, p);
+}
+
+}  // namespace qwz
