@@ -12,6 +12,7 @@
 #pragma once
 
 #include "qwz_common.cuh"
+#include "batch_kernels.h"
 #include "qwz_kernels.h"
 
 #include <math_constants.h>

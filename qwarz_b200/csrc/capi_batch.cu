@@ -4,6 +4,7 @@
 // uses the argument checks of capi.cu.
 
 #include "qwz_common.cuh"
+#include "batch_kernels.h"
 #include "qwz_kernels.h"
 #include "../../include/qwz_b200.h"
 

@@ -33,7 +33,6 @@ enum DeviceError : int {
   kErrPageRange = 2,   // physical page id outside the cache pool
   kErrSlotRange = 4,   // FP8 draft slot beyond the store capacity
   kErrTimeout = 8,     // a bounded mbarrier wait gave up
-  kErrPoolEmpty = 16,  // a step needs more pages than the pool has free
 };
 
 // Device-wide error word.  The library is one translation unit

@@ -15,6 +15,7 @@
 // than K) are collected and ranked by counting.  A second kernel, one CTA a
 // row, joins the chunks in order; no result depends on the order of atomics.
 #include "qwz_common.cuh"
+#include "batch_kernels.h"
 #include "qwz_kernels.h"
 
 #include <math_constants.h>
