@@ -446,12 +446,12 @@ int qwz_batch_append(const void* k, const void* v, void* k_cache, void* v_cache,
  * request with kv tokens sees tokens j < kv - n + s + 1 (none: the row is 0).
  *   q, out  [rows, q_heads, dim] FP16/BF16, row strides in elements (multiples
  *           of 8); q_heads is 1 to 64 times kv_heads
- *   max_rows  host bound of a request's rows; a larger request is cut there
+ *   max_rows  host bound of a request's rows
  *   workspace qwz_batch_attend_workspace_bytes(head_dim) bytes (0: bad
  *           head_dim), 16-byte aligned, for one call at a time
- * Rows outside every request are not written.  A length beyond the table or a
- * row range outside [0, rows] sets QWZ_DEVERR_TABLE_RANGE (clipped, or the
- * request skipped); a table entry outside the pool sets QWZ_DEVERR_PAGE_RANGE
+ * Rows outside every request are not written.  A length beyond the table, a
+ * row range outside [0, rows] or more than max_rows rows set
+ * QWZ_DEVERR_TABLE_RANGE (the length is clipped, the request skipped); a table entry outside the pool sets QWZ_DEVERR_PAGE_RANGE
  * and its tokens count as absent.
  */
 int64_t qwz_batch_attend_workspace_bytes(int32_t head_dim);

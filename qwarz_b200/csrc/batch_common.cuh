@@ -33,7 +33,7 @@ QWZ_DEVINL Req load_req(const BatchAttnParams& p, int b) {
   r.row0 = lo;
   r.n = hi - lo;
   r.kv = __ldg(p.kv_lens + b);
-  if (lo < 0 || hi < lo || hi > p.rows) {  // never address rows that do not exist
+  if (lo < 0 || hi < lo || hi > p.rows || r.n > p.max_rows) {  // never address rows that do not exist
     flag_error(kErrTableRange);
     r.row0 = 0;
     r.n = 0;

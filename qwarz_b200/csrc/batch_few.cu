@@ -95,26 +95,23 @@ QWZ_DEVINL void cp_async_small(uint32_t dst, const void* src) {
 // Walks the units (request, item, page) of the launch in order.
 template <int D>
 struct FewWalk {
-  int b, item, page;       // request, (head, column group) index, page
-  int items, pages;        // of request b
+  int b, head, page;       // request, KV head, page
+  int pages;               // of request b
   batch::Req r;
 
-  static QWZ_DEVINL void shape(const BatchAttnParams& p, const batch::Req& r, int& items, int& pages) {
-    const int cols = r.n * p.group;
-    items = p.kv_heads * ((cols + Few<D>::kCols - 1) / Few<D>::kCols);
-    pages = max(1, (r.kv + kPage - 1) / kPage);  // a request without tokens still has rows to write
+  static QWZ_DEVINL bool few(const BatchAttnParams& p, const batch::Req& r) {
+    return r.n > 0 && r.n * p.group <= p.few_cols;  // the others are batch_rows.cu's
   }
+  // a request without tokens still has rows to write
+  static QWZ_DEVINL int pages_of(const batch::Req& r) { return max(1, (r.kv + kPage - 1) / kPage); }
   static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b) {
     const batch::Req r = batch::load_req(p, b);
-    if (r.n == 0) return 0;
-    int items, pages;
-    shape(p, r, items, pages);
-    return (long long)items * pages;
+    return few(p, r) ? (long long)p.kv_heads * pages_of(r) : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
     r = batch::load_req(p, b);
-    shape(p, r, items, pages);
+    pages = pages_of(r);
   }
   // Unit `u` counted from the start of request b0.
   QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long u) {
@@ -124,21 +121,19 @@ struct FewWalk {
       u -= c;
     }
     enter(p, min(b, p.requests - 1));
-    item = (int)(u / pages);
+    head = (int)(u / pages);
     page = (int)(u % pages);
   }
   QWZ_DEVINL void next(const BatchAttnParams& p) {
     if (++page < pages) return;
     page = 0;
-    if (++item < items) return;
-    item = 0;
+    if (++head < p.kv_heads) return;
+    head = 0;
     for (int bb = b + 1; bb < p.requests; ++bb) {
       enter(p, bb);
-      if (r.n > 0) return;
+      if (few(p, r)) return;
     }
   }
-  QWZ_DEVINL int head(const BatchAttnParams& p) const { return item % p.kv_heads; }
-  QWZ_DEVINL int col0(const BatchAttnParams& p) const { return item / p.kv_heads * Few<D>::kCols; }
   // Table entry of the unit, unchecked (the load is in flight until it is used).
   QWZ_DEVINL int entry(const BatchAttnParams& p) const {
     return __ldg(p.block_table + (size_t)b * p.table_width + page);
@@ -227,7 +222,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
     const int valid = pre.present(p, pre_page) ? min(kFewTok, pre.r.kv - t0) : 0;
     if (valid > 0) {
       const size_t row0 = (size_t)pre_page * kPage + warp * kFewTok;
-      const size_t hd = pre.head(p);
+      const size_t hd = pre.head;
       const uint32_t dst = ring + slot * F::kStage;
       constexpr int CPR = F::kRow / 16;
 #pragma unroll
@@ -276,14 +271,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
     if (fresh) {  // ------------------------------------------- a new item
       fresh = false;
       first_page = cur.page;
-      const int c0 = cur.col0(p), hd = cur.head(p);
-      cols = min(F::kCols, cur.r.n * p.group - c0);
+      const int hd = cur.head;
+      cols = cur.r.n * p.group;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int c = nt * 8 + g;
         float amax = 0.f;
         if (c < cols) {
-          const int s = (c0 + c) / p.group, h = hd * p.group + (c0 + c) % p.group;
+          const int s = c / p.group, h = hd * p.group + c % p.group;
           const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) +
                                                             (cur.r.row0 + s) * p.q_stride + h * D + qd * (D / 4));
 #pragma unroll
@@ -316,15 +311,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
         for (int i = 0; i < 2; ++i) {
           cf[nt][i] = __shfl_sync(kFull, rowfac, 4 * (2 * qd + i));
           const int cc = nt * 8 + 2 * qd + i;
-          lim[nt][i] = cc < cols ? cur.r.kv - cur.r.n + (c0 + cc) / p.group + 1 : 0;
+          lim[nt][i] = cc < cols ? cur.r.kv - cur.r.n + cc / p.group + 1 : 0;
           m[nt][i] = -CUDART_INF_F;
           l[nt][i] = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
-      min_lim = cur.r.kv - cur.r.n + c0 / p.group + 1;
-      max_lim = cur.r.kv - cur.r.n + (c0 + cols - 1) / p.group + 1;
+      min_lim = cur.r.kv - cur.r.n + 1;
+      max_lim = cur.r.kv - cur.r.n + (cols - 1) / p.group + 1;
     }
 
     cp_async_wait<F::kStages - 2>();
@@ -525,7 +520,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
         }
       }
       __syncthreads();
-      const int c0 = cur.col0(p), hd = cur.head(p);
+      const int hd = cur.head;
       for (int idx = tid; idx < cols * (D / 2); idx += kFewThreads) {
         const int c = idx / (D / 2), d = idx % (D / 2) * 2;
         // d = D/8 gg + 2j sits in m-tile j, lane row gg: (d, col) in c0/c1, (d + 1, col) in c2/c3
@@ -539,7 +534,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
           a1 += weights[c * kFewWarps + w] * s[src + 2];
         }
         if (whole) {
-          const int s = (c0 + c) / p.group, h = hd * p.group + (c0 + c) % p.group;
+          const int s = c / p.group, h = hd * p.group + c % p.group;
           T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + s) * p.out_stride + h * D + d;
           dst[0] = InTraits<T>::from_float(a0 * col_l[c]);
           dst[1] = InTraits<T>::from_float(a1 * col_l[c]);
@@ -551,7 +546,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
         const long long last_unit = hi - 1 - cur.page + cur.pages - 1;
         meta[0] = cols;
         meta[1] = cur.r.row0;
-        meta[2] = c0;
         meta[3] = hd;
         meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
         meta[5] = (int)min(total, n_cta);  // fewer units than CTAs leave some CTAs without a record
@@ -567,7 +561,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
 
 // Merges the records of the items that more than one CTA worked on, CTA by
 // CTA in order: block (i, y) takes columns y, y + gridDim.y, ... of the item
-// that CTA i began and did not finish.
+// that CTA i began and did not finish.  
 template <typename T, int D, int COLS>
 __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
@@ -580,7 +574,7 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
   const int32_t* meta = p.meta + i0 * kBatchMeta;
   const int cols = __ldcg(meta);
   if (cols == 0) return;
-  const int row0 = __ldcg(meta + 1), c0 = __ldcg(meta + 2), hd = __ldcg(meta + 3), last = __ldcg(meta + 4);
+  const int row0 = __ldcg(meta + 1), hd = __ldcg(meta + 3), last = __ldcg(meta + 4);
   const int busy = __ldcg(meta + 5);
   const int parts = last - i0 + 1;
   constexpr size_t kRec = (size_t)COLS * (D + 2);
@@ -641,7 +635,7 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
         a.w += v.w;
       }
       const float inv = L > 0.f ? 1.f / L : 0.f;
-      const int s = (c0 + c) / p.group, h = hd * p.group + (c0 + c) % p.group;
+      const int s = c / p.group, h = hd * p.group + c % p.group;
       T* dst = reinterpret_cast<T*>(p.out) + (row0 + s) * p.out_stride + h * D + tid * 4;
       dst[0] = InTraits<T>::from_float(a.x * inv);
       dst[1] = InTraits<T>::from_float(a.y * inv);
@@ -661,7 +655,9 @@ cudaError_t launch_few(const BatchAttnParams& p, int ctas, cudaStream_t stream) 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(ctas), dim3(kFewThreads), Few<D>::kSmem, stream, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(batch_combine_kernel<T, D, Few<D>::kCols>, dim3(ctas, 8), dim3(256), 0, stream, p);
+  e = launch_pdl(batch_combine_kernel<T, D, Few<D>::kCols>, dim3(ctas, 8), dim3(256), 0, stream, p);
+  if (e != cudaSuccess || (long long)p.max_rows * p.group <= p.few_cols) return e;
+  return launch_rows<T, D>(p, ctas, stream);
 }
 
 template <typename T>
@@ -676,8 +672,12 @@ cudaError_t launch_attend(const BatchAttnParams& p, int dim, int ctas, cudaStrea
 
 }  // namespace
 
+size_t batch_few_record_bytes(int dim) {
+  return (size_t)kBatchMaxCtas * 2 * (2048 / dim) * (dim + 2) * sizeof(float);
+}
 size_t batch_workspace_bytes(int dim) {
-  return kBatchMetaBytes + (size_t)kBatchMaxCtas * 2 * (2048 / dim) * (dim + 2) * sizeof(float);
+  return kBatchMetaBytes + batch_few_record_bytes(dim) +
+         (size_t)kBatchMaxCtas * 2 * kRwRows * (dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_batch_attend(const BatchAttnParams& p, int dim, int dtype, int ctas, cudaStream_t stream) {

@@ -22,16 +22,19 @@ struct BatchAttnParams {
   const int32_t* block_table;    // [requests, table_width]
   const int32_t* cu_rows;        // [requests + 1] first row of each request
   const int32_t* kv_lens;        // [requests] tokens after the step
-  float* records;                // partial records, two per CTA
-  int32_t* meta;                 // [CTAs][kBatchMeta] what the combine has to do
+  float* records;                // partial records of batch_few.cu, two per CTA
+  float* row_records;            // and of batch_rows.cu
+  int32_t* meta;                 // [2][kBatchMaxCtas][kBatchMeta] what the combines have to do
   long long q_stride, out_stride;  // elements
   int requests, rows, table_width, num_pages, kv_heads, group;
   int max_rows;                  // upper bound of a request's rows
+  int few_cols;                  // most (row, head) columns a KV head of batch_few.cu has
   float sm_scale_log2;           // sm_scale * log2(e)
 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA
 constexpr int kBatchMaxCtas = 256;
-constexpr size_t kBatchMetaBytes = (size_t)kBatchMaxCtas * kBatchMeta * 4;
+constexpr size_t kBatchMetaBytes = 2 * (size_t)kBatchMaxCtas * kBatchMeta * 4;
+size_t batch_few_record_bytes(int dim);  // all records of batch_few.cu
 size_t batch_workspace_bytes(int dim);
 
 // Paging of many requests (batch_tables.cu).

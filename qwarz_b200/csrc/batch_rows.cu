@@ -1,0 +1,677 @@
+// Attention of many requests over one NVFP4 pool, many query rows a request
+// (verify windows, prompt chunks), sm_100a, tcgen05 with the accumulators in
+// tensor memory.  The formula is that of batch_few.cu.
+//
+// An item is one request, one KV head and 128 / group query positions: their
+// (position, head) rows are the M = 128 rows of every MMA.  It visits the
+// 128-token KV tiles up to its last row's causal limit.  One persistent CTA per
+// SM takes an equal share of all items' tiles (batch_common.cuh); 13 warps:
+//   warps 0-3   softmax, thread = row (TMEM lane); Q staging and epilogue
+//   warps 4-11  dequantise K(j) and V(j): codes straight from the pool into
+//               registers one tile ahead, FP16 into shared memory as
+//               [128 tok][D] (64-wide head-dim atoms, 128-byte swizzle): the same
+//               bytes are the K-major B operand of QK and the MN-major B
+//               operand of PV
+//   warp 12     tensor-memory owner and MMA issuer (one thread)
+// Per tile: S(j) [128 x 128] = Q K(j)^T into one of two S buffers, softmax
+// writes P(j) (FP16, 11 significant bits as the output has) over S(j), and
+// O [128 x D] += P(j) V(j) with P from tensor memory.  The MMA thread queues
+// QK(j + 1) ahead of PV(j); K(j + 1) is dequantised while PV(j - 1) runs and
+// V(j) while QK(j + 1) does, so one buffer of each suffices (192 KB at D 256).
+//
+// What bounds it (D 256): 2,048 tensor cycles a tile against 2,560 of shared
+// memory: 128 KB of QK operands, 64 KB of V and 128 KB of dequantised stores.
+#include "attn_common.cuh"
+#include "batch_common.cuh"
+#include "tc_common.cuh"
+
+namespace qwz {
+
+using namespace detail;
+
+namespace {
+
+constexpr int kRwTok = 128;                 // tokens of a tile
+constexpr int kRwRows = 128;                // MMA M
+constexpr int kRwSoft = 4;                  // softmax warps
+constexpr int kRwDq = 8;                    // dequant warps
+constexpr int kRwMma = kRwSoft + kRwDq;     // MMA warp
+constexpr int kRwWarps = kRwMma + 1;
+constexpr int kRwThreads = kRwWarps * 32;
+constexpr int kRwScan = 256;                // threads that scan the requests
+
+template <int D>
+struct Rows {
+  static constexpr int kAtoms = D / 64;
+  static constexpr int kTile = kRwTok * D * 2;           // FP16 K or V tile
+  static constexpr int kQ = 0;                           // kAtoms x [128 rows x 128 B]
+  static constexpr int kK = kQ + kRwRows * D * 2;
+  static constexpr int kV = kK + kTile;
+  static constexpr int kBars = kV + kTile;
+  static constexpr int kNumBars = 12;
+  static constexpr int kMeta = kBars + 8 * kNumBars;     // TMEM base, abort flag
+  static constexpr int kRowfac = kMeta + 16;             // [128]
+  static constexpr int kStarts = kRowfac + 4 * kRwRows;  // [kRwScan] units before each scanning thread
+  static constexpr int kSums = kStarts + 8 * kRwScan;    // [kRwWarps]
+  static constexpr int kSmem = kSums + 8 * 16 + 1024;
+  static constexpr uint32_t kTmS = 0, kTmO = 256, kTmCols = 512;
+  static constexpr size_t kRec = (size_t)kRwRows * (D + 2);  // floats of a record
+};
+
+// S, P and PV have a barrier per S buffer: a softmax warp may be a tile ahead
+// of another, and its arrival for P(j + 1) must not count for P(j); and PV's
+// completions are not all waited for, so with one barrier a waiter could be two
+// phases off and take a phase's parity for another's.
+enum RwBar : int {
+  kRwKReady, kRwKFree, kRwVReady, kRwVFree, kRwSFull0, kRwSFull1, kRwPReady0, kRwPReady1, kRwPvDone0, kRwPvDone1, kRwQReady, kRwFin
+};
+
+// Walks the units (request, head, group of positions, tile) of the launch.
+struct RowsWalk {
+  int b, h, i, tile;
+  int tiles, groups;
+  int per;                 // positions of an item
+  batch::Req r;
+
+  QWZ_DEVINL static int tiles_of(const batch::Req& r, int per, int i) {
+    const int lim = r.kv - r.n + min((i + 1) * per, r.n);
+    return max(1, (lim + kRwTok - 1) / kRwTok);
+  }
+  QWZ_DEVINL static long long head_cost(const batch::Req& r, int per) {
+    long long c = 0;
+    for (int i = 0; i * per < r.n; ++i) c += tiles_of(r, per, i);
+    return c;
+  }
+  QWZ_DEVINL static bool many(const BatchAttnParams& p, const batch::Req& r) { return r.n * p.group > p.few_cols; }
+  QWZ_DEVINL static long long cost(const BatchAttnParams& p, int b, int per) {
+    const batch::Req r = batch::load_req(p, b);
+    return many(p, r) ? p.kv_heads * head_cost(r, per) : 0;
+  }
+  QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
+    b = bb;
+    r = batch::load_req(p, b);
+    groups = (r.n + per - 1) / per;
+  }
+  QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long u) {
+    for (b = b0; b < p.requests - 1; ++b) {
+      const long long c = cost(p, b, per);
+      if (u < c) break;
+      u -= c;
+    }
+    enter(p, b);
+    const long long c = max(1LL, head_cost(r, per));
+    h = (int)(u / c);
+    u %= c;
+    for (i = 0; i < groups - 1; ++i) {
+      const int t = tiles_of(r, per, i);
+      if (u < t) break;
+      u -= t;
+    }
+    tiles = tiles_of(r, per, i);
+    tile = (int)u;
+  }
+  QWZ_DEVINL void next(const BatchAttnParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++i >= groups) {
+      i = 0;
+      if (++h >= p.kv_heads) {
+        h = 0;
+        int bb = b + 1;
+        for (; bb < p.requests; ++bb) {
+          enter(p, bb);
+          if (many(p, r)) break;
+        }
+      }
+    }
+    tiles = tiles_of(r, per, i);
+  }
+  QWZ_DEVINL int entry(const BatchAttnParams& p) const {
+    return __ldg(p.block_table + (size_t)b * p.table_width + tile / (kPage / kRwTok));
+  }
+  QWZ_DEVINL bool present(const BatchAttnParams& p, int pp) const {
+    if (r.kv <= 0) return false;
+    if (pp >= 0 && pp < p.num_pages) return true;
+    flag_error(kErrPageRange);
+    return false;
+  }
+};
+
+QWZ_DEVINL void rw_ld32(uint32_t taddr, float (&x)[32]) {
+  uint32_t a[16], b[16];
+  tc::ld_32x32b_x16(taddr, a);
+  tc::ld_32x32b_x16(taddr + 16, b);
+  tc::wait_ld();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    asm volatile("" : "+r"(a[e]), "+r"(b[e])::"memory");
+    x[e] = __uint_as_float(a[e]);
+    x[16 + e] = __uint_as_float(b[e]);
+  }
+}
+
+// Codes and scales of one thread's share of a tile: D / 64 chunks of 32 head dims.
+template <int D>
+struct RwChunks {
+  uint4 w[D / 64];
+  uint32_t s[D / 64];
+};
+
+// Thread t of the dequant warps, load k: token row and 32-dim chunk.  Eight
+// neighbouring lanes hold eight token rows of one chunk, so the swizzled 16-byte
+// stores of a quarter warp touch every bank once.
+template <int D>
+QWZ_DEVINL void rw_place(int t, int k, int& row, int& chunk) {
+  constexpr int CPR = D / 32;
+  const int idx = (k * kRwDq + (t >> 5)) * 32 + (t & 31);
+  row = (idx & 7) + 8 * (idx / (8 * CPR));
+  chunk = (idx >> 3) % CPR;
+}
+
+template <int D>
+QWZ_DEVINL void rw_load(const BatchAttnParams& p, const uint8_t* codes, const uint8_t* scales, size_t token0, int h,
+                        int valid, int t, RwChunks<D>& out) {
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    int row, c;
+    rw_place<D>(t, k, row, c);
+    out.w[k] = make_uint4(0u, 0u, 0u, 0u);
+    out.s[k] = 0u;
+    if (row < valid) {
+      const size_t at = (token0 + row) * p.kv_heads + h;
+      out.w[k] = __ldg(reinterpret_cast<const uint4*>(codes + at * (D / 2)) + c);
+      out.s[k] = __ldg(reinterpret_cast<const unsigned short*>(scales + at * (D / 16)) + c);
+    }
+  }
+}
+
+template <int D>
+QWZ_DEVINL void rw_store(uint32_t tile, int t, const RwChunks<D>& in) {
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    int row, c;
+    rw_place<D>(t, k, row, c);
+    uint32_t s01, unused;
+    e4m3x4_to_f16x2x2(in.s[k], s01, unused);
+    const uint32_t s0 = __byte_perm(s01, 0, 0x1010), s1 = __byte_perm(s01, 0, 0x3232);
+    const uint32_t base = tile + (c >> 1) * (kRwTok * 128) + row * 128;
+    const uint32_t w[4] = {in.w[k].x, in.w[k].y, in.w[k].z, in.w[k].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t h[4];
+      e2m1x8_to_f16x2x4(w[j], h);
+      const uint32_t s = j < 2 ? s0 : s1;
+      sts128(base + (((4 * (c & 1) + j) ^ (row & 7)) << 4), hmul2_u32(h[0], s), hmul2_u32(h[1], s),
+             hmul2_u32(h[2], s), hmul2_u32(h[3], s));
+    }
+  }
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_constant__ BatchAttnParams p) {
+  using R = Rows<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sraw = smem_u32(smem);
+  const uint32_t sb = (sraw + 1023u) & ~1023u;
+  uint8_t* sg = smem + (sb - sraw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto bar = [&](int i) -> uint32_t { return sb + R::kBars + 8u * (uint32_t)i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sg + R::kMeta + 4);
+  float* rowfac = reinterpret_cast<float*>(sg + R::kRowfac);
+  long long* starts = reinterpret_cast<long long*>(sg + R::kStarts);
+  long long* sums = reinterpret_cast<long long*>(sg + R::kSums);
+
+  if (tid == 0) {
+    mbar_init(bar(kRwKReady), kRwDq);
+    mbar_init(bar(kRwKFree), 1);
+    mbar_init(bar(kRwVReady), kRwDq);
+    mbar_init(bar(kRwVFree), 1);
+    mbar_init(bar(kRwSFull0), 1);
+    mbar_init(bar(kRwSFull1), 1);
+    mbar_init(bar(kRwPReady0), kRwSoft);
+    mbar_init(bar(kRwPReady1), kRwSoft);
+    mbar_init(bar(kRwPvDone0), 1);
+    mbar_init(bar(kRwPvDone1), 1);
+    mbar_init(bar(kRwQReady), kRwSoft);
+    mbar_init(bar(kRwFin), 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kRwMma) {
+    tc::tmem_alloc(sb + R::kMeta, R::kTmCols);
+    tc::tmem_relinquish();
+  }
+  griddep_wait();
+
+  // ---------------------------------------------------- this CTA's share
+  const int per_pos = kRwRows / p.group;
+  const int per = (p.requests + kRwScan - 1) / kRwScan;
+  long long mine = 0, total;
+  if (tid < kRwScan)
+    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += RowsWalk::cost(p, b, per_pos);
+  const long long before = batch::block_scan(mine, sums, total);
+  if (tid < kRwScan) starts[tid] = before;
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tbase = *reinterpret_cast<volatile uint32_t*>(sg + R::kMeta);
+  const long long n_cta = gridDim.x;
+  const long long lo = (long long)blockIdx.x * total / n_cta, hi = ((long long)blockIdx.x + 1) * total / n_cta;
+  const int units = (int)(hi - lo);
+  int32_t* meta = p.meta + (kBatchMaxCtas + blockIdx.x) * kBatchMeta;
+  RowsWalk cur;
+  cur.per = per_pos;
+  if (units > 0) {
+    int at = 0;
+    for (int step = kRwScan / 2; step > 0; step >>= 1)
+      if (starts[at + step] <= lo) at += step;
+    cur.seek(p, at * per, lo - starts[at]);
+  }
+  if (tid == 0) meta[0] = 0;
+
+  if (units == 0) {
+    // nothing to do
+  } else if (warp == kRwMma) {
+    // ------------------------------------------------------------------ MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc_qk = tc::idesc_f16_f32(kRwRows, kRwTok);
+      constexpr uint32_t idesc_pv = tc::idesc_f16_f32(kRwRows, D, /*b_mn_major=*/true);
+      const uint64_t dq = tc::smem_desc_k128(sb + R::kQ);
+      const uint64_t dk = tc::smem_desc_k128(sb + R::kK);
+      const uint64_t dv = tc::smem_desc_mn128(sb + R::kV, kRwTok * 128, 1024);
+      int item = -1;
+      bool fresh = true;  // the next QK begins an item of this CTA
+      // first tile of its item in this CTA? (PV then overwrites O), for tiles j and j + 1
+      bool first_next = false, first_cur = false;
+      auto qk = [&](int j) -> bool {
+        if (fresh) {
+          ++item;
+          if (!mbar_wait(bar(kRwQReady), item & 1)) return false;
+        }
+        first_next = fresh;
+        fresh = cur.tile + 1 == cur.tiles;
+        cur.next(p);
+        if (!mbar_wait(bar(kRwKReady), j & 1)) return false;
+        // S(j) goes where P(j - 2) was read from
+        if (j >= 2 && !mbar_wait(bar(kRwPvDone0 + (j & 1)), ((j - 2) >> 1) & 1)) return false;
+        tc::fence_after();
+        const uint32_t d = tbase + R::kTmS + 128u * (j & 1);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+          tc::mma_ss(d, dq + (uint64_t)(((ks >> 2) * (kRwRows * 128) + (ks & 3) * 32) >> 4),
+                     dk + (uint64_t)(((ks >> 2) * (kRwTok * 128) + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
+        tc::commit(bar(kRwSFull0 + (j & 1)));
+        tc::commit(bar(kRwKFree));
+        return true;
+      };
+      auto pv = [&](int j) -> bool {
+        if (!mbar_wait(bar(kRwPReady0 + (j & 1)), (j >> 1) & 1) || !mbar_wait(bar(kRwVReady), j & 1)) return false;
+        tc::fence_after();
+#pragma unroll
+        for (int kk = 0; kk < kRwTok / 16; ++kk)
+          tc::mma_ts(tbase + R::kTmO, tbase + R::kTmS + 128u * (j & 1) + 8u * kk, dv + (uint64_t)((kk * 2048) >> 4),
+                     idesc_pv, (!first_cur || kk > 0) ? 1u : 0u);
+        tc::commit(bar(kRwPvDone0 + (j & 1)));
+        tc::commit(bar(kRwVFree));
+        return true;
+      };
+      bool fine = qk(0);
+      for (int j = 0; fine && j < units; ++j) {
+        if (*abort_flag) break;
+        first_cur = first_next;
+        // a new item's Q is staged after the last softmax of the old one
+        const bool ahead = j + 1 < units && !fresh;
+        if (ahead && !(fine = qk(j + 1))) break;
+        if (!(fine = pv(j))) break;
+        if (j + 1 < units && !ahead) fine = qk(j + 1);
+      }
+      if (!fine) {
+        flag_error(kErrTimeout);
+        *abort_flag = 1;
+      }
+      tc::commit(bar(kRwFin));  // never leave with MMAs in flight
+      if (!mbar_wait(bar(kRwFin), 0)) flag_error(kErrTimeout);
+    }
+  } else if (warp >= kRwSoft) {
+    // ------------------------------------------------------------- dequant
+    const int t = tid - kRwSoft * 32;
+    RwChunks<D> kc, vc;
+    int entry = cur.entry(p);
+    auto where = [&](size_t& token0, int& valid) {
+      const int at = cur.tile * kRwTok;
+      valid = cur.present(p, entry) ? min(kRwTok, cur.r.kv - at) : 0;
+      token0 = valid > 0 ? (size_t)entry * kPage + (at & (kPage - 1)) : 0;
+    };
+    size_t token0;
+    int valid;
+    where(token0, valid);
+    rw_load<D>(p, p.k_codes, p.k_scales, token0, cur.h, valid, t, kc);
+    rw_load<D>(p, p.v_codes, p.v_scales, token0, cur.h, valid, t, vc);
+    if (units > 1) {
+      cur.next(p);
+      entry = cur.entry(p);
+    }
+    bool ok = true;
+    for (int j = 0; j < units; ++j) {
+      const bool more = j + 1 < units;
+      if (j >= 1) ok &= mbar_wait(bar(kRwKFree), (j - 1) & 1);
+      if (__any_sync(kFull, !ok || *abort_flag)) break;
+      rw_store<D>(sb + R::kK, t, kc);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kRwKReady));
+      if (more) {
+        where(token0, valid);
+        rw_load<D>(p, p.k_codes, p.k_scales, token0, cur.h, valid, t, kc);
+      }
+      if (j >= 1) ok &= mbar_wait(bar(kRwVFree), (j - 1) & 1);
+      if (__any_sync(kFull, !ok)) break;
+      rw_store<D>(sb + R::kV, t, vc);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kRwVReady));
+      if (more) {
+        rw_load<D>(p, p.v_codes, p.v_scales, token0, cur.h, valid, t, vc);
+        if (j + 2 < units) {
+          cur.next(p);
+          entry = cur.entry(p);
+        }
+      }
+    }
+    if (__any_sync(kFull, !ok) && lane == 0) {
+      flag_error(kErrTimeout);
+      *abort_flag = 1;
+    }
+  } else {
+    // ------------------------------------------------- softmax (thread = row)
+    // tcgen05.ld / st / wait are warp-collective: every branch around them is
+    // decided by a warp vote.
+    const int r = tid;
+    const int rpos = r / p.group, rhead = r % p.group;
+    const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
+    // Q rows of the walker's item -> K-major FP16 operand, each row scaled by a
+    // power of two (exact for BF16 and FP16), eight rows' loads in flight.  A
+    // warp stages the rows that its own threads are
+    auto stage_q = [&](const RowsWalk& w) {
+      constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows a load
+      const int sub = lane / LPR, ln = lane % LPR;
+      const int pos0 = w.i * per_pos, npos = min(per_pos, w.r.n - pos0);
+      const T* q = reinterpret_cast<const T*>(p.q);
+#pragma unroll 1
+      for (int base = warp * 32; base < warp * 32 + 32; base += 8) {
+        uint4 v[8 / RPI];
+#pragma unroll
+        for (int u = 0; u < 8 / RPI; ++u) {
+          const int row = base + u * RPI + sub;
+          const int pos = row / p.group;
+          v[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (pos < npos)
+            v[u] = __ldg(reinterpret_cast<const uint4*>(q + (long long)(w.r.row0 + pos0 + pos) * p.q_stride +
+                                                        (w.h * p.group + row % p.group) * D) + ln);
+        }
+#pragma unroll
+        for (int u = 0; u < 8 / RPI; ++u) {
+          const int row = base + u * RPI + sub;
+          const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          float amax = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = InTraits<T>::to_float2(x[e]);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, shfl_xor(amax, o));
+          const float sc = pow2_row_scale(amax);
+          uint32_t hh[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = InTraits<T>::to_float2(x[e]);
+            hh[e] = pack_half2(f.x * sc, f.y * sc);
+          }
+          sts128(sb + R::kQ + (ln >> 3) * (kRwRows * 128) + row * 128 + (((ln & 7) ^ (row & 7)) << 4), hh[0], hh[1],
+                 hh[2], hh[3]);
+          if (ln == 0) rowfac[row] = p.sm_scale_log2 / sc;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kRwQReady));
+    };
+
+    stage_q(cur);
+    int entry = cur.entry(p);
+    int j = 0;
+    bool ok = true;
+    while (j < units) {
+      // ------------------------------------------------------------ an item
+      const RowsWalk it = cur;
+      const int n_tiles = min(it.tiles - it.tile, units - j);
+      const int pos0 = it.i * per_pos, npos = min(per_pos, it.r.n - pos0);
+      const bool valid = rpos < npos;
+      // keys below lim are visible; rows that do not exist are all zeros in Q
+      const int lim = valid ? it.r.kv - it.r.n + pos0 + rpos + 1 : 0x7fffffff;
+      const float fac = rowfac[r];
+      float m_ref = -CUDART_INF_F, la = 0.f, lb = 0.f;
+      int done = 0;
+      for (int k = 0; k < n_tiles; ++k, ++j) {
+        const int t0 = cur.tile * kRwTok;
+        const bool here = cur.present(p, entry);
+        if (j + 1 < units) {
+          cur.next(p);
+          entry = cur.entry(p);
+        }
+        ok &= mbar_wait(bar(kRwSFull0 + (j & 1)), (j >> 1) & 1);
+        if (__any_sync(kFull, !ok || *abort_flag)) break;
+        tc::fence_after();
+        const uint32_t ts = tbase + lane_base + R::kTmS + 128u * (j & 1);
+        const int room = here ? lim - t0 : 0;  // columns below it count
+        const bool masked = !__all_sync(kFull, room >= kRwTok);
+        float mr = -CUDART_INF_F;
+#pragma unroll
+        for (int c = 0; c < kRwTok; c += 32) {
+          float x[32];
+          rw_ld32(ts + c, x);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = c + e < room ? x[e] : -CUDART_INF_F;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) mr = pf_fmax3(mr, x[e], x[e + 1]);
+        }
+        const float mt = mr * fac;
+        const bool need = mt > m_ref + kLazy;
+        const float m_new = need ? mt : m_ref;
+        const float alpha = (need && m_ref != -CUDART_INF_F) ? exp2_approx(m_ref - m_new) : 1.f;
+        const float mu = m_new == -CUDART_INF_F ? 0.f : m_new;
+        la *= alpha;
+        lb *= alpha;
+        m_ref = m_new;
+#pragma unroll
+        for (int c = 0; c < kRwTok; c += 32) {
+          float x[32];
+          rw_ld32(ts + c, x);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = c + e < room ? x[e] : -CUDART_INF_F;
+          }
+          uint32_t pw[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float p0, p1;
+            pf_ffma2(p0, p1, x[2 * e], x[2 * e + 1], fac, -mu);
+            p0 = exp2_approx(p0);
+            p1 = exp2_approx(p1);
+            pf_fadd2(la, lb, p0, p1);
+            pw[e] = pack_half2(p0, p1);
+          }
+          tc::st_32x32b_x16(ts + c / 2, pw);  // over S columns that have been read
+        }
+        if (k > 0 && __any_sync(kFull, alpha != 1.f)) {
+          ok &= mbar_wait(bar(kRwPvDone0 + ((j - 1) & 1)), ((j - 1) >> 1) & 1);
+          if (__any_sync(kFull, !ok)) break;
+          tc::fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tc::ld_32x32b_x16(tbase + lane_base + R::kTmO + c, o);
+            tc::wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tc::st_32x32b_x16(tbase + lane_base + R::kTmO + c, o);
+          }
+        }
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kRwPReady0 + (j & 1)));
+        done = k + 1;
+      }
+      if (__any_sync(kFull, done < n_tiles)) break;
+      // the next item's Q while the last PV runs (the last QK has read this one)
+      if (j < units) stage_q(cur);
+      // ---------------------------------------------------------- epilogue
+      ok &= mbar_wait(bar(kRwPvDone0 + ((j - 1) & 1)), ((j - 1) >> 1) & 1);
+      if (__any_sync(kFull, !ok)) break;
+      tc::fence_after();
+      const bool starts_here = it.tile == 0, ends_here = it.tile + n_tiles == it.tiles;
+      const float l = la + lb;
+      if (starts_here && ends_here) {
+        T* out = reinterpret_cast<T*>(p.out) + (long long)(it.r.row0 + pos0 + (valid ? rpos : 0)) * p.out_stride +
+                 (it.h * p.group + rhead) * D;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float x[32];
+          rw_ld32(tbase + lane_base + R::kTmO + c, x);
+          if (!valid) continue;
+          uint4* dst = reinterpret_cast<uint4*>(out + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const T a = InTraits<T>::from_float(x[e + 2 * i] * inv), b = InTraits<T>::from_float(x[e + 2 * i + 1] * inv);
+              w[i] = (uint32_t)(*reinterpret_cast<const uint16_t*>(&a)) |
+                     ((uint32_t)(*reinterpret_cast<const uint16_t*>(&b)) << 16);
+            }
+            dst[e / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      } else {
+        // record [D / 4][128 rows] of float4, then (m, l) a row
+        float* rec = p.row_records + (size_t)(blockIdx.x * 2 + (starts_here ? 1 : 0)) * R::kRec;
+        float4* ro = reinterpret_cast<float4*>(rec) + r;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float x[32];
+          rw_ld32(tbase + lane_base + R::kTmO + c, x);
+          if (!valid) continue;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            ro[(size_t)((c + e) / 4) * kRwRows] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+        if (valid) *reinterpret_cast<float2*>(rec + kRwRows * D + 2 * r) = make_float2(m_ref, l);
+        if (starts_here && tid == 0) {
+          const long long last_unit = lo + (j - n_tiles) + it.tiles - 1;
+          meta[0] = npos * p.group;
+          meta[1] = it.r.row0 + pos0;
+          meta[3] = it.h;
+          meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
+          meta[5] = (int)min(total, n_cta);
+        }
+      }
+      tc::fence_before();
+    }
+    if (__any_sync(kFull, !ok) && lane == 0) {
+      flag_error(kErrTimeout);
+      *abort_flag = 1;
+    }
+  }
+
+  griddep_launch_dependents();
+  tc::fence_before();
+  __syncthreads();
+  if (warp == kRwMma) {
+    tc::fence_after();
+    tc::tmem_dealloc(tbase, R::kTmCols);
+  }
+}
+
+// Merges the records of items that more than one CTA worked on, in CTA order:
+// block (i, y) takes rows 8y .. 8y + 7 of the item that CTA i began.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_constant__ BatchAttnParams p) {
+  using R = Rows<D>;
+  __shared__ float w[8][kBatchMaxCtas];
+  __shared__ float inv_l[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tid = threadIdx.x, i0 = blockIdx.x, n_cta = gridDim.x, y0 = blockIdx.y * 8;
+  const int32_t* meta = p.meta + (kBatchMaxCtas + i0) * kBatchMeta;
+  const int rows = __ldcg(meta);
+  if (y0 >= rows) return;
+  const int base = __ldcg(meta + 1), hd = __ldcg(meta + 3), parts = __ldcg(meta + 4) - i0 + 1, busy = __ldcg(meta + 5);
+  auto record = [&](int j) { return p.row_records + (size_t)((i0 + j) * 2 + (j == 0 ? 1 : 0)) * R::kRec; };
+  auto empty = [&](int j) {
+    const long long i = i0 + j;
+    return i * busy / n_cta == (i + 1) * busy / n_cta;
+  };
+  {  // one warp a row: weights of the parts
+    const int row = y0 + (tid >> 5), lane = tid & 31;
+    float M = -CUDART_INF_F;
+    for (int j = lane; j < parts; j += 32)
+      if (row < rows && !empty(j)) M = fmaxf(M, __ldcg(record(j) + kRwRows * D + 2 * row));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, shfl_xor(M, o));
+    float L = 0.f;
+    for (int j = lane; j < parts; j += 32) {
+      float wt = 0.f;
+      if (row < rows && !empty(j)) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(record(j) + kRwRows * D + 2 * row));
+        wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
+        L += wt * v.y;
+      }
+      w[tid >> 5][j] = wt;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += shfl_xor(L, o);
+    if (lane == 0) inv_l[tid >> 5] = L > 0.f ? 1.f / L : 0.f;
+  }
+  __syncthreads();
+  const int row = y0 + (tid & 7);
+  if (row >= rows) return;
+  T* out = reinterpret_cast<T*>(p.out) + (long long)(base + row / p.group) * p.out_stride + (hd * p.group + row % p.group) * D;
+  for (int d4 = tid >> 3; d4 < D / 4; d4 += 32) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = 0; j < parts; ++j) {
+      const float wj = w[tid & 7][j];
+      if (wj == 0.f) continue;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(record(j)) + (size_t)d4 * kRwRows + row);
+      a.x += wj * v.x;
+      a.y += wj * v.y;
+      a.z += wj * v.z;
+      a.w += wj * v.w;
+    }
+    const float s = inv_l[tid & 7];
+    T* dst = out + d4 * 4;
+    dst[0] = InTraits<T>::from_float(a.x * s);
+    dst[1] = InTraits<T>::from_float(a.y * s);
+    dst[2] = InTraits<T>::from_float(a.z * s);
+    dst[3] = InTraits<T>::from_float(a.w * s);
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_rows(const BatchAttnParams& p, int ctas, cudaStream_t stream) {
+  auto kernel = batch_rows_kernel<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kernel, dim3(ctas), dim3(kRwThreads), Rows<D>::kSmem, stream, p);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(batch_rows_combine_kernel<T, D>, dim3(ctas, kRwRows / 8), dim3(256), 0, stream, p);
+}
+
+}  // namespace qwz

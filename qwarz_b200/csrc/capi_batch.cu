@@ -137,6 +137,8 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   p.kv_lens = kv_lens;
   p.meta = static_cast<int32_t*>(workspace);
   p.records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + qwz::kBatchMetaBytes);
+  p.row_records = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + qwz::kBatchMetaBytes +
+                                          qwz::batch_few_record_bytes(head_dim));
   p.q_stride = q_stride;
   p.out_stride = out_stride;
   p.requests = requests;
@@ -146,6 +148,7 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
   p.max_rows = max_rows;
+  p.few_cols = 2048 / head_dim;
   p.sm_scale_log2 = sm_scale * kLog2e;
   return launched(qwz::launch_batch_attend(p, head_dim, dtype, ctas, as_stream(stream)), "qwz_batch_attend");
 }
