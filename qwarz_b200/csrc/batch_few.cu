@@ -7,21 +7,20 @@
 // Bound by HBM: a token costs D/2 + D/16 bytes of K and as many of V a head,
 // and 4 D multiply-adds a query column, far below the tensor rate.
 //
-// The (row, head of the group) pairs of one request and KV head are the
-// columns of an item: kCols of them (2048 / D, so that O^T [D x kCols] is 64
-// registers a thread at every head size).  CTA = 8 warps, one CTA per SM, and
-// a share of all items' 256-token pages (batch_common.cuh).  A warp owns 32
-// tokens of each page and streams them through a ring of its own with
-// cp.async (16-byte copies straight from the pool's rows, so any head layout,
-// page order and ragged end needs no descriptor); no warp waits for another
-// inside an item, and the ring runs on across items, so a CTA's loads never
-// drain.  A warp's 32 tokens are two 16-token MMA tiles, tokens on M and
-// columns on N: K codes become A fragments of S^T in registers, V codes A
-// fragments of O^T, P^T comes from the S^T fragment by movmatrix.  Base-2
-// online softmax, the reference maximum moves only by more than 2^8; P is
-// rounded to FP16 for its product (11 significant bits, the output's own), all
-// sums are FP32.  At an item's end the eight warps' (m, l, O) are merged in
-// shared memory in warp order.
+// The (row, head of the group) pairs of one request and KV head are the (at
+// most 8) columns of an item; its 256-token pages are shared out over the CTAs
+// together with those of all other items (batch_common.cuh).  A warp owns 32 or
+// 64 tokens of each page and streams them through a ring of its own: the codes
+// by TMA (one box of its rows of K and one of V, 128-byte swizzle, on the warp's
+// own mbarrier), the scales, whose rows can be narrower than a TMA box, by
+// cp.async.  No warp waits for another inside an item, and the ring runs on
+// across items, so a CTA's loads never drain.  Tokens are on the M side of
+// mma.sync.m16n8k16 and columns on N: K codes become A fragments of S^T in
+// registers, V codes A fragments of O^T, P^T comes from the S^T fragment by
+// movmatrix.  Base-2 online softmax, the reference maximum moves only by more
+// than 2^8; P is rounded to FP16 for its product (11 significant bits, as the
+// output has), all sums are FP32.  At an item's end the warps' (m, l, O) are
+// merged in shared memory in warp order.
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 
@@ -31,37 +30,36 @@ using namespace detail;
 
 namespace {
 
-constexpr int kFewWarps = 8;
-constexpr int kFewThreads = kFewWarps * 32;
-constexpr int kFewTok = 32;  // tokens of a page a warp owns
+constexpr int kFewCols = kBatchFewCols;  // query columns of an item
+constexpr int kFewScan = 128; // threads that scan the requests
 
 template <int D>
 struct Few {
-  static constexpr int kCols = 2048 / D;             // query columns of an item
-  static constexpr int kNT = kCols / 8;              // MMA column tiles
+  static constexpr int kWarps = D == 256 ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kTok = kPage / kWarps;        // tokens of a page a warp owns
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kCtas = D == 256 ? 1 : D == 128 ? 3 : 4;  // per SM
   static constexpr int kMT = D / 16;                 // MMA row tiles of O^T
   static constexpr int kRow = D / 2;                 // code bytes of a row
   static constexpr int kSRow = D / 16;               // scale bytes of a row
-  static constexpr int kCodes = kFewTok * kRow;
-  static constexpr int kStage = 2 * (kCodes + kFewTok * kSRow);
-  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 4 : 6;
-  static constexpr int kMergeWarp = 16 * kEpiRowF4 * 16 + kCols * 8;  // O and (m, l) of a warp
-  // D 256: the merge uses the slot that the item's last page left
-  static constexpr bool kMergeInRing = kMergeWarp <= kStage;
-  static constexpr int kRing = kFewWarps * kStages * kStage;
-  static constexpr int kMerge = kMergeInRing ? 0 : kFewWarps * kMergeWarp;
-  static constexpr int kSmem = kRing + kMerge;
+  static constexpr int kCodes = kTok * kRow;
+  static constexpr int kScales = kTok * kSRow;
+  // per CTA: code slots [warp][stage] {K, V}, scale slots, barriers
+  static constexpr int kRing = kWarps * kStages * 2 * kCodes;
+  static constexpr int kScaleRing = kWarps * kStages * 2 * kScales;
+  static constexpr int kSmem = kRing + kScaleRing + 8 * kWarps * kStages + 1024;
+  // for the merge a warp's O takes the code slot its last page left, (m, l) the scale slot
+  static_assert(kMT * 512 <= 2 * kCodes && kFewCols * 8 <= 2 * kScales, "merge area");
+  static_assert(kMT % kWarps == 0 && kTok % 32 == 0, "merge share, tile pairs");
 };
 
-// Byte offset of 16-byte chunk c of code row r: 128-byte lines of 128 / kRow
-// rows, chunks XOR-swizzled by the line so that the K reads (8 rows x 4 lanes)
-// and the V reads (rows 0, 2, 4, 6 x 8 lanes) both touch every bank once.
+// Byte offset of 16-byte chunk c of code row r as the TMA box lays it out: rows
+// of 128, 64 or 32 bytes with the swizzle of that width.
 template <int D>
 QWZ_DEVINL uint32_t few_swz(int r, int c) {
-  constexpr int rpl = 128 / Few<D>::kRow, cpr = Few<D>::kRow / 16;
-  const int line = r / rpl, ch = (r % rpl) * cpr + c;
-  const int x = D == 256 ? (line & 7) : D == 128 ? (line & 3) * 2 : (line & 1) * 2;
-  return (uint32_t)(line * 128 + ((ch ^ x) << 4));
+  const uint32_t at = (uint32_t)(r * Few<D>::kRow + c * 16);
+  return at ^ ((at >> 3) & (D == 256 ? 0x70u : D == 128 ? 0x30u : 0x10u));
 }
 
 QWZ_DEVINL uint2 few_lds64(uint32_t addr) {
@@ -92,11 +90,14 @@ QWZ_DEVINL void cp_async_small(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES));
 }
 
-// Walks the units (request, item, page) of the launch in order.
-template <int D>
+// Walks the pages (request, head, page) of the launch in order.  An item
+// weighs its pages and kOver more for what it costs beside them (its Q, the
+// merge and the store), so that CTAs with many short items get fewer pages.
 struct FewWalk {
-  int b, head, page;       // request, KV head, page
+  static constexpr int kOver = 1;
+  int b, head, page;       // request (p.requests: past the end), KV head, page
   int pages;               // of request b
+  long long base;          // weighed units before the item
   batch::Req r;
 
   static QWZ_DEVINL bool few(const BatchAttnParams& p, const batch::Req& r) {
@@ -106,39 +107,49 @@ struct FewWalk {
   static QWZ_DEVINL int pages_of(const batch::Req& r) { return max(1, (r.kv + kPage - 1) / kPage); }
   static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b) {
     const batch::Req r = batch::load_req(p, b);
-    return few(p, r) ? (long long)p.kv_heads * pages_of(r) : 0;
+    return few(p, r) ? (long long)p.kv_heads * (pages_of(r) + kOver) : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
     r = batch::load_req(p, b);
     pages = pages_of(r);
   }
-  // Unit `u` counted from the start of request b0.
-  QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long u) {
+  // Weighed unit u, `before` of which precede request b0.
+  QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long before, long long u) {
+    base = before;
+    u -= before;
     for (b = b0; b < p.requests; ++b) {
       const long long c = cost(p, b);
       if (u < c) break;
       u -= c;
+      base += c;
     }
-    enter(p, min(b, p.requests - 1));
-    head = (int)(u / pages);
-    page = (int)(u % pages);
+    head = page = 0;
+    if (b == p.requests) return;
+    enter(p, b);
+    const int w = pages + kOver;
+    head = (int)(u / w);
+    base += (long long)head * w;
+    page = max((int)(u % w) - kOver, 0);
   }
   QWZ_DEVINL void next(const BatchAttnParams& p) {
     if (++page < pages) return;
     page = 0;
+    base += pages + kOver;
     if (++head < p.kv_heads) return;
     head = 0;
     for (int bb = b + 1; bb < p.requests; ++bb) {
       enter(p, bb);
       if (few(p, r)) return;
     }
+    b = p.requests;
   }
-  // Table entry of the unit, unchecked (the load is in flight until it is used).
+  QWZ_DEVINL bool at(const FewWalk& o) const { return b == o.b && head == o.head && page == o.page; }
+  // Table entry of the page, unchecked (the load is in flight until it is used).
   QWZ_DEVINL int entry(const BatchAttnParams& p) const {
     return __ldg(p.block_table + (size_t)b * p.table_width + page);
   }
-  // Whether the unit has tokens in a page of the pool.
+  // Whether the page has tokens and lies in the pool.
   QWZ_DEVINL bool present(const BatchAttnParams& p, int pp) const {
     if (r.kv <= 0) return false;
     if (pp >= 0 && pp < p.num_pages) return true;
@@ -176,384 +187,418 @@ QWZ_DEVINL void few_v_load(uint32_t codes, uint32_t scales, int ra, int g, bool 
   e4m3x4_to_f16x2x2(__byte_perm(s[2], s[3], 0x5140), v.scd[0], v.scd[1]);
 }
 
+// O^T += V^T P^T of one 16-token tile.
+template <int D>
+QWZ_DEVINL void few_pv(const FewV<D>& v, const PFrag& pf, float (&o)[D / 16][4]) {
+#pragma unroll
+  for (int w = 0; w < FewV<D>::W; ++w) {
+    const uint32_t xab = (v.a[w] & 0x0F0F0F0Fu) | ((v.b[w] << 4) & 0xF0F0F0F0u);
+    const uint32_t yab = ((v.a[w] >> 4) & 0x0F0F0F0Fu) | (v.b[w] & 0xF0F0F0F0u);
+    const uint32_t xcd = (v.c[w] & 0x0F0F0F0Fu) | ((v.d[w] << 4) & 0xF0F0F0F0u);
+    const uint32_t ycd = ((v.c[w] >> 4) & 0x0F0F0F0Fu) | (v.d[w] & 0xF0F0F0F0u);
+    uint32_t hxab[4], hyab[4], hxcd[4], hycd[4];
+    e2m1x8_to_f16x2x4(xab, hxab);
+    e2m1x8_to_f16x2x4(yab, hyab);
+    e2m1x8_to_f16x2x4(xcd, hxcd);
+    e2m1x8_to_f16x2x4(ycd, hycd);
+    const uint32_t sab = v.sab[D == 256 ? w >> 1 : 0], scd = v.scd[D == 256 ? w >> 1 : 0];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      mma_16816(o[4 * w + kk], hmul2_u32(hxab[kk], sab), hmul2_u32(hyab[kk], sab), hmul2_u32(hxcd[kk], scd),
+                hmul2_u32(hycd[kk], scd), pf.hi0, pf.hi1);
+  }
+}
+
+// Raw S^T of the 16-token tile at row r0 - g of the slot.
+template <int D>
+QWZ_DEVINL void few_qk(uint32_t codes, uint32_t scales, int r0, int qd, const uint32_t (&qf)[D / 8], float (&s)[4]) {
+  constexpr int KW = D / 32;  // code words of a lane: 8, 4, 2
+  const int r1 = r0 + 8;
+  uint32_t kw0[KW], kw1[KW], sc0[4], sc1[4];
+  if constexpr (D == 256) {
+    uint32_t a[4], b[4], c[4], d[4];
+    lds_words(codes + few_swz<D>(r0, 2 * qd), a);
+    lds_words(codes + few_swz<D>(r0, 2 * qd + 1), b);
+    lds_words(codes + few_swz<D>(r1, 2 * qd), c);
+    lds_words(codes + few_swz<D>(r1, 2 * qd + 1), d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kw0[i] = a[i];
+      kw0[4 + i] = b[i];
+      kw1[i] = c[i];
+      kw1[4 + i] = d[i];
+    }
+    scales_bcast4(lds32(scales + r0 * 16 + 4 * qd), sc0);
+    scales_bcast4(lds32(scales + r1 * 16 + 4 * qd), sc1);
+  } else if constexpr (D == 128) {
+    lds_words(codes + few_swz<D>(r0, qd), kw0);
+    lds_words(codes + few_swz<D>(r1, qd), kw1);
+    scales_bcast4(lds16(scales + r0 * 8 + 2 * qd), sc0);
+    scales_bcast4(lds16(scales + r1 * 8 + 2 * qd), sc1);
+  } else {
+    lds_words(codes + few_swz<D>(r0, qd >> 1) + (qd & 1) * 8, kw0);
+    lds_words(codes + few_swz<D>(r1, qd >> 1) + (qd & 1) * 8, kw1);
+    scales_bcast4(lds8(scales + r0 * 4 + qd), sc0);
+    scales_bcast4(lds8(scales + r1 * 4 + qd), sc1);
+  }
+  float sa[4] = {0.f, 0.f, 0.f, 0.f}, sb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w8 = 0; w8 < KW; ++w8) {
+    uint32_t h0[4], h1[4];
+    e2m1x8_to_f16x2x4(kw0[w8], h0);
+    e2m1x8_to_f16x2x4(kw1[w8], h1);
+    const uint32_t s0 = sc0[w8 >> 1], s1 = sc1[w8 >> 1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      h0[j] = hmul2_u32(h0[j], s0);
+      h1[j] = hmul2_u32(h1[j], s1);
+    }
+    mma_16816(sa, h0[0], h1[0], h0[1], h1[1], qf[4 * w8 + 0], qf[4 * w8 + 1]);
+    mma_16816(sb, h0[2], h1[2], h0[3], h1[3], qf[4 * w8 + 2], qf[4 * w8 + 3]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = sa[i] + sb[i];
+}
+
 }  // namespace
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_constant__ BatchAttnParams p) {
+__global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
+    batch_few_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ BatchPoolMaps maps) {
   using F = Few<D>;
-  constexpr int NT = F::kNT, MT = F::kMT, QW = D / 8;
+  constexpr int MT = F::kMT, QW = D / 8, TILES = F::kTok / 16;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ long long starts[kFewThreads + 1];  // units before each thread's requests
-  __shared__ long long warp_sums[kFewWarps];
-  __shared__ float weights[F::kCols * kFewWarps];
-  __shared__ float col_l[F::kCols];
+  __shared__ long long starts[kFewScan];  // weighed units before each scanning thread's requests
+  __shared__ long long warp_sums[F::kWarps];
+  const uint32_t sraw = smem_u32(smem);
+  const uint32_t sbase = (sraw + 1023u) & ~1023u;
+  uint8_t* sgen = smem + (sbase - sraw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, qd = lane & 3;
-  const uint32_t ring = smem_u32(smem) + warp * F::kStages * F::kStage;
-
+  const uint32_t codes = sbase + warp * F::kStages * 2 * F::kCodes;
+  const uint32_t scales = sbase + F::kRing + warp * F::kStages * 2 * F::kScales;
+  const uint32_t bars = sbase + F::kRing + F::kScaleRing + warp * F::kStages * 8;
+  if (lane == 0) {
+#pragma unroll
+    for (int s = 0; s < F::kStages; ++s) mbar_init(bars + 8 * s, 1);
+    mbar_fence_init();
+    if (warp == 0) {
+      tma_prefetch_desc(&maps.k);
+      tma_prefetch_desc(&maps.v);
+    }
+  }
   griddep_wait();
 
   // ---------------------------------------------------- this CTA's share
-  const int per = (p.requests + kFewThreads - 1) / kFewThreads;
+  const int per = (p.requests + kFewScan - 1) / kFewScan;
   long long mine = 0;
-  for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += FewWalk<D>::cost(p, b);
+  if (tid < kFewScan)
+    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += FewWalk::cost(p, b);
   long long total;
-  starts[tid] = batch::block_scan(mine, warp_sums, total);
+  const long long before = batch::block_scan(mine, warp_sums, total);
+  if (tid < kFewScan) starts[tid] = before;
   __syncthreads();
   const long long n_cta = gridDim.x;
-  const long long lo = (long long)blockIdx.x * total / n_cta, hi = ((long long)blockIdx.x + 1) * total / n_cta;
-  const int units = (int)(hi - lo);
+  auto seek = [&](long long u) {
+    int at = 0;
+    for (int step = kFewScan / 2; step > 0; step >>= 1)
+      if (starts[at + step] <= u) at += step;
+    FewWalk w;
+    w.seek(p, min(at * per, p.requests), starts[at], u);
+    return w;
+  };
+  FewWalk cur = seek((long long)blockIdx.x * total / n_cta);
+  const FewWalk end = seek(((long long)blockIdx.x + 1) * total / n_cta);
   int32_t* meta = p.meta + blockIdx.x * kBatchMeta;
-  if (units == 0) {
-    if (tid == 0) meta[0] = 0;
+  if (tid == 0) meta[0] = 0;
+  if (cur.at(end)) {
     griddep_launch_dependents();
     return;
   }
-  int at = 0;
-  for (int step = kFewThreads / 2; step > 0; step >>= 1)
-    if (starts[at + step] <= lo) at += step;
-  FewWalk<D> cur;
-  cur.seek(p, at * per, lo - starts[at]);
-  FewWalk<D> pre = cur;
+  FewWalk pre = cur;
   int pre_page = pre.entry(p);
+  bool pre_more = true;
+  unsigned filled = 0;  // bit s: ring slot s holds (or will hold) a page of the pool
 
-  // Copies this warp's 32 tokens of the walker's unit into ring slot `slot`.
-  auto issue = [&](int slot) {
-    const int t0 = pre.page * kPage + warp * kFewTok;
-    const int valid = pre.present(p, pre_page) ? min(kFewTok, pre.r.kv - t0) : 0;
-    if (valid > 0) {
-      const size_t row0 = (size_t)pre_page * kPage + warp * kFewTok;
-      const size_t hd = pre.head;
-      const uint32_t dst = ring + slot * F::kStage;
-      constexpr int CPR = F::kRow / 16;
+  // Copies this warp's tokens of the next page into ring slot `slot`.
+  auto advance = [&](int slot) {
+    if (pre_more) {
+      const bool in_pool = pre.present(p, pre_page);
+      filled = in_pool ? filled | (1u << slot) : filled & ~(1u << slot);
+      if (in_pool && pre.page * kPage + warp * F::kTok < pre.r.kv) {
+        const int row0 = pre_page * kPage + warp * F::kTok;
+        if (lane == 0) {
+          const uint32_t bar = bars + 8 * slot, dst = codes + slot * 2 * F::kCodes;
+          fence_proxy_async_smem();  // the slot's last reads and merge writes before the copies
+          mbar_arrive_expect_tx(bar, 2 * F::kCodes);
+          tma_load_2d(dst, &maps.k, pre.head * F::kRow, row0, bar);
+          tma_load_2d(dst + F::kCodes, &maps.v, pre.head * F::kRow, row0, bar);
+        }
+        const size_t src = ((size_t)row0 * p.kv_heads + pre.head) * F::kSRow;
+        const size_t step = (size_t)p.kv_heads * F::kSRow;
+        const uint32_t dst = scales + slot * 2 * F::kScales;
 #pragma unroll
-      for (int i = 0; i < CPR; ++i) {
-        const int idx = i * 32 + lane, row = idx / CPR, c = idx % CPR;
-        if (row < valid) {
-          const size_t src = ((row0 + row) * p.kv_heads + hd) * F::kRow + c * 16;
-          const uint32_t off = few_swz<D>(row, c);
-          cp_async_small<16>(dst + off, p.k_codes + src);
-          cp_async_small<16>(dst + F::kCodes + off, p.v_codes + src);
+        for (int r = lane; r < F::kTok; r += 32) {
+          cp_async_small<F::kSRow>(dst + r * F::kSRow, p.k_scales + src + r * step);
+          cp_async_small<F::kSRow>(dst + F::kScales + r * F::kSRow, p.v_scales + src + r * step);
         }
       }
-      if (lane < valid) {
-        const size_t src = ((row0 + lane) * p.kv_heads + hd) * F::kSRow;
-        const uint32_t off = dst + 2 * F::kCodes + lane * F::kSRow;
-        cp_async_small<F::kSRow>(off, p.k_scales + src);
-        cp_async_small<F::kSRow>(off + kFewTok * F::kSRow, p.v_scales + src);
-      }
-    }
-  };
-
-  int issued = 0;
-  auto advance = [&](int slot) {  // one group a unit, empty past the share's end
-    if (issued < units) {
-      issue(slot);
-      if (++issued < units) {
-        pre.next(p);
+      pre.next(p);
+      pre_more = !pre.at(end);
+      if (pre_more) {
         pre_page = pre.entry(p);
+        if (pre.page == 0 && warp == 0) {  // the item's Q on its way into L1
+          constexpr int kLines = D * 2 / 128;
+          const int c = lane / kLines;
+          if (c < pre.r.n * p.group && c < kFewCols)
+            asm volatile("prefetch.global.L1 [%0];\n" ::"l"(
+                reinterpret_cast<const T*>(p.q) + (pre.r.row0 + c / p.group) * p.q_stride +
+                (pre.head * p.group + c % p.group) * D + (lane % kLines) * 64));
+        }
       }
     }
-    cp_async_commit();
+    cp_async_commit();  // one group a page, empty past the share's end
   };
 #pragma unroll
   for (int s = 0; s < F::kStages - 1; ++s) advance(s);
 
-  float o[NT][MT][4];
-  float m[NT][2], l[NT][2], cf[NT][2];
-  int lim[NT][2];
-  uint32_t qf[NT][QW];
-  int first_page = 0, min_lim = 0, max_lim = 0, cols = 0;
-  bool fresh = true;
-  if (tid == 0) meta[0] = 0;
+  float o[MT][4];
+  float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f, cf0 = 0.f, cf1 = 0.f;
+  int lim0 = 0, lim1 = 0, min_lim = 0, max_lim = 0, cols = 0, first_page = 0;
+  uint32_t qf[QW];
+  bool fresh = true, ok = true;
   int slot = 0, fill = F::kStages - 1;
+  unsigned phases = 0;  // parity of each slot's barrier
 
-  for (int k = 0; k < units; ++k) {
+  while (true) {
     if (fresh) {  // ------------------------------------------- a new item
       fresh = false;
       first_page = cur.page;
-      const int hd = cur.head;
       cols = cur.r.n * p.group;
+      float amax = 0.f;
+      if (g < cols) {
+        const uint4* src = reinterpret_cast<const uint4*>(
+            reinterpret_cast<const T*>(p.q) + (cur.r.row0 + g / p.group) * p.q_stride +
+            (cur.head * p.group + g % p.group) * D + qd * (D / 4));
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int c = nt * 8 + g;
-        float amax = 0.f;
-        if (c < cols) {
-          const int s = c / p.group, h = hd * p.group + c % p.group;
-          const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) +
-                                                            (cur.r.row0 + s) * p.q_stride + h * D + qd * (D / 4));
-#pragma unroll
-          for (int i = 0; i < QW / 4; ++i) {
-            const uint4 v = __ldg(src + i);
-            qf[nt][4 * i + 0] = v.x;
-            qf[nt][4 * i + 1] = v.y;
-            qf[nt][4 * i + 2] = v.z;
-            qf[nt][4 * i + 3] = v.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < QW; ++i) qf[nt][i] = 0u;
+        for (int i = 0; i < QW / 4; ++i) {
+          const uint4 v = __ldg(src + i);
+          qf[4 * i + 0] = v.x;
+          qf[4 * i + 1] = v.y;
+          qf[4 * i + 2] = v.z;
+          qf[4 * i + 3] = v.w;
         }
+      } else {
 #pragma unroll
-        for (int i = 0; i < QW; ++i) {
-          const float2 f = InTraits<T>::to_float2(qf[nt][i]);
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-        amax = fmaxf(amax, shfl_xor(amax, 1));
-        amax = fmaxf(amax, shfl_xor(amax, 2));
-        const float sc = pow2_row_scale(amax);
-#pragma unroll
-        for (int i = 0; i < QW; ++i) {
-          const float2 f = InTraits<T>::to_float2(qf[nt][i]);
-          qf[nt][i] = pack_half2(f.x * sc, f.y * sc);
-        }
-        const float rowfac = p.sm_scale_log2 / sc;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          cf[nt][i] = __shfl_sync(kFull, rowfac, 4 * (2 * qd + i));
-          const int cc = nt * 8 + 2 * qd + i;
-          lim[nt][i] = cc < cols ? cur.r.kv - cur.r.n + cc / p.group + 1 : 0;
-          m[nt][i] = -CUDART_INF_F;
-          l[nt][i] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+        for (int i = 0; i < QW; ++i) qf[i] = 0u;
       }
+#pragma unroll
+      for (int i = 0; i < QW; ++i) {
+        const float2 f = InTraits<T>::to_float2(qf[i]);
+        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+      amax = fmaxf(amax, shfl_xor(amax, 1));
+      amax = fmaxf(amax, shfl_xor(amax, 2));
+      const float sc = pow2_row_scale(amax);
+#pragma unroll
+      for (int i = 0; i < QW; ++i) {
+        const float2 f = InTraits<T>::to_float2(qf[i]);
+        qf[i] = pack_half2(f.x * sc, f.y * sc);
+      }
+      const float rowfac = p.sm_scale_log2 / sc;
+      cf0 = __shfl_sync(kFull, rowfac, 8 * qd);
+      cf1 = __shfl_sync(kFull, rowfac, 8 * qd + 4);
       min_lim = cur.r.kv - cur.r.n + 1;
-      max_lim = cur.r.kv - cur.r.n + (cols - 1) / p.group + 1;
+      max_lim = cur.r.kv;
+      lim0 = 2 * qd < cols ? min_lim + 2 * qd / p.group : 0;
+      lim1 = 2 * qd + 1 < cols ? min_lim + (2 * qd + 1) / p.group : 0;
+      m0 = m1 = -CUDART_INF_F;
+      l0 = l1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     }
 
     cp_async_wait<F::kStages - 2>();
+    const int tw = cur.page * kPage + warp * F::kTok;
+    const bool here = ((filled >> slot) & 1u) != 0u && tw < max_lim;
+    if (here) {  // this warp's copy was issued
+      if (ok && !mbar_wait(bars + 8 * slot, (phases >> slot) & 1u)) {
+        flag_error(kErrTimeout);
+        ok = false;  // nothing is waited for any more, the result is marked by the error
+      }
+      phases ^= 1u << slot;
+    }
     __syncwarp();
-    const bool here = cur.present(p, cur.entry(p));
+    const uint32_t kc = codes + slot * 2 * F::kCodes, vc = kc + F::kCodes;
+    const uint32_t ks = scales + slot * 2 * F::kScales, vs = ks + F::kScales;
     advance(fill);
     fill = fill + 1 == F::kStages ? 0 : fill + 1;
 
-    const uint32_t st = ring + slot * F::kStage;
-    const uint32_t k_codes = st, v_codes = st + F::kCodes;
-    const uint32_t k_scales = st + 2 * F::kCodes, v_scales = k_scales + kFewTok * F::kSRow;
-    const int tw = cur.page * kPage + warp * kFewTok;
-    if (tw < max_lim && here) {
-      const bool tail = tw + kFewTok > min_lim;
-      // ------------------------------------------------ S^T of both tiles
-      float t[NT][8];
+    if (here) {
+      const bool tail = tw + F::kTok > min_lim;
+      const int end_row = cur.r.kv - tw;
+      float t[TILES][4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float sa[NT][4], sb[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sa[nt][i] = sb[nt][i] = 0.f;
-        const int r0 = 16 * half + g, r1 = r0 + 8;
-        constexpr int KW = D / 32;  // code words of a lane: 8, 4, 2
-        uint32_t kw0[KW], kw1[KW], sc0[4], sc1[4];
-        if constexpr (D == 256) {
-          uint32_t(&a)[4] = reinterpret_cast<uint32_t(&)[4]>(kw0[0]);
-          uint32_t(&b)[4] = reinterpret_cast<uint32_t(&)[4]>(kw0[4]);
-          uint32_t(&c)[4] = reinterpret_cast<uint32_t(&)[4]>(kw1[0]);
-          uint32_t(&d)[4] = reinterpret_cast<uint32_t(&)[4]>(kw1[4]);
-          lds_words(k_codes + few_swz<D>(r0, 2 * qd), a);
-          lds_words(k_codes + few_swz<D>(r0, 2 * qd + 1), b);
-          lds_words(k_codes + few_swz<D>(r1, 2 * qd), c);
-          lds_words(k_codes + few_swz<D>(r1, 2 * qd + 1), d);
-          scales_bcast4(lds32(k_scales + r0 * 16 + 4 * qd), sc0);
-          scales_bcast4(lds32(k_scales + r1 * 16 + 4 * qd), sc1);
-        } else if constexpr (D == 128) {
-          lds_words(k_codes + few_swz<D>(r0, qd), kw0);
-          lds_words(k_codes + few_swz<D>(r1, qd), kw1);
-          scales_bcast4(lds16(k_scales + r0 * 8 + 2 * qd), sc0);
-          scales_bcast4(lds16(k_scales + r1 * 8 + 2 * qd), sc1);
-        } else {
-          lds_words(k_codes + few_swz<D>(r0, qd >> 1) + (qd & 1) * 8, kw0);
-          lds_words(k_codes + few_swz<D>(r1, qd >> 1) + (qd & 1) * 8, kw1);
-          scales_bcast4(lds8(k_scales + r0 * 4 + qd), sc0);
-          scales_bcast4(lds8(k_scales + r1 * 4 + qd), sc1);
-        }
-#pragma unroll
-        for (int w8 = 0; w8 < KW; ++w8) {
-          uint32_t h0[4], h1[4];
-          e2m1x8_to_f16x2x4(kw0[w8], h0);
-          e2m1x8_to_f16x2x4(kw1[w8], h1);
-          const uint32_t s0 = sc0[w8 >> 1], s1 = sc1[w8 >> 1];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            h0[j] = hmul2_u32(h0[j], s0);
-            h1[j] = hmul2_u32(h1[j], s1);
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816(sa[nt], h0[0], h1[0], h0[1], h1[1], qf[nt][4 * w8 + 0], qf[nt][4 * w8 + 1]);
-            mma_16816(sb[nt], h0[2], h1[2], h0[3], h1[3], qf[nt][4 * w8 + 2], qf[nt][4 * w8 + 3]);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = (sa[nt][i] + sb[nt][i]) * cf[nt][i & 1];
-            if (tail && tw + 16 * half + g + 8 * (i >> 1) >= lim[nt][i & 1]) x = -CUDART_INF_F;
-            t[nt][4 * half + i] = x;
-          }
+      for (int i = 0; i < TILES; ++i) {
+        few_qk<D>(kc, ks, 16 * i + g, qd, qf, t[i]);
+        t[i][0] *= cf0;
+        t[i][1] *= cf1;
+        t[i][2] *= cf0;
+        t[i][3] *= cf1;
       }
-
+      if (tail) {
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+          const int at = tw + 16 * i + g;
+          if (at >= lim0) t[i][0] = -CUDART_INF_F;
+          if (at >= lim1) t[i][1] = -CUDART_INF_F;
+          if (at + 8 >= lim0) t[i][2] = -CUDART_INF_F;
+          if (at + 8 >= lim1) t[i][3] = -CUDART_INF_F;
+        }
+      }
       // V codes first: their shared-memory latency hides behind the softmax
-      const int end = cur.r.kv - tw;
       FewV<D> va, vb;
-      few_v_load<D>(v_codes, v_scales, 2 * qd, g, tail, end, va);
-      few_v_load<D>(v_codes, v_scales, 2 * qd + 16, g, tail, end, vb);
+      few_v_load<D>(vc, vs, 2 * qd, g, tail, end_row, va);
+      few_v_load<D>(vc, vs, 2 * qd + 16, g, tail, end_row, vb);
 
-      // ------------------------------------------------ online softmax
-      PFrag pa[NT], pb[NT];
+      float mx0 = fmaxf(t[0][0], t[0][2]), mx1 = fmaxf(t[0][1], t[0][3]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float mx0 = fmaxf(fmaxf(t[nt][0], t[nt][2]), fmaxf(t[nt][4], t[nt][6]));
-        float mx1 = fmaxf(fmaxf(t[nt][1], t[nt][3]), fmaxf(t[nt][5], t[nt][7]));
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          mx0 = fmaxf(mx0, shfl_xor(mx0, off));
-          mx1 = fmaxf(mx1, shfl_xor(mx1, off));
-        }
-        if (__any_sync(kFull, (mx0 > m[nt][0] + kLazy) || (mx1 > m[nt][1] + kLazy))) {
-          const float n0 = fmaxf(m[nt][0], mx0), n1 = fmaxf(m[nt][1], mx1);
-          const float a0 = (n0 == -CUDART_INF_F) ? 1.f : exp2_approx(m[nt][0] - n0);
-          const float a1 = (n1 == -CUDART_INF_F) ? 1.f : exp2_approx(m[nt][1] - n1);
-          m[nt][0] = n0;
-          m[nt][1] = n1;
-          l[nt][0] *= a0;
-          l[nt][1] *= a1;
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            o[nt][j][0] *= a0;
-            o[nt][j][1] *= a1;
-            o[nt][j][2] *= a0;
-            o[nt][j][3] *= a1;
-          }
-        }
-        const float mu0 = (m[nt][0] == -CUDART_INF_F) ? 0.f : m[nt][0];
-        const float mu1 = (m[nt][1] == -CUDART_INF_F) ? 0.f : m[nt][1];
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          t[nt][i] = exp2_approx(t[nt][i] - mu0);
-          t[nt][i + 1] = exp2_approx(t[nt][i + 1] - mu1);
-        }
-        l[nt][0] += (t[nt][0] + t[nt][2]) + (t[nt][4] + t[nt][6]);
-        l[nt][1] += (t[nt][1] + t[nt][3]) + (t[nt][5] + t[nt][7]);
-        pa[nt] = p_fragments(t[nt][0], t[nt][1], t[nt][2], t[nt][3]);
-        pb[nt] = p_fragments(t[nt][4], t[nt][5], t[nt][6], t[nt][7]);
+      for (int i = 1; i < TILES; ++i) {
+        mx0 = fmaxf(mx0, fmaxf(t[i][0], t[i][2]));
+        mx1 = fmaxf(mx1, fmaxf(t[i][1], t[i][3]));
       }
-
-      // ------------------------------------------------ O^T += V^T P^T
 #pragma unroll
-      for (int w = 0; w < FewV<D>::W; ++w) {
+      for (int off = 4; off < 32; off <<= 1) {
+        mx0 = fmaxf(mx0, shfl_xor(mx0, off));
+        mx1 = fmaxf(mx1, shfl_xor(mx1, off));
+      }
+      if (__any_sync(kFull, (mx0 > m0 + kLazy) || (mx1 > m1 + kLazy))) {
+        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        const float a0 = (n0 == -CUDART_INF_F) ? 1.f : exp2_approx(m0 - n0);
+        const float a1 = (n1 == -CUDART_INF_F) ? 1.f : exp2_approx(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= a0;
+        l1 *= a1;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const FewV<D>& v = half ? vb : va;
-          const uint32_t xab = (v.a[w] & 0x0F0F0F0Fu) | ((v.b[w] << 4) & 0xF0F0F0F0u);
-          const uint32_t yab = ((v.a[w] >> 4) & 0x0F0F0F0Fu) | (v.b[w] & 0xF0F0F0F0u);
-          const uint32_t xcd = (v.c[w] & 0x0F0F0F0Fu) | ((v.d[w] << 4) & 0xF0F0F0F0u);
-          const uint32_t ycd = ((v.c[w] >> 4) & 0x0F0F0F0Fu) | (v.d[w] & 0xF0F0F0F0u);
-          uint32_t hxab[4], hyab[4], hxcd[4], hycd[4];
-          e2m1x8_to_f16x2x4(xab, hxab);
-          e2m1x8_to_f16x2x4(yab, hyab);
-          e2m1x8_to_f16x2x4(xcd, hxcd);
-          e2m1x8_to_f16x2x4(ycd, hycd);
-          const uint32_t sab = v.sab[D == 256 ? w >> 1 : 0], scd = v.scd[D == 256 ? w >> 1 : 0];
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t a0 = hmul2_u32(hxab[kk], sab), a1 = hmul2_u32(hyab[kk], sab);
-            const uint32_t a2 = hmul2_u32(hxcd[kk], scd), a3 = hmul2_u32(hycd[kk], scd);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_16816(o[nt][4 * w + kk], a0, a1, a2, a3, half ? pb[nt].hi0 : pa[nt].hi0,
-                        half ? pb[nt].hi1 : pa[nt].hi1);
-          }
+        for (int j = 0; j < MT; ++j) {
+          o[j][0] *= a0;
+          o[j][1] *= a1;
+          o[j][2] *= a0;
+          o[j][3] *= a1;
         }
+      }
+      const float mu0 = (m0 == -CUDART_INF_F) ? 0.f : m0;
+      const float mu1 = (m1 == -CUDART_INF_F) ? 0.f : m1;
+      PFrag pf[TILES];
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        t[i][0] = exp2_approx(t[i][0] - mu0);
+        t[i][1] = exp2_approx(t[i][1] - mu1);
+        t[i][2] = exp2_approx(t[i][2] - mu0);
+        t[i][3] = exp2_approx(t[i][3] - mu1);
+        l0 += t[i][0] + t[i][2];
+        l1 += t[i][1] + t[i][3];
+        pf[i] = p_fragments(t[i][0], t[i][1], t[i][2], t[i][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < TILES; i += 2) {
+        few_pv<D>(va, pf[i], o);
+        if (i + 2 < TILES) few_v_load<D>(vc, vs, 2 * qd + 16 * (i + 2), g, tail, end_row, va);
+        few_pv<D>(vb, pf[i + 1], o);
+        if (i + 3 < TILES) few_v_load<D>(vc, vs, 2 * qd + 16 * (i + 3), g, tail, end_row, vb);
       }
     }
 
-    if (cur.page + 1 == cur.pages || k + 1 == units) {  // --------- item's end
-      uint8_t* area = F::kMergeInRing ? smem + slot * F::kStage : smem + F::kRing;
-      constexpr int kPitch = F::kMergeInRing ? F::kStages * F::kStage : F::kMergeWarp;
+    FewWalk nxt = cur;
+    nxt.next(p);
+    const bool last = nxt.at(end);
+    if (nxt.page == 0 || last) {  // ------------------------------ item's end
+      constexpr int kPitch = F::kStages * 2 * F::kCodes;
+      uint8_t* area = sgen + slot * 2 * F::kCodes;  // of warp 0
+      auto ml_of = [&](int w) {
+        return reinterpret_cast<float2*>(sgen + F::kRing + (w * F::kStages + slot) * 2 * F::kScales);
+      };
       float4* red = reinterpret_cast<float4*>(area + warp * kPitch);
-      float* ml = reinterpret_cast<float*>(red + 16 * kEpiRowF4);
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l0 += shfl_xor(l0, off);
+        l1 += shfl_xor(l1, off);
+      }
       __syncwarp();
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) l[nt][i] += shfl_xor(l[nt][i], off);
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-          red[(nt * MT + j) * kEpiRowF4 + lane] =
-              make_float4(o[nt][j][0], o[nt][j][1], o[nt][j][2], o[nt][j][3]);
-        if (g == 0) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ml[(nt * 8 + 2 * qd + i) * 2 + 0] = m[nt][i];
-            ml[(nt * 8 + 2 * qd + i) * 2 + 1] = l[nt][i];
-          }
-        }
+      for (int j = 0; j < MT; ++j) red[j * 32 + lane] = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+      if (g == 0) {
+        ml_of(warp)[2 * qd] = make_float2(m0, l0);
+        ml_of(warp)[2 * qd + 1] = make_float2(m1, l1);
       }
       const bool starts_here = first_page == 0, ends_here = cur.page + 1 == cur.pages;
       const bool whole = starts_here && ends_here;
-      float* rec = p.records + (size_t)(blockIdx.x * 2 + (starts_here ? 1 : 0)) * (F::kCols * (D + 2));
+      float* rec = p.records + (size_t)(blockIdx.x * 2 + (starts_here ? 1 : 0)) * (kFewCols * (D + 2));
       __syncthreads();
-      if (tid < F::kCols) {
-        float mm[kFewWarps], M = -CUDART_INF_F, ls = 0.f;
+      // the lane's two columns: weights of the warps
+      float w0[F::kWarps], w1[F::kWarps], M0 = -CUDART_INF_F, M1 = -CUDART_INF_F, L0 = 0.f, L1 = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
-          const float* s = reinterpret_cast<const float*>(area + w * kPitch + 16 * kEpiRowF4 * 16) + tid * 2;
-          mm[w] = s[0];
-          M = fmaxf(M, mm[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
-          const float* s = reinterpret_cast<const float*>(area + w * kPitch + 16 * kEpiRowF4 * 16) + tid * 2;
-          const float wt = mm[w] == -CUDART_INF_F ? 0.f : exp2_approx(mm[w] - M);
-          weights[tid * kFewWarps + w] = wt;
-          ls += wt * s[1];
-        }
-        col_l[tid] = ls > 0.f ? 1.f / ls : 0.f;
-        if (!whole) {
-          rec[F::kCols * D + 2 * tid] = M;
-          rec[F::kCols * D + 2 * tid + 1] = ls;
-        }
+      for (int w = 0; w < F::kWarps; ++w) {
+        w0[w] = ml_of(w)[2 * qd].x;
+        w1[w] = ml_of(w)[2 * qd + 1].x;
+        M0 = fmaxf(M0, w0[w]);
+        M1 = fmaxf(M1, w1[w]);
       }
-      __syncthreads();
-      const int hd = cur.head;
-      for (int idx = tid; idx < cols * (D / 2); idx += kFewThreads) {
-        const int c = idx / (D / 2), d = idx % (D / 2) * 2;
-        // d = D/8 gg + 2j sits in m-tile j, lane row gg: (d, col) in c0/c1, (d + 1, col) in c2/c3
-        const int gg = d / (D / 8), j = d % (D / 8) / 2;
-        const int src = ((((c >> 3) * MT + j) * kEpiRowF4) + 4 * gg + ((c & 7) >> 1)) * 4 + (c & 1);
-        float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) {
-          const float* s = reinterpret_cast<const float*>(area + w * kPitch);
-          a0 += weights[c * kFewWarps + w] * s[src];
-          a1 += weights[c * kFewWarps + w] * s[src + 2];
+      for (int w = 0; w < F::kWarps; ++w) {
+        w0[w] = w0[w] == -CUDART_INF_F ? 0.f : exp2_approx(w0[w] - M0);
+        w1[w] = w1[w] == -CUDART_INF_F ? 0.f : exp2_approx(w1[w] - M1);
+        L0 += w0[w] * ml_of(w)[2 * qd].y;
+        L1 += w1[w] * ml_of(w)[2 * qd + 1].y;
+      }
+      const float i0 = L0 > 0.f ? 1.f / L0 : 0.f, i1 = L1 > 0.f ? 1.f / L1 : 0.f;
+      if (!whole && warp == 0 && g == 0) {
+        float2* ml = reinterpret_cast<float2*>(rec + kFewCols * D);
+        ml[2 * qd] = make_float2(M0, L0);
+        ml[2 * qd + 1] = make_float2(M1, L1);
+      }
+#pragma unroll
+      for (int jj = 0; jj < MT / F::kWarps; ++jj) {
+        const int j = jj * F::kWarps + warp;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < F::kWarps; ++w) {
+          const float4 v = reinterpret_cast<const float4*>(area + w * kPitch)[j * 32 + lane];
+          a.x += w0[w] * v.x;
+          a.y += w1[w] * v.y;
+          a.z += w0[w] * v.z;
+          a.w += w1[w] * v.w;
         }
-        if (whole) {
-          const int s = c / p.group, h = hd * p.group + c % p.group;
-          T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + s) * p.out_stride + h * D + d;
-          dst[0] = InTraits<T>::from_float(a0 * col_l[c]);
-          dst[1] = InTraits<T>::from_float(a1 * col_l[c]);
-        } else {
-          *reinterpret_cast<float2*>(rec + c * D + d) = make_float2(a0, a1);
+        // (x, z): d = D/8 g + 2j and d + 1 of column 2qd; (y, w): of column 2qd + 1
+        const int d = D / 8 * g + 2 * j;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 2 * qd + e;
+          if (c >= cols) continue;
+          const float x = e ? a.y : a.x, y = e ? a.w : a.z, inv = e ? i1 : i0;
+          if (whole) {
+            T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + c / p.group) * p.out_stride +
+                     (cur.head * p.group + c % p.group) * D + d;
+            const T h[2] = {InTraits<T>::from_float(x * inv), InTraits<T>::from_float(y * inv)};
+            *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
+          } else {
+            *reinterpret_cast<float2*>(rec + c * D + d) = make_float2(x, y);
+          }
         }
       }
       if (starts_here && !ends_here && tid == 0) {  // the rest of the item is the next CTAs'
-        const long long last_unit = hi - 1 - cur.page + cur.pages - 1;
+        const long long last_unit = cur.base + FewWalk::kOver + cur.pages - 1;
         meta[0] = cols;
         meta[1] = cur.r.row0;
-        meta[3] = hd;
+        meta[3] = cur.head;
         meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
         meta[5] = (int)min(total, n_cta);  // fewer units than CTAs leave some CTAs without a record
       }
       __syncthreads();
       fresh = true;
     }
-    cur.next(p);
+    if (last) break;
+    cur = nxt;
     slot = slot + 1 == F::kStages ? 0 : slot + 1;
   }
   griddep_launch_dependents();
@@ -561,11 +606,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) batch_few_kernel(const __grid_
 
 // Merges the records of the items that more than one CTA worked on, CTA by
 // CTA in order: block (i, y) takes columns y, y + gridDim.y, ... of the item
-// that CTA i began and did not finish.  
-template <typename T, int D, int COLS>
+// that CTA i began and did not finish.
+template <typename T, int D>
 __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ float w[256];
+  __shared__ float w[kBatchMaxCtas];
   __shared__ float red[8];
   __shared__ float4 acc_s[kGroups][kLanes];
   griddep_wait();
@@ -577,7 +622,7 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
   const int row0 = __ldcg(meta + 1), hd = __ldcg(meta + 3), last = __ldcg(meta + 4);
   const int busy = __ldcg(meta + 5);
   const int parts = last - i0 + 1;
-  constexpr size_t kRec = (size_t)COLS * (D + 2);
+  constexpr size_t kRec = (size_t)kFewCols * (D + 2);
   // CTA i0 left its part in record 1, the later ones in record 0
   auto record = [&](int j) { return p.records + (size_t)((i0 + j) * 2 + (j == 0 ? 1 : 0)) * kRec; };
   auto empty = [&](int j) {
@@ -585,13 +630,10 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
     return i * busy / n_cta == (i + 1) * busy / n_cta;
   };
   for (int c = blockIdx.y; c < cols; c += gridDim.y) {
-    float m = -CUDART_INF_F, l = 0.f;
-    if (tid < parts && !empty(tid)) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(record(tid) + COLS * D + 2 * c));
-      m = v.x;
-      l = v.y;
-    }
-    float M = m;
+    auto stat = [&](int j) { return __ldcg(reinterpret_cast<const float2*>(record(j) + kFewCols * D + 2 * c)); };
+    float M = -CUDART_INF_F;
+    for (int j = tid; j < parts; j += 256)
+      if (!empty(j)) M = fmaxf(M, stat(j).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if ((tid & 31) == 0) red[tid >> 5] = M;
@@ -600,9 +642,16 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
 #pragma unroll
     for (int i = 1; i < 8; ++i) M = fmaxf(M, red[i]);
     __syncthreads();
-    const float wt = m == -CUDART_INF_F ? 0.f : exp2_approx(m - M);
-    w[tid] = wt;
-    float L = wt * l;
+    float L = 0.f;
+    for (int j = tid; j < parts; j += 256) {
+      float wt = 0.f;
+      if (!empty(j)) {
+        const float2 v = stat(j);
+        wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
+        L += wt * v.y;
+      }
+      w[j] = wt;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     if ((tid & 31) == 0) red[tid >> 5] = L;
@@ -649,41 +698,42 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
 namespace {
 
 template <typename T, int D>
-cudaError_t launch_few(const BatchAttnParams& p, int ctas, cudaStream_t stream) {
+cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int sms, cudaStream_t stream) {
+  using F = Few<D>;
+  const int ctas = sms * F::kCtas;
   auto kernel = batch_few_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(ctas), dim3(kFewThreads), Few<D>::kSmem, stream, p);
+  e = launch_pdl(kernel, dim3(ctas), dim3(F::kThreads), F::kSmem, stream, p, maps);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(batch_combine_kernel<T, D, Few<D>::kCols>, dim3(ctas, 8), dim3(256), 0, stream, p);
+  e = launch_pdl(batch_combine_kernel<T, D>, dim3(ctas, kFewCols), dim3(256), 0, stream, p);
   if (e != cudaSuccess || (long long)p.max_rows * p.group <= p.few_cols) return e;
-  return launch_rows<T, D>(p, ctas, stream);
+  return launch_rows<T, D>(p, sms, stream);
 }
 
 template <typename T>
-cudaError_t launch_attend(const BatchAttnParams& p, int dim, int ctas, cudaStream_t stream) {
+cudaError_t launch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int sms, cudaStream_t stream) {
   switch (dim) {
-    case 64: return launch_few<T, 64>(p, ctas, stream);
-    case 128: return launch_few<T, 128>(p, ctas, stream);
-    case 256: return launch_few<T, 256>(p, ctas, stream);
+    case 64: return launch_few<T, 64>(p, maps, sms, stream);
+    case 128: return launch_few<T, 128>(p, maps, sms, stream);
+    case 256: return launch_few<T, 256>(p, maps, sms, stream);
   }
   return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-size_t batch_few_record_bytes(int dim) {
-  return (size_t)kBatchMaxCtas * 2 * (2048 / dim) * (dim + 2) * sizeof(float);
-}
+size_t batch_few_record_bytes(int dim) { return (size_t)kBatchMaxCtas * 2 * kFewCols * (dim + 2) * sizeof(float); }
 size_t batch_workspace_bytes(int dim) {
-  return kBatchMetaBytes + batch_few_record_bytes(dim) +
-         (size_t)kBatchMaxCtas * 2 * kRwRows * (dim + 2) * sizeof(float);
+  return kBatchMetaBytes + batch_few_record_bytes(dim) + (size_t)kBatchMaxSms * 2 * kRwRows * (dim + 2) * sizeof(float);
 }
+int batch_few_box_rows(int dim) { return dim == 256 ? Few<256>::kTok : dim == 128 ? Few<128>::kTok : Few<64>::kTok; }
 
-cudaError_t launch_batch_attend(const BatchAttnParams& p, int dim, int dtype, int ctas, cudaStream_t stream) {
+cudaError_t launch_batch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
+                                cudaStream_t stream) {
   if (p.requests <= 0 || p.rows <= 0) return cudaSuccess;
-  return dtype == kDtypeBF16 ? launch_attend<__nv_bfloat16>(p, dim, ctas, stream)
-                             : launch_attend<__half>(p, dim, ctas, stream);
+  return dtype == kDtypeBF16 ? launch_attend<__nv_bfloat16>(p, maps, dim, sms, stream)
+                             : launch_attend<__half>(p, maps, dim, sms, stream);
 }
 
 }  // namespace qwz

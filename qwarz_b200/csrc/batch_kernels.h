@@ -3,6 +3,7 @@
 // ABI is include/qwz_b200.h).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -32,7 +33,16 @@ struct BatchAttnParams {
   float sm_scale_log2;           // sm_scale * log2(e)
 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA
-constexpr int kBatchMaxCtas = 256;
+constexpr int kBatchMaxSms = 256;
+constexpr int kBatchMaxCtas = 4 * kBatchMaxSms;  // batch_few.cu has up to 4 CTAs an SM
+
+// TMA descriptors of the pool's codes as [P * 256 rows, kv_heads * dim / 2
+// bytes], boxes of one head's dim / 2 bytes x batch_few_box_rows(dim) rows.
+struct alignas(64) BatchPoolMaps {
+  CUtensorMap k, v;
+};
+int batch_few_box_rows(int dim);
+constexpr int kBatchFewCols = 8;
 constexpr size_t kBatchMetaBytes = 2 * (size_t)kBatchMaxCtas * kBatchMeta * 4;
 size_t batch_few_record_bytes(int dim);  // all records of batch_few.cu
 size_t batch_workspace_bytes(int dim);
@@ -89,6 +99,7 @@ cudaError_t launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_
 
 cudaError_t launch_batch_tables(const BatchTablesParams& p, int sms, cudaStream_t stream);
 cudaError_t launch_batch_append(const BatchAppendParams& p, int dtype, cudaStream_t stream);
-cudaError_t launch_batch_attend(const BatchAttnParams& p, int dim, int dtype, int ctas, cudaStream_t stream);
+cudaError_t launch_batch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
+                                cudaStream_t stream);
 
 }  // namespace qwz

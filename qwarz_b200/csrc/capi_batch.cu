@@ -25,12 +25,12 @@ int check_row_stride(int64_t stride, int64_t width, const char* what) {
   return QWZ_OK;
 }
 
-// CTAs of an attention launch: one per SM of the current device.
-int batch_ctas() {
+// SMs of the current device (0: none).
+int batch_sms() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return 0;
-  return sms < qwz::kBatchMaxCtas ? sms : qwz::kBatchMaxCtas;
+  return sms < qwz::kBatchMaxSms ? sms : qwz::kBatchMaxSms;
 }
 
 }  // namespace
@@ -52,7 +52,7 @@ int qwz_batch_tables(const int32_t* lengths, const int32_t* new_rows, const int3
   if (ring_size < 1) return fail(QWZ_EINVAL, "ring_size must be positive");
   if (held_out == held || kv_lens == lengths || ring_out == ring_state || cu_rows == lengths || cu_rows == held)
     return fail(QWZ_EINVAL, "outputs must not share storage with inputs");
-  const int sms = batch_ctas();
+  const int sms = batch_sms();
   if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
   qwz::BatchTablesParams p{lengths, new_rows, held, ring_state, ring, block_table, cu_rows, kv_lens, held_out,
                            ring_out, slots, positions, request_of, requests, table_width, ring_size, rows};
@@ -123,8 +123,17 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   if ((rc = check_row_stride(q_stride, width, "q"))) return rc;
   if ((rc = check_row_stride(out_stride, width, "out"))) return rc;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(QWZ_EINVAL, "sm_scale must be positive and finite");
-  const int ctas = batch_ctas();
-  if (ctas <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
+  const int sms = batch_sms();
+  if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
+  qwz::BatchPoolMaps maps;
+  const uint64_t pool_rows = (uint64_t)num_pages * qwz::kPage, row_bytes = (uint64_t)num_kv_heads * head_dim / 2;
+  const CUtensorMapSwizzle swizzle = head_dim == 256   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                       : CU_TENSOR_MAP_SWIZZLE_32B;
+  const uint32_t box_rows = (uint32_t)qwz::batch_few_box_rows(head_dim);
+  rc = encode_2d(&maps.k, k_cache, row_bytes, pool_rows, head_dim / 2, box_rows, swizzle);
+  if (!rc) rc = encode_2d(&maps.v, v_cache, row_bytes, pool_rows, head_dim / 2, box_rows, swizzle);
+  if (rc) return rc;
   qwz::BatchAttnParams p{};
   p.q = q;
   p.out = out;
@@ -148,9 +157,9 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
   p.max_rows = max_rows;
-  p.few_cols = 2048 / head_dim;
+  p.few_cols = qwz::kBatchFewCols;
   p.sm_scale_log2 = sm_scale * kLog2e;
-  return launched(qwz::launch_batch_attend(p, head_dim, dtype, ctas, as_stream(stream)), "qwz_batch_attend");
+  return launched(qwz::launch_batch_attend(p, maps, head_dim, dtype, sms, as_stream(stream)), "qwz_batch_attend");
 }
 
 int64_t qwz_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top, int32_t dtype) {

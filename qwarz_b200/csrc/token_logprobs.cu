@@ -87,13 +87,21 @@ QWZ_DEVINL float max_nan(float a, float b) {  // NaN wins
 
 constexpr float kLog2eF = 1.4426950408889634f;
 
+// Makes the raw words opaque between two passes over them: otherwise the
+// compiler keeps every unpacked FP32 value of the first pass (64 registers)
+// for the second instead of unpacking again.
+QWZ_DEVINL void lp_opaque(uint4 (&raw)[kLpVecs]) {
+#pragma unroll
+  for (int i = 0; i < kLpVecs; ++i) asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y), "+r"(raw[i].z), "+r"(raw[i].w));
+}
+
 // Bytes of one chunk's record: m, s, t, (pad), K keys.
 QWZ_DEVINL size_t lp_record(int top) { return 16 + 8 * (size_t)top; }
 
 }  // namespace
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) lp_chunk_kernel(const __grid_constant__ LogprobParams p) {
+__global__ void __launch_bounds__(kLpThreads, 4) lp_chunk_kernel(const __grid_constant__ LogprobParams p) {
   using L = LpTraits<T>;
   constexpr int E = L::E;
   __shared__ float red[3][kLpThreads / 32];
@@ -166,6 +174,7 @@ __global__ void __launch_bounds__(kLpThreads) lp_chunk_kernel(const __grid_const
     if (rb == K - 1) tau_s = b;
   }
 
+  lp_opaque(raw);
   const float mu = M == -CUDART_INF_F ? 0.f : M;
   float s = 0.f, t = 0.f;
 #pragma unroll
@@ -210,6 +219,7 @@ __global__ void __launch_bounds__(kLpThreads) lp_chunk_kernel(const __grid_const
 
   // candidates: at or above tau; where fewer than K groups hold anything above
   // -inf, all that is above -inf and the first K places (the lowest indices)
+  lp_opaque(raw);
   const float tau = tau_s;
   const bool open = tau == -CUDART_INF_F;
   const int first = max(0, v0 * E - skew);
@@ -248,6 +258,7 @@ __global__ void __launch_bounds__(kLpThreads) lp_chunk_kernel(const __grid_const
     unsigned long long last = ~0ull;
     for (int k = 0; k < K; ++k) {
       unsigned long long top = 0ull;
+      lp_opaque(raw);
 #pragma unroll
       for (int i = 0; i < kLpVecs; ++i) {
         float x[E];
