@@ -8,9 +8,10 @@
 // and 4 D multiply-adds a query column, far below the tensor rate.
 //
 // The (row, head of the group) pairs of one request and KV head are the (at
-// most 8) columns of an item; its 256-token pages are shared out over the CTAs
-// together with those of all other items (batch_common.cuh).  A warp owns 32 or
-// 64 tokens of each page and streams them through a ring of its own: the codes
+// most 8) columns of an item.  A CTA has one KV head and a share of all
+// requests' units of 128 or 256 tokens (batch_common.cuh); the CTAs of the other heads work
+// on the same tokens at the same time.  A warp owns 32
+// or 64 tokens of a unit and streams them through a ring of its own: the codes
 // by TMA (one box of its rows of K and one of V, 128-byte swizzle, on the warp's
 // own mbarrier), the scales, whose rows can be narrower than a TMA box, by
 // cp.async.  No warp waits for another inside an item, and the ring runs on
@@ -31,15 +32,21 @@ using namespace detail;
 namespace {
 
 constexpr int kFewCols = kBatchFewCols;  // query columns of an item
-constexpr int kFewScan = 128; // threads that scan the requests
+constexpr int kFewScan = 128;  // threads that scan the requests
 
 template <int D>
 struct Few {
-  static constexpr int kWarps = D == 256 ? 8 : 4;
+  // measured at 524,288 tokens of 24/4/256 and 262,144 of 32/8/128 (us):
+  //   D 256: 4 warps x 32 tokens, 3 stages, 2 CTAs 125; 8 x 32, 3, 1 CTA 126
+  //     (short items: 187 against 248 at 1,024 x 512 tokens); 4 x 32, 2, 3 CTAs 148
+  //   D 128: 4 x 64, 2, 3 CTAs 78; 4 x 32, 3, 4 CTAs 81; 8 x 32, 3, 2 CTAs 80
+  //   D 64:  4 x 64, 2, 4 CTAs 37; 4 x 64, 3, 4 CTAs 39; 4 x 32, 3, 5 CTAs 45
+  static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTok = kPage / kWarps;        // tokens of a page a warp owns
-  static constexpr int kStages = D == 128 ? 2 : 3;
-  static constexpr int kCtas = D == 256 ? 1 : D == 128 ? 3 : 4;  // per SM
+  static constexpr int kTok = D == 256 ? 32 : 64;    // tokens of a unit a warp owns
+  static constexpr int kUnit = kWarps * kTok;        // tokens of a unit of work (divides a page)
+  static constexpr int kStages = D == 256 ? 3 : 2;
+  static constexpr int kCtas = D == 256 ? 2 : D == 128 ? 3 : 4;  // per SM
   static constexpr int kMT = D / 16;                 // MMA row tiles of O^T
   static constexpr int kRow = D / 2;                 // code bytes of a row
   static constexpr int kSRow = D / 16;               // scale bytes of a row
@@ -49,7 +56,7 @@ struct Few {
   static constexpr int kRing = kWarps * kStages * 2 * kCodes;
   static constexpr int kScaleRing = kWarps * kStages * 2 * kScales;
   static constexpr int kSmem = kRing + kScaleRing + 8 * kWarps * kStages + 1024;
-  // for the merge a warp's O takes the code slot its last page left, (m, l) the scale slot
+  // for the merge a warp's O takes the code slot its last unit left, (m, l) the scale slot
   static_assert(kMT * 512 <= 2 * kCodes && kFewCols * 8 <= 2 * kScales, "merge area");
   static_assert(kMT % kWarps == 0 && kTok % 32 == 0, "merge share, tile pairs");
 };
@@ -90,29 +97,30 @@ QWZ_DEVINL void cp_async_small(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES));
 }
 
-// Walks the pages (request, head, page) of the launch in order.  An item
-// weighs its pages and kOver more for what it costs beside them (its Q, the
-// merge and the store), so that CTAs with many short items get fewer pages.
+// Walks the units (request, U tokens) of one KV head in order.  A request
+// weighs its units and kOver more for what its item costs beside them (its Q,
+// the merge and the store), so that CTAs with many short items get fewer.
+template <int U>
 struct FewWalk {
-  static constexpr int kOver = 1;
-  int b, head, page;       // request (p.requests: past the end), KV head, page
-  int pages;               // of request b
-  long long base;          // weighed units before the item
+  static constexpr int kOver = 256 / U;
+  int b, unit;             // request (p.requests: past the end), unit
+  int units;               // of request b
+  long long base;          // weighed units before the request
   batch::Req r;
 
   static QWZ_DEVINL bool few(const BatchAttnParams& p, const batch::Req& r) {
     return r.n > 0 && r.n * p.group <= p.few_cols;  // the others are batch_rows.cu's
   }
   // a request without tokens still has rows to write
-  static QWZ_DEVINL int pages_of(const batch::Req& r) { return max(1, (r.kv + kPage - 1) / kPage); }
+  static QWZ_DEVINL int units_of(const batch::Req& r) { return max(1, (r.kv + U - 1) / U); }
   static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b) {
     const batch::Req r = batch::load_req(p, b);
-    return few(p, r) ? (long long)p.kv_heads * (pages_of(r) + kOver) : 0;
+    return few(p, r) ? units_of(r) + kOver : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
     r = batch::load_req(p, b);
-    pages = pages_of(r);
+    units = units_of(r);
   }
   // Weighed unit u, `before` of which precede request b0.
   QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long before, long long u) {
@@ -124,32 +132,29 @@ struct FewWalk {
       u -= c;
       base += c;
     }
-    head = page = 0;
+    unit = 0;
     if (b == p.requests) return;
     enter(p, b);
-    const int w = pages + kOver;
-    head = (int)(u / w);
-    base += (long long)head * w;
-    page = max((int)(u % w) - kOver, 0);
+    unit = max((int)u - kOver, 0);
   }
-  QWZ_DEVINL void next(const BatchAttnParams& p) {
-    if (++page < pages) return;
-    page = 0;
-    base += pages + kOver;
-    if (++head < p.kv_heads) return;
-    head = 0;
+  // To the next request that has work here.
+  QWZ_DEVINL void next_request(const BatchAttnParams& p) {
+    unit = 0;
+    base += units + kOver;
     for (int bb = b + 1; bb < p.requests; ++bb) {
       enter(p, bb);
       if (few(p, r)) return;
     }
     b = p.requests;
   }
-  QWZ_DEVINL bool at(const FewWalk& o) const { return b == o.b && head == o.head && page == o.page; }
-  // Table entry of the page, unchecked (the load is in flight until it is used).
+  QWZ_DEVINL bool at(const FewWalk& o) const { return b == o.b && unit == o.unit; }
+  // Units from here on, of this request, before the walk's end.
+  QWZ_DEVINL int left(int end_b, int end_unit) const { return (b == end_b ? end_unit : units) - unit; }
+  // Table entry of the unit's page, unchecked (the load is in flight until it is used).
   QWZ_DEVINL int entry(const BatchAttnParams& p) const {
-    return __ldg(p.block_table + (size_t)b * p.table_width + page);
+    return __ldg(p.block_table + (size_t)b * p.table_width + unit / (kPage / U));
   }
-  // Whether the page has tokens and lies in the pool.
+  // Whether the unit has tokens and lies in the pool.
   QWZ_DEVINL bool present(const BatchAttnParams& p, int pp) const {
     if (r.kv <= 0) return false;
     if (pp >= 0 && pp < p.num_pages) return true;
@@ -266,10 +271,9 @@ template <typename T, int D>
 __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
     batch_few_kernel(const __grid_constant__ BatchAttnParams p, const __grid_constant__ BatchPoolMaps maps) {
   using F = Few<D>;
+  using Walk = FewWalk<F::kUnit>;
   constexpr int MT = F::kMT, QW = D / 8, TILES = F::kTok / 16;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ long long starts[kFewScan];  // weighed units before each scanning thread's requests
-  __shared__ long long warp_sums[F::kWarps];
   const uint32_t sraw = smem_u32(smem);
   const uint32_t sbase = (sraw + 1023u) & ~1023u;
   uint8_t* sgen = smem + (sbase - sraw);
@@ -289,96 +293,124 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   griddep_wait();
 
   // ---------------------------------------------------- this CTA's share
+  // (the ring's memory holds the scan until the first copy)
+  long long* starts = reinterpret_cast<long long*>(sgen);  // weighed units before each scanning thread's requests
+  long long* warp_sums = starts + kFewScan;
   const int per = (p.requests + kFewScan - 1) / kFewScan;
   long long mine = 0;
   if (tid < kFewScan)
-    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += FewWalk::cost(p, b);
+    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b);
   long long total;
   const long long before = batch::block_scan(mine, warp_sums, total);
   if (tid < kFewScan) starts[tid] = before;
   __syncthreads();
-  const long long n_cta = gridDim.x;
+  const int hd = blockIdx.x, split = blockIdx.y, cta = split * gridDim.x + hd;
+  const long long splits = gridDim.y;
   auto seek = [&](long long u) {
     int at = 0;
     for (int step = kFewScan / 2; step > 0; step >>= 1)
       if (starts[at + step] <= u) at += step;
-    FewWalk w;
+    Walk w;
     w.seek(p, min(at * per, p.requests), starts[at], u);
     return w;
   };
-  FewWalk cur = seek((long long)blockIdx.x * total / n_cta);
-  const FewWalk end = seek(((long long)blockIdx.x + 1) * total / n_cta);
-  int32_t* meta = p.meta + blockIdx.x * kBatchMeta;
+  Walk cur = seek(split * total / splits);
+  int end_b, end_unit;
+  bool none;
+  {
+    const Walk end = seek((split + 1) * total / splits);
+    end_b = end.b;
+    end_unit = end.unit;
+    none = cur.at(end);
+  }
+  __syncthreads();
+  int32_t* meta = p.meta + cta * kBatchMeta;
   if (tid == 0) meta[0] = 0;
-  if (cur.at(end)) {
+  if (none) {
     griddep_launch_dependents();
     return;
   }
-  FewWalk pre = cur;
-  int pre_page = pre.entry(p);
-  bool pre_more = true;
-  unsigned filled = 0;  // bit s: ring slot s holds (or will hold) a page of the pool
 
-  // Copies this warp's tokens of the next page into ring slot `slot`.
+  // The loads run kStages - 1 units ahead of the math, with their own place.
+  int pre_b = cur.b, pre_unit = cur.unit, pre_left = cur.left(end_b, end_unit), pre_kv = cur.r.kv;
+  const int32_t* pre_row = p.block_table + (size_t)pre_b * p.table_width;
+  constexpr int kPerPage = kPage / F::kUnit;
+  int pre_page = __ldg(pre_row + pre_unit / kPerPage);
+  unsigned filled = 0;  // bit s: ring slot s holds (or will hold) tokens of the pool
+  const int step = p.kv_heads * F::kSRow;  // scale bytes of a token row
+  const uint8_t* ks_lane = p.k_scales + hd * F::kSRow + (size_t)lane * step;
+  const uint8_t* vs_lane = p.v_scales + hd * F::kSRow + (size_t)lane * step;
+
+  // Copies this warp's tokens of the next unit into ring slot `slot`.
   auto advance = [&](int slot) {
-    if (pre_more) {
-      const bool in_pool = pre.present(p, pre_page);
+    if (pre_left > 0) {
+      bool in_pool = pre_page >= 0 && pre_page < p.num_pages;
+      if (!in_pool && pre_kv > 0) flag_error(kErrPageRange);  // a bad entry: its tokens count as absent
+      in_pool = in_pool && pre_kv > 0;
       filled = in_pool ? filled | (1u << slot) : filled & ~(1u << slot);
-      if (in_pool && pre.page * kPage + warp * F::kTok < pre.r.kv) {
-        const int row0 = pre_page * kPage + warp * F::kTok;
+      const int t0 = pre_unit * F::kUnit + warp * F::kTok;
+      if (in_pool && t0 < pre_kv) {
+        const int row0 = pre_page * kPage + (t0 & (kPage - 1));
         if (lane == 0) {
           const uint32_t bar = bars + 8 * slot, dst = codes + slot * 2 * F::kCodes;
           fence_proxy_async_smem();  // the slot's last reads and merge writes before the copies
           mbar_arrive_expect_tx(bar, 2 * F::kCodes);
-          tma_load_2d(dst, &maps.k, pre.head * F::kRow, row0, bar);
-          tma_load_2d(dst + F::kCodes, &maps.v, pre.head * F::kRow, row0, bar);
+          tma_load_2d(dst, &maps.k, hd * F::kRow, row0, bar);
+          tma_load_2d(dst + F::kCodes, &maps.v, hd * F::kRow, row0, bar);
         }
-        const size_t src = ((size_t)row0 * p.kv_heads + pre.head) * F::kSRow;
-        const size_t step = (size_t)p.kv_heads * F::kSRow;
-        const uint32_t dst = scales + slot * 2 * F::kScales;
+        const uint8_t* kp = ks_lane + (size_t)(unsigned)row0 * (unsigned)step;
+        const uint8_t* vp = vs_lane + (size_t)(unsigned)row0 * (unsigned)step;
+        const uint32_t dst = scales + slot * 2 * F::kScales + lane * F::kSRow;
 #pragma unroll
-        for (int r = lane; r < F::kTok; r += 32) {
-          cp_async_small<F::kSRow>(dst + r * F::kSRow, p.k_scales + src + r * step);
-          cp_async_small<F::kSRow>(dst + F::kScales + r * F::kSRow, p.v_scales + src + r * step);
+        for (int r = 0; r < F::kTok; r += 32) {
+          cp_async_small<F::kSRow>(dst + r * F::kSRow, kp + r * step);
+          cp_async_small<F::kSRow>(dst + F::kScales + r * F::kSRow, vp + r * step);
         }
       }
-      pre.next(p);
-      pre_more = !pre.at(end);
-      if (pre_more) {
-        pre_page = pre.entry(p);
-        if (pre.page == 0 && warp == 0) {  // the item's Q on its way into L1
-          constexpr int kLines = D * 2 / 128;
-          const int c = lane / kLines;
-          if (c < pre.r.n * p.group && c < kFewCols)
-            asm volatile("prefetch.global.L1 [%0];\n" ::"l"(
-                reinterpret_cast<const T*>(p.q) + (pre.r.row0 + c / p.group) * p.q_stride +
-                (pre.head * p.group + c % p.group) * D + (lane % kLines) * 64));
+      ++pre_unit;
+      if (--pre_left == 0 && pre_b != end_b) {  // on to the next request
+        batch::Req r = {0, 0, 0};
+        while (++pre_b < p.requests) {
+          r = batch::load_req(p, pre_b);
+          if (Walk::few(p, r)) break;
+        }
+        if (pre_b < p.requests) {
+          pre_unit = 0;
+          pre_left = pre_b == end_b ? end_unit : Walk::units_of(r);
+          pre_kv = r.kv;
+          pre_row = p.block_table + (size_t)pre_b * p.table_width;
+          if (pre_left > 0 && warp == 0) {  // the item's Q on its way into L1
+            constexpr int kLines = D * 2 / 128;
+            const int c = lane / kLines;
+            if (c < r.n * p.group && c < kFewCols)
+              asm volatile("prefetch.global.L1 [%0];\n" ::"l"(reinterpret_cast<const T*>(p.q) +
+                                                             (r.row0 + c / p.group) * p.q_stride +
+                                                             (hd * p.group + c % p.group) * D + (lane % kLines) * 64));
+          }
         }
       }
+      if (pre_left > 0) pre_page = __ldg(pre_row + pre_unit / kPerPage);
     }
-    cp_async_commit();  // one group a page, empty past the share's end
+    cp_async_commit();  // one group a unit, empty past the share's end
   };
 #pragma unroll
   for (int s = 0; s < F::kStages - 1; ++s) advance(s);
 
   float o[MT][4];
-  float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f, cf0 = 0.f, cf1 = 0.f;
-  int lim0 = 0, lim1 = 0, min_lim = 0, max_lim = 0, cols = 0, first_page = 0;
   uint32_t qf[QW];
-  bool fresh = true, ok = true;
+  bool ok = true;
   int slot = 0, fill = F::kStages - 1;
   unsigned phases = 0;  // parity of each slot's barrier
 
-  while (true) {
-    if (fresh) {  // ------------------------------------------- a new item
-      fresh = false;
-      first_page = cur.page;
-      cols = cur.r.n * p.group;
+  while (true) {  // ------------------------------------------------ an item
+    const int first_unit = cur.unit, cols = cur.r.n * p.group;
+    float cf0, cf1;
+    {
       float amax = 0.f;
       if (g < cols) {
         const uint4* src = reinterpret_cast<const uint4*>(
             reinterpret_cast<const T*>(p.q) + (cur.r.row0 + g / p.group) * p.q_stride +
-            (cur.head * p.group + g % p.group) * D + qd * (D / 4));
+            (hd * p.group + g % p.group) * D + qd * (D / 4));
 #pragma unroll
         for (int i = 0; i < QW / 4; ++i) {
           const uint4 v = __ldg(src + i);
@@ -407,44 +439,40 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       const float rowfac = p.sm_scale_log2 / sc;
       cf0 = __shfl_sync(kFull, rowfac, 8 * qd);
       cf1 = __shfl_sync(kFull, rowfac, 8 * qd + 4);
-      min_lim = cur.r.kv - cur.r.n + 1;
-      max_lim = cur.r.kv;
-      lim0 = 2 * qd < cols ? min_lim + 2 * qd / p.group : 0;
-      lim1 = 2 * qd + 1 < cols ? min_lim + (2 * qd + 1) / p.group : 0;
-      m0 = m1 = -CUDART_INF_F;
-      l0 = l1 = 0.f;
+    }
+    const int min_lim = cur.r.kv - cur.r.n + 1;
+    const int lim0 = 2 * qd < cols ? min_lim + 2 * qd / p.group : 0;
+    const int lim1 = 2 * qd + 1 < cols ? min_lim + (2 * qd + 1) / p.group : 0;
+    // reference maxima in base-2 units, and the raw scores that move them
+    float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, top0 = -CUDART_INF_F, top1 = -CUDART_INF_F;
+    float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    }
+    for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-    cp_async_wait<F::kStages - 2>();
-    const int tw = cur.page * kPage + warp * F::kTok;
-    const bool here = ((filled >> slot) & 1u) != 0u && tw < max_lim;
-    if (here) {  // this warp's copy was issued
-      if (ok && !mbar_wait(bars + 8 * slot, (phases >> slot) & 1u)) {
-        flag_error(kErrTimeout);
-        ok = false;  // nothing is waited for any more, the result is marked by the error
+    int tw = cur.unit * F::kUnit + warp * F::kTok;
+    for (int n = cur.left(end_b, end_unit); n > 0; --n, tw += F::kUnit) {
+      cp_async_wait<F::kStages - 2>();
+      const bool here = ((filled >> slot) & 1u) != 0u && tw < cur.r.kv;
+      if (here) {  // this warp's copy was issued
+        if (ok && !mbar_wait(bars + 8 * slot, (phases >> slot) & 1u)) {
+          flag_error(kErrTimeout);
+          ok = false;  // nothing is waited for any more, the result is marked by the error
+        }
+        phases ^= 1u << slot;
       }
-      phases ^= 1u << slot;
-    }
-    __syncwarp();
-    const uint32_t kc = codes + slot * 2 * F::kCodes, vc = kc + F::kCodes;
-    const uint32_t ks = scales + slot * 2 * F::kScales, vs = ks + F::kScales;
-    advance(fill);
-    fill = fill + 1 == F::kStages ? 0 : fill + 1;
+      __syncwarp();
+      const uint32_t kc = codes + slot * 2 * F::kCodes, vc = kc + F::kCodes;
+      const uint32_t ks = scales + slot * 2 * F::kScales, vs = ks + F::kScales;
+      advance(fill);
+      fill = fill + 1 == F::kStages ? 0 : fill + 1;
+      slot = slot + 1 == F::kStages ? 0 : slot + 1;
+      if (!here) continue;
 
-    if (here) {
       const bool tail = tw + F::kTok > min_lim;
       const int end_row = cur.r.kv - tw;
       float t[TILES][4];
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
-        few_qk<D>(kc, ks, 16 * i + g, qd, qf, t[i]);
-        t[i][0] *= cf0;
-        t[i][1] *= cf1;
-        t[i][2] *= cf0;
-        t[i][3] *= cf1;
-      }
+      for (int i = 0; i < TILES; ++i) few_qk<D>(kc, ks, 16 * i + g, qd, qf, t[i]);
       if (tail) {
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
@@ -460,23 +488,27 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       few_v_load<D>(vc, vs, 2 * qd, g, tail, end_row, va);
       few_v_load<D>(vc, vs, 2 * qd + 16, g, tail, end_row, vb);
 
+      // The maxima move only when some score exceeds its reference by 2^8: one
+      // vote a unit, and the reduction over the lanes only then.
       float mx0 = fmaxf(t[0][0], t[0][2]), mx1 = fmaxf(t[0][1], t[0][3]);
 #pragma unroll
       for (int i = 1; i < TILES; ++i) {
         mx0 = fmaxf(mx0, fmaxf(t[i][0], t[i][2]));
         mx1 = fmaxf(mx1, fmaxf(t[i][1], t[i][3]));
       }
+      if (__any_sync(kFull, mx0 > top0 || mx1 > top1)) {
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        mx0 = fmaxf(mx0, shfl_xor(mx0, off));
-        mx1 = fmaxf(mx1, shfl_xor(mx1, off));
-      }
-      if (__any_sync(kFull, (mx0 > m0 + kLazy) || (mx1 > m1 + kLazy))) {
-        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        for (int off = 4; off < 32; off <<= 1) {
+          mx0 = fmaxf(mx0, shfl_xor(mx0, off));
+          mx1 = fmaxf(mx1, shfl_xor(mx1, off));
+        }
+        const float n0 = fmaxf(m0, mx0 * cf0), n1 = fmaxf(m1, mx1 * cf1);
         const float a0 = (n0 == -CUDART_INF_F) ? 1.f : exp2_approx(m0 - n0);
         const float a1 = (n1 == -CUDART_INF_F) ? 1.f : exp2_approx(m1 - n1);
         m0 = n0;
         m1 = n1;
+        top0 = (m0 + kLazy) / cf0;
+        top1 = (m1 + kLazy) / cf1;
         l0 *= a0;
         l1 *= a1;
 #pragma unroll
@@ -492,10 +524,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       PFrag pf[TILES];
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        t[i][0] = exp2_approx(t[i][0] - mu0);
-        t[i][1] = exp2_approx(t[i][1] - mu1);
-        t[i][2] = exp2_approx(t[i][2] - mu0);
-        t[i][3] = exp2_approx(t[i][3] - mu1);
+        t[i][0] = exp2_approx(fmaf(t[i][0], cf0, -mu0));
+        t[i][1] = exp2_approx(fmaf(t[i][1], cf1, -mu1));
+        t[i][2] = exp2_approx(fmaf(t[i][2], cf0, -mu0));
+        t[i][3] = exp2_approx(fmaf(t[i][3], cf1, -mu1));
         l0 += t[i][0] + t[i][2];
         l1 += t[i][1] + t[i][3];
         pf[i] = p_fragments(t[i][0], t[i][1], t[i][2], t[i][3]);
@@ -509,14 +541,12 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       }
     }
 
-    FewWalk nxt = cur;
-    nxt.next(p);
-    const bool last = nxt.at(end);
-    if (nxt.page == 0 || last) {  // ------------------------------ item's end
+    {  // ---------------------------------------------------- the item's end
       constexpr int kPitch = F::kStages * 2 * F::kCodes;
-      uint8_t* area = sgen + slot * 2 * F::kCodes;  // of warp 0
+      const int used = fill;  // the slot that the last unit left (the next copy's)
+      uint8_t* area = sgen + used * 2 * F::kCodes;  // of warp 0
       auto ml_of = [&](int w) {
-        return reinterpret_cast<float2*>(sgen + F::kRing + (w * F::kStages + slot) * 2 * F::kScales);
+        return reinterpret_cast<float2*>(sgen + F::kRing + (w * F::kStages + used) * 2 * F::kScales);
       };
       float4* red = reinterpret_cast<float4*>(area + warp * kPitch);
 #pragma unroll
@@ -531,9 +561,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         ml_of(warp)[2 * qd] = make_float2(m0, l0);
         ml_of(warp)[2 * qd + 1] = make_float2(m1, l1);
       }
-      const bool starts_here = first_page == 0, ends_here = cur.page + 1 == cur.pages;
+      const bool starts_here = first_unit == 0, ends_here = cur.b != end_b;
       const bool whole = starts_here && ends_here;
-      float* rec = p.records + (size_t)(blockIdx.x * 2 + (starts_here ? 1 : 0)) * (kFewCols * (D + 2));
+      float* rec = p.records + (size_t)(cta * 2 + (starts_here ? 1 : 0)) * (kFewCols * (D + 2));
       __syncthreads();
       // the lane's two columns: weights of the warps
       float w0[F::kWarps], w1[F::kWarps], M0 = -CUDART_INF_F, M1 = -CUDART_INF_F, L0 = 0.f, L1 = 0.f;
@@ -578,7 +608,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
           const float x = e ? a.y : a.x, y = e ? a.w : a.z, inv = e ? i1 : i0;
           if (whole) {
             T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + c / p.group) * p.out_stride +
-                     (cur.head * p.group + c % p.group) * D + d;
+                     (hd * p.group + c % p.group) * D + d;
             const T h[2] = {InTraits<T>::from_float(x * inv), InTraits<T>::from_float(y * inv)};
             *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
           } else {
@@ -587,26 +617,24 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         }
       }
       if (starts_here && !ends_here && tid == 0) {  // the rest of the item is the next CTAs'
-        const long long last_unit = cur.base + FewWalk::kOver + cur.pages - 1;
+        const long long last_unit = cur.base + Walk::kOver + cur.units - 1;
         meta[0] = cols;
         meta[1] = cur.r.row0;
-        meta[3] = cur.head;
-        meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
-        meta[5] = (int)min(total, n_cta);  // fewer units than CTAs leave some CTAs without a record
+        meta[4] = (int)(((last_unit + 1) * splits - 1) / total);
+        meta[5] = (int)min(total, splits);  // fewer units than splits leave some without a record
       }
       __syncthreads();
-      fresh = true;
     }
-    if (last) break;
-    cur = nxt;
-    slot = slot + 1 == F::kStages ? 0 : slot + 1;
+    if (cur.b == end_b) break;
+    cur.next_request(p);
+    if (cur.b == p.requests || (cur.b == end_b && end_unit == 0)) break;
   }
   griddep_launch_dependents();
 }
 
-// Merges the records of the items that more than one CTA worked on, CTA by
-// CTA in order: block (i, y) takes columns y, y + gridDim.y, ... of the item
-// that CTA i began and did not finish.
+// Merges the records of the items that more than one CTA worked on, in the
+// order of the splits: block (head, split, y) takes columns y, y + gridDim.z,
+// ... of the item that this split began and did not finish.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
@@ -615,21 +643,20 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
   __shared__ float4 acc_s[kGroups][kLanes];
   griddep_wait();
   griddep_launch_dependents();
-  const int tid = threadIdx.x, i0 = blockIdx.x, n_cta = gridDim.x;
-  const int32_t* meta = p.meta + i0 * kBatchMeta;
+  const int tid = threadIdx.x, hd = blockIdx.x, heads = gridDim.x, i0 = blockIdx.y;
+  const long long splits = gridDim.y;
+  const int32_t* meta = p.meta + (i0 * heads + hd) * kBatchMeta;
   const int cols = __ldcg(meta);
   if (cols == 0) return;
-  const int row0 = __ldcg(meta + 1), hd = __ldcg(meta + 3), last = __ldcg(meta + 4);
-  const int busy = __ldcg(meta + 5);
-  const int parts = last - i0 + 1;
+  const int row0 = __ldcg(meta + 1), parts = __ldcg(meta + 4) - i0 + 1, busy = __ldcg(meta + 5);
   constexpr size_t kRec = (size_t)kFewCols * (D + 2);
-  // CTA i0 left its part in record 1, the later ones in record 0
-  auto record = [&](int j) { return p.records + (size_t)((i0 + j) * 2 + (j == 0 ? 1 : 0)) * kRec; };
+  // split i0 left its part in record 1, the later ones in record 0
+  auto record = [&](int j) { return p.records + (size_t)(((i0 + j) * heads + hd) * 2 + (j == 0 ? 1 : 0)) * kRec; };
   auto empty = [&](int j) {
     const long long i = i0 + j;
-    return i * busy / n_cta == (i + 1) * busy / n_cta;
+    return i * busy / splits == (i + 1) * busy / splits;
   };
-  for (int c = blockIdx.y; c < cols; c += gridDim.y) {
+  for (int c = blockIdx.z; c < cols; c += gridDim.z) {
     auto stat = [&](int j) { return __ldcg(reinterpret_cast<const float2*>(record(j) + kFewCols * D + 2 * c)); };
     float M = -CUDART_INF_F;
     for (int j = tid; j < parts; j += 256)
@@ -700,13 +727,15 @@ namespace {
 template <typename T, int D>
 cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int sms, cudaStream_t stream) {
   using F = Few<D>;
-  const int ctas = sms * F::kCtas;
+  // the heads of a token range run side by side: their slices of a token row
+  // share DRAM pages and sectors
+  const dim3 grid(p.kv_heads, max(1, sms * F::kCtas / p.kv_heads));
   auto kernel = batch_few_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(ctas), dim3(F::kThreads), F::kSmem, stream, p, maps);
+  e = launch_pdl(kernel, grid, dim3(F::kThreads), F::kSmem, stream, p, maps);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(batch_combine_kernel<T, D>, dim3(ctas, kFewCols), dim3(256), 0, stream, p);
+  e = launch_pdl(batch_combine_kernel<T, D>, dim3(grid.x, grid.y, kFewCols), dim3(256), 0, stream, p);
   if (e != cudaSuccess || (long long)p.max_rows * p.group <= p.few_cols) return e;
   return launch_rows<T, D>(p, sms, stream);
 }

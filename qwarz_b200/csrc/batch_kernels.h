@@ -90,10 +90,13 @@ struct LogprobParams {
   int32_t* top_ids;              // [rows, top]
   void* workspace;               // [rows, chunks] records
   long long stride;
-  int rows, vocab, top, chunks, ids64;
+  int rows, vocab, top;
+  int chunks, chunk_tiles;       // parts of a row, tiles of a part
+  int ids64;
 };
 enum : int { kDtypeF32 = 2 };    // logits only
-int logprob_chunks(int vocab, int itemsize);
+void logprob_parts(int rows, int vocab, int itemsize, int* parts, int* tiles_each);
+long long logprob_records(int rows, int vocab, int itemsize);
 size_t logprob_record_bytes(int top);
 cudaError_t launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t stream);
 
