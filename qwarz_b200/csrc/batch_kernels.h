@@ -88,17 +88,16 @@ struct LogprobParams {
   float* entropy;                // [rows]
   float* top_logprobs;           // [rows, top]
   int32_t* top_ids;              // [rows, top]
-  void* workspace;               // [rows, chunks] records
+  void* workspace;               // records of parts of rows
   long long stride;
   int rows, vocab, top;
-  int chunks, chunk_tiles;       // parts of a row, tiles of a part
   int ids64;
+  int row_tiles, ctas;           // set by the launch: tiles of a row, CTAs of the first kernel
 };
 enum : int { kDtypeF32 = 2 };    // logits only
-void logprob_parts(int rows, int vocab, int itemsize, int* parts, int* tiles_each);
-long long logprob_records(int rows, int vocab, int itemsize);
+long long logprob_records(int rows);
 size_t logprob_record_bytes(int top);
-cudaError_t launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t stream);
+cudaError_t launch_token_logprobs(LogprobParams p, int dtype, int sms, cudaStream_t stream);
 
 cudaError_t launch_batch_tables(const BatchTablesParams& p, int sms, cudaStream_t stream);
 cudaError_t launch_batch_append(const BatchAppendParams& p, int dtype, cudaStream_t stream);

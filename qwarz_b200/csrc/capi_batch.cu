@@ -164,7 +164,7 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
 
 int64_t qwz_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top, int32_t dtype) {
   if (rows < 0 || vocab < 1 || vocab > (1 << 30) || top < 0 || top > 32 || dtype < 0 || dtype > QWZ_DTYPE_F32) return 0;
-  return qwz::logprob_records(rows, vocab, dtype == QWZ_DTYPE_F32 ? 4 : 2) * (int64_t)qwz::logprob_record_bytes(top);
+  return qwz::logprob_records(rows) * (int64_t)qwz::logprob_record_bytes(top);
 }
 
 int qwz_token_logprobs(const void* logits, const void* ids, int32_t ids64, float* logprob, float* entropy,
@@ -184,12 +184,11 @@ int qwz_token_logprobs(const void* logits, const void* ids, int32_t ids64, float
   if (!workspace || !aligned(workspace, 16)) return fail(QWZ_EINVAL, "workspace must be a non-null 16-byte aligned pointer");
   if (workspace_bytes < qwz_token_logprobs_workspace_bytes(rows, vocab, top, dtype))
     return fail(QWZ_EINVAL, "workspace smaller than qwz_token_logprobs_workspace_bytes");
-  int parts, tiles;
-  qwz::logprob_parts(rows, vocab, item, &parts, &tiles);
-  qwz::LogprobParams p{logits, ids, logprob, entropy, top_logprobs, top_ids, workspace, stride, rows, vocab, top,
-                       parts, tiles, ids64};
-  if ((int64_t)rows * p.chunks > 0x7fffffff) return fail(QWZ_EINVAL, "rows x vocab too large for one call");
-  return launched(qwz::launch_token_logprobs(p, dtype, as_stream(stream)), "qwz_token_logprobs");
+  const int sms = batch_sms();
+  if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
+  qwz::LogprobParams p{logits, ids, logprob, entropy, top_logprobs, top_ids, workspace, stride, rows, vocab, top, ids64,
+                       0, 0};
+  return launched(qwz::launch_token_logprobs(p, dtype, sms, as_stream(stream)), "qwz_token_logprobs");
 }
 
 }  // extern "C"

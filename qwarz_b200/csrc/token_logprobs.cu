@@ -1,9 +1,11 @@
 // Log probabilities of given tokens, entropy and the top alternatives of rows
 // of logits (sm_100a): what a verify step or a sampler takes from the logits
 // that follow the attention.  For a row x of V logits, M = max x:
-//   s = sum e^(x - M),  t = sum (x - M) e^(x - M)
-//   log p(id) = (x_id - M) - ln s,  H = ln s - t / s,
-//   top K by (value, then lowest index).
+//   a_i = x_i log2 e - R,  s = sum 2^a,  t = sum a 2^a
+//   log p(id) = ln 2 (a_id - log2 s),  H = ln 2 (log2 s - t / s),
+//   top K by (value, then lowest index),
+// R being near the maximum in base-2 units: each a is one fused multiply-add of
+// the same R, so R's own rounding cancels.
 //
 // One pass over the logits; bound by HBM (and, for 16-bit logits, by the
 // exponentials: 16 a cycle and SM allow 1.4 times the rate at which the logits
@@ -32,8 +34,10 @@ constexpr int kLpThreads = 256;
 constexpr int kLpVecs = 4;                              // 16-byte loads of a tile a thread
 constexpr int kLpTileVecs = kLpThreads * kLpVecs;       // 16 KB
 constexpr int kLpCand = 1024;                           // candidates ranked by counting
-constexpr int kLpParts = 16 * 148;                      // parts of all rows that a launch aims at
-constexpr float kLpMove = 8.f;                          // a thread's reference moves past this
+constexpr int kLpCtasPerSm = 4;
+constexpr int kLpMaxCtas = 4 * 256;
+constexpr int kLpAgain = 4;                             // a long part's tau is made again after this tile
+constexpr float kLpMove = 8.f;                          // a thread's reference moves past this (base 2)
 constexpr int kLpMergeCand = 1024;
 
 template <typename T>
@@ -101,16 +105,7 @@ QWZ_DEVINL float max_nan(float a, float b) {  // NaN wins
 }
 
 constexpr float kLog2eF = 1.4426950408889634f;
-
-// (d0, d1) += (a0, a1) * (b0, b1)
-QWZ_DEVINL void lp_ffma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
-  uint64_t d;
-  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%1, %2};\n mov.b64 b, {%3, %4};\n mov.b64 c, {%5, %6};\n"
-      " fma.rn.f32x2 %0, a, b, c;\n}\n"
-      : "=l"(d)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(d0), "f"(d1));
-  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(d0), "=f"(d1) : "l"(d));
-}
+constexpr float kLn2F = 0.6931471805599453f;
 
 // Bytes of one chunk's record: m, s, t, (pad), K keys.
 QWZ_DEVINL size_t lp_record(int top) { return 16 + 8 * (size_t)top; }
@@ -146,20 +141,32 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
   __shared__ float tau_s;
   __shared__ int n_cand;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int row = blockIdx.x / p.chunks, part = blockIdx.x % p.chunks;
   const int K = p.top;
   griddep_wait();
+  // this CTA's tiles of the concatenation of all rows' tiles
+  const long long total = (long long)p.rows * p.row_tiles;
+  long long at = (long long)blockIdx.x * total / gridDim.x;
+  const long long stop = ((long long)blockIdx.x + 1) * total / gridDim.x;
+  while (at < stop) {  // a part: tiles of one row
+  const int row = (int)(at / p.row_tiles), tile0 = (int)(at % p.row_tiles);
+  const int tiles = (int)min(stop - at, (long long)(p.row_tiles - tile0));
+  at += tiles;
 
   const T* x0 = reinterpret_cast<const T*>(p.logits) + (long long)row * p.stride;
   const int skew = (int)((reinterpret_cast<uintptr_t>(x0) / sizeof(T)) % E);  // elements past a 16-byte boundary
-  const int v0 = part * p.chunk_tiles * kLpTileVecs;
-  const int vecs = (p.vocab + skew + E - 1) / E;
-  const int tiles = max(0, min(p.chunk_tiles, (vecs - v0 + kLpTileVecs - 1) / kLpTileVecs));
+  const int v0 = tile0 * kLpTileVecs;
   // places of the part
-  const int first = max(0, v0 * E - skew), last_pos = min(p.vocab, (v0 + p.chunk_tiles * kLpTileVecs) * E - skew);
+  const int first = max(0, v0 * E - skew), last_pos = min(p.vocab, (v0 + tiles * kLpTileVecs) * E - skew);
 
   // this thread's vectors of a tile, absent places as -inf
   auto load = [&](int tile, uint4(&raw)[kLpVecs]) {
+    const int begin = (v0 + tile * kLpTileVecs) * E - skew;
+    if (begin >= 0 && begin + kLpTileVecs * E <= p.vocab) {  // wholly inside the row
+      const uint4* src = reinterpret_cast<const uint4*>(x0 + begin) + tid;
+#pragma unroll
+      for (int i = 0; i < kLpVecs; ++i) raw[i] = __ldg(src + i * kLpThreads);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLpVecs; ++i) {
       const int pos = (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew;
@@ -197,54 +204,76 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
     if ((lane & 3) == 0) gmax[tid >> 2] = v;
-    if (tid == 0) n_cand = 0;
     __syncthreads();
     if (warp == 0) lp_kth(gmax, K, lane, &tau_s);
     __syncthreads();
     return tau_s;
   };
-  // Candidates of a vector: at or above tau; where tau is -inf (fewer than K
-  // groups hold anything above it), all that is above -inf and the first K
-  // places (the lowest indices).
-  auto collect = [&](const uint4& v, int pos, float tau) {
-    float x[E];
-    L::unpack(v, x);
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const bool take = tau == -CUDART_INF_F ? x[j] > -CUDART_INF_F || pos + j < first + K : x[j] >= tau;
-      if (take && pos + j >= first && pos + j < last_pos) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at < kLpCand) cand[at] = lp_key(x[j], (uint32_t)(pos + j));
+  // Candidates: at or above tau; where tau is -inf (fewer than K groups hold
+  // anything above it), all that is above -inf and the first K places (the lowest
+  // indices).  Vectors that hold any are rare, so the warp takes them one by one,
+  // a lane an element, which reads it again (from L1).
+  auto wanted = [&](float vmax, int pos, float tau) {
+    return tau == -CUDART_INF_F ? vmax > tau || pos < first + K : vmax >= tau;
+  };
+  auto collect = [&](int tile, unsigned mine, float tau) {  // mine: bit i = this lane's vector i
+    unsigned any = __ballot_sync(0xffffffffu, mine != 0u);
+    while (any) {
+      const int src = __ffs(any) - 1;
+      any &= any - 1;
+      unsigned h = __shfl_sync(0xffffffffu, mine, src);
+      while (h) {
+        const int i = __ffs(h) - 1;
+        h &= h - 1;
+        const int pos = (v0 + tile * kLpTileVecs + i * kLpThreads + warp * 32 + src) * E - skew + lane;
+        if (lane < E && pos >= first && pos < last_pos) {
+          const float x = L::one(x0 + pos);
+          if (wanted(x, pos, tau)) {
+            const int at = atomicAdd(&n_cand, 1);
+            if (at < kLpCand) cand[at] = lp_key(x, (uint32_t)pos);
+          }
+        }
       }
     }
   };
 
-  uint4 raw[kLpVecs];
-  load(0, raw);
+  uint4 raw[kLpVecs], cur[kLpVecs];
+  load(0, cur);
+  if (tiles > 1) load(1, raw);
   float r = -CUDART_INF_F, tmax = -CUDART_INF_F, tau = CUDART_INF_F;
   if (K > 0) {
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) tmax = fmaxf(tmax, vec_max(raw[i]));
+    for (int i = 0; i < kLpVecs; ++i) {
+      tmax = fmaxf(tmax, vec_max(cur[i]));
+      if (tiles > 1) tmax = fmaxf(tmax, vec_max(raw[i]));
+    }
+    if (tid == 0) n_cand = 0;
     tau = threshold(tmax);
   }
-  float s = 0.f, t = 0.f, s1 = 0.f, t1 = 0.f;
+  float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};  // two chains each
   for (int tile = 0; tile < tiles; ++tile) {
-    uint4 cur[kLpVecs];
     float vm[kLpVecs], m = -CUDART_INF_F;
+    if (tile > 0) {
 #pragma unroll
-    for (int i = 0; i < kLpVecs; ++i) cur[i] = raw[i];
-    if (tile + 1 < tiles) load(tile + 1, raw);
+      for (int i = 0; i < kLpVecs; ++i) cur[i] = raw[i];
+      if (tile + 1 < tiles) load(tile + 1, raw);
+    }
 #pragma unroll
     for (int i = 0; i < kLpVecs; ++i) {
       vm[i] = vec_max(cur[i]);
       m = fmaxf(m, vm[i]);
     }
-    if (m > r + kLpMove || (r == -CUDART_INF_F && m > r)) {  // a new reference
-      const float d = r - m, w = r == -CUDART_INF_F ? 0.f : exp2_approx(d * kLog2eF);
-      t = r == -CUDART_INF_F ? t : w * (t + t1 + d * (s + s1));  // (sums without a reference are 0 or NaN)
-      s = r == -CUDART_INF_F ? s : w * (s + s1);
-      s1 = t1 = 0.f;
-      r = m;
+    const float m2 = m * kLog2eF;
+    if (m2 > r + kLpMove || (r == -CUDART_INF_F && m2 > r)) {  // a new reference
+      if (r != -CUDART_INF_F) {  // (sums without a reference are 0 or NaN)
+        const float d = r - m2, w = exp2_approx(d);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          t[e] = w * fmaf(d, s[e], t[e]);
+          s[e] *= w;
+        }
+      }
+      r = m2;
     }
     tmax = fmaxf(tmax, m);
     const float mu = r == -CUDART_INF_F ? 0.f : r;
@@ -253,32 +282,25 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       float x[E];
       L::unpack(cur[i], x);
 #pragma unroll
-      for (int j = 0; j < E; j += 2) {  // packed FP32 pairs
-        pf_fadd2(x[j], x[j + 1], -mu, -mu);
-        const float d0 = max_nan(x[j], -1000.f), d1 = max_nan(x[j + 1], -1000.f);  // -inf: e = 0 and d e = 0
-        float e0, e1;
-        pf_ffma2(e0, e1, d0, d1, kLog2eF, 0.f);
-        e0 = exp2_approx(e0);
-        e1 = exp2_approx(e1);
-        pf_fadd2(s, s1, e0, e1);
-        lp_ffma2(t, t1, d0, d1, e0, e1);
+      for (int j = 0; j < E; ++j) {
+        const float a = max_nan(fmaf(x[j], kLog2eF, -mu), -2000.f);  // -inf: e = 0 and a e = 0
+        const float e = exp2_approx(a);
+        s[j & 1] += e;
+        t[j & 1] = fmaf(a, e, t[j & 1]);
       }
     }
-    if (K > 0 && (m >= tau || tau == -CUDART_INF_F)) {
-#pragma unroll 1
-      for (int i = 0; i < kLpVecs; ++i) {
-        const uint4 v = i == 0 ? cur[0] : i == 1 ? cur[1] : i == 2 ? cur[2] : cur[3];
-        const float best_of = i == 0 ? vm[0] : i == 1 ? vm[1] : i == 2 ? vm[2] : vm[3];
-        if (best_of >= tau || tau == -CUDART_INF_F)
-          collect(v, (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau);
-      }
+    if (K > 0) {
+      unsigned mine = 0;
+#pragma unroll
+      for (int i = 0; i < kLpVecs; ++i)
+        if (wanted(vm[i], (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau)) mine |= 1u << i;
+      collect(tile, mine, tau);
+      if (tile == kLpAgain && tiles > 2 * kLpAgain) tau = fmaxf(tau, threshold(tmax));
     }
   }
-  s += s1;
-  t += t1;
 
-  // the part's maximum, and the threads' sums relative to it
-  float M = r;
+  // the part's reference, and the threads' sums relative to it
+  float M = r, sum = s[0] + s[1], tsum = t[0] + t[1];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if (lane == 0) red[0][warp] = M;
@@ -287,49 +309,69 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
 #pragma unroll
   for (int i = 1; i < kLpThreads / 32; ++i) M = fmaxf(M, red[0][i]);
   if (r != -CUDART_INF_F) {
-    const float d = r - M, w = exp2_approx(d * kLog2eF);
-    t = w * (t + d * s);
-    s = w * s;
+    const float d = r - M, w = exp2_approx(d);
+    tsum = w > 0.f ? w * fmaf(d, sum, tsum) : 0.f;
+    sum *= w;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    t += __shfl_xor_sync(0xffffffffu, t, o);
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    tsum += __shfl_xor_sync(0xffffffffu, tsum, o);
   }
   if (lane == 0) {
-    red[1][warp] = s;
-    red[2][warp] = t;
+    red[1][warp] = sum;
+    red[2][warp] = tsum;
   }
   __syncthreads();
-  uint8_t* rec = reinterpret_cast<uint8_t*>(p.workspace) + ((size_t)row * p.chunks + part) * lp_record(K);
+  // (CTA + row) numbers the parts of the launch without gaps within a row
+  uint8_t* rec = reinterpret_cast<uint8_t*>(p.workspace) + ((size_t)blockIdx.x + row) * lp_record(K);
   if (tid == 0) {
-    s = t = 0.f;
+    sum = tsum = 0.f;
 #pragma unroll
     for (int i = 0; i < kLpThreads / 32; ++i) {
-      s += red[1][i];
-      t += red[2][i];
+      sum += red[1][i];
+      tsum += red[2][i];
     }
     float* f = reinterpret_cast<float*>(rec);
     f[0] = M;
-    f[1] = s;
-    f[2] = t;
+    f[1] = sum;
+    f[2] = tsum;
   }
   if (K > 0) {
-    if (n_cand > kLpCand) {  // (the same for all threads: the list is complete)
+    // The whole part's maxima give a closer bound, which most of the list does
+    // not reach; a list that overflowed is made again with it.
+    int n = n_cand;
+    tau = threshold(tmax);
+    if (n > kLpCand) {
+      if (tid == 0) n_cand = 0;
       __syncthreads();
-      tau = threshold(tmax);
 #pragma unroll 1
       for (int tile = 0; tile < tiles; ++tile) {
         load(tile, raw);
-#pragma unroll 1
-        for (int i = 0; i < kLpVecs; ++i) {
-          const uint4 v = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
-          collect(v, (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau);
-        }
+        unsigned mine = 0;
+#pragma unroll
+        for (int i = 0; i < kLpVecs; ++i)
+          if (wanted(vec_max(raw[i]), (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau)) mine |= 1u << i;
+        collect(tile, mine, tau);
       }
       __syncthreads();
+      n = n_cand;
+    } else if (tau > -CUDART_INF_F) {
+      const unsigned long long least = lp_key(tau, 0xffffffffu);
+      unsigned long long mine[kLpCand / kLpThreads];
+#pragma unroll
+      for (int i = 0; i < kLpCand / kLpThreads; ++i) {
+        const int at = i * kLpThreads + tid;
+        mine[i] = at < n ? cand[at] : 0ull;
+      }
+      if (tid == 0) n_cand = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kLpCand / kLpThreads; ++i)
+        if (mine[i] >= least) cand[atomicAdd(&n_cand, 1)] = mine[i];
+      __syncthreads();
+      n = n_cand;
     }
-    const int n = n_cand;
     unsigned long long* keys = reinterpret_cast<unsigned long long*>(rec + 16);
     if (n <= kLpCand) {
       for (int c = tid; c < max(n, K); c += kLpThreads) {
@@ -362,6 +404,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       }
     }
   }
+  __syncthreads();  // the next part's list takes the place of this one's
+  }
   griddep_launch_dependents();
 }
 
@@ -374,11 +418,15 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
   const int K = p.top;
   griddep_wait();
   griddep_launch_dependents();
-  const uint8_t* recs = reinterpret_cast<const uint8_t*>(p.workspace) + (size_t)row * p.chunks * lp_record(K);
+  // the parts of this row: those of CTAs c0 .. c1
+  const long long total = (long long)p.rows * p.row_tiles, t0 = (long long)row * p.row_tiles, t1 = t0 + p.row_tiles - 1;
+  const int c0 = (int)(((t0 + 1) * p.ctas - 1) / total), c1 = (int)(((t1 + 1) * p.ctas - 1) / total);
+  const int parts = c1 - c0 + 1;
+  const uint8_t* recs = reinterpret_cast<const uint8_t*>(p.workspace) + ((size_t)c0 + row) * lp_record(K);
   auto stat = [&](int c) { return reinterpret_cast<const float*>(recs + c * lp_record(K)); };
 
   float M = -CUDART_INF_F;
-  for (int c = tid; c < p.chunks; c += kLpThreads) M = fmaxf(M, __ldcg(stat(c)));
+  for (int c = tid; c < parts; c += kLpThreads) M = fmaxf(M, __ldcg(stat(c)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if (lane == 0) red[0][warp] = M;
@@ -388,13 +436,13 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
   for (int i = 1; i < kLpThreads / 32; ++i) M = fmaxf(M, red[0][i]);
   __syncthreads();
   float s = 0.f, t = 0.f;
-  for (int c = tid; c < p.chunks; c += kLpThreads) {
+  for (int c = tid; c < parts; c += kLpThreads) {
     const float m = __ldcg(stat(c)), sc = __ldcg(stat(c) + 1), tc = __ldcg(stat(c) + 2);
     if (m == -CUDART_INF_F) {
       s += sc;  // 0, or NaN
       continue;
     }
-    const float d = m - M, w = exp2_approx(d * kLog2eF);
+    const float d = m - M, w = exp2_approx(d);
     s += w * sc;
     t += w > 0.f ? w * (tc + d * sc) : 0.f;
   }
@@ -414,12 +462,12 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
     s += red[0][i];
     t += red[1][i];
   }
-  const float ln_s = logf(s);
+  const float log2_s = log2f(s);
   const bool none = M == -CUDART_INF_F && s == 0.f;  // no token is possible
-  auto logprob = [&](float x) { return none ? (x != x ? x : -CUDART_INF_F) : (x - M) - ln_s; };
+  auto logprob = [&](float x) { return none ? (x != x ? x : -CUDART_INF_F) : kLn2F * (fmaf(x, kLog2eF, -M) - log2_s); };
 
   if (tid == 0) {
-    p.entropy[row] = none ? 0.f : ln_s - t / s;
+    p.entropy[row] = none ? 0.f : kLn2F * (log2_s - t / s);
     const long long id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + row)
                                  : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + row);
     float lp = 0.f;  // id < 0: no token
@@ -436,11 +484,11 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
   // the best K so far, then as many chunks' lists as fit beside them
   int have = 0;
   const int lists = (kLpMergeCand - 32) / K;
-  for (int c0 = 0; c0 < p.chunks; c0 += lists) {
-    const int n_lists = min(lists, p.chunks - c0), n = have + n_lists * K;
+  for (int l0 = 0; l0 < parts; l0 += lists) {
+    const int n_lists = min(lists, parts - l0), n = have + n_lists * K;
     if (tid < have) cand[tid] = sorted[tid];
     for (int i = tid; i < n_lists * K; i += kLpThreads)
-      cand[have + i] = __ldcg(reinterpret_cast<const unsigned long long*>(recs + (c0 + i / K) * lp_record(K) + 16) + i % K);
+      cand[have + i] = __ldcg(reinterpret_cast<const unsigned long long*>(recs + (l0 + i / K) * lp_record(K) + 16) + i % K);
     __syncthreads();
     if (tid < K) sorted[tid] = 0ull;
     __syncthreads();
@@ -471,19 +519,9 @@ int lp_tiles(int vocab, int itemsize) {
 
 }  // namespace
 
-// Parts of a row: about kLpParts of all rows (16 an SM, four rounds of the
-// resident CTAs: 448 rows of 151,000 take five of four tiles), a tile at least.
-void logprob_parts(int rows, int vocab, int itemsize, int* parts, int* tiles_each) {
-  const int tiles = lp_tiles(vocab, itemsize);
-  const int want = max(1, min(tiles, (kLpParts + rows - 1) / max(rows, 1)));
-  *tiles_each = (tiles + want - 1) / want;
-  *parts = (tiles + *tiles_each - 1) / *tiles_each;
-}
-
-// Records that any call of up to `rows` rows needs.
-long long logprob_records(int rows, int vocab, int itemsize) {
-  return min((long long)rows * lp_tiles(vocab, itemsize), (long long)kLpParts + rows);
-}
+// Records that any call of up to `rows` rows needs: a part begins with a CTA or
+// with a row.
+long long logprob_records(int rows) { return (long long)kLpMaxCtas + rows; }
 
 size_t logprob_record_bytes(int top) { return 16 + 8 * (size_t)top; }
 
@@ -491,15 +529,17 @@ namespace {
 
 template <typename T>
 cudaError_t launch_lp(const LogprobParams& p, cudaStream_t stream) {
-  cudaError_t e = launch_pdl(lp_part_kernel<T>, dim3((unsigned)p.chunks * p.rows), dim3(kLpThreads), 0, stream, p);
+  cudaError_t e = launch_pdl(lp_part_kernel<T>, dim3(p.ctas), dim3(kLpThreads), 0, stream, p);
   if (e != cudaSuccess) return e;
   return launch_pdl(lp_merge_kernel<T>, dim3(p.rows), dim3(kLpThreads), 0, stream, p);
 }
 
 }  // namespace
 
-cudaError_t launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t stream) {
+cudaError_t launch_token_logprobs(LogprobParams p, int dtype, int sms, cudaStream_t stream) {
   if (p.rows <= 0) return cudaSuccess;
+  p.row_tiles = lp_tiles(p.vocab, dtype == kDtypeF32 ? 4 : 2);
+  p.ctas = (int)min((long long)p.rows * p.row_tiles, (long long)min(kLpMaxCtas, sms * kLpCtasPerSm));
   switch (dtype) {
     case kDtypeF16: return launch_lp<__half>(p, stream);
     case kDtypeBF16: return launch_lp<__nv_bfloat16>(p, stream);

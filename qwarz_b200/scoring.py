@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _contig, _cuda, _p, _stream
+from .batch import _device, _raw_stream
 
 _CODES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 MAX_TOP = 32
@@ -32,24 +32,31 @@ def token_logprobs(logits, ids, logprob, entropy, top_logprobs, top_ids, workspa
     Writes logprob [T] = log p(ids), entropy [T] (nats) and, for top_logprobs /
     top_ids [T, K] (FP32 / int32, K 0 to 32), the K most likely tokens, equal
     logits by lowest index.  ids < 0 gives 0; -inf logits are impossible tokens."""
-    dev = _cuda(logits, ids, logprob, entropy, top_logprobs, top_ids, workspace)
-    if logits.dim() != 2 or logits.dtype not in _CODES or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError("logits must be float16, bfloat16 or float32 [rows, vocab] with contiguous rows")
+    dev = _device(logits, (ids, logprob, entropy, top_logprobs, top_ids, workspace))
+    code = _CODES.get(logits.dtype)
+    if logits.dim() != 2 or code is None:
+        raise ValueError("logits must be float16, bfloat16 or float32 [rows, vocab]")
     T, V = logits.shape
-    if ids.dtype not in (torch.int32, torch.int64) or ids.numel() != T:
+    stride, one = logits.stride()
+    if one != 1 and V > 1:
+        raise ValueError("logits must have contiguous rows")
+    if ids.dtype not in (torch.int64, torch.int32) or ids.numel() != T:
         raise ValueError("ids must be int32 or int64, one per row")
-    if top_ids.dim() != 2 or top_ids.shape[0] != T or top_logprobs.shape != top_ids.shape:
+    K = top_ids.shape[-1]
+    if top_ids.shape != (T, K) or top_logprobs.shape != (T, K):
         raise ValueError("top_logprobs and top_ids must be [rows, K]")
     if logprob.numel() != T or entropy.numel() != T:
         raise ValueError("logprob and entropy must have one entry per row")
-    if logprob.dtype != torch.float32 or entropy.dtype != torch.float32 or top_logprobs.dtype != torch.float32 \
-            or top_ids.dtype != torch.int32:
+    f32 = torch.float32
+    if logprob.dtype is not f32 or entropy.dtype is not f32 or top_logprobs.dtype is not f32 \
+            or top_ids.dtype is not torch.int32:
         raise ValueError("logprob, entropy and top_logprobs must be float32, top_ids int32")
-    for name, t in (("ids", ids), ("logprob", logprob), ("entropy", entropy), ("top_logprobs", top_logprobs),
-                    ("top_ids", top_ids), ("workspace", workspace)):
-        _contig(name, t)
-    lib = _lib.load()
-    _lib.check(lib.qwz_token_logprobs(
-        _p(logits), _p(ids), int(ids.dtype == torch.int64), _p(logprob), _p(entropy), _p(top_logprobs), _p(top_ids),
-        _p(workspace), workspace.numel() * workspace.element_size(), T, V, top_ids.shape[1], logits.stride(0),
-        _CODES[logits.dtype], _stream(dev)), "qwz_token_logprobs")
+    if not (ids.is_contiguous() and logprob.is_contiguous() and entropy.is_contiguous()
+            and top_logprobs.is_contiguous() and top_ids.is_contiguous() and workspace.is_contiguous()):
+        raise ValueError("ids, the outputs and the workspace must be contiguous")
+    rc = _lib.load().qwz_token_logprobs(
+        logits.data_ptr(), ids.data_ptr(), int(ids.dtype is torch.int64), logprob.data_ptr(), entropy.data_ptr(),
+        top_logprobs.data_ptr(), top_ids.data_ptr(), workspace.data_ptr(), workspace.nbytes, T, V, K, stride, code,
+        _raw_stream(dev))
+    if rc:
+        _lib.check(rc, "qwz_token_logprobs")
