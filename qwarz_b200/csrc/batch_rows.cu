@@ -5,22 +5,28 @@
 // An item is one request, one KV head and 128 / group query positions: their
 // (position, head) rows are the M = 128 rows of every MMA.  It visits the
 // 128-token KV tiles up to its last row's causal limit.  One persistent CTA per
-// SM takes an equal share of all items' tiles (batch_common.cuh); 13 warps:
-//   warps 0-3   softmax, thread = row (TMEM lane); Q staging and epilogue
-//   warps 4-11  dequantise K(j) and V(j): codes straight from the pool into
+// SM takes an equal share of all items' tiles (batch_common.cuh); 17 warps:
+//   warps 0-7   softmax, thread = row (TMEM lane), in two groups of four that
+//               take the even and the odd tiles; Q staging and epilogue (half of
+//               the head dims a group)
+//   warps 8-15  dequantise K(j) and V(j): codes straight from the pool into
 //               registers one tile ahead, FP16 into shared memory as
 //               [128 tok][D] (64-wide head-dim atoms, 128-byte swizzle): the same
 //               bytes are the K-major B operand of QK and the MN-major B
 //               operand of PV
-//   warp 12     tensor-memory owner and MMA issuer (one thread)
-// Per tile: S(j) [128 x 128] = Q K(j)^T into one of two S buffers, softmax
+//   warp 16     tensor-memory owner and MMA issuer (one thread)
+// Per tile: S(j) [128 x 128] = Q K(j)^T into the group's S buffer, softmax
 // writes P(j) (FP16, 11 significant bits as the output has) over S(j), and
-// O [128 x D] += P(j) V(j) with P from tensor memory.  The MMA thread queues
-// QK(j + 1) ahead of PV(j); K(j + 1) is dequantised while PV(j - 1) runs and
-// V(j) while QK(j + 1) does, so one buffer of each suffices (192 KB at D 256).
+// O [128 x D] += P(j) V(j) with P from tensor memory.  A row's reference maximum
+// moves only by more than 2^8; it is handed from one group's warp to the other's
+// before the exponentials, so the two groups' exponentials overlap.  The MMA
+// thread queues QK(j + 1) ahead of PV(j).  K and V have two buffers each below D
+// 256 and one at D 256 (192 KB of operands): there K(j + 1) is dequantised while
+// PV(j - 1) runs and V(j) while QK(j + 1) does.
 //
-// What bounds it (D 256): 2,048 tensor cycles a tile against 2,560 of shared
-// memory: 128 KB of QK operands, 64 KB of V and 128 KB of dequantised stores.
+// What bounds it: 128 rows x 128 exponentials are 1,024 cycles a tile (16 a
+// cycle and SM), the MMAs 8 D; at D 256 shared memory carries 320 KB a tile (128
+// of QK operands, 64 of V, 128 of dequantised stores), 2,560 cycles.
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 #include "tc_common.cuh"
@@ -33,37 +39,49 @@ namespace {
 
 constexpr int kRwTok = 128;                 // tokens of a tile
 constexpr int kRwRows = 128;                // MMA M
-constexpr int kRwSoft = 4;                  // softmax warps
+constexpr int kRwSoft = 8;                  // softmax warps, two groups
 constexpr int kRwDq = 8;                    // dequant warps
 constexpr int kRwMma = kRwSoft + kRwDq;     // MMA warp
 constexpr int kRwWarps = kRwMma + 1;
 constexpr int kRwThreads = kRwWarps * 32;
 constexpr int kRwScan = 256;                // threads that scan the requests
 
-template <int D>
-struct Rows {
-  static constexpr int kAtoms = D / 64;
-  static constexpr int kTile = kRwTok * D * 2;           // FP16 K or V tile
-  static constexpr int kQ = 0;                           // kAtoms x [128 rows x 128 B]
-  static constexpr int kK = kQ + kRwRows * D * 2;
-  static constexpr int kV = kK + kTile;
-  static constexpr int kBars = kV + kTile;
-  static constexpr int kNumBars = 12;
-  static constexpr int kMeta = kBars + 8 * kNumBars;     // TMEM base, abort flag
-  static constexpr int kRowfac = kMeta + 16;             // [128]
-  static constexpr int kStarts = kRowfac + 4 * kRwRows;  // [kRwScan] units before each scanning thread
-  static constexpr int kSums = kStarts + 8 * kRwScan;    // [kRwWarps]
-  static constexpr int kSmem = kSums + 8 * 16 + 1024;
-  static constexpr uint32_t kTmS = 0, kTmO = 256, kTmCols = 512;
-  static constexpr size_t kRec = (size_t)kRwRows * (D + 2);  // floats of a record
+// Every barrier whose phases are not all waited for by everyone is per tile
+// parity or per warp pair, so that a waiter is never two phases off.
+enum RwBar : int {
+  kRwKReady = 0,            // [2] K buffer written
+  kRwKFree = 2,             // [2] QK has read it
+  kRwVReady = 4,            // [2]
+  kRwVFree = 6,             // [2]
+  kRwSFull = 8,             // [2] S(j) is there (j's parity)
+  kRwPReady = 10,           // [2] P(j) is written
+  kRwPvDone = 12,           // [2] PV(j) is done
+  kRwRef = 14,              // [4 warps][2] the reference maxima after tile j
+  kRwSum = 22,              // [4 warps] both groups' row sums of the item
+  kRwQReady = 26,           // the item's Q is staged
+  kRwEpi = 27,              // the item's O has been read
+  kRwFin = 28,
+  kRwNumBars = 29
 };
 
-// S, P and PV have a barrier per S buffer: a softmax warp may be a tile ahead
-// of another, and its arrival for P(j + 1) must not count for P(j); and PV's
-// completions are not all waited for, so with one barrier a waiter could be two
-// phases off and take a phase's parity for another's.
-enum RwBar : int {
-  kRwKReady, kRwKFree, kRwVReady, kRwVFree, kRwSFull0, kRwSFull1, kRwPReady0, kRwPReady1, kRwPvDone0, kRwPvDone1, kRwQReady, kRwFin
+template <int D>
+struct Rows {
+  static constexpr int kBufs = D == 256 ? 1 : 2;         // K and V buffers
+  static constexpr int kTile = kRwTok * D * 2;           // FP16 K or V tile
+  static constexpr int kQ = 0;                           // D / 64 atoms of [128 rows x 128 B]
+  static constexpr int kK = kQ + kRwRows * D * 2;
+  static constexpr int kV = kK + kBufs * kTile;
+  static constexpr int kBars = kV + kBufs * kTile;
+  static constexpr int kMeta = kBars + 8 * ((kRwNumBars + 1) / 2 * 2);  // TMEM base, abort flag
+  static constexpr int kRowfac = kMeta + 16;             // [2][128] by item parity
+  static constexpr int kRef = kRowfac + 8 * kRwRows;     // [2][128] by tile parity
+  static constexpr int kSum = kRef + 8 * kRwRows;        // [2][2][128] by item parity and group
+  static constexpr int kStarts = kSum + 16 * kRwRows;     // [kRwScan] units before each scanning thread
+  static constexpr int kSums = kStarts + 8 * kRwScan;    // [kRwWarps]
+  static constexpr int kSmem = kSums + 8 * 32 + 1024;
+  static_assert(kSmem <= 227 * 1024 && kStarts % 8 == 0, "shared memory");
+  static constexpr uint32_t kTmS = 0, kTmO = 256, kTmCols = 512;
+  static constexpr size_t kRec = (size_t)kRwRows * (D + 2);  // floats of a record
 };
 
 // Walks the units (request, head, group of positions, tile) of the launch.
@@ -157,44 +175,43 @@ struct RwChunks {
   uint32_t s[D / 64];
 };
 
-// Thread t of the dequant warps, load k: token row and 32-dim chunk.  Eight
-// neighbouring lanes hold eight token rows of one chunk, so the swizzled 16-byte
-// stores of a quarter warp touch every bank once.
+// Thread t of the dequant warps, load 0: token row and 32-dim chunk; load k is
+// kRwStep<D> rows further.  Eight neighbouring lanes hold eight token rows of one
+// chunk, so the swizzled 16-byte stores of a quarter warp touch every bank once.
 template <int D>
-QWZ_DEVINL void rw_place(int t, int k, int& row, int& chunk) {
+constexpr int kRwStep = 8 * kRwDq * 32 / (8 * (D / 32));
+template <int D>
+QWZ_DEVINL void rw_place(int t, int& row, int& chunk) {
   constexpr int CPR = D / 32;
-  const int idx = (k * kRwDq + (t >> 5)) * 32 + (t & 31);
-  row = (idx & 7) + 8 * (idx / (8 * CPR));
-  chunk = (idx >> 3) % CPR;
+  row = (t & 7) + 8 * (t / (8 * CPR));
+  chunk = (t >> 3) % CPR;
 }
 
+// codes and scales point at the thread's row 0 of the pool; token0: first token.
 template <int D>
-QWZ_DEVINL void rw_load(const BatchAttnParams& p, const uint8_t* codes, const uint8_t* scales, size_t token0, int h,
-                        int valid, int t, RwChunks<D>& out) {
+QWZ_DEVINL void rw_load(const uint8_t* codes, const uint8_t* scales, size_t token0, int kv_heads, int row, int valid,
+                        RwChunks<D>& out) {
+  const uint8_t* c = codes + token0 * (size_t)(kv_heads * (D / 2));
+  const uint8_t* s = scales + token0 * (size_t)(kv_heads * (D / 16));
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) {
-    int row, c;
-    rw_place<D>(t, k, row, c);
     out.w[k] = make_uint4(0u, 0u, 0u, 0u);
     out.s[k] = 0u;
-    if (row < valid) {
-      const size_t at = (token0 + row) * p.kv_heads + h;
-      out.w[k] = __ldg(reinterpret_cast<const uint4*>(codes + at * (D / 2)) + c);
-      out.s[k] = __ldg(reinterpret_cast<const unsigned short*>(scales + at * (D / 16)) + c);
+    if (row + k * kRwStep<D> < valid) {
+      out.w[k] = __ldg(reinterpret_cast<const uint4*>(c + k * kRwStep<D> * kv_heads * (D / 2)));
+      out.s[k] = __ldg(reinterpret_cast<const unsigned short*>(s + k * kRwStep<D> * kv_heads * (D / 16)));
     }
   }
 }
 
 template <int D>
-QWZ_DEVINL void rw_store(uint32_t tile, int t, const RwChunks<D>& in) {
+QWZ_DEVINL void rw_store(uint32_t tile, int row, int c, const RwChunks<D>& in) {
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) {
-    int row, c;
-    rw_place<D>(t, k, row, c);
     uint32_t s01, unused;
     e4m3x4_to_f16x2x2(in.s[k], s01, unused);
     const uint32_t s0 = __byte_perm(s01, 0, 0x1010), s1 = __byte_perm(s01, 0, 0x3232);
-    const uint32_t base = tile + (c >> 1) * (kRwTok * 128) + row * 128;
+    const uint32_t base = tile + (c >> 1) * (kRwTok * 128) + (row + k * kRwStep<D>) * 128;
     const uint32_t w[4] = {in.w[k].x, in.w[k].y, in.w[k].z, in.w[k].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -212,6 +229,7 @@ QWZ_DEVINL void rw_store(uint32_t tile, int t, const RwChunks<D>& in) {
 template <typename T, int D>
 __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_constant__ BatchAttnParams p) {
   using R = Rows<D>;
+  constexpr int NB = R::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sraw = smem_u32(smem);
   const uint32_t sb = (sraw + 1023u) & ~1023u;
@@ -220,21 +238,28 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
   auto bar = [&](int i) -> uint32_t { return sb + R::kBars + 8u * (uint32_t)i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sg + R::kMeta + 4);
   float* rowfac = reinterpret_cast<float*>(sg + R::kRowfac);
+  float* ref_s = reinterpret_cast<float*>(sg + R::kRef);
+  float* sum_s = reinterpret_cast<float*>(sg + R::kSum);
   long long* starts = reinterpret_cast<long long*>(sg + R::kStarts);
   long long* sums = reinterpret_cast<long long*>(sg + R::kSums);
 
   if (tid == 0) {
-    mbar_init(bar(kRwKReady), kRwDq);
-    mbar_init(bar(kRwKFree), 1);
-    mbar_init(bar(kRwVReady), kRwDq);
-    mbar_init(bar(kRwVFree), 1);
-    mbar_init(bar(kRwSFull0), 1);
-    mbar_init(bar(kRwSFull1), 1);
-    mbar_init(bar(kRwPReady0), kRwSoft);
-    mbar_init(bar(kRwPReady1), kRwSoft);
-    mbar_init(bar(kRwPvDone0), 1);
-    mbar_init(bar(kRwPvDone1), 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kRwKReady + i), kRwDq);
+      mbar_init(bar(kRwKFree + i), 1);
+      mbar_init(bar(kRwVReady + i), kRwDq);
+      mbar_init(bar(kRwVFree + i), 1);
+      mbar_init(bar(kRwSFull + i), 1);
+      mbar_init(bar(kRwPReady + i), kRwSoft / 2);
+      mbar_init(bar(kRwPvDone + i), 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mbar_init(bar(kRwRef + i), 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mbar_init(bar(kRwSum + i), 2);
     mbar_init(bar(kRwQReady), kRwSoft);
+    mbar_init(bar(kRwEpi), kRwSoft);
     mbar_init(bar(kRwFin), 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -281,7 +306,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       const uint64_t dq = tc::smem_desc_k128(sb + R::kQ);
       const uint64_t dk = tc::smem_desc_k128(sb + R::kK);
       const uint64_t dv = tc::smem_desc_mn128(sb + R::kV, kRwTok * 128, 1024);
-      int item = -1;
+      int item = -1, item_cur = 0;  // items of this CTA: of the last QK, of the current tile
       bool fresh = true;  // the next QK begins an item of this CTA
       // first tile of its item in this CTA? (PV then overwrites O), for tiles j and j + 1
       bool first_next = false, first_cur = false;
@@ -293,34 +318,42 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         first_next = fresh;
         fresh = cur.tile + 1 == cur.tiles;
         cur.next(p);
-        if (!mbar_wait(bar(kRwKReady), j & 1)) return false;
+        const int kb = j % NB;
+        if (!mbar_wait(bar(kRwKReady + kb), (j / NB) & 1)) return false;
         // S(j) goes where P(j - 2) was read from
-        if (j >= 2 && !mbar_wait(bar(kRwPvDone0 + (j & 1)), ((j - 2) >> 1) & 1)) return false;
+        if (j >= 2 && !mbar_wait(bar(kRwPvDone + (j & 1)), ((j - 2) >> 1) & 1)) return false;
         tc::fence_after();
         const uint32_t d = tbase + R::kTmS + 128u * (j & 1);
+        const uint64_t dkj = dk + (uint64_t)((kb * R::kTile) >> 4);
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
           tc::mma_ss(d, dq + (uint64_t)(((ks >> 2) * (kRwRows * 128) + (ks & 3) * 32) >> 4),
-                     dk + (uint64_t)(((ks >> 2) * (kRwTok * 128) + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
-        tc::commit(bar(kRwSFull0 + (j & 1)));
-        tc::commit(bar(kRwKFree));
+                     dkj + (uint64_t)(((ks >> 2) * (kRwTok * 128) + (ks & 3) * 32) >> 4), idesc_qk, ks > 0);
+        tc::commit(bar(kRwSFull + (j & 1)));
+        tc::commit(bar(kRwKFree + kb));
         return true;
       };
       auto pv = [&](int j) -> bool {
-        if (!mbar_wait(bar(kRwPReady0 + (j & 1)), (j >> 1) & 1) || !mbar_wait(bar(kRwVReady), j & 1)) return false;
+        const int vb = j % NB;
+        if (!mbar_wait(bar(kRwPReady + (j & 1)), (j >> 1) & 1) || !mbar_wait(bar(kRwVReady + vb), (j / NB) & 1))
+          return false;
+        // a new item's first PV overwrites O: all of the old one has been read
+        if (first_cur && item_cur > 0 && !mbar_wait(bar(kRwEpi), (item_cur - 1) & 1)) return false;
         tc::fence_after();
+        const uint64_t dvj = dv + (uint64_t)((vb * R::kTile) >> 4);
 #pragma unroll
         for (int kk = 0; kk < kRwTok / 16; ++kk)
-          tc::mma_ts(tbase + R::kTmO, tbase + R::kTmS + 128u * (j & 1) + 8u * kk, dv + (uint64_t)((kk * 2048) >> 4),
+          tc::mma_ts(tbase + R::kTmO, tbase + R::kTmS + 128u * (j & 1) + 8u * kk, dvj + (uint64_t)((kk * 2048) >> 4),
                      idesc_pv, (!first_cur || kk > 0) ? 1u : 0u);
-        tc::commit(bar(kRwPvDone0 + (j & 1)));
-        tc::commit(bar(kRwVFree));
+        tc::commit(bar(kRwPvDone + (j & 1)));
+        tc::commit(bar(kRwVFree + vb));
         return true;
       };
       bool fine = qk(0);
       for (int j = 0; fine && j < units; ++j) {
         if (*abort_flag) break;
         first_cur = first_next;
+        item_cur = item;
         // a new item's Q is staged after the last softmax of the old one
         const bool ahead = j + 1 < units && !fresh;
         if (ahead && !(fine = qk(j + 1))) break;
@@ -336,19 +369,27 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     }
   } else if (warp >= kRwSoft) {
     // ------------------------------------------------------------- dequant
-    const int t = tid - kRwSoft * 32;
+    int row, chunk;
+    rw_place<D>(tid - kRwSoft * 32, row, chunk);
+    const uint8_t* kc0 = p.k_codes + (size_t)row * p.kv_heads * (D / 2) + chunk * 16;
+    const uint8_t* vc0 = p.v_codes + (size_t)row * p.kv_heads * (D / 2) + chunk * 16;
+    const uint8_t* ks0 = p.k_scales + (size_t)row * p.kv_heads * (D / 16) + chunk * 2;
+    const uint8_t* vs0 = p.v_scales + (size_t)row * p.kv_heads * (D / 16) + chunk * 2;
     RwChunks<D> kc, vc;
     int entry = cur.entry(p);
-    auto where = [&](size_t& token0, int& valid) {
+    size_t token0;
+    int valid, head;
+    auto where = [&]() {
       const int at = cur.tile * kRwTok;
       valid = cur.present(p, entry) ? min(kRwTok, cur.r.kv - at) : 0;
       token0 = valid > 0 ? (size_t)entry * kPage + (at & (kPage - 1)) : 0;
+      head = cur.h;
     };
-    size_t token0;
-    int valid;
-    where(token0, valid);
-    rw_load<D>(p, p.k_codes, p.k_scales, token0, cur.h, valid, t, kc);
-    rw_load<D>(p, p.v_codes, p.v_scales, token0, cur.h, valid, t, vc);
+    auto load_k = [&]() { rw_load<D>(kc0 + head * (D / 2), ks0 + head * (D / 16), token0, p.kv_heads, row, valid, kc); };
+    auto load_v = [&]() { rw_load<D>(vc0 + head * (D / 2), vs0 + head * (D / 16), token0, p.kv_heads, row, valid, vc); };
+    where();
+    load_k();
+    load_v();
     if (units > 1) {
       cur.next(p);
       entry = cur.entry(p);
@@ -356,24 +397,25 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     bool ok = true;
     for (int j = 0; j < units; ++j) {
       const bool more = j + 1 < units;
-      if (j >= 1) ok &= mbar_wait(bar(kRwKFree), (j - 1) & 1);
+      const int kb = j % NB;
+      if (j >= NB) ok &= mbar_wait(bar(kRwKFree + kb), (j / NB - 1) & 1);
       if (__any_sync(kFull, !ok || *abort_flag)) break;
-      rw_store<D>(sb + R::kK, t, kc);
+      rw_store<D>(sb + R::kK + kb * R::kTile, row, chunk, kc);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kRwKReady));
+      if (lane == 0) mbar_arrive(bar(kRwKReady + kb));
       if (more) {
-        where(token0, valid);
-        rw_load<D>(p, p.k_codes, p.k_scales, token0, cur.h, valid, t, kc);
+        where();
+        load_k();
       }
-      if (j >= 1) ok &= mbar_wait(bar(kRwVFree), (j - 1) & 1);
+      if (j >= NB) ok &= mbar_wait(bar(kRwVFree + kb), (j / NB - 1) & 1);
       if (__any_sync(kFull, !ok)) break;
-      rw_store<D>(sb + R::kV, t, vc);
+      rw_store<D>(sb + R::kV + kb * R::kTile, row, chunk, vc);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kRwVReady));
+      if (lane == 0) mbar_arrive(bar(kRwVReady + kb));
       if (more) {
-        rw_load<D>(p, p.v_codes, p.v_scales, token0, cur.h, valid, t, vc);
+        load_v();
         if (j + 2 < units) {
           cur.next(p);
           entry = cur.entry(p);
@@ -388,22 +430,25 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     // ------------------------------------------------- softmax (thread = row)
     // tcgen05.ld / st / wait are warp-collective: every branch around them is
     // decided by a warp vote.
-    const int r = tid;
+    const int grp = warp >> 2, wq = warp & 3;  // tiles of parity grp; TMEM lane quadrant
+    const int r = 32 * wq + lane;
     const int rpos = r / p.group, rhead = r % p.group;
-    const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
-    // Q rows of the walker's item -> K-major FP16 operand, each row scaled by a
-    // power of two (exact for BF16 and FP16), eight rows' loads in flight.  A
-    // warp stages the rows that its own threads are
-    auto stage_q = [&](const RowsWalk& w) {
+    const uint32_t lane_base = (uint32_t)(32 * wq) << 16;
+    const uint32_t ts = tbase + lane_base + R::kTmS + 128u * grp, to = tbase + lane_base + R::kTmO;
+    bool ok = true;
+    // 16 of the quadrant's Q rows of the walker's item -> K-major FP16 operand,
+    // each row scaled by a power of two (exact for BF16 and FP16)
+    auto stage_q = [&](const RowsWalk& w, int item) {
       constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows a load
       const int sub = lane / LPR, ln = lane % LPR;
       const int pos0 = w.i * per_pos, npos = min(per_pos, w.r.n - pos0);
       const T* q = reinterpret_cast<const T*>(p.q);
 #pragma unroll 1
-      for (int base = warp * 32; base < warp * 32 + 32; base += 8) {
-        uint4 v[8 / RPI];
+      for (int base = 32 * wq + 16 * grp; base < 32 * wq + 16 * grp + 16; base += 4) {
+        constexpr int U = RPI < 4 ? 4 / RPI : 1;
+        uint4 v[U];
 #pragma unroll
-        for (int u = 0; u < 8 / RPI; ++u) {
+        for (int u = 0; u < U; ++u) {
           const int row = base + u * RPI + sub;
           const int pos = row / p.group;
           v[u] = make_uint4(0u, 0u, 0u, 0u);
@@ -412,7 +457,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
                                                         (w.h * p.group + row % p.group) * D) + ln);
         }
 #pragma unroll
-        for (int u = 0; u < 8 / RPI; ++u) {
+        for (int u = 0; u < U; ++u) {
           const int row = base + u * RPI + sub;
           const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
           float amax = 0.f;
@@ -432,7 +477,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           }
           sts128(sb + R::kQ + (ln >> 3) * (kRwRows * 128) + row * 128 + (((ln & 7) ^ (row & 7)) << 4), hh[0], hh[1],
                  hh[2], hh[3]);
-          if (ln == 0) rowfac[row] = p.sm_scale_log2 / sc;
+          if (ln == 0) rowfac[(item & 1) * kRwRows + row] = p.sm_scale_log2 / sc;
         }
       }
       fence_proxy_async_smem();
@@ -440,21 +485,24 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       if (lane == 0) mbar_arrive(bar(kRwQReady));
     };
 
-    stage_q(cur);
+    stage_q(cur, 0);
     int entry = cur.entry(p);
-    int j = 0;
-    bool ok = true;
-    while (j < units) {
+    int j = 0;  // tile of the CTA
+    for (int item = 0; j < units; ++item) {
       // ------------------------------------------------------------ an item
-      const RowsWalk it = cur;
-      const int n_tiles = min(it.tiles - it.tile, units - j);
-      const int pos0 = it.i * per_pos, npos = min(per_pos, it.r.n - pos0);
-      const bool valid = rpos < npos;
+      const int pos0 = cur.i * per_pos, npos = min(per_pos, cur.r.n - pos0);
+      const int tile0 = cur.tile, n_tiles = min(cur.tiles - tile0, units - j), head = cur.h;
+      const int row0 = cur.r.row0 + pos0;
+      const bool starts_here = tile0 == 0, ends_here = tile0 + n_tiles == cur.tiles, valid = rpos < npos;
+      const int all_tiles = cur.tiles;
       // keys below lim are visible; rows that do not exist are all zeros in Q
-      const int lim = valid ? it.r.kv - it.r.n + pos0 + rpos + 1 : 0x7fffffff;
-      const float fac = rowfac[r];
-      float m_ref = -CUDART_INF_F, la = 0.f, lb = 0.f;
-      int done = 0;
+      const int lim = valid ? cur.r.kv - cur.r.n + pos0 + rpos + 1 : 0x7fffffff;
+      const int last = j + n_tiles - 1;
+      ok &= mbar_wait(bar(kRwQReady), item & 1);  // the other warps' row factors
+      if (__any_sync(kFull, !ok || *abort_flag)) break;
+      const float fac = rowfac[(item & 1) * kRwRows + r];
+      float m_own = -CUDART_INF_F, la = 0.f, lb = 0.f;  // the row sum relative to m_own
+      bool fine = true;
       for (int k = 0; k < n_tiles; ++k, ++j) {
         const int t0 = cur.tile * kRwTok;
         const bool here = cur.present(p, entry);
@@ -462,10 +510,13 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           cur.next(p);
           entry = cur.entry(p);
         }
-        ok &= mbar_wait(bar(kRwSFull0 + (j & 1)), (j >> 1) & 1);
-        if (__any_sync(kFull, !ok || *abort_flag)) break;
+        if ((j & 1) != grp) continue;
+        ok &= mbar_wait(bar(kRwSFull + grp), (j >> 1) & 1);
+        if (__any_sync(kFull, !ok || *abort_flag)) {
+          fine = false;
+          break;
+        }
         tc::fence_after();
-        const uint32_t ts = tbase + lane_base + R::kTmS + 128u * (j & 1);
         const int room = here ? lim - t0 : 0;  // columns below it count
         const bool masked = !__all_sync(kFull, room >= kRwTok);
         float mr = -CUDART_INF_F;
@@ -481,13 +532,26 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           for (int e = 0; e < 32; e += 2) mr = pf_fmax3(mr, x[e], x[e + 1]);
         }
         const float mt = mr * fac;
+        float m_ref = -CUDART_INF_F;
+        if (k > 0) {  // the reference after tile j - 1, from the other group's warp
+          ok &= mbar_wait(bar(kRwRef + 2 * wq + (grp ^ 1)), ((j - 1) >> 1) & 1);
+          if (__any_sync(kFull, !ok)) {
+            fine = false;
+            break;
+          }
+          m_ref = ref_s[(grp ^ 1) * kRwRows + r];
+        }
         const bool need = mt > m_ref + kLazy;
         const float m_new = need ? mt : m_ref;
+        ref_s[grp * kRwRows + r] = m_new;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kRwRef + 2 * wq + grp));
         const float alpha = (need && m_ref != -CUDART_INF_F) ? exp2_approx(m_ref - m_new) : 1.f;
+        const float own = m_own != -CUDART_INF_F ? exp2_approx(m_own - m_new) : 1.f;
         const float mu = m_new == -CUDART_INF_F ? 0.f : m_new;
-        la *= alpha;
-        lb *= alpha;
-        m_ref = m_new;
+        la *= own;
+        lb *= own;
+        m_own = m_new;
 #pragma unroll
         for (int c = 0; c < kRwTok; c += 32) {
           float x[32];
@@ -509,42 +573,57 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           tc::st_32x32b_x16(ts + c / 2, pw);  // over S columns that have been read
         }
         if (k > 0 && __any_sync(kFull, alpha != 1.f)) {
-          ok &= mbar_wait(bar(kRwPvDone0 + ((j - 1) & 1)), ((j - 1) >> 1) & 1);
-          if (__any_sync(kFull, !ok)) break;
+          ok &= mbar_wait(bar(kRwPvDone + (grp ^ 1)), ((j - 1) >> 1) & 1);
+          if (__any_sync(kFull, !ok)) {
+            fine = false;
+            break;
+          }
           tc::fence_after();
 #pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             uint32_t o[16];
-            tc::ld_32x32b_x16(tbase + lane_base + R::kTmO + c, o);
+            tc::ld_32x32b_x16(to + c, o);
             tc::wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tc::st_32x32b_x16(tbase + lane_base + R::kTmO + c, o);
+            for (int e = 0; e < 16; ++e) {
+              asm volatile("" : "+r"(o[e])::"memory");
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            }
+            tc::st_32x32b_x16(to + c, o);
           }
         }
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kRwPReady0 + (j & 1)));
-        done = k + 1;
+        if (lane == 0) mbar_arrive(bar(kRwPReady + grp));
       }
-      if (__any_sync(kFull, done < n_tiles)) break;
-      // the next item's Q while the last PV runs (the last QK has read this one)
-      if (j < units) stage_q(cur);
+      if (!fine) break;
+      // the next item's Q while the last PV runs, once the last QK has read this one
+      ok &= mbar_wait(bar(kRwSFull + (last & 1)), (last >> 1) & 1);
+      if (__any_sync(kFull, !ok)) break;
+      if (j < units) stage_q(cur, item + 1);
+      // the row's reference and sum over both groups
+      ok &= mbar_wait(bar(kRwRef + 2 * wq + (last & 1)), (last >> 1) & 1);
+      if (__any_sync(kFull, !ok)) break;
+      const float m_fin = ref_s[(last & 1) * kRwRows + r];
+      float* sums_of = sum_s + (item & 1) * 2 * kRwRows;
+      sums_of[grp * kRwRows + r] = m_own != -CUDART_INF_F ? (la + lb) * exp2_approx(m_own - m_fin) : 0.f;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kRwSum + wq));
+      ok &= mbar_wait(bar(kRwSum + wq), item & 1);
       // ---------------------------------------------------------- epilogue
-      ok &= mbar_wait(bar(kRwPvDone0 + ((j - 1) & 1)), ((j - 1) >> 1) & 1);
+      ok &= mbar_wait(bar(kRwPvDone + (last & 1)), (last >> 1) & 1);
       if (__any_sync(kFull, !ok)) break;
       tc::fence_after();
-      const bool starts_here = it.tile == 0, ends_here = it.tile + n_tiles == it.tiles;
-      const float l = la + lb;
+      const float l = sums_of[r] + sums_of[kRwRows + r];
       if (starts_here && ends_here) {
-        T* out = reinterpret_cast<T*>(p.out) + (long long)(it.r.row0 + pos0 + (valid ? rpos : 0)) * p.out_stride +
-                 (it.h * p.group + rhead) * D;
+        T* out = reinterpret_cast<T*>(p.out) + (long long)(row0 + (valid ? rpos : 0)) * p.out_stride +
+                 (head * p.group + rhead) * D;
         const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = grp * (D / 2); c < (grp + 1) * (D / 2); c += 32) {
           float x[32];
-          rw_ld32(tbase + lane_base + R::kTmO + c, x);
+          rw_ld32(to + c, x);
           if (!valid) continue;
           uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
@@ -564,25 +643,27 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         float* rec = p.row_records + (size_t)(blockIdx.x * 2 + (starts_here ? 1 : 0)) * R::kRec;
         float4* ro = reinterpret_cast<float4*>(rec) + r;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = grp * (D / 2); c < (grp + 1) * (D / 2); c += 32) {
           float x[32];
-          rw_ld32(tbase + lane_base + R::kTmO + c, x);
+          rw_ld32(to + c, x);
           if (!valid) continue;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             ro[(size_t)((c + e) / 4) * kRwRows] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         }
-        if (valid) *reinterpret_cast<float2*>(rec + kRwRows * D + 2 * r) = make_float2(m_ref, l);
+        if (valid && grp == 0) *reinterpret_cast<float2*>(rec + kRwRows * D + 2 * r) = make_float2(m_fin, l);
         if (starts_here && tid == 0) {
-          const long long last_unit = lo + (j - n_tiles) + it.tiles - 1;
+          const long long last_unit = lo + (j - n_tiles) + all_tiles - 1;
           meta[0] = npos * p.group;
-          meta[1] = it.r.row0 + pos0;
-          meta[3] = it.h;
+          meta[1] = row0;
+          meta[3] = head;
           meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
           meta[5] = (int)min(total, n_cta);
         }
       }
       tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kRwEpi));
     }
     if (__any_sync(kFull, !ok) && lane == 0) {
       flag_error(kErrTimeout);
