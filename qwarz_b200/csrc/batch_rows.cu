@@ -9,8 +9,8 @@
 //   warps 0-7   softmax, thread = row (TMEM lane), in two groups of four that
 //               take the even and the odd tiles; Q staging and epilogue (half of
 //               the head dims a group)
-//   warps 8-15  dequantise K(j) and V(j): codes straight from the pool into
-//               registers one tile ahead, FP16 into shared memory as
+//   warps 8-11  dequantise K(j), warps 12-15 V(j): codes straight from the pool
+//               into registers one tile ahead, FP16 into shared memory as
 //               [128 tok][D] (64-wide head-dim atoms, 128-byte swizzle): the same
 //               bytes are the K-major B operand of QK and the MN-major B
 //               operand of PV
@@ -40,8 +40,8 @@ namespace {
 constexpr int kRwTok = 128;                 // tokens of a tile
 constexpr int kRwRows = 128;                // MMA M
 constexpr int kRwSoft = 8;                  // softmax warps, two groups
-constexpr int kRwDq = 8;                    // dequant warps
-constexpr int kRwMma = kRwSoft + kRwDq;     // MMA warp
+constexpr int kRwDq = 4;                    // dequant warps of K, and of V
+constexpr int kRwMma = kRwSoft + 2 * kRwDq;  // MMA warp
 constexpr int kRwWarps = kRwMma + 1;
 constexpr int kRwThreads = kRwWarps * 32;
 constexpr int kRwScan = 256;                // threads that scan the requests
@@ -168,18 +168,18 @@ QWZ_DEVINL void rw_ld32(uint32_t taddr, float (&x)[32]) {
   }
 }
 
-// Codes and scales of one thread's share of a tile: D / 64 chunks of 32 head dims.
+// Codes and scales of one thread's share of a tile: D / 32 chunks of 32 head dims.
 template <int D>
 struct RwChunks {
-  uint4 w[D / 64];
-  uint32_t s[D / 64];
+  uint4 w[D / 32];
+  uint32_t s[D / 32];
 };
 
 // Thread t of the dequant warps, load 0: token row and 32-dim chunk; load k is
 // kRwStep<D> rows further.  Eight neighbouring lanes hold eight token rows of one
 // chunk, so the swizzled 16-byte stores of a quarter warp touch every bank once.
 template <int D>
-constexpr int kRwStep = 8 * kRwDq * 32 / (8 * (D / 32));
+constexpr int kRwStep = kRwDq * 32 / (D / 32);
 template <int D>
 QWZ_DEVINL void rw_place(int t, int& row, int& chunk) {
   constexpr int CPR = D / 32;
@@ -194,7 +194,7 @@ QWZ_DEVINL void rw_load(const uint8_t* codes, const uint8_t* scales, size_t toke
   const uint8_t* c = codes + token0 * (size_t)(kv_heads * (D / 2));
   const uint8_t* s = scales + token0 * (size_t)(kv_heads * (D / 16));
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k) {
+  for (int k = 0; k < D / 32; ++k) {
     out.w[k] = make_uint4(0u, 0u, 0u, 0u);
     out.s[k] = 0u;
     if (row + k * kRwStep<D> < valid) {
@@ -207,7 +207,7 @@ QWZ_DEVINL void rw_load(const uint8_t* codes, const uint8_t* scales, size_t toke
 template <int D>
 QWZ_DEVINL void rw_store(uint32_t tile, int row, int c, const RwChunks<D>& in) {
 #pragma unroll
-  for (int k = 0; k < D / 64; ++k) {
+  for (int k = 0; k < D / 32; ++k) {
     uint32_t s01, unused;
     e4m3x4_to_f16x2x2(in.s[k], s01, unused);
     const uint32_t s0 = __byte_perm(s01, 0, 0x1010), s1 = __byte_perm(s01, 0, 0x3232);
@@ -369,53 +369,37 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     }
   } else if (warp >= kRwSoft) {
     // ------------------------------------------------------------- dequant
+    const bool is_k = warp < kRwSoft + kRwDq;
     int row, chunk;
-    rw_place<D>(tid - kRwSoft * 32, row, chunk);
-    const uint8_t* kc0 = p.k_codes + (size_t)row * p.kv_heads * (D / 2) + chunk * 16;
-    const uint8_t* vc0 = p.v_codes + (size_t)row * p.kv_heads * (D / 2) + chunk * 16;
-    const uint8_t* ks0 = p.k_scales + (size_t)row * p.kv_heads * (D / 16) + chunk * 2;
-    const uint8_t* vs0 = p.v_scales + (size_t)row * p.kv_heads * (D / 16) + chunk * 2;
-    RwChunks<D> kc, vc;
+    rw_place<D>(tid - (is_k ? kRwSoft : kRwSoft + kRwDq) * 32, row, chunk);
+    const uint8_t* c0 = (is_k ? p.k_codes : p.v_codes) + (size_t)row * p.kv_heads * (D / 2) + chunk * 16;
+    const uint8_t* s0 = (is_k ? p.k_scales : p.v_scales) + (size_t)row * p.kv_heads * (D / 16) + chunk * 2;
+    const uint32_t tiles = sb + (is_k ? R::kK : R::kV);
+    const int ready = is_k ? kRwKReady : kRwVReady, free = is_k ? kRwKFree : kRwVFree;
+    RwChunks<D> regs;
     int entry = cur.entry(p);
-    size_t token0;
-    int valid, head;
-    auto where = [&]() {
+    auto load = [&]() {
       const int at = cur.tile * kRwTok;
-      valid = cur.present(p, entry) ? min(kRwTok, cur.r.kv - at) : 0;
-      token0 = valid > 0 ? (size_t)entry * kPage + (at & (kPage - 1)) : 0;
-      head = cur.h;
+      const int valid = cur.present(p, entry) ? min(kRwTok, cur.r.kv - at) : 0;
+      const size_t token0 = valid > 0 ? (size_t)entry * kPage + (at & (kPage - 1)) : 0;
+      rw_load<D>(c0 + cur.h * (D / 2), s0 + cur.h * (D / 16), token0, p.kv_heads, row, valid, regs);
     };
-    auto load_k = [&]() { rw_load<D>(kc0 + head * (D / 2), ks0 + head * (D / 16), token0, p.kv_heads, row, valid, kc); };
-    auto load_v = [&]() { rw_load<D>(vc0 + head * (D / 2), vs0 + head * (D / 16), token0, p.kv_heads, row, valid, vc); };
-    where();
-    load_k();
-    load_v();
+    load();
     if (units > 1) {
       cur.next(p);
       entry = cur.entry(p);
     }
     bool ok = true;
     for (int j = 0; j < units; ++j) {
-      const bool more = j + 1 < units;
-      const int kb = j % NB;
-      if (j >= NB) ok &= mbar_wait(bar(kRwKFree + kb), (j / NB - 1) & 1);
+      const int b = j % NB;
+      if (j >= NB) ok &= mbar_wait(bar(free + b), (j / NB - 1) & 1);
       if (__any_sync(kFull, !ok || *abort_flag)) break;
-      rw_store<D>(sb + R::kK + kb * R::kTile, row, chunk, kc);
+      rw_store<D>(tiles + b * R::kTile, row, chunk, regs);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kRwKReady + kb));
-      if (more) {
-        where();
-        load_k();
-      }
-      if (j >= NB) ok &= mbar_wait(bar(kRwVFree + kb), (j / NB - 1) & 1);
-      if (__any_sync(kFull, !ok)) break;
-      rw_store<D>(sb + R::kV + kb * R::kTile, row, chunk, vc);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kRwVReady + kb));
-      if (more) {
-        load_v();
+      if (lane == 0) mbar_arrive(bar(ready + b));
+      if (j + 1 < units) {
+        load();
         if (j + 2 < units) {
           cur.next(p);
           entry = cur.entry(p);
