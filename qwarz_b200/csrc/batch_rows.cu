@@ -168,6 +168,12 @@ QWZ_DEVINL void rw_ld32(uint32_t taddr, float (&x)[32]) {
   }
 }
 
+// Columns at or past `room` do not count.
+QWZ_DEVINL void rw_mask(float (&x)[32], int room) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) x[e] = e < room ? x[e] : -CUDART_INF_F;
+}
+
 // Codes and scales of one thread's share of a tile: D / 32 chunks of 32 head dims.
 template <int D>
 struct RwChunks {
@@ -503,15 +509,14 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         tc::fence_after();
         const int room = here ? lim - t0 : 0;  // columns below it count
         const bool masked = !__all_sync(kFull, room >= kRwTok);
+        // (loops, not unrolled over the columns: with three roles in one kernel
+        // the instruction cache is short)
         float mr = -CUDART_INF_F;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kRwTok; c += 32) {
           float x[32];
           rw_ld32(ts + c, x);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = c + e < room ? x[e] : -CUDART_INF_F;
-          }
+          if (masked) rw_mask(x, room - c);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mr = pf_fmax3(mr, x[e], x[e + 1]);
         }
@@ -536,14 +541,11 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         la *= own;
         lb *= own;
         m_own = m_new;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < kRwTok; c += 32) {
           float x[32];
           rw_ld32(ts + c, x);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = c + e < room ? x[e] : -CUDART_INF_F;
-          }
+          if (masked) rw_mask(x, room - c);
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
