@@ -80,7 +80,10 @@ struct Rows {
   static constexpr int kSums = kStarts + 8 * kRwScan;    // [kRwWarps]
   static constexpr int kSmem = kSums + 8 * 32 + 1024;
   static_assert(kSmem <= 227 * 1024 && kStarts % 8 == 0, "shared memory");
-  static constexpr uint32_t kTmS = 0, kTmO = 256, kTmCols = 512;
+  // tensor memory: S of even and odd tiles, O; P has columns of its own where
+  // they fit, so that S is free for QK(j + 2) as soon as the softmax has read it
+  static constexpr bool kOwnP = D <= 128;
+  static constexpr uint32_t kTmS = 0, kTmO = 256, kTmP = kOwnP ? 384 : 0, kTmPStep = kOwnP ? 64 : 128, kTmCols = 512;
   static constexpr size_t kRec = (size_t)kRwRows * (D + 2);  // floats of a record
 };
 
@@ -312,7 +315,8 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       const uint64_t dq = tc::smem_desc_k128(sb + R::kQ);
       const uint64_t dk = tc::smem_desc_k128(sb + R::kK);
       const uint64_t dv = tc::smem_desc_mn128(sb + R::kV, kRwTok * 128, 1024);
-      int item = -1, item_cur = 0;  // items of this CTA: of the last QK, of the current tile
+      int item = -1, item_cur = -1;  // items of this CTA: of the last QK, of the current tile
+      unsigned firsts = 0;           // bit j % 4: tile j is its item's first here
       bool fresh = true;  // the next QK begins an item of this CTA
       // first tile of its item in this CTA? (PV then overwrites O), for tiles j and j + 1
       bool first_next = false, first_cur = false;
@@ -326,8 +330,9 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         cur.next(p);
         const int kb = j % NB;
         if (!mbar_wait(bar(kRwKReady + kb), (j / NB) & 1)) return false;
-        // S(j) goes where P(j - 2) was read from
-        if (j >= 2 && !mbar_wait(bar(kRwPvDone + (j & 1)), ((j - 2) >> 1) & 1)) return false;
+        // S(j) goes where P(j - 2) was read from (with a P of its own: where S(j - 2)
+        // was read, and PV(j - 2) has waited for that)
+        if (!R::kOwnP && j >= 2 && !mbar_wait(bar(kRwPvDone + (j & 1)), ((j - 2) >> 1) & 1)) return false;
         tc::fence_after();
         const uint32_t d = tbase + R::kTmS + 128u * (j & 1);
         const uint64_t dkj = dk + (uint64_t)((kb * R::kTile) >> 4);
@@ -341,30 +346,40 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       };
       auto pv = [&](int j) -> bool {
         const int vb = j % NB;
-        if (!mbar_wait(bar(kRwPReady + (j & 1)), (j >> 1) & 1) || !mbar_wait(bar(kRwVReady + vb), (j / NB) & 1))
-          return false;
+        if (!mbar_wait(bar(kRwVReady + vb), (j / NB) & 1)) return false;
         // a new item's first PV overwrites O: all of the old one has been read
         if (first_cur && item_cur > 0 && !mbar_wait(bar(kRwEpi), (item_cur - 1) & 1)) return false;
         tc::fence_after();
         const uint64_t dvj = dv + (uint64_t)((vb * R::kTile) >> 4);
 #pragma unroll
         for (int kk = 0; kk < kRwTok / 16; ++kk)
-          tc::mma_ts(tbase + R::kTmO, tbase + R::kTmS + 128u * (j & 1) + 8u * kk, dvj + (uint64_t)((kk * 2048) >> 4),
+          tc::mma_ts(tbase + R::kTmO, tbase + R::kTmP + R::kTmPStep * (j & 1) + 8u * kk, dvj + (uint64_t)((kk * 2048) >> 4),
                      idesc_pv, (!first_cur || kk > 0) ? 1u : 0u);
         tc::commit(bar(kRwPvDone + (j & 1)));
         tc::commit(bar(kRwVFree + vb));
         return true;
       };
-      bool fine = qk(0);
+      // QK runs one tile ahead of PV, two once P(j) is there where P has columns
+      // of its own; a new item's first QK comes after the old one's last PV (its Q
+      // is staged after the last softmax)
+      int next = 0;  // tile of the next QK
+      bool fine = true;
       for (int j = 0; fine && j < units; ++j) {
         if (*abort_flag) break;
-        first_cur = first_next;
-        item_cur = item;
-        // a new item's Q is staged after the last softmax of the old one
-        const bool ahead = j + 1 < units && !fresh;
-        if (ahead && !(fine = qk(j + 1))) break;
-        if (!(fine = pv(j))) break;
-        if (j + 1 < units && !ahead) fine = qk(j + 1);
+        while (fine && next < units && next <= j + 1 && (!fresh || next == j)) {
+          fine = qk(next);
+          firsts = (firsts & ~(1u << (next & 3))) | ((first_next ? 1u : 0u) << (next & 3));
+          ++next;
+        }
+        if (!fine || !(fine = mbar_wait(bar(kRwPReady + (j & 1)), (j >> 1) & 1))) break;
+        if (R::kOwnP && next == j + 2 && next < units && !fresh) {
+          if (!(fine = qk(next))) break;
+          firsts = (firsts & ~(1u << (next & 3))) | ((first_next ? 1u : 0u) << (next & 3));
+          ++next;
+        }
+        first_cur = ((firsts >> (j & 3)) & 1u) != 0u;
+        item_cur += first_cur ? 1 : 0;
+        fine = pv(j);
       }
       if (!fine) {
         flag_error(kErrTimeout);
@@ -425,6 +440,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     const int rpos = r / p.group, rhead = r % p.group;
     const uint32_t lane_base = (uint32_t)(32 * wq) << 16;
     const uint32_t ts = tbase + lane_base + R::kTmS + 128u * grp, to = tbase + lane_base + R::kTmO;
+    const uint32_t tp = tbase + lane_base + R::kTmP + R::kTmPStep * grp;
     bool ok = true;
     // 16 of the quadrant's Q rows of the walker's item -> K-major FP16 operand,
     // each row scaled by a power of two (exact for BF16 and FP16)
@@ -541,6 +557,14 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         la *= own;
         lb *= own;
         m_own = m_new;
+        if (R::kOwnP && j >= 2) {  // PV(j - 2) has read this P
+          ok &= mbar_wait(bar(kRwPvDone + grp), ((j - 2) >> 1) & 1);
+          if (__any_sync(kFull, !ok)) {
+            fine = false;
+            break;
+          }
+          tc::fence_after();
+        }
 #pragma unroll 1
         for (int c = 0; c < kRwTok; c += 32) {
           float x[32];
@@ -556,7 +580,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
             pf_fadd2(la, lb, p0, p1);
             pw[e] = pack_half2(p0, p1);
           }
-          tc::st_32x32b_x16(ts + c / 2, pw);  // over S columns that have been read
+          tc::st_32x32b_x16(tp + c / 2, pw);  // (on top of S: over columns that have been read)
         }
         if (k > 0 && __any_sync(kFull, alpha != 1.f)) {
           ok &= mbar_wait(bar(kRwPvDone + (grp ^ 1)), ((j - 1) >> 1) & 1);
