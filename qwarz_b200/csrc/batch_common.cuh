@@ -20,6 +20,12 @@
 namespace qwz {
 namespace batch {
 
+// A row's weights are 2^(score - m).  The reference m is set kLift below the
+// maximum and moves when a score exceeds it by more than kRoom, so that weights
+// lie below 2^15 and, rounded to FP16, keep their 11 bits down to 2^-21 of the
+// largest (with m at the maximum itself they would lose them at 2^-14).
+constexpr float kLift = 7.f, kRoom = 15.f;
+
 // Rows and tokens of request b, clipped to what the buffers hold.
 struct Req {
   int row0;  // first row in q / out

@@ -18,8 +18,7 @@
 // across items, so a CTA's loads never drain.  Tokens are on the M side of
 // mma.sync.m16n8k16 and columns on N: K codes become A fragments of S^T in
 // registers, V codes A fragments of O^T, P^T comes from the S^T fragment by
-// movmatrix.  Base-2 online softmax, the reference maximum moves only by more
-// than 2^8; P is rounded to FP16 for its product (11 significant bits, as the
+// movmatrix.  Base-2 online softmax with a reference that seldom moves; P is rounded to FP16 for its product (11 significant bits, as the
 // output has), all sums are FP32.  At an item's end the warps' (m, l, O) are
 // merged in shared memory in warp order.
 #include "attn_common.cuh"
@@ -488,7 +487,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       few_v_load<D>(vc, vs, 2 * qd, g, tail, end_row, va);
       few_v_load<D>(vc, vs, 2 * qd + 16, g, tail, end_row, vb);
 
-      // The maxima move only when some score exceeds its reference by 2^8: one
+      // The references move only when some score exceeds one by 2^15: one
       // vote a unit, and the reduction over the lanes only then.
       float mx0 = fmaxf(t[0][0], t[0][2]), mx1 = fmaxf(t[0][1], t[0][3]);
 #pragma unroll
@@ -502,13 +501,13 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
           mx0 = fmaxf(mx0, shfl_xor(mx0, off));
           mx1 = fmaxf(mx1, shfl_xor(mx1, off));
         }
-        const float n0 = fmaxf(m0, mx0 * cf0), n1 = fmaxf(m1, mx1 * cf1);
+        const float n0 = fmaxf(m0, mx0 * cf0 - batch::kLift), n1 = fmaxf(m1, mx1 * cf1 - batch::kLift);
         const float a0 = (n0 == -CUDART_INF_F) ? 1.f : exp2_approx(m0 - n0);
         const float a1 = (n1 == -CUDART_INF_F) ? 1.f : exp2_approx(m1 - n1);
         m0 = n0;
         m1 = n1;
-        top0 = (m0 + kLazy) / cf0;
-        top1 = (m1 + kLazy) / cf1;
+        top0 = (m0 + batch::kRoom) / cf0;
+        top1 = (m1 + batch::kRoom) / cf1;
         l0 *= a0;
         l1 *= a1;
 #pragma unroll
@@ -528,9 +527,14 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         t[i][1] = exp2_approx(fmaf(t[i][1], cf1, -mu1));
         t[i][2] = exp2_approx(fmaf(t[i][2], cf0, -mu0));
         t[i][3] = exp2_approx(fmaf(t[i][3], cf1, -mu1));
-        l0 += t[i][0] + t[i][2];
-        l1 += t[i][1] + t[i][3];
-        pf[i] = p_fragments(t[i][0], t[i][1], t[i][2], t[i][3]);
+        // P rounded to FP16 once; the sums take the rounded weights, so a row's
+        // weights add up to one and a rounding of a dominant weight cancels
+        const uint32_t a = pack_half2(t[i][0], t[i][1]), b = pack_half2(t[i][2], t[i][3]);
+        const float2 fa = InTraits<__half>::to_float2(a), fb = InTraits<__half>::to_float2(b);
+        l0 += fa.x + fb.x;
+        l1 += fa.y + fb.y;
+        pf[i].hi0 = movmatrix_trans(a);
+        pf[i].hi1 = movmatrix_trans(b);
       }
 #pragma unroll
       for (int i = 0; i < TILES; i += 2) {

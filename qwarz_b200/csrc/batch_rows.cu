@@ -17,8 +17,8 @@
 //   warp 16     tensor-memory owner and MMA issuer (one thread)
 // Per tile: S(j) [128 x 128] = Q K(j)^T into the group's S buffer, softmax
 // writes P(j) (FP16, 11 significant bits as the output has) over S(j), and
-// O [128 x D] += P(j) V(j) with P from tensor memory.  A row's reference maximum
-// moves only by more than 2^8; it is handed from one group's warp to the other's
+// O [128 x D] += P(j) V(j) with P from tensor memory.  A row's reference
+// seldom moves (batch_common.cuh); it is handed from one group's warp to the other's
 // before the exponentials, so the two groups' exponentials overlap.  The MMA
 // thread queues QK(j + 1) ahead of PV(j).  K and V have two buffers each below D
 // 256 and one at D 256 (192 KB of operands): there K(j + 1) is dequantised while
@@ -546,8 +546,8 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           }
           m_ref = ref_s[(grp ^ 1) * kRwRows + r];
         }
-        const bool need = mt > m_ref + kLazy;
-        const float m_new = need ? mt : m_ref;
+        const bool need = mt > m_ref + batch::kRoom;
+        const float m_new = need ? mt - batch::kLift : m_ref;
         ref_s[grp * kRwRows + r] = m_new;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kRwRef + 2 * wq + grp));
@@ -575,10 +575,9 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           for (int e = 0; e < 16; ++e) {
             float p0, p1;
             pf_ffma2(p0, p1, x[2 * e], x[2 * e + 1], fac, -mu);
-            p0 = exp2_approx(p0);
-            p1 = exp2_approx(p1);
-            pf_fadd2(la, lb, p0, p1);
-            pw[e] = pack_half2(p0, p1);
+            pw[e] = pack_half2(exp2_approx(p0), exp2_approx(p1));
+            const float2 f = InTraits<__half>::to_float2(pw[e]);  // the sum is of the rounded weights
+            pf_fadd2(la, lb, f.x, f.y);
           }
           tc::st_32x32b_x16(tp + c / 2, pw);  // (on top of S: over columns that have been read)
         }

@@ -180,7 +180,7 @@ int qwz_token_logprobs(const void* logits, const void* ids, int32_t ids64, float
   if (top > 0 && (!top_logprobs || !top_ids)) return fail(QWZ_EINVAL, "top_logprobs and top_ids are required");
   const int item = dtype == QWZ_DTYPE_F32 ? 4 : 2;
   if (!aligned(logits, item)) return fail(QWZ_EINVAL, "logits must be aligned to their element");
-  if (stride < vocab && rows > 1) return fail(QWZ_EINVAL, "the row stride must hold a row");
+  if (stride < vocab && stride != 0 && rows > 1) return fail(QWZ_EINVAL, "the row stride must hold a row (or be 0)");
   if (!workspace || !aligned(workspace, 16)) return fail(QWZ_EINVAL, "workspace must be a non-null 16-byte aligned pointer");
   if (workspace_bytes < qwz_token_logprobs_workspace_bytes(rows, vocab, top, dtype))
     return fail(QWZ_EINVAL, "workspace smaller than qwz_token_logprobs_workspace_bytes");

@@ -1,11 +1,9 @@
 // Log probabilities of given tokens, entropy and the top alternatives of rows
 // of logits (sm_100a): what a verify step or a sampler takes from the logits
 // that follow the attention.  For a row x of V logits, M = max x:
-//   a_i = x_i log2 e - R,  s = sum 2^a,  t = sum a 2^a
-//   log p(id) = ln 2 (a_id - log2 s),  H = ln 2 (log2 s - t / s),
-//   top K by (value, then lowest index),
-// R being near the maximum in base-2 units: each a is one fused multiply-add of
-// the same R, so R's own rounding cancels.
+//   s = sum e^(x - M),  t = sum (x - M) e^(x - M)
+//   log p(id) = (x_id - M) - ln s,  H = ln s - t / s,
+//   top K by (value, then lowest index).
 //
 // One pass over the logits; bound by HBM (and, for 16-bit logits, by the
 // exponentials: 16 a cycle and SM allow 1.4 times the rate at which the logits
@@ -37,7 +35,7 @@ constexpr int kLpCand = 1024;                           // candidates ranked by 
 constexpr int kLpCtasPerSm = 4;
 constexpr int kLpMaxCtas = 4 * 256;
 constexpr int kLpAgain = 4;                             // a long part's tau is made again after this tile
-constexpr float kLpMove = 8.f;                          // a thread's reference moves past this (base 2)
+constexpr float kLpMove = 8.f;                          // a thread's reference moves past this
 constexpr int kLpMergeCand = 1024;
 
 template <typename T>
@@ -105,7 +103,6 @@ QWZ_DEVINL float max_nan(float a, float b) {  // NaN wins
 }
 
 constexpr float kLog2eF = 1.4426950408889634f;
-constexpr float kLn2F = 0.6931471805599453f;
 
 // Bytes of one chunk's record: m, s, t, (pad), K keys.
 QWZ_DEVINL size_t lp_record(int top) { return 16 + 8 * (size_t)top; }
@@ -263,17 +260,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       vm[i] = vec_max(cur[i]);
       m = fmaxf(m, vm[i]);
     }
-    const float m2 = m * kLog2eF;
-    if (m2 > r + kLpMove || (r == -CUDART_INF_F && m2 > r)) {  // a new reference
+    if (m > r + kLpMove || (r == -CUDART_INF_F && m > r)) {  // a new reference
       if (r != -CUDART_INF_F) {  // (sums without a reference are 0 or NaN)
-        const float d = r - m2, w = exp2_approx(d);
+        const float d = max_nan(r - m, -1000.f), w = exp2_approx(d * kLog2eF);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           t[e] = w * fmaf(d, s[e], t[e]);
           s[e] *= w;
         }
       }
-      r = m2;
+      r = m;
     }
     tmax = fmaxf(tmax, m);
     const float mu = r == -CUDART_INF_F ? 0.f : r;
@@ -283,10 +279,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       L::unpack(cur[i], x);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float a = max_nan(fmaf(x[j], kLog2eF, -mu), -2000.f);  // -inf: e = 0 and a e = 0
-        const float e = exp2_approx(a);
+        const float d = max_nan(x[j] - mu, -1000.f);  // -inf: e = 0 and d e = 0
+        const float e = exp2_approx(d * kLog2eF);
         s[j & 1] += e;
-        t[j & 1] = fmaf(a, e, t[j & 1]);
+        t[j & 1] = fmaf(d, e, t[j & 1]);
       }
     }
     if (K > 0) {
@@ -309,8 +305,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
 #pragma unroll
   for (int i = 1; i < kLpThreads / 32; ++i) M = fmaxf(M, red[0][i]);
   if (r != -CUDART_INF_F) {
-    const float d = r - M, w = exp2_approx(d);
-    tsum = w > 0.f ? w * fmaf(d, sum, tsum) : 0.f;
+    const float d = max_nan(r - M, -1000.f), w = exp2_approx(d * kLog2eF);
+    tsum = w * fmaf(d, sum, tsum);
     sum *= w;
   }
 #pragma unroll
@@ -442,9 +438,9 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
       s += sc;  // 0, or NaN
       continue;
     }
-    const float d = m - M, w = exp2_approx(d);
+    const float d = max_nan(m - M, -1000.f), w = exp2_approx(d * kLog2eF);
     s += w * sc;
-    t += w > 0.f ? w * (tc + d * sc) : 0.f;
+    t += w * fmaf(d, sc, tc);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -462,12 +458,12 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
     s += red[0][i];
     t += red[1][i];
   }
-  const float log2_s = log2f(s);
+  const float ln_s = logf(s);
   const bool none = M == -CUDART_INF_F && s == 0.f;  // no token is possible
-  auto logprob = [&](float x) { return none ? (x != x ? x : -CUDART_INF_F) : kLn2F * (fmaf(x, kLog2eF, -M) - log2_s); };
+  auto logprob = [&](float x) { return none ? (x != x ? x : -CUDART_INF_F) : (x - M) - ln_s; };
 
   if (tid == 0) {
-    p.entropy[row] = none ? 0.f : kLn2F * (log2_s - t / s);
+    p.entropy[row] = none ? 0.f : ln_s - t / s;
     const long long id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + row)
                                  : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + row);
     float lp = 0.f;  // id < 0: no token

@@ -1,0 +1,393 @@
+"""The operators that serve many requests from one NVFP4 pool (qwarz_b200.batch)
+against plain 64-bit forms (oracle/batch.py)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import batch as obatch
+from oracle import nvfp4
+from qwarz_b200 import _lib, batch, ops
+
+pytestmark = pytest.mark.gpu
+PAGE = 256
+
+
+@pytest.fixture(autouse=True)
+def clean_errors(cuda):
+    _lib.device_error(clear=True)
+    yield
+    assert _lib.device_error(clear=True) == 0  # a test that expects a bit clears it itself
+
+
+def i32(x, dev="cuda"):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+# ------------------------------------------------------------------- tables
+def run_tables(lengths, new_rows, held, pool, width, rows, head=0, seed=0, count=None):
+    g = np.random.default_rng(seed)
+    ids = g.permutation(pool)
+    total = int(np.sum(held))
+    table = np.full((len(lengths), width), -1)
+    at = 0
+    for b, h in enumerate(held):
+        table[b, :h] = ids[at:at + h]
+        at += h
+    count = pool - total if count is None else count
+    ring = np.full(pool, -1)
+    ring[(head + np.arange(count)) % pool] = ids[total:total + count]
+    want, why = obatch.build_tables(lengths, new_rows, held, ring, (head, count), table, rows)
+    R = len(lengths)
+    got = {"block_table": i32(table), "ring": i32(ring), "cu_rows": i32([-7] * (R + 1)), "kv_lens": i32([-7] * R),
+           "held_out": i32([-7] * R), "ring_out": i32([-7, -7]), "slots": i32([-7] * rows),
+           "positions": i32([-7] * rows), "request_of": i32([-7] * rows)}
+    for _ in range(2):  # the same state gives the same step again
+        batch.build_tables(i32(lengths), i32(new_rows), i32(held), got["ring"], i32([head, count]), got["block_table"],
+                           got["cu_rows"], got["kv_lens"], got["held_out"], got["ring_out"], got["slots"],
+                           got["positions"], got["request_of"])
+        for name, t in got.items():
+            assert np.array_equal(t.cpu().numpy(), want[name]), name
+    return want, why
+
+
+@pytest.mark.parametrize("lengths,new_rows,held,extra", [
+    ([0], [1], [0], 0),                                   # the first token of a request
+    ([255], [1], [1], 0), ([256], [1], [1], 0),           # to and past a page's end
+    ([0, 5, 700], [0, 0, 0], [0, 1, 3], 0),               # nothing to do
+    ([0, 300, 511, 512, 1], [600, 7, 1, 1, 513], [0, 2, 2, 2, 1], 3),  # windows and chunks, rows past the end
+    ([100, 900, 40, 0], [-1, 8, -1, 300], [2, 4, 1, 0], 5),  # requests that end, held pages beyond the length
+])
+def test_tables_small(lengths, new_rows, held, extra):
+    rows = sum(max(n, 0) for n in new_rows) + extra
+    _, why = run_tables(lengths, new_rows, held, 24, 8, rows, head=20)
+    assert not why
+
+
+def test_tables_denied():
+    # 3 free pages: request 1 does not get its 2, nor does any later one that needs some; one without need goes on
+    want, why = run_tables([0, 0, 0, 10], [512, 512, 1, 1], [0, 0, 0, 1], 10, 4, 1026, count=3)
+    assert why == {"empty"} and want["kv_lens"].tolist() == [512, 0, 0, 11]
+    assert _lib.device_error(clear=True) == 16
+    # a request longer than its table row
+    want, why = run_tables([1000, 3], [100, 1], [4, 1], 12, 4, 101)
+    assert why == {"wide"} and want["kv_lens"].tolist() == [0, 4]
+    assert _lib.device_error(clear=True) == 1
+
+
+@pytest.mark.parametrize("R", [1, 33, 1024, 1500])
+def test_tables_many(R):
+    g = np.random.default_rng(R)
+    lengths = g.integers(0, 3000, R)
+    new_rows = g.choice([0, 1, 1, 7, 300, -1], R)
+    held = -(-lengths // PAGE) + g.integers(0, 2, R)
+    rows = int(np.maximum(new_rows, 0).sum()) + 11
+    pool = int(held.sum() + R * 3 + 8)
+    _, why = run_tables(lengths, new_rows, held, pool, 16, rows, head=pool - 5, seed=R)
+    assert not why
+
+
+# ------------------------------------------------------------------- append
+def without_nan(x):
+    """The device writers' rule for NaN, which the oracle's numpy maximum does not
+    have: NaN does not count for a block's maximum and is stored as +6 times the
+    scale (a block of nothing else as 0)."""
+    b = x.reshape(*x.shape[:-1], -1, 16)
+    top = np.abs(np.where(np.isnan(b), 0.0, b)).max(-1, keepdims=True)
+    return np.where(np.isnan(b), top, b).reshape(x.shape).astype(np.float32)
+
+
+@pytest.mark.parametrize("heads,dim", [(4, 256), (8, 128), (1, 64), (3, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_bytes(heads, dim, dtype, packed):
+    T, pages = 77, 3
+    g = torch.Generator().manual_seed(heads * dim)
+    x = torch.randn(T, 4 * heads, dim, generator=g) * torch.exp(2 * torch.randn(T, 4 * heads, 1, generator=g))
+    x[3, :, :16] = 0.0
+    x[4, :, 0] = torch.inf
+    x[5, :, 1] = -torch.inf
+    x[6, :, 2] = torch.nan
+    x[7] = torch.nan
+    x[8] *= 1e-30
+    x[9] = 60000.0
+    x[10, :, :16] = torch.tensor([6.0, 0.25, -0.25, 0.75, -0.75, 1.25, 1.75, 2.5, -2.5, 3.5, 5.0, -5.0, 1e-3, -1e-3, 4.5, 2.25])
+    x = x.to(dtype)
+    k, v = (x[:, heads:2 * heads], x[:, 3 * heads:]) if packed else (x[:, :heads].contiguous(), x[:, heads:2 * heads].contiguous())
+    slots = torch.randperm(pages * PAGE, generator=g)[:T].to(torch.int32)
+    slots[20] = -1
+    shapes = {"k_cache": dim // 2, "v_cache": dim // 2, "k_scales": dim // 16, "v_scales": dim // 16}
+    pool = {n: torch.full((pages, PAGE, heads, w), 0xAB, dtype=torch.uint8, device="cuda") for n, w in shapes.items()}
+    xd = x.cuda()
+    kd, vd = ((xd[:, heads:2 * heads], xd[:, 3 * heads:]) if packed
+              else (xd[:, :heads].contiguous(), xd[:, heads:2 * heads].contiguous()))
+    held = [torch.empty(T, heads, dim, dtype=dtype, device="cuda") for _ in range(2)]
+    batch.append(kd, vd, *pool.values(), slots.cuda(), k_held=held[0], v_held=held[1])
+    for rows, cn, sn, h in ((k, "k_cache", "k_scales", held[0]), (v, "v_cache", "v_scales", held[1])):
+        codes, scales = nvfp4.quantize_rows(without_nan(rows.float().numpy()))
+        want_c, want_s = (np.full(tuple(pool[n].shape), 0xAB, np.uint8).reshape(pages * PAGE, heads, -1) for n in (cn, sn))
+        for i, s in enumerate(slots.tolist()):
+            if s >= 0:
+                want_c[s], want_s[s] = codes[i], scales[i]
+        assert np.array_equal(pool[cn].cpu().numpy().reshape(want_c.shape), want_c)
+        assert np.array_equal(pool[sn].cpu().numpy().reshape(want_s.shape), want_s)
+        values = obatch.dequant(torch.from_numpy(codes), torch.from_numpy(scales))
+        assert torch.equal(h.double().cpu(), values)  # exact in the input's type, the unstored row too
+
+
+def test_append_matches_the_single_sequence_writer():
+    T, P = 300, 4
+    k = torch.randn(T, 4, 256, device="cuda").half()
+    v = torch.randn(T, 4, 256, device="cuda").half()
+    v[5, 0, 3], v[5, 1, 2], v[5, 2, 7], v[6, 0, :40] = torch.nan, torch.inf, -torch.inf, torch.nan
+    table = i32([[2, 0, 3]])
+    one = [torch.zeros(P, PAGE, 4, w, dtype=torch.uint8, device="cuda") for w in (128, 128, 16, 16)]
+    many = [t.clone() for t in one]
+    ops.nvfp4_append(k, v, *one, table, i32([100]))
+    pos = torch.arange(100, 100 + T, device="cuda")
+    slots = (table[0, pos // PAGE] * PAGE + pos % PAGE).to(torch.int32)
+    batch.append(k, v, *many, slots)
+    assert all(torch.equal(a, b) for a, b in zip(one, many))
+
+
+def test_append_slot_outside_the_pool():
+    pool = [torch.zeros(2, PAGE, 1, w, dtype=torch.uint8, device="cuda") for w in (32, 32, 4, 4)]
+    k = torch.ones(3, 1, 64, device="cuda").half()
+    batch.append(k, k, *pool, i32([0, 2 * PAGE, 0x7fffffff]))
+    assert _lib.device_error(clear=True) == 4
+    assert int((pool[0] != 0).sum()) == 32
+
+
+# ------------------------------------------------------------------- attend
+def make_pool(pages, heads, dim, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = [torch.randint(0, 256, (pages, PAGE, heads, dim // 2), generator=g, device="cuda", dtype=torch.uint8)
+             for _ in range(2)]
+    scales = [(0.1 + torch.rand(pages, PAGE, heads, dim // 16, generator=g, device="cuda")).to(torch.float8_e4m3fn)
+              for _ in range(2)]
+    return codes[0], codes[1], scales[0], scales[1]
+
+
+def make_tables(kv_lens, width, pages, seed):
+    ids = np.random.default_rng(seed).permutation(pages)
+    table, at = np.full((len(kv_lens), width), -1), 0
+    for b, kv in enumerate(kv_lens):
+        n = -(-max(kv, 0) // PAGE)
+        table[b, :n] = ids[at:at + n]
+        at += n
+    return i32(table)
+
+
+def check(out, ref, mag, dtype):
+    """P is rounded to FP16 once (2^-11 of each weight), scores and sums are FP32
+    (well below 3e-5 of a weight), and the output is rounded to its type."""
+    eps = 2.0 ** -10 if dtype == torch.float16 else 2.0 ** -7
+    ulp = torch.exp2(torch.floor(torch.log2(ref.abs().clamp(min=2.0 ** -14)))) * eps
+    tol = (2.0 ** -11 + 3e-5) * mag + ulp + 1e-7
+    err = (out.double() - ref).abs()
+    assert torch.isfinite(out).all()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def run_attend(rows, kv_lens, heads, kv_heads, dim, dtype, seed=0, spare=0, gap=0, table=None, pool=None, q_scale=1.0):
+    width = max(1, max(-(-max(kv, 0) // PAGE) for kv in kv_lens))
+    pages = sum(-(-max(kv, 0) // PAGE) for kv in kv_lens) + 2
+    pool = pool or make_pool(pages, kv_heads, dim, seed)
+    table = make_tables(kv_lens, width, pages, seed) if table is None else table
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    T = int(cu[-1]) + spare
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    q = (torch.randn(T, heads + gap, dim, generator=g, device="cuda") * q_scale).to(dtype)[:, :heads]
+    out = torch.full((T, heads + gap, dim), 7.0, dtype=dtype, device="cuda")[:, :heads]
+    ws = batch.attend_workspace("cuda", dim)
+    args = (q, *pool, table, i32(cu), i32(kv_lens))
+    want, mag = obatch.attend(*args, out, dim ** -0.5)
+    batch.attend(*args, out, ws, max_rows=max(max(rows), 1))
+    check(out, want, mag, dtype)
+    again = out.clone()
+    batch.attend(*args, out, ws, max_rows=max(max(rows), 1) + 3)
+    assert torch.equal(out, again)  # no result depends on timing
+    return args, out, ws
+
+
+LENGTHS = [1, 2, 15, 31, 33, 64, 127, 128, 129, 255, 256, 257, 600, 1025]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (8, 8, 64), (14, 2, 64), (7, 1, 128), (16, 1, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attend_decode(heads, kv_heads, dim, dtype):
+    run_attend([1] * len(LENGTHS), LENGTHS, heads, kv_heads, dim, dtype, seed=dim)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (8, 8, 64), (14, 2, 64), (16, 1, 256), (64, 1, 64)])
+@pytest.mark.parametrize("n", [2, 7, 8, 9, 30])
+def test_attend_windows(heads, kv_heads, dim, n):
+    kv = [k for k in LENGTHS if k >= n]
+    run_attend([n] * len(kv), kv, heads, kv_heads, dim, torch.bfloat16, seed=n)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (14, 2, 64)])
+def test_attend_mixed_step(heads, kv_heads, dim):
+    """Decode rows, windows, prompt chunks, whole prompts and idle requests in one
+    call; rows past the step's end and a strided q and out."""
+    run_attend([1, 0, 7, 200, 300, 0, 1, 129, 2], [5, 40, 300, 1000, 300, 0, 2000, 130, 257], heads, kv_heads, dim,
+               torch.float16, spare=5, gap=kv_heads)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128)])
+def test_attend_rows_that_see_nothing(heads, kv_heads, dim):
+    """More rows than tokens (the first rows see none) and a request without
+    tokens: those rows are 0."""
+    _, out, _ = run_attend([1, 9, 1, 40, 3], [0, 4, 3, 17, 1], heads, kv_heads, dim, torch.float16)
+    assert int(out[0].count_nonzero()) == 0 and int(out[1:6].count_nonzero()) == 0
+    assert int(out[11:34].count_nonzero()) == 0 and int(out[51:53].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("rows,kv", [([1], [30000]), ([7], [30000]), ([1] * 700, [90] * 700), ([5] * 90, [300] * 90),
+                                     ([1, 1, 1], [40000, 1, 513])])
+def test_attend_work_split(rows, kv):
+    """One long request over all CTAs; many short items a CTA."""
+    run_attend(rows, kv, 24, 4, 256, torch.float16)
+
+
+def test_attend_large_scores():
+    """Scores of hundreds: the reference maximum moves often."""
+    run_attend([1, 7, 40], [3000, 2000, 1000], 24, 4, 256, torch.float16, q_scale=60.0)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [9, 9]])
+def test_attend_page_order_and_stale_bytes(rows):
+    """Another physical order of the same pages gives the same bits, and what
+    lies in the pool past a request's end (NaN scales too) does not matter."""
+    kv, dim = [700, 300], 256
+    pool = make_pool(8, 4, dim, 3)
+    ids = np.arange(5)
+    table = np.full((2, 3), -1)
+    table[0], table[1, :2] = ids[:3], ids[3:5]
+    args, out, ws = run_attend(rows, kv, 24, 4, dim, torch.float16, pool=pool, table=i32(table))
+    order = torch.tensor([6, 2, 7, 0, 5])
+    other = [t.clone() for t in pool]
+    for t, u in zip(pool, other):
+        u.view(torch.uint8).fill_(0x7F)  # NaN as a scale
+        u[order] = t[:5]
+    moved = np.full((2, 3), -1)
+    moved[0], moved[1, :2] = order[:3], order[3:5]
+    for t in other:
+        flat = t.view(torch.uint8)
+        flat[order[2], 700 - 512:] = 0x7F
+        flat[order[4], 300 - 256:] = 0x7F
+    out2 = torch.empty_like(out)
+    batch.attend(args[0], *other, i32(moved), args[6], args[7], out2, ws, max_rows=max(rows))
+    assert torch.equal(out, out2)
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [10, 10, 10]])
+def test_attend_bad_pages_and_ranges(rows):
+    """Table entries outside the pool count as absent tokens; lengths beyond the
+    table are cut; both set their bits and nothing else happens."""
+    kv = [600, 600, 600]
+    pool = make_pool(9, 4, 256, 5)
+    table = i32([[0, -1, 2], [3, 4, 999], [-5, 9, 77]])
+    run_attend(rows, kv, 24, 4, 256, torch.float16, pool=pool, table=table)
+    assert _lib.device_error(clear=True) == 2
+    q = torch.randn(2, 24, 256, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    ws = batch.attend_workspace("cuda", 256)
+    good = i32([[0, 1], [2, 3]])
+    batch.attend(q, *pool, good, i32([0, 1, 2]), i32([512, 5000]), out, ws, max_rows=1)
+    assert _lib.device_error(clear=True) == 1
+    want = torch.empty_like(out)
+    batch.attend(q, *pool, good, i32([0, 1, 2]), i32([512, 512]), want, ws, max_rows=1)
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    batch.attend(q, *pool, good, i32([0, 1, 9]), i32([512, 512]), out, ws, max_rows=8)  # rows that do not exist
+    assert _lib.device_error(clear=True) == 1
+    # (without request 1 the work is split elsewhere: the last bit may differ)
+    assert float((out[0].float() - want[0].float()).abs().max()) <= 2.0 ** -10 * float(want[0].float().abs().max())
+    assert bool((out[1] == 7.0).all())
+
+
+def test_attend_offsets_past_32_bits():
+    """A pool of more than 4 GB of codes a tensor; the pages used lie at its end."""
+    pages = 34000  # x 128 KB
+    shapes = ((128, torch.uint8), (128, torch.uint8), (16, torch.uint8), (16, torch.uint8))
+    big = [torch.zeros(pages, PAGE, 4, w, dtype=d, device="cuda") for w, d in shapes]
+    small = make_pool(6, 4, 256, 9)
+    at = torch.tensor([33999, 33990, 20000, 33000, 32768, 16384])
+    for b, s in zip(big, small):
+        b[at] = s.view(torch.uint8)
+    for rows in ([1, 1], [8, 8]):
+        args, out, ws = run_attend(rows, [700, 500], 24, 4, 256, torch.float16, pool=small,
+                                   table=i32([[0, 1, 2], [3, 4, -1]]))
+        out2 = torch.empty_like(out)
+        batch.attend(args[0], *big, i32([[33999, 33990, 20000], [33000, 32768, -1]]), args[6], args[7], out2, ws,
+                     max_rows=max(rows))
+        assert torch.equal(out, out2)
+    k = torch.randn(2, 4, 256, device="cuda").half()
+    batch.append(k, k, *big, i32([33998 * PAGE + 255, 16385 * PAGE]))
+    want, _ = nvfp4.quantize_rows(k.float().cpu().numpy())
+    assert np.array_equal(big[0][33998, 255].cpu().numpy(), want[0])
+    assert np.array_equal(big[1][16385, 0].cpu().numpy(), want[1])
+
+
+def test_attend_matches_the_single_sequence_kernels():
+    pool = make_pool(20, 4, 256, 11)
+    table = i32([list(range(18))])
+    for n, pre in ((1, 4000), (7, 4000), (40, 2000)):
+        q = torch.randn(n, 24, 256, device="cuda").half()
+        out, one = torch.empty_like(q), torch.empty_like(q)
+        batch.attend(q, *pool, table, i32([0, n]), i32([pre + n]), out, batch.attend_workspace("cuda", 256), max_rows=n)
+        if n > 8:
+            ops.nvfp4_prefill(q, *pool, table, i32([pre]), one)
+        else:
+            po, pml = ops.split_workspace("cuda", n, 16)
+            ops.attn_split(q, pool[0], pool[1], table, i32([pre]), po, pml, pool[2], pool[3], 16)
+            ops.attn_combine(po, pml, one, 16)
+        scale = float(one.abs().max())
+        assert float((out.float() - one.float()).abs().max()) <= 2.0 ** -10 * 2 * scale  # two roundings of P
+
+
+def test_step_in_a_graph_and_on_a_stream():
+    """tables + append + attend captured once; lengths change between replays; all
+    of it on a stream of its own."""
+    R, W, rows, dim = 3, 4, 16, 128
+    state = {"lengths": i32([0, 0, 0]), "new": i32([1, 1, 1]), "held": i32([0, 0, 0]),
+             "ring": i32(list(range(12))), "ring_state": i32([0, 12]), "table": i32(np.full((R, W), -1)),
+             "cu": i32([0] * 4), "kv": i32([0] * 3), "held_out": i32([0] * 3), "ring_out": i32([0, 0])}
+    maps = [i32([0] * rows) for _ in range(3)]
+    pool = [torch.zeros(12, PAGE, 2, w, dtype=torch.uint8, device="cuda") for w in (64, 64, 8, 8)]
+    q = torch.zeros(rows, 6, dim, device="cuda").half()
+    k, v = (torch.zeros(rows, 2, dim, device="cuda").half() for _ in range(2))
+    out, ws = torch.zeros_like(q), batch.attend_workspace("cuda", dim)
+
+    def step():
+        batch.build_tables(state["lengths"], state["new"], state["held"], state["ring"], state["ring_state"],
+                           state["table"], state["cu"], state["kv"], state["held_out"], state["ring_out"], *maps)
+        batch.append(k, v, *pool, maps[0])
+        batch.attend(q, *pool, state["table"], state["cu"], state["kv"], out, ws, max_rows=8)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for t in (state["held"], state["lengths"]):
+            t.zero_()
+        g = torch.Generator(device="cuda").manual_seed(0)
+        for new in ([5, 1, 0], [1, 7, 3], [1, 8, 1], [2, 0, 7]):
+            n = sum(new)
+            state["new"].copy_(i32(new))
+            for t in (q, k, v):
+                t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+            graph.replay()
+            want, mag = obatch.attend(q, *pool, state["table"], state["cu"], state["kv"], out, dim ** -0.5)
+            check(out[:n], want[:n], mag[:n], torch.float16)
+            state["held"].copy_(state["held_out"])
+            state["ring_state"].copy_(state["ring_out"])
+            state["lengths"].copy_(state["kv"])
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    assert state["lengths"].tolist() == [9, 16, 11]
