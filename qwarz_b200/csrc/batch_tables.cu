@@ -74,32 +74,44 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   int freed = lo32(batch::block_scan(v, sums, pages));
   const int rows = lo32(total);
 
-  // the requests: CTA 0 writes the per-request words, the table entries and
-  // the ring are shared out by request
+  // the requests: CTA 0 writes the per-request words; the table entries and the
+  // ring are shared out by request, a warp copies one request's pages at a time
   const int F = p.ring_size;
   auto ring_at = [&](long long i) { return (int)((head + i) % F); };
   const bool state_ok = head >= 0 && head < F && count >= 0 && count <= F;
   int row = lo32(before);
   first = hi32(before);
-  for (int b = b_lo; b < b_hi; ++b) {
-    const TabReq t = tab_req(p, b);
+  for (int k = 0; k < per; ++k) {
+    const int b = b_lo + k;
+    const bool mine = b < b_hi;
+    TabReq t = {0, 0, 0, 0, false, false};
+    if (mine) t = tab_req(p, b);
     const bool no = denied(t, first);
-    if (blockIdx.x == 0) {
+    if (mine && blockIdx.x == 0) {
       p.cu_rows[b] = row;
       p.kv_lens[b] = (t.ends || no) ? 0 : t.len + t.n;
       p.held_out[b] = t.ends ? 0 : t.held + (no ? 0 : t.grow);
       if (no) flag_error(t.wide ? kErrTableRange : kErrPoolEmpty);
     }
-    if ((unsigned)b % gridDim.x == blockIdx.x && state_ok) {
-      int32_t* table = p.block_table + (size_t)b * p.table_width;
-      if (!no)
-        for (int j = 0; j < t.grow; ++j) table[t.held + j] = __ldg(p.ring + ring_at((long long)first + j));
-      if (t.ends)
-        for (int j = 0; j < t.held; ++j) {
-          const long long at = (long long)count + freed + j;
+    const int pages_moved = t.ends ? t.held : no ? 0 : t.grow;
+    unsigned work = __ballot_sync(0xffffffffu, mine && state_ok && pages_moved > 0 &&
+                                                   (unsigned)b % gridDim.x == blockIdx.x);
+    while (work) {
+      const int src = __ffs(work) - 1;
+      work &= work - 1;
+      const int n = __shfl_sync(0xffffffffu, pages_moved, src), ends = __shfl_sync(0xffffffffu, (int)t.ends, src);
+      const int have = __shfl_sync(0xffffffffu, t.held, src);
+      const int from = __shfl_sync(0xffffffffu, t.ends ? freed : first, src);
+      int32_t* table = p.block_table + (size_t)__shfl_sync(0xffffffffu, b, src) * p.table_width;
+      for (int j = tid & 31; j < n; j += 32) {
+        if (ends) {
+          const long long at = (long long)count + from + j;
           if (at < F) p.ring[ring_at(at)] = table[j];
           else flag_error(kErrPoolEmpty);  // more pages than the ring has places
+        } else {
+          table[have + j] = __ldg(p.ring + ring_at((long long)from + j));
         }
+      }
     }
     row += t.n;
     first += t.grow;
