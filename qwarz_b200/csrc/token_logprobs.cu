@@ -109,22 +109,22 @@ QWZ_DEVINL size_t lp_record(int top) { return 16 + 8 * (size_t)top; }
 
 }  // namespace
 
-// The K-th largest (1 <= K <= 64) of 64 values in shared memory, by one warp.
-QWZ_DEVINL void lp_kth(const float* v64, int K, int lane, float* out) {
-  const float a = v64[lane], b = v64[lane + 32];
-  int ra = 0, rb = 0;
-#pragma unroll 4
-  for (int i = 0; i < 64; i += 4) {
-    const float4 v = *reinterpret_cast<const float4*>(v64 + i);
+// The K-th largest (1 <= K <= 64) of 64 values in shared memory, by 256 threads:
+// four threads rank a value against sixteen others each.
+QWZ_DEVINL void lp_kth(const float* v64, int K, int tid, float* out) {
+  const int at = tid >> 2, from = (tid & 3) * 16;
+  const float a = v64[at];
+  int rank = 0;
+#pragma unroll
+  for (int i = 0; i < 16; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(v64 + from + i);
     const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      ra += (w[j] > a || (w[j] == a && i + j < lane)) ? 1 : 0;
-      rb += (w[j] > b || (w[j] == b && i + j < lane + 32)) ? 1 : 0;
-    }
+    for (int j = 0; j < 4; ++j) rank += (w[j] > a || (w[j] == a && from + i + j < at)) ? 1 : 0;
   }
-  if (ra == K - 1) *out = a;
-  if (rb == K - 1) *out = b;
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+  if (rank == K - 1 && (tid & 3) == 0) *out = a;
 }
 
 template <typename T>
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
     if ((lane & 3) == 0) gmax[tid >> 2] = v;
     __syncthreads();
-    if (warp == 0) lp_kth(gmax, K, lane, &tau_s);
+    lp_kth(gmax, K, tid, &tau_s);
     __syncthreads();
     return tau_s;
   };
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     // The whole part's maxima give a closer bound, which most of the list does
     // not reach; a list that overflowed is made again with it.
     int n = n_cand;
-    tau = threshold(tmax);
+    if (tiles > 2 || n > kLpCand) tau = threshold(tmax);
     if (n > kLpCand) {
       if (tid == 0) n_cand = 0;
       __syncthreads();
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       }
       __syncthreads();
       n = n_cand;
-    } else if (tau > -CUDART_INF_F) {
+    } else if (tiles > 2 && tau > -CUDART_INF_F) {
       const unsigned long long least = lp_key(tau, 0xffffffffu);
       unsigned long long mine[kLpCand / kLpThreads];
 #pragma unroll
@@ -420,6 +420,17 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
   const int parts = c1 - c0 + 1;
   const uint8_t* recs = reinterpret_cast<const uint8_t*>(p.workspace) + ((size_t)c0 + row) * lp_record(K);
   auto stat = [&](int c) { return reinterpret_cast<const float*>(recs + c * lp_record(K)); };
+  // the given token's logit and the first lists, on their way while the sums are joined
+  long long id = -1;
+  float x_id = 0.f;
+  if (tid == 0) {
+    id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + row)
+                 : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + row);
+    if (id >= 0 && id < p.vocab)
+      x_id = LpTraits<T>::one(reinterpret_cast<const T*>(p.logits) + (long long)row * p.stride + id);
+  }
+  if (K > 0 && tid < parts * K)
+    cand[tid] = __ldcg(reinterpret_cast<const unsigned long long*>(recs + tid / K * lp_record(K) + 16) + tid % K);
 
   float M = -CUDART_INF_F;
   for (int c = tid; c < parts; c += kLpThreads) M = fmaxf(M, __ldcg(stat(c)));
@@ -464,14 +475,12 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
 
   if (tid == 0) {
     p.entropy[row] = none ? 0.f : ln_s - t / s;
-    const long long id = p.ids64 ? __ldg(reinterpret_cast<const long long*>(p.ids) + row)
-                                 : (long long)__ldg(reinterpret_cast<const int*>(p.ids) + row);
     float lp = 0.f;  // id < 0: no token
     if (id >= p.vocab) {
       flag_error(kErrSlotRange);
       lp = CUDART_NAN_F;
     } else if (id >= 0) {
-      lp = logprob(LpTraits<T>::one(reinterpret_cast<const T*>(p.logits) + (long long)row * p.stride + id));
+      lp = logprob(x_id);
     }
     p.logprob[row] = lp;
   }
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
   for (int l0 = 0; l0 < parts; l0 += lists) {
     const int n_lists = min(lists, parts - l0), n = have + n_lists * K;
     if (tid < have) cand[tid] = sorted[tid];
-    for (int i = tid; i < n_lists * K; i += kLpThreads)
+    for (int i = tid + (l0 == 0 ? kLpThreads : 0); i < n_lists * K; i += kLpThreads)
       cand[have + i] = __ldcg(reinterpret_cast<const unsigned long long*>(recs + (l0 + i / K) * lp_record(K) + 16) + i % K);
     __syncthreads();
     if (tid < K) sorted[tid] = 0ull;
