@@ -637,45 +637,18 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
 }
 
 // Merges the records of the items that more than one CTA worked on, in the
-// order of the splits, GROUPS warps a column, warp i of them the parts i, i +
-// GROUPS, ...  Block (head, y, z) takes columns of the item that split y began
-// and did not finish, or with LIST of the y-th such item.
-constexpr int kCombineWarps = 16;
-constexpr int kCombineThreads = kCombineWarps * 32;
-
-template <typename T, int D, int GROUPS, bool LIST>
-__global__ void __launch_bounds__(kCombineThreads)
-    batch_combine_kernel(const __grid_constant__ BatchAttnParams p, int splits) {
-  constexpr int kVecs = (D + 127) / 128;  // float4s of a lane (D 64: half the lanes)
-  constexpr int kColsHere = kCombineWarps / GROUPS;
-  extern __shared__ float weights[];  // [warps][splits / GROUPS + 1]
-  __shared__ float4 others[kCombineWarps][D / 4];
+// order of the splits: block (head, split, y) takes columns y, y + gridDim.z,
+// ... of the item that this split began and did not finish.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ float w[kBatchMaxCtas];
+  __shared__ float red[8];
+  __shared__ float4 acc_s[kGroups][kLanes];
   griddep_wait();
   griddep_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.z * kColsHere + warp % kColsHere, grp = warp / kColsHere;
-  const int hd = blockIdx.x, heads = gridDim.x;
-  int i0 = blockIdx.y;
-  if constexpr (LIST) {
-    __shared__ int counts[kCombineWarps], found;
-    if (threadIdx.x == 0) found = -1;
-    int before = 0;
-    for (int base = 0; base < splits; base += kCombineThreads) {
-      const int i = base + threadIdx.x;
-      const bool begun = i < splits && __ldcg(p.meta + (i * heads + hd) * kBatchMeta) != 0;
-      const unsigned any = __ballot_sync(0xffffffffu, begun);
-      if (lane == 0) counts[warp] = __popc(any);
-      __syncthreads();
-      int rank = before + __popc(any & ((1u << lane) - 1u));
-      for (int k = 0; k < kCombineWarps; ++k) {
-        rank += k < warp ? counts[k] : 0;
-        before += counts[k];
-      }
-      if (begun && rank == (int)blockIdx.y) found = i;
-      __syncthreads();
-    }
-    i0 = found;
-    if (i0 < 0) return;
-  }
+  const int tid = threadIdx.x, hd = blockIdx.x, heads = gridDim.x, i0 = blockIdx.y;
+  const long long splits = gridDim.y;
   const int32_t* meta = p.meta + (i0 * heads + hd) * kBatchMeta;
   const int cols = __ldcg(meta);
   if (cols == 0) return;
@@ -683,7 +656,98 @@ __global__ void __launch_bounds__(kCombineThreads)
   constexpr size_t kRec = (size_t)kFewCols * (D + 2);
   // split i0 left its part in record 1, the later ones in record 0
   auto record = [&](int j) { return p.records + (size_t)(((i0 + j) * heads + hd) * 2 + (j == 0 ? 1 : 0)) * kRec; };
-  float* w = weights + warp * (splits / GROUPS + 1);
+  auto empty = [&](int j) {
+    const long long i = i0 + j;
+    return i * busy / splits == (i + 1) * busy / splits;
+  };
+  for (int c = blockIdx.z; c < cols; c += gridDim.z) {
+    auto stat = [&](int j) { return __ldcg(reinterpret_cast<const float2*>(record(j) + kFewCols * D + 2 * c)); };
+    float M = -CUDART_INF_F;
+    for (int j = tid; j < parts; j += 256)
+      if (!empty(j)) M = fmaxf(M, stat(j).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if ((tid & 31) == 0) red[tid >> 5] = M;
+    __syncthreads();
+    M = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) M = fmaxf(M, red[i]);
+    __syncthreads();
+    float L = 0.f;
+    for (int j = tid; j < parts; j += 256) {
+      float wt = 0.f;
+      if (!empty(j)) {
+        const float2 v = stat(j);
+        wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
+        L += wt * v.y;
+      }
+      w[j] = wt;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if ((tid & 31) == 0) red[tid >> 5] = L;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) L += red[i];
+    const int grp = tid / kLanes, ln = tid % kLanes;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = grp; j < parts; j += kGroups) {
+      const float wj = w[j];
+      if (wj == 0.f) continue;
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(record(j) + c * D) + ln);
+      a.x += wj * v.x;
+      a.y += wj * v.y;
+      a.z += wj * v.z;
+      a.w += wj * v.w;
+    }
+    acc_s[grp][ln] = a;
+    __syncthreads();
+    if (tid < kLanes) {
+      a = acc_s[0][tid];
+#pragma unroll
+      for (int i = 1; i < kGroups; ++i) {
+        const float4 v = acc_s[i][tid];
+        a.x += v.x;
+        a.y += v.y;
+        a.z += v.z;
+        a.w += v.w;
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const int s = c / p.group, h = hd * p.group + c % p.group;
+      T* dst = reinterpret_cast<T*>(p.out) + (row0 + s) * p.out_stride + h * D + tid * 4;
+      dst[0] = InTraits<T>::from_float(a.x * inv);
+      dst[1] = InTraits<T>::from_float(a.y * inv);
+      dst[2] = InTraits<T>::from_float(a.z * inv);
+      dst[3] = InTraits<T>::from_float(a.w * inv);
+    }
+    __syncthreads();
+  }
+}
+
+// The same with a warp a column and a block an item: for many requests, whose
+// items have a few parts each.
+constexpr int kCombineThreads = kFewCols * 32;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kCombineThreads)
+    batch_combine_short_kernel(const __grid_constant__ BatchAttnParams p, int splits) {
+  constexpr int kVecs = (D + 127) / 128;  // float4s of a lane (D 64: half the lanes)
+  extern __shared__ float weights[];      // [warps][splits]
+  griddep_wait();
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = warp;
+  const int hd = blockIdx.x, heads = gridDim.x;
+  const int i0 = blockIdx.y;
+  const int32_t* meta = p.meta + (i0 * heads + hd) * kBatchMeta;
+  const int cols = __ldcg(meta);
+  if (cols == 0) return;
+  const int row0 = __ldcg(meta + 1), parts = __ldcg(meta + 4) - i0 + 1, busy = __ldcg(meta + 5);
+  constexpr size_t kRec = (size_t)kFewCols * (D + 2);
+  // split i0 left its part in record 1, the later ones in record 0
+  auto record = [&](int j) { return p.records + (size_t)(((i0 + j) * heads + hd) * 2 + (j == 0 ? 1 : 0)) * kRec; };
+  float* w = weights + warp * splits;
   float4 a[kVecs];
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -703,15 +767,15 @@ __global__ void __launch_bounds__(kCombineThreads)
       const float2 v = stat(j);
       const float wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
       L += wt * v.y;
-      if (j % GROUPS == grp) w[j / GROUPS] = wt;
+      w[j] = wt;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     __syncwarp();
     if (mine) {
 #pragma unroll 4
-      for (int j = grp; j < parts; j += GROUPS) {
-        const float wj = w[j / GROUPS];
+      for (int j = 0; j < parts; ++j) {
+        const float wj = w[j];
         if (wj == 0.f) continue;  // (a split without units has no record)
         const float4* src = reinterpret_cast<const float4*>(record(j) + c * D) + lane;
 #pragma unroll
@@ -723,28 +787,15 @@ __global__ void __launch_bounds__(kCombineThreads)
           a[v].w += wj * x.w;
         }
       }
-      if (grp > 0)
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) others[warp][lane + 32 * v] = a[v];
     }
   }
-  __syncthreads();
-  if (grp > 0 || c >= cols || !mine) return;
+  if (c >= cols || !mine) return;
   const float inv = L > 0.f ? 1.f / L : 0.f;
   T* dst = reinterpret_cast<T*>(p.out) + (row0 + c / p.group) * p.out_stride + (hd * p.group + c % p.group) * D;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 1; i < GROUPS; ++i) {
-      const float4 y = others[warp + i * kColsHere][lane + 32 * v];
-      x.x += y.x;
-      x.y += y.y;
-      x.z += y.z;
-      x.w += y.w;
-    }
-    T h[4] = {InTraits<T>::from_float((a[v].x + x.x) * inv), InTraits<T>::from_float((a[v].y + x.y) * inv),
-              InTraits<T>::from_float((a[v].z + x.z) * inv), InTraits<T>::from_float((a[v].w + x.w) * inv)};
+    T h[4] = {InTraits<T>::from_float(a[v].x * inv), InTraits<T>::from_float(a[v].y * inv),
+              InTraits<T>::from_float(a[v].z * inv), InTraits<T>::from_float(a[v].w * inv)};
     *reinterpret_cast<uint2*>(dst + (lane + 32 * v) * 4) = *reinterpret_cast<const uint2*>(h);
   }
 }
@@ -762,16 +813,14 @@ cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int 
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, grid, dim3(F::kThreads), F::kSmem, stream, p, maps);
   if (e != cudaSuccess) return e;
-  // Few requests: their items have many parts, which 16 warps a column share, and
-  // there are few blocks to launch; otherwise an item has a few parts, and one
-  // block takes all its columns (measured: see the table of cases).
+  // Few requests have items of many parts: a block a column (one request of 4,000
+  // tokens: 15 us a call against 17 with a warp a column); otherwise a warp a
+  // column (256 requests: 100 us a call against 106 with a block a column).
   const int splits = (int)grid.y;
-  const auto weights = [&](int groups) { return kCombineWarps * (splits / groups + 1) * sizeof(float); };
-  const unsigned cols = (unsigned)min((long long)kFewCols, max(1LL, (long long)p.max_rows * p.group));
   e = p.requests * 4 <= splits
-          ? launch_pdl(batch_combine_kernel<T, D, 16, true>, dim3(grid.x, p.requests, cols), dim3(kCombineThreads),
-                       weights(16), stream, p, splits)
-          : launch_pdl(batch_combine_kernel<T, D, 2, false>, grid, dim3(kCombineThreads), weights(2), stream, p, splits);
+          ? launch_pdl(batch_combine_kernel<T, D>, dim3(grid.x, grid.y, kFewCols), dim3(256), 0, stream, p)
+          : launch_pdl(batch_combine_short_kernel<T, D>, grid, dim3(kCombineThreads), kFewCols * splits * sizeof(float),
+                       stream, p, splits);
   if (e != cudaSuccess || (long long)p.max_rows * p.group <= p.few_cols) return e;
   return launch_rows<T, D>(p, sms, stream);
 }
