@@ -4,23 +4,35 @@
 //   out[r, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q_r.k_j - max),
 //   j < kv - n + s + 1 for row s of the n rows of a request with kv tokens.
 //
-// Bound by HBM: a token costs D/2 + D/16 bytes of K and as many of V a head,
-// and 4 D multiply-adds a query column, far below the tensor rate.
+// A token costs D/2 + D/16 bytes of K and as many of V a head, and 4 D
+// multiply-adds a query column, far below the tensor rate.  What bounds it is
+// the work between: each pair of codes is converted and each pair of halves
+// scaled on the way to a fragment, and with those instructions taken out the
+// loads alone run at 92 % of the measured copy bandwidth.
 //
-// The (row, head of the group) pairs of one request and KV head are the (at
-// most 8) columns of an item.  A CTA has one KV head and a share of all
-// requests' units of 128 or 256 tokens (batch_common.cuh); the CTAs of the other heads work
-// on the same tokens at the same time.  A warp owns 32
-// or 64 tokens of a unit and streams them through a ring of its own: the codes
-// by TMA (one box of its rows of K and one of V, 128-byte swizzle, on the warp's
-// own mbarrier), the scales, whose rows can be narrower than a TMA box, by
-// cp.async.  No warp waits for another inside an item, and the ring runs on
-// across items, so a CTA's loads never drain.  Tokens are on the M side of
-// mma.sync.m16n8k16 and columns on N: K codes become A fragments of S^T in
-// registers, V codes A fragments of O^T, P^T comes from the S^T fragment by
-// movmatrix.  Base-2 online softmax with a reference that seldom moves; P is rounded to FP16 for its product (11 significant bits, as the
-// output has), all sums are FP32.  At an item's end the warps' (m, l, O) are
-// merged in shared memory in warp order.
+// The (row, head of the group) pairs of one request and KV head are the columns
+// of an item, eight at most (9 to 16 heads of a group make two items that run
+// side by side, the second reading the tokens from L2).  A CTA has one KV head and
+// a share of all requests' units of 128 or 256 tokens (batch_common.cuh); the CTAs
+// of the other heads work on the same tokens at the same time, so that the slices
+// of a token's row leave HBM together.  A warp owns 32 or 64 tokens of a unit and
+// streams them through a ring of its own: the codes by TMA (one box of its rows
+// of K and one of V, on the warp's own mbarrier), the scales, whose rows can be
+// narrower than a TMA box, by cp.async.  No warp waits for another inside an
+// item, and the ring runs on across items, so a CTA's loads never drain.  Tokens
+// are on the M side of mma.sync.m16n8k16 and columns on N, where eight columns
+// fill the tile (tcgen05 would take the operands from shared memory, four bytes of
+// FP16 written and read there for each byte of codes): K codes become A
+// fragments of S^T in registers, V codes A fragments of O^T, P^T comes from the
+// S^T fragment by movmatrix.  Base-2 online softmax with a reference that seldom
+// moves; P is rounded to FP16 for its product (11 significant bits, as the output
+// has), all sums are FP32.  At an item's end the warps' (m, l, O) are merged in
+// shared memory in warp order.
+//
+// Measured: 524,288 tokens in one request, 24/4/256, 122 us (4.9 TB/s, 76 % of
+// the measured copy bandwidth); 64 requests of 256 to 32,768 tokens, 24/4/256,
+// 112 us (72 %); 256 of 32/8/128, 100 us (47 %: short items, whose ends cost
+// two units each); one of 4,000 tokens 15 us, the latency of two launches.
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 
@@ -107,14 +119,17 @@ struct FewWalk {
   long long base;          // weighed units before the request
   batch::Req r;
 
-  static QWZ_DEVINL bool few(const BatchAttnParams& p, const batch::Req& r) {
-    return r.n > 0 && r.n * p.group <= p.few_cols;  // the others are batch_rows.cu's
+  // whether request r has columns of the group that begins at c0 (those with more
+  // than few_cols are batch_rows.cu's)
+  static QWZ_DEVINL bool few(const BatchAttnParams& p, const batch::Req& r, int c0) {
+    const int cols = r.n * p.group;
+    return cols > c0 && cols <= p.few_cols;
   }
   // a request without tokens still has rows to write
   static QWZ_DEVINL int units_of(const batch::Req& r) { return max(1, (r.kv + U - 1) / U); }
-  static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b) {
+  static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b, int c0) {
     const batch::Req r = batch::load_req(p, b);
-    return few(p, r) ? units_of(r) + kOver : 0;
+    return few(p, r, c0) ? units_of(r) + kOver : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
@@ -122,11 +137,11 @@ struct FewWalk {
     units = units_of(r);
   }
   // Weighed unit u, `before` of which precede request b0.
-  QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long before, long long u) {
+  QWZ_DEVINL void seek(const BatchAttnParams& p, int c0, int b0, long long before, long long u) {
     base = before;
     u -= before;
     for (b = b0; b < p.requests; ++b) {
-      const long long c = cost(p, b);
+      const long long c = cost(p, b, c0);
       if (u < c) break;
       u -= c;
       base += c;
@@ -137,12 +152,12 @@ struct FewWalk {
     unit = max((int)u - kOver, 0);
   }
   // To the next request that has work here.
-  QWZ_DEVINL void next_request(const BatchAttnParams& p) {
+  QWZ_DEVINL void next_request(const BatchAttnParams& p, int c0) {
     unit = 0;
     base += units + kOver;
     for (int bb = b + 1; bb < p.requests; ++bb) {
       enter(p, bb);
-      if (few(p, r)) return;
+      if (few(p, r, c0)) return;
     }
     b = p.requests;
   }
@@ -291,6 +306,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   }
   griddep_wait();
 
+  // x: KV head and group of columns, y: share
+  const int hd = blockIdx.x / p.col_groups, c0 = blockIdx.x % p.col_groups * kFewCols;
+  const int split = blockIdx.y, cta = split * gridDim.x + blockIdx.x;
+  const long long splits = gridDim.y;
   // ---------------------------------------------------- this CTA's share
   // (the ring's memory holds the scan until the first copy)
   long long* starts = reinterpret_cast<long long*>(sgen);  // weighed units before each scanning thread's requests
@@ -298,19 +317,17 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   const int per = (p.requests + kFewScan - 1) / kFewScan;
   long long mine = 0;
   if (tid < kFewScan)
-    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b);
+    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, c0);
   long long total;
   const long long before = batch::block_scan(mine, warp_sums, total);
   if (tid < kFewScan) starts[tid] = before;
   __syncthreads();
-  const int hd = blockIdx.x, split = blockIdx.y, cta = split * gridDim.x + hd;
-  const long long splits = gridDim.y;
   auto seek = [&](long long u) {
     int at = 0;
     for (int step = kFewScan / 2; step > 0; step >>= 1)
       if (starts[at + step] <= u) at += step;
     Walk w;
-    w.seek(p, min(at * per, p.requests), starts[at], u);
+    w.seek(p, c0, min(at * per, p.requests), starts[at], u);
     return w;
   };
   Walk cur = seek(split * total / splits);
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         batch::Req r = {0, 0, 0};
         while (++pre_b < p.requests) {
           r = batch::load_req(p, pre_b);
-          if (Walk::few(p, r)) break;
+          if (Walk::few(p, r, c0)) break;
         }
         if (pre_b < p.requests) {
           pre_unit = 0;
@@ -380,8 +397,8 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
           pre_row = p.block_table + (size_t)pre_b * p.table_width;
           if (pre_left > 0 && warp == 0) {  // the item's Q on its way into L1
             constexpr int kLines = D * 2 / 128;
-            const int c = lane / kLines;
-            if (c < r.n * p.group && c < kFewCols)
+            const int c = c0 + lane / kLines;
+            if (c < r.n * p.group && c < c0 + kFewCols)
               asm volatile("prefetch.global.L1 [%0];\n" ::"l"(reinterpret_cast<const T*>(p.q) +
                                                              (r.row0 + c / p.group) * p.q_stride +
                                                              (hd * p.group + c % p.group) * D + (lane % kLines) * 64));
@@ -402,14 +419,14 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   unsigned phases = 0;  // parity of each slot's barrier
 
   while (true) {  // ------------------------------------------------ an item
-    const int first_unit = cur.unit, cols = cur.r.n * p.group;
+    const int first_unit = cur.unit, cols = min(kFewCols, cur.r.n * p.group - c0);
     float cf0, cf1;
     {
       float amax = 0.f;
       if (g < cols) {
         const uint4* src = reinterpret_cast<const uint4*>(
-            reinterpret_cast<const T*>(p.q) + (cur.r.row0 + g / p.group) * p.q_stride +
-            (hd * p.group + g % p.group) * D + qd * (D / 4));
+            reinterpret_cast<const T*>(p.q) + (cur.r.row0 + (c0 + g) / p.group) * p.q_stride +
+            (hd * p.group + (c0 + g) % p.group) * D + qd * (D / 4));
 #pragma unroll
         for (int i = 0; i < QW / 4; ++i) {
           const uint4 v = __ldg(src + i);
@@ -439,9 +456,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       cf0 = __shfl_sync(kFull, rowfac, 8 * qd);
       cf1 = __shfl_sync(kFull, rowfac, 8 * qd + 4);
     }
-    const int min_lim = cur.r.kv - cur.r.n + 1;
-    const int lim0 = 2 * qd < cols ? min_lim + 2 * qd / p.group : 0;
-    const int lim1 = 2 * qd + 1 < cols ? min_lim + (2 * qd + 1) / p.group : 0;
+    const int lim_base = cur.r.kv - cur.r.n + 1, min_lim = lim_base + c0 / p.group;
+    const int lim0 = 2 * qd < cols ? lim_base + (c0 + 2 * qd) / p.group : 0;
+    const int lim1 = 2 * qd + 1 < cols ? lim_base + (c0 + 2 * qd + 1) / p.group : 0;
     // reference maxima in base-2 units, and the raw scores that move them
     float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, top0 = -CUDART_INF_F, top1 = -CUDART_INF_F;
     float l0 = 0.f, l1 = 0.f;
@@ -611,8 +628,8 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
           if (c >= cols) continue;
           const float x = e ? a.y : a.x, y = e ? a.w : a.z, inv = e ? i1 : i0;
           if (whole) {
-            T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + c / p.group) * p.out_stride +
-                     (hd * p.group + c % p.group) * D + d;
+            T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + (c0 + c) / p.group) * p.out_stride +
+                     (hd * p.group + (c0 + c) % p.group) * D + d;
             const T h[2] = {InTraits<T>::from_float(x * inv), InTraits<T>::from_float(y * inv)};
             *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(h);
           } else {
@@ -630,7 +647,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       __syncthreads();
     }
     if (cur.b == end_b) break;
-    cur.next_request(p);
+    cur.next_request(p, c0);
     if (cur.b == p.requests || (cur.b == end_b && end_unit == 0)) break;
   }
   griddep_launch_dependents();
@@ -715,7 +732,8 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
         a.w += v.w;
       }
       const float inv = L > 0.f ? 1.f / L : 0.f;
-      const int s = c / p.group, h = hd * p.group + c % p.group;
+      const int cc = hd % p.col_groups * kFewCols + c;  // column of the KV head
+      const int s = cc / p.group, h = hd / p.col_groups * p.group + cc % p.group;
       T* dst = reinterpret_cast<T*>(p.out) + (row0 + s) * p.out_stride + h * D + tid * 4;
       dst[0] = InTraits<T>::from_float(a.x * inv);
       dst[1] = InTraits<T>::from_float(a.y * inv);
@@ -791,7 +809,9 @@ __global__ void __launch_bounds__(kCombineThreads)
   }
   if (c >= cols || !mine) return;
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  T* dst = reinterpret_cast<T*>(p.out) + (row0 + c / p.group) * p.out_stride + (hd * p.group + c % p.group) * D;
+  const int cc = hd % p.col_groups * kFewCols + c;  // column of the KV head
+  T* dst = reinterpret_cast<T*>(p.out) + (row0 + cc / p.group) * p.out_stride +
+           (hd / p.col_groups * p.group + cc % p.group) * D;
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) {
     T h[4] = {InTraits<T>::from_float(a[v].x * inv), InTraits<T>::from_float(a[v].y * inv),
@@ -807,7 +827,8 @@ cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int 
   using F = Few<D>;
   // the heads of a token range run side by side: their slices of a token row
   // share DRAM pages and sectors
-  const dim3 grid(p.kv_heads, max(1, sms * F::kCtas / p.kv_heads));
+  const int heads = p.kv_heads * p.col_groups;
+  const dim3 grid(heads, max(1, sms * F::kCtas / heads));
   auto kernel = batch_few_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;

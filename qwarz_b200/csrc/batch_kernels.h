@@ -30,6 +30,7 @@ struct BatchAttnParams {
   int requests, rows, table_width, num_pages, kv_heads, group;
   int max_rows;                  // upper bound of a request's rows
   int few_cols;                  // most (row, head) columns a KV head of batch_few.cu has
+  int col_groups;                // groups of eight of them
   float sm_scale_log2;           // sm_scale * log2(e)
 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA

@@ -24,9 +24,21 @@
 // 256 and one at D 256 (192 KB of operands): there K(j + 1) is dequantised while
 // PV(j - 1) runs and V(j) while QK(j + 1) does.
 //
-// What bounds it: 128 rows x 128 exponentials are 1,024 cycles a tile (16 a
-// cycle and SM), the MMAs 8 D; at D 256 shared memory carries 320 KB a tile (128
-// of QK operands, 64 of V, 128 of dequantised stores), 2,560 cycles.
+// What bounds it: a tile's MMAs take 8 D cycles, its 128 x 128 exponentials 1,024
+// (16 a cycle and SM).  At D 256 shared memory carries 320 KB a tile (128 of QK
+// operands, 64 of V, 128 of dequantised stores: 2,560 cycles) and the four warps
+// that dequantise K are busy for about 5,400 cycles a tile (3,000 converting and
+// storing, 2,400 issuing loads), which is the period measured; a second K buffer
+// does not fit.  At D 128 the period is about 2,500 cycles, the softmax's chain
+// from S(j) to P(j).  Converting once a tile for all 128 rows is why this kernel
+// starts at 9 columns (17 where a group has more than 8 heads): batch_few.cu
+// converts for every eight.
+//
+// Measured, 24/4/256: 16 requests of 4,096 to 32,768 tokens, 7 rows each, 174 us
+// (22 % of the HBM rate, 13 % of the measured bf16 rate in useful rows, two thirds
+// of the tile's rows being empty); a step of prompt chunks, windows and decode
+// rows, 466 us (32 % of the measured bf16 rate).  16 x 7 rows at 32,768 tokens of
+// 32/8/128: 376 us.
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 #include "tc_common.cuh"

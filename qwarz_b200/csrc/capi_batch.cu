@@ -157,7 +157,13 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   p.kv_heads = num_kv_heads;
   p.group = num_q_heads / num_kv_heads;
   p.max_rows = max_rows;
-  p.few_cols = qwz::kBatchFewCols;
+  // Decode rows of 9 to 16 heads a KV head are two groups of columns in batch_few.cu:
+  // 8 requests of 32,768 tokens, 48/4/256: 124 us against 193 in batch_rows.cu; 512 of
+  // 512 tokens, 96/8/64: 124 against 316.  What has more columns goes to batch_rows.cu.
+  // The group of heads alone decides, so that a request's result does not depend on
+  // max_rows.
+  p.col_groups = p.group > qwz::kBatchFewCols && p.group <= 2 * qwz::kBatchFewCols ? 2 : 1;
+  p.few_cols = p.col_groups * qwz::kBatchFewCols;
   p.sm_scale_log2 = sm_scale * kLog2e;
   return launched(qwz::launch_batch_attend(p, maps, head_dim, dtype, sms, as_stream(stream)), "qwz_batch_attend");
 }

@@ -5,19 +5,25 @@
 //   log p(id) = (x_id - M) - ln s,  H = ln s - t / s,
 //   top K by (value, then lowest index).
 //
-// One pass over the logits; bound by HBM (and, for 16-bit logits, by the
-// exponentials: 16 a cycle and SM allow 1.4 times the rate at which the logits
-// arrive).  A CTA streams a part of one row, four 16-byte loads a thread in
-// flight while the four before them are summed; the sums are FP32, relative to
-// a maximum of the thread's own that moves only when a logit exceeds it by more
-// than 8, so nothing waits inside the loop.  Top K: the K-th largest of 64 group
-// maxima (four threads each) of the part's first tile is a lower bound tau of the
-// part's K-th largest value; whatever reaches it (about K times the number of
-// tiles) goes to a list in shared memory that is ranked by counting at the end.
-// A list that overflows is made again with the tau of the whole part's maxima,
-// and where equal values overflow that, K rounds of a maximum find the K.  A
-// second kernel, one CTA a row, joins the parts in order; no result depends on
-// the order of atomics.
+// One pass over the logits.  A CTA streams an equal share of all rows' 16 KB
+// tiles (a share may end one row and begin others: a part a row), four 16-byte
+// loads a thread in flight while the four before them are summed; the sums are
+// FP32, relative to a maximum of the thread's own that moves only when a logit
+// exceeds it by more than 8, so nothing waits inside the loop.  Top K: the K-th
+// largest of 64 group maxima (four threads each) of the part's first tile is a
+// lower bound tau of the part's K-th largest value; whatever reaches it (about K
+// times the number of tiles) goes to a list in shared memory that is ranked by
+// counting at the end.  A list that overflows is made again with the tau of the
+// whole part's maxima, and where equal values overflow that, K rounds of a
+// maximum find the K.  A second kernel, one CTA a row, joins the parts in order;
+// no result depends on the order of atomics.
+//
+// What bounds it: instructions, about 14 an element and warp (unpack, compare,
+// subtract, exponential, two sums), where HBM would allow 5 for 16-bit logits.
+// Measured: 448 rows of 151,000 BF16 logits, top 20, 62 us (2.2 TB/s, 34 % of
+// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 10.7 us and 7 rows
+// of 131,072 BF16, top 8, 12.8 us: the latency of two launches and of one part's
+// ranking.  A CTA a row took 203 us for the first of these.
 #include "qwz_common.cuh"
 #include "batch_kernels.h"
 #include "qwz_kernels.h"
