@@ -227,6 +227,13 @@ def test_attend_windows(heads, kv_heads, dim, n):
     run_attend([n] * len(kv), kv, heads, kv_heads, dim, torch.bfloat16, seed=n)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(9, 1, 256), (24, 2, 128), (32, 2, 64), (51, 3, 64)])
+def test_attend_wide_groups(heads, kv_heads, dim):
+    """9 to 17 heads a KV head: decode rows beside windows and requests without tokens."""
+    run_attend([1, 1, 0, 2, 1, 5, 1, 1], [700, 1, 9, 300, 0, 513, 256, 2049], heads, kv_heads, dim, torch.float16,
+               seed=heads, gap=kv_heads)
+
+
 @pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (14, 2, 64)])
 def test_attend_mixed_step(heads, kv_heads, dim):
     """Decode rows, windows, prompt chunks, whole prompts and idle requests in one
@@ -391,3 +398,18 @@ def test_step_in_a_graph_and_on_a_stream():
     torch.cuda.current_stream().wait_stream(stream)
     torch.cuda.synchronize()
     assert state["lengths"].tolist() == [9, 16, 11]
+
+
+def test_example_serves_requests():
+    """examples/batched_verify.py: pages are neither lost nor held twice, requests
+    end, drafts are accepted."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "batched_verify.py"
+    spec = importlib.util.spec_from_file_location("batched_verify", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.serve(requests=6, steps=25, seed=1, say=lambda *_: None)
+    assert got["free"] + got["held"] == got["pages"]
+    assert got["lengths"] == got["done"] and got["finished"] > 0 and 0 < got["accepted"] <= got["drafted"]
