@@ -10,18 +10,23 @@
 // loads a thread in flight while the four before them are summed; the sums are
 // FP32, relative to a maximum of the thread's own that moves only when a logit
 // exceeds it by more than 8, so nothing waits inside the loop.  Top K: the K-th
-// largest of 64 group maxima (four threads each) of the part's first tile is a
-// lower bound tau of the part's K-th largest value; whatever reaches it (about K
-// times the number of tiles) goes to a list in shared memory that is ranked by
-// counting at the end.  A list that overflows is made again with the tau of the
-// whole part's maxima, and where equal values overflow that, K rounds of a
-// maximum find the K.  A second kernel, one CTA a row, joins the parts in order;
-// no result depends on the order of atomics.
+// largest of 64 group maxima (four threads each) of the part's first tiles is a
+// lower bound tau of the part's K-th largest value; the places of the vectors
+// that reach it (about K a tile) go to a list, and at the end, with the tau of
+// the whole part's maxima, their elements are read again and ranked by counting
+// (reading them at once, a warp a vector, took 61 us where this takes 53).  If
+// the list overflows, the part is read again with that tau, and where equal
+// values overflow the candidates, K rounds of a maximum find the K.  A second
+// kernel, one CTA a row, joins the parts in order; no result depends on the order
+// of atomics.
 //
-// What bounds it: instructions, about 14 an element and warp (unpack, compare,
-// subtract, exponential, two sums), where HBM would allow 5 for 16-bit logits.
-// Measured: 448 rows of 151,000 BF16 logits, top 20, 62 us (2.2 TB/s, 34 % of
-// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 10.7 us and 7 rows
+// What bounds it: the exponentials, 16 a cycle and SM, would take 15 us of the
+// first case below and HBM 21; with what stands around them (unpack, difference,
+// two sums, maxima; two elements an instruction made no difference) the sums alone
+// take 39, the search for the top 20 another 14, a part's beginning and end being
+// half of that.
+// Measured: 448 rows of 151,000 BF16 logits, top 20, 53 us (2.6 TB/s, 40 % of
+// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 10.4 us and 7 rows
 // of 131,072 BF16, top 8, 12.8 us: the latency of two launches and of one part's
 // ranking.  A CTA a row took 203 us for the first of these.
 #include "qwz_common.cuh"
@@ -38,6 +43,7 @@ constexpr int kLpThreads = 256;
 constexpr int kLpVecs = 4;                              // 16-byte loads of a tile a thread
 constexpr int kLpTileVecs = kLpThreads * kLpVecs;       // 16 KB
 constexpr int kLpCand = 1024;                           // candidates ranked by counting
+constexpr int kLpList = 1024;                           // vectors that may hold candidates
 constexpr int kLpCtasPerSm = 4;
 constexpr int kLpMaxCtas = 4 * 256;
 constexpr int kLpAgain = 4;                             // a long part's tau is made again after this tile
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
   __shared__ unsigned long long cand[kLpCand];
   __shared__ unsigned long long best;
   __shared__ float tau_s;
-  __shared__ int n_cand;
+  __shared__ int n_cand, n_vec, list[kLpList];  // candidates; places of vectors that may hold some
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int K = p.top;
   griddep_wait();
@@ -214,30 +220,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
   };
   // Candidates: at or above tau; where tau is -inf (fewer than K groups hold
   // anything above it), all that is above -inf and the first K places (the lowest
-  // indices).  Vectors that hold any are rare, so the warp takes them one by one,
-  // a lane an element, which reads it again (from L1).
+  // indices).
   auto wanted = [&](float vmax, int pos, float tau) {
     return tau == -CUDART_INF_F ? vmax > tau || pos < first + K : vmax >= tau;
   };
-  auto collect = [&](int tile, unsigned mine, float tau) {  // mine: bit i = this lane's vector i
-    unsigned any = __ballot_sync(0xffffffffu, mine != 0u);
-    while (any) {
-      const int src = __ffs(any) - 1;
-      any &= any - 1;
-      unsigned h = __shfl_sync(0xffffffffu, mine, src);
-      while (h) {
-        const int i = __ffs(h) - 1;
-        h &= h - 1;
-        const int pos = (v0 + tile * kLpTileVecs + i * kLpThreads + warp * 32 + src) * E - skew + lane;
-        if (lane < E && pos >= first && pos < last_pos) {
-          const float x = L::one(x0 + pos);
-          if (wanted(x, pos, tau)) {
-            const int at = atomicAdd(&n_cand, 1);
-            if (at < kLpCand) cand[at] = lp_key(x, (uint32_t)pos);
-          }
-        }
+  auto place = [&](int tile, int i) { return (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew; };
+  // the candidates of the vector at `pos`, which is read again
+  auto expand = [&](int pos, float tau) {
+    float x[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = pos + j >= first && pos + j < last_pos ? L::one(x0 + pos + j) : CUDART_NAN_F;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (pos + j >= first && pos + j < last_pos && wanted(x[j], pos + j, tau)) {
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < kLpCand) cand[at] = lp_key(x[j], (uint32_t)(pos + j));
       }
-    }
   };
 
   uint4 raw[kLpVecs], cur[kLpVecs];
@@ -250,7 +248,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       tmax = fmaxf(tmax, vec_max(cur[i]));
       if (tiles > 1) tmax = fmaxf(tmax, vec_max(raw[i]));
     }
-    if (tid == 0) n_cand = 0;
+    if (tid == 0) n_cand = n_vec = 0;
     tau = threshold(tmax);
   }
   float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};  // two chains each
@@ -292,11 +290,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
       }
     }
     if (K > 0) {
-      unsigned mine = 0;
 #pragma unroll
       for (int i = 0; i < kLpVecs; ++i)
-        if (wanted(vm[i], (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau)) mine |= 1u << i;
-      collect(tile, mine, tau);
+        if (wanted(vm[i], place(tile, i), tau)) {
+          const int at = atomicAdd(&n_vec, 1);
+          if (at < kLpList) list[at] = place(tile, i);
+        }
       if (tile == kLpAgain && tiles > 2 * kLpAgain) tau = fmaxf(tau, threshold(tmax));
     }
   }
@@ -340,40 +339,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     f[2] = tsum;
   }
   if (K > 0) {
-    // The whole part's maxima give a closer bound, which most of the list does
-    // not reach; a list that overflowed is made again with it.
-    int n = n_cand;
-    if (tiles > 2 || n > kLpCand) tau = threshold(tmax);
-    if (n > kLpCand) {
-      if (tid == 0) n_cand = 0;
-      __syncthreads();
+    // The whole part's maxima give a closer bound, which most of the listed
+    // vectors do not reach.
+    if (tiles > 2) tau = threshold(tmax);
+    if (n_vec <= kLpList) {
+      for (int c = tid; c < n_vec; c += kLpThreads) expand(list[c], tau);
+    } else {  // the list overflowed
 #pragma unroll 1
       for (int tile = 0; tile < tiles; ++tile) {
         load(tile, raw);
-        unsigned mine = 0;
 #pragma unroll
         for (int i = 0; i < kLpVecs; ++i)
-          if (wanted(vec_max(raw[i]), (v0 + tile * kLpTileVecs + i * kLpThreads + tid) * E - skew, tau)) mine |= 1u << i;
-        collect(tile, mine, tau);
+          if (wanted(vec_max(raw[i]), place(tile, i), tau)) expand(place(tile, i), tau);
       }
-      __syncthreads();
-      n = n_cand;
-    } else if (tiles > 2 && tau > -CUDART_INF_F) {
-      const unsigned long long least = lp_key(tau, 0xffffffffu);
-      unsigned long long mine[kLpCand / kLpThreads];
-#pragma unroll
-      for (int i = 0; i < kLpCand / kLpThreads; ++i) {
-        const int at = i * kLpThreads + tid;
-        mine[i] = at < n ? cand[at] : 0ull;
-      }
-      if (tid == 0) n_cand = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kLpCand / kLpThreads; ++i)
-        if (mine[i] >= least) cand[atomicAdd(&n_cand, 1)] = mine[i];
-      __syncthreads();
-      n = n_cand;
     }
+    __syncthreads();
+    const int n = n_cand;
     unsigned long long* keys = reinterpret_cast<unsigned long long*>(rec + 16);
     if (n <= kLpCand) {
       for (int c = tid; c < max(n, K); c += kLpThreads) {
