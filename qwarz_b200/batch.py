@@ -23,6 +23,7 @@ from .ops import PAGE, _contig, _dtype_code
 _I32 = torch.int32
 _U8 = torch.uint8
 _SCALES = (torch.float8_e4m3fn, torch.uint8)
+_current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the handle alone; a Stream object costs 2 us a call
 
 
@@ -35,6 +36,18 @@ def _device(first, rest) -> int:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on different devices: {first.device} vs {t.device}")
     return dev
+
+
+def _launch(dev, name, *args) -> None:
+    """Calls `name` on the current stream of device `dev`, which need not be the current device."""
+    fn = getattr(_lib.load(), name)
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _int32(names, tensors) -> None:
@@ -103,12 +116,11 @@ def build_tables(lengths, new_rows, held, ring, ring_state, block_table, cu_rows
         raise ValueError("cu_rows has requests + 1 entries, ring_state and ring_out have 2")
     if positions.numel() != T or request_of.numel() != T:
         raise ValueError("slots, positions and request_of must have the same length")
-    rc = _lib.load().qwz_batch_tables(
+    _launch(
+        dev, "qwz_batch_tables",
         lengths.data_ptr(), new_rows.data_ptr(), held.data_ptr(), ring.data_ptr(), ring_state.data_ptr(),
         block_table.data_ptr(), cu_rows.data_ptr(), kv_lens.data_ptr(), held_out.data_ptr(), ring_out.data_ptr(),
-        slots.data_ptr(), positions.data_ptr(), request_of.data_ptr(), R, width, ring.numel(), T, _raw_stream(dev))
-    if rc:
-        _lib.check(rc, "qwz_batch_tables")
+        slots.data_ptr(), positions.data_ptr(), request_of.data_ptr(), R, width, ring.numel(), T)
 
 
 def append(k, v, k_cache, v_cache, k_scales, v_scales, slots, k_held=None, v_held=None) -> None:
@@ -132,11 +144,10 @@ def append(k, v, k_cache, v_cache, k_scales, v_scales, slots, k_held=None, v_hel
                 raise ValueError("k_held and v_held must have k's shape and dtype")
             _contig("k_held and v_held", t)
             held[i] = t.data_ptr()
-    rc = _lib.load().qwz_batch_append(
+    _launch(
+        dev, "qwz_batch_append",
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-        slots.data_ptr(), held[0], held[1], T, k_stride, v_stride, heads, dim, P, _dtype_code(dtype), _raw_stream(dev))
-    if rc:
-        _lib.check(rc, "qwz_batch_append")
+        slots.data_ptr(), held[0], held[1], T, k_stride, v_stride, heads, dim, P, _dtype_code(dtype))
 
 
 def attend_workspace(device, head_dim: int) -> torch.Tensor:
@@ -171,10 +182,9 @@ def attend(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_len
         raise ValueError("block_table must be [requests, width], cu_rows [requests + 1], kv_lens [requests]")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    rc = _lib.load().qwz_batch_attend(
+    _launch(
+        dev, "qwz_batch_attend",
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
         block_table.data_ptr(), cu_rows.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
         workspace.nbytes, T, R, max_rows, width, P, q_heads, heads, dim, q_stride, out_stride,
-        dim ** -0.5 if sm_scale is None else float(sm_scale), _dtype_code(dtype), _raw_stream(dev))
-    if rc:
-        _lib.check(rc, "qwz_batch_attend")
+        dim ** -0.5 if sm_scale is None else float(sm_scale), _dtype_code(dtype))

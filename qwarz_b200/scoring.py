@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .batch import _device, _raw_stream
+from .batch import _device, _launch
 
 _CODES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 MAX_TOP = 32
@@ -54,9 +54,7 @@ def token_logprobs(logits, ids, logprob, entropy, top_logprobs, top_ids, workspa
     if not (ids.is_contiguous() and logprob.is_contiguous() and entropy.is_contiguous()
             and top_logprobs.is_contiguous() and top_ids.is_contiguous() and workspace.is_contiguous()):
         raise ValueError("ids, the outputs and the workspace must be contiguous")
-    rc = _lib.load().qwz_token_logprobs(
+    _launch(
+        dev, "qwz_token_logprobs",
         logits.data_ptr(), ids.data_ptr(), int(ids.dtype is torch.int64), logprob.data_ptr(), entropy.data_ptr(),
-        top_logprobs.data_ptr(), top_ids.data_ptr(), workspace.data_ptr(), workspace.nbytes, T, V, K, stride, code,
-        _raw_stream(dev))
-    if rc:
-        _lib.check(rc, "qwz_token_logprobs")
+        top_logprobs.data_ptr(), top_ids.data_ptr(), workspace.data_ptr(), workspace.nbytes, T, V, K, stride, code)

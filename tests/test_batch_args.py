@@ -98,3 +98,31 @@ def test_cpu_tensors_are_refused():
         batch.attend(x, *[t] * 9, max_rows=1)
     with pytest.raises(ValueError, match="no CPU fallback"):
         scoring.token_logprobs(torch.zeros(2, 8), *[t] * 6)
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_launches_on_the_tensors_device(monkeypatch, current):
+    """The call runs with the tensors' device current and on its stream, whichever was current before."""
+    seen, now = [], [current]
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.was, now[0] = now[0], self.dev
+
+        def __exit__(self, *_):
+            now[0] = self.was
+
+    class Lib:
+        def qwz_op(self, *args):
+            seen.append((now[0], args))
+            return 0
+
+    monkeypatch.setattr(batch, "_current_device", lambda: now[0])
+    monkeypatch.setattr(batch, "_raw_stream", lambda dev: 100 + dev)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(batch._lib, "load", Lib)
+    batch._launch(1, "qwz_op", 7, 8)
+    assert seen == [(1, (7, 8, 101))] and now == [current]
