@@ -7,6 +7,8 @@ A drop-in for the attention hot path of the Qwarz engine:
   draft_attention   `DecodeAttention` over the FP8 shadow KV
                     (engine/forward/draft_attention.py)
   sharded           sequence-page sharding over the GPUs of one node (new)
+  batch             many requests over one pool: tables, writer, attention (new)
+  scoring           log probabilities, entropy, top tokens of logits (new)
   ops               torch wrappers of the C ABI (include/qwz_b200.h)
   contract          the split/combine ABI fixtures the reference tests assert
 The kernels live in libqwz_b200.so, built from csrc/ by `python -m qwarz_b200.build`.
