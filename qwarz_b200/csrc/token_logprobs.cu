@@ -14,7 +14,7 @@
 // lower bound tau of the part's K-th largest value; the places of the vectors
 // that reach it (about K a tile) go to a list, and at the end, with the tau of
 // the whole part's maxima, their elements are read again and ranked by counting
-// (reading them at once, a warp a vector, took 61 us where this takes 53).  If
+// (reading them at once, a warp a vector, took 61 us where this took 53).  If
 // the list overflows, the part is read again with that tau, and where equal
 // values overflow the candidates, K rounds of a maximum find the K.  A second
 // kernel, one CTA a row, joins the parts in order; no result depends on the order
@@ -23,11 +23,11 @@
 // What bounds it: the exponentials, 16 a cycle and SM, would take 15 us of the
 // first case below and HBM 21; with what stands around them (unpack, difference,
 // two sums, maxima; two elements an instruction made no difference) the sums alone
-// take 39, the search for the top 20 another 14, a part's beginning and end being
-// half of that.
-// Measured: 448 rows of 151,000 BF16 logits, top 20, 53 us (2.6 TB/s, 40 % of
-// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 10.4 us and 7 rows
-// of 131,072 BF16, top 8, 12.8 us: the latency of two launches and of one part's
+// take 39, the search for the top 20 another 12, a part's beginning and end being
+// half of that.  2, 3, 5, 6 or 8 CTAs an SM are 1 to 15 us slower than 4.
+// Measured: 448 rows of 151,000 BF16 logits, top 20, 51 us (2.6 TB/s, 41 % of
+// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 8.5 us and 7 rows
+// of 131,072 BF16, top 8, 8.7 us: the latency of two launches and of one part's
 // ranking.  A CTA a row took 203 us for the first of these.
 #include "qwz_common.cuh"
 #include "batch_kernels.h"
@@ -483,12 +483,16 @@ __global__ void __launch_bounds__(kLpThreads) lp_merge_kernel(const __grid_const
       cand[have + i] = __ldcg(reinterpret_cast<const unsigned long long*>(recs + (l0 + i / K) * lp_record(K) + 16) + i % K);
     __syncthreads();
     if (tid < K) sorted[tid] = 0ull;
+    if (tid < 16 && n + tid < kLpMergeCand) cand[n + tid] = 0ull;  // the last sixteen are whole
     __syncthreads();
     for (int i = tid; i < n; i += kLpThreads) {
       const unsigned long long mine = cand[i];
       if (mine == 0ull) continue;
-      int rank = 0;
-      for (int j = 0; j < n && rank < K; ++j) rank += cand[j] > mine ? 1 : 0;
+      int rank = 0;  // looked at every sixteen: every one costs 4 us of a 13 us call
+      for (int j = 0; j < n && rank < K; j += 16) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) rank += cand[j + e] > mine ? 1 : 0;
+      }
       if (rank < K) sorted[rank] = mine;
     }
     __syncthreads();
