@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ float w[kBatchMaxCtas];
+  __shared__ float w[kBatchMaxCtas], sums[kBatchMaxCtas];
   __shared__ float red[8];
   __shared__ float4 acc_s[kGroups][kLanes];
   griddep_wait();
@@ -680,8 +680,13 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
   for (int c = blockIdx.z; c < cols; c += gridDim.z) {
     auto stat = [&](int j) { return __ldcg(reinterpret_cast<const float2*>(record(j) + kFewCols * D + 2 * c)); };
     float M = -CUDART_INF_F;
-    for (int j = tid; j < parts; j += 256)
-      if (!empty(j)) M = fmaxf(M, stat(j).x);
+    for (int j = tid; j < parts; j += 256) {
+      const float2 v = stat(j);
+      const bool skip = empty(j);  // its record is another call's
+      w[j] = skip ? -CUDART_INF_F : v.x;
+      sums[j] = skip ? 0.f : v.y;
+      M = fmaxf(M, w[j]);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if ((tid & 31) == 0) red[tid >> 5] = M;
@@ -692,12 +697,8 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
     __syncthreads();
     float L = 0.f;
     for (int j = tid; j < parts; j += 256) {
-      float wt = 0.f;
-      if (!empty(j)) {
-        const float2 v = stat(j);
-        wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
-        L += wt * v.y;
-      }
+      const float wt = w[j] == -CUDART_INF_F ? 0.f : exp2_approx(w[j] - M);
+      L += wt * sums[j];
       w[j] = wt;
     }
 #pragma unroll
@@ -709,15 +710,14 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
     for (int i = 0; i < 8; ++i) L += red[i];
     const int grp = tid / kLanes, ln = tid % kLanes;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int j = grp; j < parts; j += kGroups) {
       const float wj = w[j];
-      if (wj == 0.f) continue;
       const float4 v = __ldcg(reinterpret_cast<const float4*>(record(j) + c * D) + ln);
-      a.x += wj * v.x;
-      a.y += wj * v.y;
-      a.z += wj * v.z;
-      a.w += wj * v.w;
+      a.x += wj == 0.f ? 0.f : wj * v.x;  // (v can be anything where wj is 0)
+      a.y += wj == 0.f ? 0.f : wj * v.y;
+      a.z += wj == 0.f ? 0.f : wj * v.z;
+      a.w += wj == 0.f ? 0.f : wj * v.w;
     }
     acc_s[grp][ln] = a;
     __syncthreads();
