@@ -444,6 +444,7 @@ int qwz_batch_append(const void* k, const void* v, void* k_cache, void* v_cache,
 /*
  * Attention of every request's rows over its pages: row s of the n rows of a
  * request with kv tokens sees tokens j < kv - n + s + 1 (none: the row is 0).
+ * A NaN or +inf score makes its head's row NaN.
  *   q, out  [rows, q_heads, dim] FP16/BF16, row strides in elements (multiples
  *           of 8); q_heads is 1 to 64 times kv_heads
  *   max_rows  host bound of a request's rows

@@ -52,6 +52,13 @@ QWZ_DEVINL Req load_req(const BatchAttnParams& p, int b) {
   return r;
 }
 
+// Weight of a part (m, l) of a row whose parts have the maximum M.  A part
+// without tokens (m -inf, l 0) has none; one that saw nothing but NaN scores (m
+// -inf, l NaN) makes the row NaN, as it would be in one piece.
+QWZ_DEVINL float part_weight(float m, float l, float M) {
+  return m == -CUDART_INF_F ? 0.f * l : exp2_approx(m - M);
+}
+
 // Exclusive scan of one value a thread over the CTA (blockDim.x <= 1024, a
 // multiple of 32); returns the thread's prefix, the CTA's total in `total`.
 QWZ_DEVINL long long block_scan(long long v, long long* warp_sums, long long& total) {

@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
     __syncthreads();
     float L = 0.f;
     for (int j = tid; j < parts; j += 256) {
-      const float wt = w[j] == -CUDART_INF_F ? 0.f : exp2_approx(w[j] - M);
+      const float wt = batch::part_weight(w[j], sums[j], M);
       L += wt * sums[j];
       w[j] = wt;
     }
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     for (int j = lane; j < parts; j += 32) {
       const float2 v = stat(j);
-      const float wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
+      const float wt = batch::part_weight(v.x, v.y, M);
       L += wt * v.y;
       w[j] = wt;
     }

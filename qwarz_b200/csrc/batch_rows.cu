@@ -628,7 +628,8 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       if (__any_sync(kFull, !ok)) break;
       const float m_fin = ref_s[(last & 1) * kRwRows + r];
       float* sums_of = sum_s + (item & 1) * 2 * kRwRows;
-      sums_of[grp * kRwRows + r] = m_own != -CUDART_INF_F ? (la + lb) * exp2_approx(m_own - m_fin) : 0.f;
+      // (without a reference of its own the group's sum is 0, or NaN from NaN scores)
+      sums_of[grp * kRwRows + r] = m_own != -CUDART_INF_F ? (la + lb) * exp2_approx(m_own - m_fin) : la + lb;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kRwSum + wq));
       ok &= mbar_wait(bar(kRwSum + wq), item & 1);
@@ -732,7 +733,7 @@ __global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_co
       float wt = 0.f;
       if (row < rows && !empty(j)) {
         const float2 v = __ldcg(reinterpret_cast<const float2*>(record(j) + kRwRows * D + 2 * row));
-        wt = v.x == -CUDART_INF_F ? 0.f : exp2_approx(v.x - M);
+        wt = batch::part_weight(v.x, v.y, M);
         L += wt * v.y;
       }
       w[tid >> 5][j] = wt;

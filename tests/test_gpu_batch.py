@@ -413,3 +413,19 @@ def test_example_serves_requests():
     got = example.serve(requests=6, steps=25, seed=1, say=lambda *_: None)
     assert got["free"] + got["held"] == got["pages"]
     assert got["lengths"] == got["done"] and got["finished"] > 0 and 0 < got["accepted"] <= got["drafted"]
+
+
+@pytest.mark.parametrize("rows,kv", [([1, 1], [700, 40]), ([1], [30000]), ([9, 9], [700, 300]), ([7], [30000])])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attend_nan_query(rows, kv, value):
+    """A query element that is not finite makes its row and head NaN and nothing
+    else, whether one CTA has the item (the short ones) or many share it."""
+    args, out, ws = run_attend(rows, kv, 24, 4, 256, torch.float16)
+    want, mag = obatch.attend(*args, out, 256 ** -0.5)
+    q = args[0].clone()
+    q[-1, 5, 100] = value
+    got = torch.empty_like(out)
+    batch.attend(q, *args[1:], got, ws, max_rows=max(rows))
+    assert bool(got[-1, 5].isnan().all())
+    got[-1, 5] = out[-1, 5]
+    check(got, want, mag, torch.float16)
