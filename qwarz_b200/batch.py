@@ -164,8 +164,9 @@ def attend(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_len
     """Attention of the rows q [T, q_heads, dim] of all requests over their
     pages, into out (same shape and type; row strides any multiple of 8).
     Row s of a request's n rows sees its first kv - n + s + 1 tokens; a row
-    that sees none is 0, one with a NaN or +inf score NaN.  `max_rows` is a host bound of the rows a request
-    has (1 for a decode step).  q_heads is 1 to 64 times kv_heads."""
+    that sees none is 0, one with a NaN or +inf score NaN.  `max_rows` is a
+    host bound of the rows a request has (1 for a decode step).  q_heads is 1
+    to 64 times kv_heads."""
     dev = _device(q, (k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace))
     P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)
     q_heads = q.shape[1] if q.dim() == 3 else 0

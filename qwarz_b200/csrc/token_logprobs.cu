@@ -16,9 +16,9 @@
 // the whole part's maxima, their elements are read again and ranked by counting
 // (reading them at once, a warp a vector, took 61 us where this took 53).  If
 // the list overflows, the part is read again with that tau, and where equal
-// values overflow the candidates, K rounds of a maximum find the K.  A second
-// kernel, one CTA a row, joins the parts in order; no result depends on the order
-// of atomics.
+// values overflow the candidates, or NaN stands among nothing but -inf, K rounds
+// of a maximum find the K.  A second kernel, one CTA a row, joins the parts in
+// order; no result depends on the order of atomics.
 //
 // What bounds it: the exponentials, 16 a cycle and SM, would take 15 us of the
 // first case below and HBM 21; with what stands around them (unpack, difference,
@@ -342,7 +342,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     // The whole part's maxima give a closer bound, which most of the listed
     // vectors do not reach.
     if (tiles > 2) tau = threshold(tmax);
-    if (n_vec <= kLpList) {
+    // Without a bound the first K places stand for the -inf tokens, which holds
+    // as long as none of them is NaN (a NaN, or +inf, is in the part's sum).
+    bool nan = false;
+    if (tau == -CUDART_INF_F) {
+#pragma unroll 1
+      for (int i = 0; i < kLpThreads / 32; ++i) nan |= red[1][i] != red[1][i];
+    }
+    if (nan) {
+      // ranked below without a list
+    } else if (n_vec <= kLpList) {
       for (int c = tid; c < n_vec; c += kLpThreads) expand(list[c], tau);
     } else {  // the list overflowed
 #pragma unroll 1
@@ -356,7 +365,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
     __syncthreads();
     const int n = n_cand;
     unsigned long long* keys = reinterpret_cast<unsigned long long*>(rec + 16);
-    if (n <= kLpCand) {
+    if (!nan && n <= kLpCand) {
       for (int c = tid; c < max(n, K); c += kLpThreads) {
         if (c < n) {
           const unsigned long long mine = cand[c];
@@ -368,7 +377,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) lp_part_kernel(const __grid_con
         }
       }
     } else {
-      // many equal values: K rounds of the largest key below the last one
+      // many equal values, or NaN among -inf: K rounds of the largest key below the last one
       unsigned long long last = ~0ull;
       for (int k = 0; k < K; ++k) {
         unsigned long long top = 0ull;

@@ -136,3 +136,24 @@ def test_workspace_of_a_larger_call():
         x, ids = logits_of(T, V, dtype, T)
         got, want = run(x, ids, 20, ws), run(x, ids, 20)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [1, 4, 32])
+def test_nan_ranks_after_impossible_tokens(dtype, top):
+    """Rows of -inf with few finite logits and NaN at their beginning, in later
+    parts, and everywhere: NaN takes no place from a -inf token."""
+    x = torch.full((7, 50001), -torch.inf, device="cuda")
+    x[0, 0] = torch.nan
+    x[1, :40] = torch.nan
+    x[1, [100, 30000, 50000]] = torch.tensor([1.0, 3.0, 2.0], device="cuda")
+    x[2, ::2] = torch.nan
+    x[3] = torch.nan
+    x[3, 49999] = -torch.inf
+    x[4, :] = torch.nan
+    x[5, 1:49000] = torch.nan
+    x[5, 20000] = 5.0
+    x[6, 3] = torch.inf
+    x[6, 4:9] = torch.nan
+    check(x.to(dtype), torch.tensor([0, 30000, 1, 49999, 7, 20000, -1], device="cuda"), top)
+    check(x[:, :40].to(dtype), torch.tensor([0, 39, 1, 2, 7, 20, -1], device="cuda"), top)
