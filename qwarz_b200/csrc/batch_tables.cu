@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   __shared__ long long sums[32];
   const int tid = threadIdx.x;
   griddep_wait();
-  const int head = __ldg(p.ring_state), count = __ldg(p.ring_state + 1);
+  const int F = p.ring_size, head = __ldg(p.ring_state), count = __ldg(p.ring_state + 1);
+  const bool state_ok = head >= 0 && head < F && count >= 0 && count <= F;  // else no page moves and no row has a slot
   const int per = (p.requests + kTabThreads - 1) / kTabThreads;
   const int b_lo = min(tid * per, p.requests), b_hi = min(b_lo + per, p.requests);
 
@@ -63,7 +64,9 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   const long long before = batch::block_scan(v, sums, total);
   starts[tid] = before;
   // granted and freed pages: a request is granted while the pool lasts
-  auto denied = [&](const TabReq& t, int first) { return t.n > 0 && (t.wide || (t.grow > 0 && first + t.grow > count)); };
+  auto denied = [&](const TabReq& t, int first) {
+    return t.n > 0 && (!state_ok || t.wide || (t.grow > 0 && first + t.grow > count));
+  };
   v = 0;
   int first = hi32(before);
   for (int b = b_lo; b < b_hi; ++b) {
@@ -77,9 +80,7 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
 
   // the requests: CTA 0 writes the per-request words; the table entries and the
   // ring are shared out by request, a warp copies one request's pages at a time
-  const int F = p.ring_size;
   auto ring_at = [&](long long i) { return (int)((head + i) % F); };
-  const bool state_ok = head >= 0 && head < F && count >= 0 && count <= F;
   int row = lo32(before);
   first = hi32(before);
   for (int k = 0; k < per; ++k) {
@@ -91,8 +92,8 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
     if (mine && blockIdx.x == 0) {
       p.cu_rows[b] = row;
       p.kv_lens[b] = (t.ends || no) ? 0 : t.len + t.n;
-      p.held_out[b] = t.ends ? 0 : t.held + (no ? 0 : t.grow);
-      if (no) flag_error(t.wide ? kErrTableRange : kErrPoolEmpty);
+      p.held_out[b] = t.ends && state_ok ? 0 : t.held + (no || t.ends ? 0 : t.grow);
+      if (no && (t.wide || state_ok)) flag_error(t.wide ? kErrTableRange : kErrPoolEmpty);
     }
     const int pages_moved = t.ends ? t.held : no ? 0 : t.grow;
     unsigned work = __ballot_sync(0xffffffffu, mine && state_ok && pages_moved > 0 &&
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   if (blockIdx.x == 0 && tid == 0) {
     p.cu_rows[p.requests] = rows;
     p.ring_out[0] = state_ok ? ring_at(hi32(pages)) : head;
-    p.ring_out[1] = (int)min((long long)count - hi32(pages) + lo32(pages), (long long)F);
+    p.ring_out[1] = state_ok ? (int)min((long long)count - hi32(pages) + lo32(pages), (long long)F) : count;
     if (!state_ok) flag_error(kErrPageRange);
     if (rows > p.rows) flag_error(kErrSlotRange);  // rows past the slot map's end get no slot
   }
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
       }
       req = b;
       pos = t.len + off;
-      if (!denied(t, first) && state_ok) {
+      if (!denied(t, first)) {
         const int j = pos / kPage;
         int page;
         if (j < t.held) page = p.block_table[(size_t)b * p.table_width + j];

@@ -88,6 +88,29 @@ def test_tables_many(R):
     assert not why
 
 
+@pytest.mark.parametrize("head,count", [(16, 3), (-1, 3), (2, 17), (2, -1)])
+def test_tables_bad_ring_state(head, count):
+    """A ring state that cannot be: no page moves, no request keeps rows of the
+    step (all slots -1, kv_lens 0 where there are rows), and the state that
+    comes out is the one that went in."""
+    lengths, new_rows, held, width, rows = [10, 300, 0, 700, 5, 900], [3, -1, 600, 1, 0, 200], [1, 2, 0, 3, 1, 4], 4, 810
+    table = np.arange(24).reshape(6, 4)
+    ring = np.arange(16) + 30
+    out = {"cu_rows": i32([-7] * 7), "kv_lens": i32([-7] * 6), "held_out": i32([-7] * 6), "ring_out": i32([-7, -7]),
+           "slots": i32([-7] * rows), "positions": i32([-7] * rows), "request_of": i32([-7] * rows)}
+    table_d, ring_d = i32(table), i32(ring)
+    batch.build_tables(i32(lengths), i32(new_rows), i32(held), ring_d, i32([head, count]), table_d, *out.values())
+    assert _lib.device_error(clear=True) == 2 | 1  # the state, and the last request, which does not fit its table row
+    got = {k: t.tolist() for k, t in out.items()}
+    assert got["cu_rows"] == [0, 3, 3, 603, 604, 604, 804]
+    assert got["kv_lens"] == [0, 0, 0, 0, 5, 0]
+    assert got["held_out"] == held and got["ring_out"] == [head, count]
+    assert np.array_equal(table_d.cpu().numpy(), table) and np.array_equal(ring_d.cpu().numpy(), ring)
+    assert got["slots"] == [-1] * rows
+    assert got["request_of"] == [0] * 3 + [2] * 600 + [3] + [5] * 200 + [-1] * 6
+    assert got["positions"] == [10, 11, 12] + list(range(600)) + [700] + list(range(900, 1100)) + [0] * 6
+
+
 # ------------------------------------------------------------------- append
 def without_nan(x):
     """The device writers' rule for NaN, which the oracle's numpy maximum does not
