@@ -10,8 +10,10 @@
 // b, position p = lengths[b] + r, gets slot table[b][p / 256] * 256 + p % 256.
 // All of it is a few bytes a request and 12 bytes a row: the launch and the
 // latency of one scan bound it, so every CTA scans all requests by itself (two
-// packed 64-bit scans) instead of waiting for another CTA, and then fills its
-// part of the rows and of the tables.  Measured: 5.7 us for 8 requests, 8.5 us for
+// scans of a pair) instead of waiting for another CTA, and then fills its part of
+// the rows and of the tables.  Requests that are denied count with all they ask
+// for, which need not fit 32 bits together: sums stop at 2^31 - 1, beyond every
+// row of the slot map and every free page.  Measured: 5.7 us for 8 requests, 8.5 us for
 // 2,048 with prompts (a thread copying a request's pages: 22 us).
 #include "batch_common.cuh"
 #include "nvfp4_quant.cuh"
@@ -40,15 +42,39 @@ QWZ_DEVINL TabReq tab_req(const BatchTablesParams& p, int b) {
   return t;
 }
 
-QWZ_DEVINL long long pack(int lo, int hi) { return ((long long)hi << 32) | (unsigned)lo; }
-QWZ_DEVINL int lo32(long long v) { return (int)(unsigned)v; }
-QWZ_DEVINL int hi32(long long v) { return (int)(v >> 32); }
+// Sum of two counts, at most 2^31 - 1 (associative for counts).
+QWZ_DEVINL int add_sat(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
+QWZ_DEVINL int2 add_sat(int2 a, int2 b) { return make_int2(add_sat(a.x, b.x), add_sat(a.y, b.y)); }
+
+// Exclusive scan of a pair of counts a thread over the CTA; the CTA's total in
+// `total`.
+QWZ_DEVINL int2 tab_scan(int2 v, int2* warp_sums, int2& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int2 y = make_int2(__shfl_up_sync(0xffffffffu, v.x, o), __shfl_up_sync(0xffffffffu, v.y, o));
+    if (lane >= o) v = add_sat(v, y);
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int2 before = make_int2(0, 0);
+  total = make_int2(0, 0);
+#pragma unroll
+  for (int w = 0; w < kTabThreads / 32; ++w) {
+    const int2 s = warp_sums[w];
+    if (w < warp) before = add_sat(before, s);
+    total = add_sat(total, s);
+  }
+  __syncthreads();
+  const int2 y = make_int2(__shfl_up_sync(0xffffffffu, v.x, 1), __shfl_up_sync(0xffffffffu, v.y, 1));
+  return lane > 0 ? add_sat(before, y) : before;
+}
 
 }  // namespace
 
 __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_constant__ BatchTablesParams p) {
-  __shared__ long long starts[kTabThreads];  // (rows, grown pages) before each thread's requests
-  __shared__ long long sums[32];
+  __shared__ int2 starts[kTabThreads];  // (rows, grown pages) before each thread's requests
+  __shared__ int2 sums[kTabThreads / 32];
   const int tid = threadIdx.x;
   griddep_wait();
   const int F = p.ring_size, head = __ldg(p.ring_state), count = __ldg(p.ring_state + 1);
@@ -56,33 +82,33 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   const int per = (p.requests + kTabThreads - 1) / kTabThreads;
   const int b_lo = min(tid * per, p.requests), b_hi = min(b_lo + per, p.requests);
 
-  long long v = 0, total;
+  int2 v = make_int2(0, 0), total;
   for (int b = b_lo; b < b_hi; ++b) {
     const TabReq t = tab_req(p, b);
-    v += pack(t.n, t.grow);
+    v = add_sat(v, make_int2(t.n, t.grow));
   }
-  const long long before = batch::block_scan(v, sums, total);
+  const int2 before = tab_scan(v, sums, total);
   starts[tid] = before;
   // granted and freed pages: a request is granted while the pool lasts
   auto denied = [&](const TabReq& t, int first) {
-    return t.n > 0 && (!state_ok || t.wide || (t.grow > 0 && first + t.grow > count));
+    return t.n > 0 && (!state_ok || t.wide || (t.grow > 0 && t.grow > count - first));
   };
-  v = 0;
-  int first = hi32(before);
+  v = make_int2(0, 0);
+  int first = before.y;
   for (int b = b_lo; b < b_hi; ++b) {
     const TabReq t = tab_req(p, b);
-    v += pack(t.ends ? t.held : 0, denied(t, first) ? 0 : t.grow);
-    first += t.grow;
+    v = add_sat(v, make_int2(t.ends ? t.held : 0, denied(t, first) ? 0 : t.grow));
+    first = add_sat(first, t.grow);
   }
-  long long pages;
-  int freed = lo32(batch::block_scan(v, sums, pages));
-  const int rows = lo32(total);
+  int2 pages;
+  int freed = tab_scan(v, sums, pages).x;
+  const int rows = total.x;
 
   // the requests: CTA 0 writes the per-request words; the table entries and the
   // ring are shared out by request, a warp copies one request's pages at a time
   auto ring_at = [&](long long i) { return (int)((head + i) % F); };
-  int row = lo32(before);
-  first = hi32(before);
+  int row = before.x;
+  first = before.y;
   for (int k = 0; k < per; ++k) {
     const int b = b_lo + k;
     const bool mine = b < b_hi;
@@ -115,14 +141,14 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
         }
       }
     }
-    row += t.n;
-    first += t.grow;
-    freed += t.ends ? t.held : 0;
+    row = add_sat(row, t.n);
+    first = add_sat(first, t.grow);
+    freed = add_sat(freed, t.ends ? t.held : 0);
   }
   if (blockIdx.x == 0 && tid == 0) {
     p.cu_rows[p.requests] = rows;
-    p.ring_out[0] = state_ok ? ring_at(hi32(pages)) : head;
-    p.ring_out[1] = state_ok ? (int)min((long long)count - hi32(pages) + lo32(pages), (long long)F) : count;
+    p.ring_out[0] = state_ok ? ring_at(pages.y) : head;
+    p.ring_out[1] = state_ok ? (int)min((long long)count - pages.y + pages.x, (long long)F) : count;
     if (!state_ok) flag_error(kErrPageRange);
     if (rows > p.rows) flag_error(kErrSlotRange);  // rows past the slot map's end get no slot
   }
@@ -133,18 +159,18 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
     if (r < rows) {
       int at = 0;
       for (int step = kTabThreads / 2; step > 0; step >>= 1)
-        if (lo32(starts[at + step]) <= r) at += step;
-      int off = (int)r - lo32(starts[at]);
-      first = hi32(starts[at]);
+        if (starts[at + step].x <= r) at += step;
+      int off = (int)r - starts[at].x;
+      first = starts[at].y;
       int b = at * per;
       TabReq t = tab_req(p, b);
       while (off >= t.n && b + 1 < p.requests) {
         off -= t.n;
-        first += t.grow;
+        first = add_sat(first, t.grow);
         t = tab_req(p, ++b);
       }
       req = b;
-      pos = t.len + off;
+      pos = add_sat(t.len, off);
       if (!denied(t, first)) {
         const int j = pos / kPage;
         int page;

@@ -111,6 +111,48 @@ def test_tables_bad_ring_state(head, count):
     assert got["positions"] == [10, 11, 12] + list(range(600)) + [700] + list(range(900, 1100)) + [0] * 6
 
 
+@pytest.mark.parametrize("wide", [1, 2, 3, 700])
+def test_tables_rows_past_32_bits(wide):
+    """Requests whose rows do not fit their tables, and whose sum does not fit 32
+    bits: they are denied, the others get their pages in order, row offsets stop
+    at the largest int32."""
+    big = 2 ** 31 - 1
+    lengths, new_rows = [0] + [0] * wide + [2048, 255, 0], [2] + [big] * wide + [3, 2, 300]
+    held, pool, width, rows = [0] + [0] * wide + [8, 1, 0], 24, 8, 9
+    table, ring = np.full((len(held), width), -1), np.arange(pool) + 50
+    table[-3], table[-2, 0] = np.arange(8), 8
+    want, why = obatch.build_tables(lengths, new_rows, held, ring, (20, 10), table, rows)
+    assert why == {"wide"} and want["ring_out"].tolist() == [0, 6]
+    want["cu_rows"] = np.minimum(want["cu_rows"], big)
+    R = len(held)
+    out = {"block_table": i32(table), "ring": i32(ring), "cu_rows": i32([-7] * (R + 1)), "kv_lens": i32([-7] * R),
+           "held_out": i32([-7] * R), "ring_out": i32([-7, -7]), "slots": i32([-7] * rows),
+           "positions": i32([-7] * rows), "request_of": i32([-7] * rows)}
+    names = list(out)
+    batch.build_tables(i32(lengths), i32(new_rows), i32(held), out["ring"], i32([20, 10]), out["block_table"],
+                       *[out[n] for n in names[2:]])
+    assert _lib.device_error(clear=True) == 1 | 4  # a table row too short, more rows than the slot map has
+    for name, t in out.items():
+        assert np.array_equal(t.cpu().numpy(), want[name]), name
+
+
+def test_tables_pages_past_32_bits():
+    """Denied requests may ask for more pages together than 32 bits count."""
+    R, width = 520, 1 << 22
+    lengths = [0] + [2 ** 30 - 1] * (R - 2) + [5]
+    new_rows, held = [1] + [1] * (R - 2) + [1], [0] * (R - 1) + [1]
+    table = torch.empty(R, width, dtype=torch.int32, device="cuda")
+    table[R - 1, 0] = 3
+    ring = i32([7, 8, 9, -1])
+    out = [i32([-7] * (R + 1)), i32([-7] * R), i32([-7] * R), i32([-7, -7])] + [i32([-7] * R) for _ in range(3)]
+    batch.build_tables(i32(lengths), i32(new_rows), i32(held), ring, i32([0, 3]), table, *out)
+    assert _lib.device_error(clear=True) == 16
+    assert out[0].tolist() == list(range(R + 1)) and out[3].tolist() == [1, 2]
+    assert out[1].tolist() == [1] + [0] * (R - 2) + [6] and out[2].tolist() == [1] + [0] * (R - 2) + [1]
+    assert out[4].tolist() == [7 * PAGE] + [-1] * (R - 2) + [3 * PAGE + 5]
+    assert out[5].tolist() == [0] + [2 ** 30 - 1] * (R - 2) + [5]
+
+
 # ------------------------------------------------------------------- append
 def without_nan(x):
     """The device writers' rule for NaN, which the oracle's numpy maximum does not
