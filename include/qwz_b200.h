@@ -422,10 +422,12 @@ int qwz_k8v4_gather(const void* words, const void* scales, const int32_t* block_
  * not fit its table row (QWZ_DEVERR_TABLE_RANGE), or, from the first one that
  * the free pages do not cover on, any request that needs a page
  * (QWZ_DEVERR_POOL_EMPTY), is denied: it takes no page, its rows get slot -1
- * and its kv_lens is 0.  A request that ends has kv_lens 0 and held_out 0.  A
- * ring_state with first outside 0 .. ring_size - 1 or count outside
- * 0 .. ring_size sets QWZ_DEVERR_PAGE_RANGE: every request with rows is denied,
- * those that end keep their pages, and ring_out is ring_state.
+ * and its kv_lens is 0.  A request that ends has kv_lens 0 and held_out 0.
+ * From the first one whose pages find no place behind the free ones of the ring
+ * on, those that end keep their pages (held_out held, QWZ_DEVERR_POOL_EMPTY) and
+ * can be ended again.  A ring_state with first outside 0 .. ring_size - 1 or
+ * count outside 0 .. ring_size sets QWZ_DEVERR_PAGE_RANGE: every request with
+ * rows is denied, those that end keep their pages, and ring_out is ring_state.
  */
 int qwz_batch_tables(const int32_t* lengths, const int32_t* new_rows, const int32_t* held, int32_t* ring,
                      const int32_t* ring_state, int32_t* block_table, int32_t* cu_rows, int32_t* kv_lens,

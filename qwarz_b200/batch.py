@@ -99,7 +99,9 @@ def build_tables(lengths, new_rows, held, ring, ring_state, block_table, cu_rows
     `request_of`; these may be longer than the step has rows (the rest gets
     -1, 0, -1).  To commit a step, use held_out, ring_out and the lengths
     that were kept (rejected rows need no undoing: their slots are written
-    again) as the next step's inputs.  All tensors int32."""
+    again) as the next step's inputs.  A request that could not be served has
+    kv_lens 0 and slots of -1, and keeps held_out = held; the device error word
+    says why (include/qwz_b200.h).  All tensors int32."""
     dev = _device(lengths, (new_rows, held, ring, ring_state, block_table, cu_rows, kv_lens, held_out, ring_out,
                             slots, positions, request_of))
     _int32(("lengths", "new_rows", "held", "ring", "ring_state", "block_table", "cu_rows", "kv_lens", "held_out",

@@ -6,15 +6,17 @@
 // new[b] rows, or ends (new[b] < 0).  With
 //   grow[b] = max(0, ceil((lengths[b] + new[b]) / 256) - held[b])  (new[b] > 0)
 // pages are taken from a ring of free ids in request order (exclusive scan of
-// grow), those of requests that end go behind the free ones.  Row r of request
-// b, position p = lengths[b] + r, gets slot table[b][p / 256] * 256 + p % 256.
+// grow), those of requests that end go behind the free ones as far as the ring
+// has places there.  Row r of request b, position p = lengths[b] + r, gets slot
+// table[b][p / 256] * 256 + p % 256.
 // All of it is a few bytes a request and 12 bytes a row: the launch and the
-// latency of one scan bound it, so every CTA scans all requests by itself (two
-// scans of a pair) instead of waiting for another CTA, and then fills its part of
-// the rows and of the tables.  Requests that are denied count with all they ask
-// for, which need not fit 32 bits together: sums stop at 2^31 - 1, beyond every
-// row of the slot map and every free page.  Measured: 5.7 us for 8 requests, 8.5 us for
-// 2,048 with prompts (a thread copying a request's pages: 22 us).
+// latency of one scan bound it, so every CTA scans all requests by itself (one
+// scan of three counts) instead of waiting for another CTA, and then fills its
+// part of the rows and of the tables.  Requests that are denied count with all
+// they ask for, which need not fit 32 bits together: sums stop at 2^31 - 1, beyond
+// every row of the slot map and every free page.  Measured: 4.8 us for 8 requests,
+// 7.1 us for 2,048 with prompts (a thread copying a request's pages: 22 us; two
+// scans, of pages asked for and of pages granted: 6.5 and 9.0 us).
 #include "batch_common.cuh"
 #include "nvfp4_quant.cuh"
 
@@ -44,29 +46,38 @@ QWZ_DEVINL TabReq tab_req(const BatchTablesParams& p, int b) {
 
 // Sum of two counts, at most 2^31 - 1 (associative for counts).
 QWZ_DEVINL int add_sat(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
-QWZ_DEVINL int2 add_sat(int2 a, int2 b) { return make_int2(add_sat(a.x, b.x), add_sat(a.y, b.y)); }
+// Rows, pages asked for and pages of requests that end.
+struct TabSum {
+  int rows, grow, freed;
+};
+QWZ_DEVINL TabSum add_sat(TabSum a, TabSum b) {
+  return {add_sat(a.rows, b.rows), add_sat(a.grow, b.grow), add_sat(a.freed, b.freed)};
+}
+QWZ_DEVINL TabSum tab_sum(const TabReq& t) { return {t.n, t.grow, t.ends ? t.held : 0}; }
+QWZ_DEVINL TabSum tab_shfl_up(TabSum v, int o) {
+  return {__shfl_up_sync(0xffffffffu, v.rows, o), __shfl_up_sync(0xffffffffu, v.grow, o),
+          __shfl_up_sync(0xffffffffu, v.freed, o)};
+}
 
-// Exclusive scan of a pair of counts a thread over the CTA; the CTA's total in
-// `total`.
-QWZ_DEVINL int2 tab_scan(int2 v, int2* warp_sums, int2& total) {
+// Exclusive scan over the CTA; all threads' rows in `rows`.
+QWZ_DEVINL TabSum tab_scan(TabSum v, TabSum* warp_sums, int& rows) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int2 y = make_int2(__shfl_up_sync(0xffffffffu, v.x, o), __shfl_up_sync(0xffffffffu, v.y, o));
+    const TabSum y = tab_shfl_up(v, o);
     if (lane >= o) v = add_sat(v, y);
   }
   if (lane == 31) warp_sums[warp] = v;
   __syncthreads();
-  int2 before = make_int2(0, 0);
-  total = make_int2(0, 0);
+  TabSum before = {0, 0, 0};
+  rows = 0;
 #pragma unroll
   for (int w = 0; w < kTabThreads / 32; ++w) {
-    const int2 s = warp_sums[w];
+    const TabSum s = warp_sums[w];
     if (w < warp) before = add_sat(before, s);
-    total = add_sat(total, s);
+    rows = add_sat(rows, s.rows);
   }
-  __syncthreads();
-  const int2 y = make_int2(__shfl_up_sync(0xffffffffu, v.x, 1), __shfl_up_sync(0xffffffffu, v.y, 1));
+  const TabSum y = tab_shfl_up(v, 1);
   return lane > 0 ? add_sat(before, y) : before;
 }
 
@@ -74,7 +85,8 @@ QWZ_DEVINL int2 tab_scan(int2 v, int2* warp_sums, int2& total) {
 
 __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_constant__ BatchTablesParams p) {
   __shared__ int2 starts[kTabThreads];  // (rows, grown pages) before each thread's requests
-  __shared__ int2 sums[kTabThreads / 32];
+  __shared__ TabSum sums[kTabThreads / 32];
+  __shared__ int granted_s, put_back_s;
   const int tid = threadIdx.x;
   griddep_wait();
   const int F = p.ring_size, head = __ldg(p.ring_state), count = __ldg(p.ring_state + 1);
@@ -82,73 +94,71 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   const int per = (p.requests + kTabThreads - 1) / kTabThreads;
   const int b_lo = min(tid * per, p.requests), b_hi = min(b_lo + per, p.requests);
 
-  int2 v = make_int2(0, 0), total;
-  for (int b = b_lo; b < b_hi; ++b) {
-    const TabReq t = tab_req(p, b);
-    v = add_sat(v, make_int2(t.n, t.grow));
-  }
-  const int2 before = tab_scan(v, sums, total);
-  starts[tid] = before;
-  // granted and freed pages: a request is granted while the pool lasts
+  if (tid == 0) granted_s = put_back_s = 0;
+  TabSum v = {0, 0, 0};
+  for (int b = b_lo; b < b_hi; ++b) v = add_sat(v, tab_sum(tab_req(p, b)));
+  int rows;
+  v = tab_scan(v, sums, rows);  // before this thread's requests
+  starts[tid] = make_int2(v.rows, v.grow);
+  // granted and freed pages: a request is granted while the pool lasts, one that
+  // ends puts its pages back while the ring has room (places that this step takes
+  // from do not count: another CTA may not have read them yet)
   auto denied = [&](const TabReq& t, int first) {
     return t.n > 0 && (!state_ok || t.wide || (t.grow > 0 && t.grow > count - first));
   };
-  v = make_int2(0, 0);
-  int first = before.y;
-  for (int b = b_lo; b < b_hi; ++b) {
-    const TabReq t = tab_req(p, b);
-    v = add_sat(v, make_int2(t.ends ? t.held : 0, denied(t, first) ? 0 : t.grow));
-    first = add_sat(first, t.grow);
-  }
-  int2 pages;
-  int freed = tab_scan(v, sums, pages).x;
-  const int rows = total.x;
+  auto kept = [&](const TabReq& t, int freed) { return t.ends && t.held > 0 && (!state_ok || t.held > F - count - freed); };
 
   // the requests: CTA 0 writes the per-request words; the table entries and the
   // ring are shared out by request, a warp copies one request's pages at a time
   auto ring_at = [&](long long i) { return (int)((head + i) % F); };
-  int row = before.x;
-  first = before.y;
+  int granted = 0, put_back = 0;  // pages, up to the thread's last request that has any
   for (int k = 0; k < per; ++k) {
     const int b = b_lo + k;
     const bool mine = b < b_hi;
     TabReq t = {0, 0, 0, 0, false, false};
     if (mine) t = tab_req(p, b);
-    const bool no = denied(t, first);
+    const bool no = denied(t, v.grow), stays = kept(t, v.freed);
+    if (t.grow > 0 && !no) granted = v.grow + t.grow;
+    if (t.ends && t.held > 0 && !stays) put_back = v.freed + t.held;
     if (mine && blockIdx.x == 0) {
-      p.cu_rows[b] = row;
+      p.cu_rows[b] = v.rows;
       p.kv_lens[b] = (t.ends || no) ? 0 : t.len + t.n;
-      p.held_out[b] = t.ends && state_ok ? 0 : t.held + (no || t.ends ? 0 : t.grow);
-      if (no && (t.wide || state_ok)) flag_error(t.wide ? kErrTableRange : kErrPoolEmpty);
+      p.held_out[b] = t.ends ? (stays ? t.held : 0) : t.held + (no ? 0 : t.grow);
+      if (no && t.wide) flag_error(kErrTableRange);
+      else if ((no || stays) && state_ok) flag_error(kErrPoolEmpty);
     }
-    const int pages_moved = t.ends ? t.held : no ? 0 : t.grow;
-    unsigned work = __ballot_sync(0xffffffffu, mine && state_ok && pages_moved > 0 &&
-                                                   (unsigned)b % gridDim.x == blockIdx.x);
+    const int pages_moved = t.ends ? (stays ? 0 : t.held) : no ? 0 : t.grow;
+    unsigned work = __ballot_sync(0xffffffffu, mine && pages_moved > 0 && (unsigned)b % gridDim.x == blockIdx.x);
     while (work) {
       const int src = __ffs(work) - 1;
       work &= work - 1;
       const int n = __shfl_sync(0xffffffffu, pages_moved, src), ends = __shfl_sync(0xffffffffu, (int)t.ends, src);
       const int have = __shfl_sync(0xffffffffu, t.held, src);
-      const int from = __shfl_sync(0xffffffffu, t.ends ? freed : first, src);
+      const int from = __shfl_sync(0xffffffffu, t.ends ? v.freed : v.grow, src);
       int32_t* table = p.block_table + (size_t)__shfl_sync(0xffffffffu, b, src) * p.table_width;
       for (int j = tid & 31; j < n; j += 32) {
         if (ends) {
-          const long long at = (long long)count + from + j;
-          if (at < F) p.ring[ring_at(at)] = table[j];
-          else flag_error(kErrPoolEmpty);  // more pages than the ring has places
+          p.ring[ring_at((long long)count + from + j)] = table[j];
         } else {
           table[have + j] = __ldg(p.ring + ring_at((long long)from + j));
         }
       }
     }
-    row = add_sat(row, t.n);
-    first = add_sat(first, t.grow);
-    freed = add_sat(freed, t.ends ? t.held : 0);
+    v = add_sat(v, tab_sum(t));
   }
+  if (blockIdx.x == 0) {  // no request is served after one that was not: the furthest is the sum
+    granted = __reduce_max_sync(0xffffffffu, granted);
+    put_back = __reduce_max_sync(0xffffffffu, put_back);
+    if ((tid & 31) == 0) {
+      atomicMax(&granted_s, granted);
+      atomicMax(&put_back_s, put_back);
+    }
+  }
+  __syncthreads();  // (and `starts` is whole)
   if (blockIdx.x == 0 && tid == 0) {
     p.cu_rows[p.requests] = rows;
-    p.ring_out[0] = state_ok ? ring_at(pages.y) : head;
-    p.ring_out[1] = state_ok ? (int)min((long long)count - pages.y + pages.x, (long long)F) : count;
+    p.ring_out[0] = state_ok ? ring_at(granted_s) : head;
+    p.ring_out[1] = state_ok ? count - granted_s + put_back_s : count;
     if (!state_ok) flag_error(kErrPageRange);
     if (rows > p.rows) flag_error(kErrSlotRange);  // rows past the slot map's end get no slot
   }
@@ -160,8 +170,7 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
       int at = 0;
       for (int step = kTabThreads / 2; step > 0; step >>= 1)
         if (starts[at + step].x <= r) at += step;
-      int off = (int)r - starts[at].x;
-      first = starts[at].y;
+      int off = (int)r - starts[at].x, first = starts[at].y;
       int b = at * per;
       TabReq t = tab_req(p, b);
       while (off >= t.n && b + 1 < p.requests) {

@@ -153,6 +153,31 @@ def test_tables_pages_past_32_bits():
     assert out[5].tolist() == [0] + [2 ** 30 - 1] * (R - 2) + [5]
 
 
+def test_tables_ring_without_room():
+    """Pages that find no place behind the free ones stay with the request that
+    ends, and so do those of any that ends after it: no page is lost, and the
+    count is of pages that are in the ring."""
+    table = i32([[1, 2, -1], [3, -1, -1], [4, 5, -1], [6, -1, -1], [-1, -1, -1]])
+    ring = i32([40, 41, -1, -1, 42])  # 42, 40, 41 are free
+    out = {"cu_rows": i32([-7] * 6), "kv_lens": i32([-7] * 5), "held_out": i32([-7] * 5), "ring_out": i32([-7, -7]),
+           "slots": i32([-7] * 3), "positions": i32([-7] * 3), "request_of": i32([-7] * 3)}
+    for _ in range(2):
+        batch.build_tables(i32([300, 10, 400, 20, 0]), i32([3, -1, -1, -1, -1]), i32([2, 1, 2, 1, 0]), ring,
+                           i32([4, 3]), table, *out.values())
+        assert _lib.device_error(clear=True) == 16
+        got = {k: t.tolist() for k, t in out.items()}
+        assert ring.tolist() == [40, 41, 3, -1, 42]  # one of two places taken: request 2 needs two, request 3 comes after it
+        assert got["held_out"] == [2, 0, 2, 1, 0] and got["ring_out"] == [4, 4]
+        assert got["kv_lens"] == [303, 0, 0, 0, 0] and got["cu_rows"] == [0, 3, 3, 3, 3, 3]
+    # ended again once there is room
+    ring2 = i32([40, 41, 3, -1, -1, -1, -1, 42])
+    batch.build_tables(i32([303, 0, 0, 0, 0]), i32([300, 0, -1, -1, 0]), i32([2, 0, 2, 1, 0]), ring2, i32([7, 4]), table,
+                       out["cu_rows"], out["kv_lens"], out["held_out"], out["ring_out"],
+                       *[i32([0] * 300) for _ in range(3)])
+    assert ring2.tolist() == [40, 41, 3, 4, 5, 6, -1, 42]
+    assert out["held_out"].tolist() == [3, 0, 0, 0, 0] and out["ring_out"].tolist() == [0, 6]
+
+
 # ------------------------------------------------------------------- append
 def without_nan(x):
     """The device writers' rule for NaN, which the oracle's numpy maximum does not
