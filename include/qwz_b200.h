@@ -414,10 +414,10 @@ int qwz_k8v4_gather(const void* words, const void* scales, const int32_t* block_
  *                 places first .. first + count - 1 modulo ring_size
  * Pages are taken from the ring in request order and entered in block_table
  * (in place); those of requests that end are put back behind the free ones.
- * Outputs (no storage shared with the inputs, so a step may be built again
- * from the same state): cu_rows, kv_lens, held_out [R], ring_out [2], and for
- * row r < rows slots[r], positions[r] (token position), request_of[r].  Rows
- * past cu_rows[R] get slot -1, position 0, request -1.  More than `rows` rows
+ * Outputs (no storage shared with any of the above, so a step may be built again
+ * from the same state; ring and block_table share none with what is read
+ * either): cu_rows, kv_lens, held_out [R], ring_out [2], and for row r < rows
+ * slots[r], positions[r] (token position), request_of[r].  Rows past cu_rows[R] get slot -1, position 0, request -1.  More than `rows` rows
  * set QWZ_DEVERR_SLOT_RANGE; cu_rows stops at 2^31 - 1.  A request that does
  * not fit its table row (QWZ_DEVERR_TABLE_RANGE), or, from the first one that
  * the free pages do not cover on, any request that needs a page

@@ -50,8 +50,27 @@ int qwz_batch_tables(const int32_t* lengths, const int32_t* new_rows, const int3
   if (requests < 1 || requests > (1 << 20)) return fail(QWZ_EINVAL, "requests must be in 1..2^20");
   if (table_width < 1 || table_width > (1 << 22)) return fail(QWZ_EINVAL, "table_width must be in 1..2^22");
   if (ring_size < 1) return fail(QWZ_EINVAL, "ring_size must be positive");
-  if (held_out == held || kv_lens == lengths || ring_out == ring_state || cu_rows == lengths || cu_rows == held)
-    return fail(QWZ_EINVAL, "outputs must not share storage with inputs");
+  // every CTA reads all of the inputs while others write
+  struct Array {
+    const int32_t* at;
+    int64_t n;
+  };
+  const Array both[] = {{ring, ring_size}, {block_table, (int64_t)requests * table_width}};  // read and written
+  const Array reads[] = {{lengths, requests}, {new_rows, requests}, {held, requests}, {ring_state, 2}};
+  const Array writes[] = {{cu_rows, requests + 1}, {kv_lens, requests}, {held_out, requests}, {ring_out, 2},
+                          {slots, rows},           {positions, rows},   {request_of, rows}};
+  auto shared = [](const Array& a, const Array& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.n > 0 && b.n > 0 && x < y + 4 * (uintptr_t)b.n && y < x + 4 * (uintptr_t)a.n;
+  };
+  bool clash = shared(both[0], both[1]);
+  for (const Array& r : reads) {
+    for (const Array& w : writes) clash |= shared(r, w);
+    for (const Array& w : both) clash |= shared(r, w);
+  }
+  for (const Array& r : both)
+    for (const Array& w : writes) clash |= shared(r, w);
+  if (clash) return fail(QWZ_EINVAL, "outputs must not share storage with inputs");
   const int sms = batch_sms();
   if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
   qwz::BatchTablesParams p{lengths, new_rows, held, ring_state, ring, block_table, cu_rows, kv_lens, held_out,

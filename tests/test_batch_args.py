@@ -36,6 +36,18 @@ def test_tables(lib, addr, change, needle):
     refused(lib, lib.qwz_batch_tables(*args), needle)
 
 
+@pytest.mark.parametrize("out,other,at", [
+    (7, 1, 0), (8, 0, 0), (8, 1, 0), (9, 0, 0), (9, 2, 4), (6, 1, 0), (6, 4, 0), (10, 0, 0), (11, 2, 0), (12, 3, 0),
+    (7, 0, 4), (7, 0, -4), (6, 5, 64), (5, 0, 0), (5, 3, 0), (3, 2, 0),   # in part; tables and ring, which are written too
+])
+def test_tables_shared_storage(lib, addr, out, other, at):
+    """An array that is written and shares bytes with one that is read is refused:
+    every CTA reads all of the inputs while others write."""
+    args = [addr + 256 * i for i in range(13)] + [4, 8, 16, 32, None]
+    args[out] = args[other] + at
+    refused(lib, lib.qwz_batch_tables(*args), "share storage")
+
+
 @pytest.mark.parametrize("change,needle", [
     ({0: None}, "k, v and slots"), ({2: None}, "required"), ({0: "odd"}, "aligned"), ({10: 4 * 256 - 8}, "k: the row stride"),
     ({11: 4 * 256 + 4}, "v: the row stride"), ({12: 0}, "num_kv_heads"), ({13: 96}, "head_dim"), ({14: 0}, "num_pages"),
