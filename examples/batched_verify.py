@@ -137,7 +137,8 @@ def serve(requests=8, steps=20, seed=0, say=print):
             targets += [-1] * (len(row) - 1) + guess + [-1]
             new.append(len(row) + len(guess))
         out = server.step(model, torch.tensor(new, dtype=torch.int32, device=device),
-                          torch.tensor(tokens, device=device), torch.tensor(targets, device=device), max(max(new), 1))
+                          torch.tensor(tokens, dtype=torch.long, device=device),
+                          torch.tensor(targets, dtype=torch.long, device=device), max(max(new), 1))
         logprob, _, ids = (t.cpu() for t in out)
         for r, p in enumerate(plan):
             if p is None:

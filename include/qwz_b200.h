@@ -456,10 +456,11 @@ int qwz_batch_append(const void* k, const void* v, void* k_cache, void* v_cache,
  *   max_rows  host bound of a request's rows
  *   workspace qwz_batch_attend_workspace_bytes(head_dim) bytes (0: bad
  *           head_dim), 16-byte aligned, for one call at a time
- * Rows outside every request are not written.  A length beyond the table, a
- * row range outside [0, rows] or more than max_rows rows set
- * QWZ_DEVERR_TABLE_RANGE (the length is clipped, the request skipped); a table entry outside the pool sets QWZ_DEVERR_PAGE_RANGE
- * and its tokens count as absent.
+ * A call without rows or requests does nothing.  Rows outside every request are
+ * not written.  A length beyond the table, a row range outside [0, rows] or more
+ * than max_rows rows set QWZ_DEVERR_TABLE_RANGE (the length is clipped, the
+ * request skipped); a table entry outside the pool sets QWZ_DEVERR_PAGE_RANGE and
+ * its tokens count as absent.
  */
 int64_t qwz_batch_attend_workspace_bytes(int32_t head_dim);
 int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,

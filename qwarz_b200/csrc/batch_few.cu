@@ -866,7 +866,6 @@ int batch_few_box_rows(int dim) { return dim == 256 ? Few<256>::kTok : dim == 12
 
 cudaError_t launch_batch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
                                 cudaStream_t stream) {
-  if (p.requests <= 0 || p.rows <= 0) return cudaSuccess;
   return dtype == kDtypeBF16 ? launch_attend<__nv_bfloat16>(p, maps, dim, sms, stream)
                              : launch_attend<__half>(p, maps, dim, sms, stream);
 }

@@ -128,11 +128,6 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   if (rc) return rc;
   rc = check_batch_pool(k_cache, v_cache, k_scales, v_scales, num_pages, num_kv_heads, head_dim);
   if (rc) return rc;
-  if (!q || !out || !aligned(q, 16) || !aligned(out, 16)) return fail(QWZ_EINVAL, "q and out must be non-null 16-byte aligned pointers");
-  if (!block_table || !cu_rows || !kv_lens) return fail(QWZ_EINVAL, "block_table, cu_rows and kv_lens are required");
-  if (!workspace || !aligned(workspace, 16)) return fail(QWZ_EINVAL, "workspace must be a non-null 16-byte aligned pointer");
-  if (workspace_bytes < (int64_t)qwz::batch_workspace_bytes(head_dim))
-    return fail(QWZ_EINVAL, "workspace smaller than qwz_batch_attend_workspace_bytes(head_dim)");
   if (rows < 0 || requests < 0 || requests > (1 << 20)) return fail(QWZ_EINVAL, "rows and requests must be >= 0 (requests at most 2^20)");
   if (max_rows < 1) return fail(QWZ_EINVAL, "max_rows must be positive");
   if (table_width < 1 || table_width > (1 << 22)) return fail(QWZ_EINVAL, "table_width must be in 1..2^22");
@@ -142,6 +137,12 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   if ((rc = check_row_stride(q_stride, width, "q"))) return rc;
   if ((rc = check_row_stride(out_stride, width, "out"))) return rc;
   if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(QWZ_EINVAL, "sm_scale must be positive and finite");
+  if (rows == 0 || requests == 0) return QWZ_OK;
+  if (!q || !out || !aligned(q, 16) || !aligned(out, 16)) return fail(QWZ_EINVAL, "q and out must be non-null 16-byte aligned pointers");
+  if (!block_table || !cu_rows || !kv_lens) return fail(QWZ_EINVAL, "block_table, cu_rows and kv_lens are required");
+  if (!workspace || !aligned(workspace, 16)) return fail(QWZ_EINVAL, "workspace must be a non-null 16-byte aligned pointer");
+  if (workspace_bytes < (int64_t)qwz::batch_workspace_bytes(head_dim))
+    return fail(QWZ_EINVAL, "workspace smaller than qwz_batch_attend_workspace_bytes(head_dim)");
   const int sms = batch_sms();
   if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
   qwz::BatchPoolMaps maps;

@@ -76,6 +76,19 @@ def test_attend(lib, addr, change, needle):
     refused(lib, lib.qwz_batch_attend(*args), needle)
 
 
+@pytest.mark.parametrize("change", [{11: 0}, {0: None, 8: None, 11: 0}, {5: None, 6: None, 7: None, 12: 0}])
+def test_attend_without_work(lib, addr, change):
+    """No rows or no requests: nothing is launched, whatever the pointers (those
+    of empty tensors are null); the sizes are checked all the same."""
+    size = lib.qwz_batch_attend_workspace_bytes(256)
+    args = [addr + 256 * i for i in range(10)] + [size, 4, 2, 1, 4, 8, 24, 4, 256, 6144, 6144, 0.0625, 0, None]
+    for i, value in change.items():
+        args[i] = value
+    assert lib.qwz_batch_attend(*args) == _lib.QWZ_OK
+    args[16] = 23
+    refused(lib, lib.qwz_batch_attend(*args), "num_q_heads")
+
+
 def test_workspace_sizes(lib):
     assert lib.qwz_batch_attend_workspace_bytes(100) == 0
     sizes = [lib.qwz_batch_attend_workspace_bytes(d) for d in (64, 128, 256)]

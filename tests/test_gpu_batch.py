@@ -519,3 +519,39 @@ def test_attend_nan_query(rows, kv, value):
     assert bool(got[-1, 5].isnan().all())
     got[-1, 5] = out[-1, 5]
     check(got, want, mag, torch.float16)
+
+
+def test_step_without_rows():
+    """Every request is idle or ends: pages go back, no row is attended, written
+    or scored."""
+    from qwarz_b200 import scoring
+
+    pool = make_pool(6, 4, 256, 0)
+    before = [t.clone() for t in pool]
+    ring, table = i32([5, -1, -1, -1, -1, -1]), i32([[0, 1], [2, -1], [3, 4]])
+    cu, kv, held_out, ring_out, maps = i32([-7] * 4), i32([-7] * 3), i32([-7] * 3), i32([-7] * 2), [i32([]) for _ in range(3)]
+    batch.build_tables(i32([300, 20, 500]), i32([-1, 0, -1]), i32([2, 1, 2]), ring, i32([0, 1]), table, cu, kv, held_out,
+                       ring_out, *maps)
+    rows = torch.empty(0, 32, 256, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(0, 24, 256, dtype=torch.bfloat16, device="cuda")
+    batch.append(rows[:, 24:28], rows[:, 28:], *pool, maps[0])
+    batch.attend(rows[:, :24], *pool, table, cu, kv, out, batch.attend_workspace("cuda", 256), max_rows=1)
+    scoring.token_logprobs(torch.empty(0, 100, device="cuda"), torch.empty(0, dtype=torch.long, device="cuda"),
+                           torch.empty(0, device="cuda"), torch.empty(0, device="cuda"), torch.empty(0, 2, device="cuda"),
+                           torch.empty(0, 2, dtype=torch.int32, device="cuda"), scoring.workspace("cuda", 0, 100, 2))
+    assert ring.tolist() == [5, 0, 1, 3, 4, -1] and ring_out.tolist() == [0, 5] and cu.tolist() == [0] * 4
+    assert kv.tolist() == [0, 20, 0] and held_out.tolist() == [0, 1, 0]
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pool, before))
+
+
+def test_example_serves_one_request():
+    """A server of one slot has steps without rows, when its request ends."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "batched_verify.py"
+    spec = importlib.util.spec_from_file_location("batched_verify", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.serve(requests=1, steps=8, seed=13, say=lambda *_: None)
+    assert got["free"] + got["held"] == got["pages"] and got["finished"] > 0 and got["lengths"] == got["done"]
