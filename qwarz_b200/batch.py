@@ -83,7 +83,7 @@ def _rows(name: str, t, heads: int, dim: int):
     row, head, one = t.stride()
     if one != 1 or (head != dim and heads > 1):
         raise ValueError(f"{name} must have head and dim contiguous")
-    return shape[0], row if shape[0] > 1 else max(row, heads * dim)
+    return shape[0], row if shape[0] > 1 else heads * dim
 
 
 def build_tables(lengths, new_rows, held, ring, ring_state, block_table, cu_rows, kv_lens, held_out, ring_out,

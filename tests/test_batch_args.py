@@ -151,3 +151,10 @@ def test_launches_on_the_tensors_device(monkeypatch, current):
     monkeypatch.setattr(batch._lib, "load", Lib)
     batch._launch(1, "qwz_op", 7, 8)
     assert seen == [(1, (7, 8, 101))] and now == [current]
+
+
+@pytest.mark.parametrize("rows,stride", [(1, 1001), (1, 0), (1, 256), (0, 1001), (0, 0)])
+def test_stride_of_one_row(rows, stride):
+    """The row stride of at most one row means nothing, whatever the view gives."""
+    assert batch._rows("k", torch.empty_strided((rows, 4, 64), (stride, 64, 1)), 4, 64) == (rows, 256)
+    assert batch._rows("k", torch.empty_strided((2, 4, 64), (1001, 64, 1)), 4, 64) == (2, 1001)

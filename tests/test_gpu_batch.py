@@ -555,3 +555,23 @@ def test_example_serves_one_request():
     spec.loader.exec_module(example)
     got = example.serve(requests=1, steps=8, seed=13, say=lambda *_: None)
     assert got["free"] + got["held"] == got["pages"] and got["finished"] > 0 and got["lengths"] == got["done"]
+
+
+def test_one_row_of_any_stride():
+    """One row whose view has a stride that rows could not have."""
+    def view(x):
+        return torch.empty(2 * 1001 * x.shape[1], dtype=x.dtype, device="cuda").as_strided(
+            x.shape, (1001, x.shape[2], 1)).copy_(x)
+
+    pool = make_pool(2, 2, 64, 8)
+    ws, table, cu, kv = batch.attend_workspace("cuda", 64), i32([[1, 0]]), i32([0, 1]), i32([300])
+    q = torch.randn(1, 6, 64, device="cuda").half()
+    want, out = torch.empty_like(q), view(torch.zeros_like(q))
+    batch.attend(q, *pool, table, cu, kv, want, ws, max_rows=1)
+    batch.attend(view(q), *pool, table, cu, kv, out, ws, max_rows=1)
+    assert torch.equal(out, want)
+    k = torch.randn(1, 2, 64, device="cuda").half()
+    other = [t.clone() for t in pool]
+    batch.append(k, k, *pool, i32([7]))
+    batch.append(view(k), view(k), *other, i32([7]))
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pool, other))
