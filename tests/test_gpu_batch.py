@@ -575,3 +575,12 @@ def test_one_row_of_any_stride():
     batch.append(k, k, *pool, i32([7]))
     batch.append(view(k), view(k), *other, i32([7]))
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pool, other))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (64, 8, 64)])
+@pytest.mark.parametrize("rows,kv", [([7], [30001]), ([12, 7, 3, 40], [9000, 20001, 3000, 12345])])
+def test_attend_long_windows_below_dim_256(heads, kv_heads, dim, rows, kv):
+    """A dozen tiles and more a CTA: every buffer, barrier and parity of the
+    many-row kernel's two-buffer form comes round several times, with changes of
+    item between."""
+    run_attend(rows, kv, heads, kv_heads, dim, torch.float16, seed=dim)
