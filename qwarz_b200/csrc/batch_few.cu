@@ -353,6 +353,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   constexpr int kPerPage = kPage / F::kUnit;
   int pre_page = __ldg(pre_row + pre_unit / kPerPage);
   unsigned filled = 0;  // bit s: ring slot s holds (or will hold) tokens of the pool
+  // False once a wait gave up: nothing more is copied, what is on its way is still
+  // waited for, and the result is marked by the error.
+  bool ok = true;
+  unsigned late = 0, phases = 0;  // bits of slots: whose wait gave up; their barriers' parity
   const int step = p.kv_heads * F::kSRow;  // scale bytes of a token row
   const uint8_t* ks_lane = p.k_scales + hd * F::kSRow + (size_t)lane * step;
   const uint8_t* vs_lane = p.v_scales + hd * F::kSRow + (size_t)lane * step;
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
     if (pre_left > 0) {
       bool in_pool = pre_page >= 0 && pre_page < p.num_pages;
       if (!in_pool && pre_kv > 0) flag_error(kErrPageRange);  // a bad entry: its tokens count as absent
-      in_pool = in_pool && pre_kv > 0;
+      in_pool = in_pool && pre_kv > 0 && ok;
       filled = in_pool ? filled | (1u << slot) : filled & ~(1u << slot);
       const int t0 = pre_unit * F::kUnit + warp * F::kTok;
       if (in_pool && t0 < pre_kv) {
@@ -414,9 +418,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
 
   float o[MT][4];
   uint32_t qf[QW];
-  bool ok = true;
   int slot = 0, fill = F::kStages - 1;
-  unsigned phases = 0;  // parity of each slot's barrier
 
   while (true) {  // ------------------------------------------------ an item
     const int first_unit = cur.unit, cols = min(kFewCols, cur.r.n * p.group - c0);
@@ -470,9 +472,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
       cp_async_wait<F::kStages - 2>();
       const bool here = ((filled >> slot) & 1u) != 0u && tw < cur.r.kv;
       if (here) {  // this warp's copy was issued
-        if (ok && !mbar_wait(bars + 8 * slot, (phases >> slot) & 1u)) {
+        if (!__all_sync(kFull, mbar_wait(bars + 8 * slot, (phases >> slot) & 1u))) {
           flag_error(kErrTimeout);
-          ok = false;  // nothing is waited for any more, the result is marked by the error
+          ok = false;
+          late |= 1u << slot;
         }
         phases ^= 1u << slot;
       }
@@ -649,6 +652,11 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
     if (cur.b == end_b) break;
     cur.next_request(p, c0);
     if (cur.b == p.requests || (cur.b == end_b && end_unit == 0)) break;
+  }
+  if (!ok) {  // never leave with copies in flight
+    cp_async_wait<0>();
+    for (int s = 0; s < F::kStages; ++s)
+      if ((late >> s) & 1u) mbar_wait(bars + 8 * s, ((phases >> s) & 1u) ^ 1u);
   }
   griddep_launch_dependents();
 }
