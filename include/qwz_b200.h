@@ -417,12 +417,13 @@ int qwz_k8v4_gather(const void* words, const void* scales, const int32_t* block_
  * Outputs (no storage shared with any of the above, so a step may be built again
  * from the same state; ring and block_table share none with what is read
  * either): cu_rows, kv_lens, held_out [R], ring_out [2], and for row r < rows
- * slots[r], positions[r] (token position), request_of[r].  Rows past cu_rows[R] get slot -1, position 0, request -1.  More than `rows` rows
- * set QWZ_DEVERR_SLOT_RANGE; cu_rows stops at 2^31 - 1.  A request that does
- * not fit its table row (QWZ_DEVERR_TABLE_RANGE), or, from the first one that
- * the free pages do not cover on, any request that needs a page
- * (QWZ_DEVERR_POOL_EMPTY), is denied: it takes no page, its rows get slot -1
- * and its kv_lens is 0.  A request that ends has kv_lens 0 and held_out 0.
+ * slots[r], positions[r] (token position), request_of[r].  Rows past cu_rows[R]
+ * get slot -1, position 0, request -1.  More than `rows` rows set
+ * QWZ_DEVERR_SLOT_RANGE; cu_rows stops at 2^31 - 1.  A request that does not fit
+ * its table row (QWZ_DEVERR_TABLE_RANGE), or, from the first one that the free
+ * pages do not cover on, any request that needs a page (QWZ_DEVERR_POOL_EMPTY),
+ * is denied: it takes no page, its rows get slot -1 and its kv_lens is 0.  A
+ * request that ends has kv_lens 0 and held_out 0.
  * From the first one whose pages find no place behind the free ones of the ring
  * on, those that end keep their pages (held_out held, QWZ_DEVERR_POOL_EMPTY) and
  * can be ended again.  A ring_state with first outside 0 .. ring_size - 1 or

@@ -8,7 +8,9 @@
 // multiply-adds a query column, far below the tensor rate.  What bounds it is
 // the work between: each pair of codes is converted and each pair of halves
 // scaled on the way to a fragment, and with those instructions taken out the
-// loads alone run at 92 % of the measured copy bandwidth.
+// loads alone run at 92 % of the measured copy bandwidth.  They do not fill a
+// unit, though (ALU 51 %, issue slots 54 %, DRAM 57 %): eight warps an SM, at 236
+// registers, wait on their own chains.
 //
 // The (row, head of the group) pairs of one request and KV head are the columns
 // of an item, eight at most (9 to 16 heads of a group make two items that run
@@ -32,7 +34,7 @@
 // Measured: 524,288 tokens in one request, 24/4/256, 122 us (4.9 TB/s, 76 % of
 // the measured copy bandwidth); 64 requests of 256 to 32,768 tokens, 24/4/256,
 // 112 us (72 %); 256 of 32/8/128, 100 us (47 %: short items, whose ends cost
-// two units each); one of 4,000 tokens 15 us, the latency of two launches.
+// two units each); one of 4,000 tokens 14 us, the latency of two launches.
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 
@@ -843,7 +845,7 @@ cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int 
   e = launch_pdl(kernel, grid, dim3(F::kThreads), F::kSmem, stream, p, maps);
   if (e != cudaSuccess) return e;
   // Few requests have items of many parts: a block a column (one request of 4,000
-  // tokens: 15 us a call against 17 with a warp a column); otherwise a warp a
+  // tokens: 14 us a call against 17 with a warp a column); otherwise a warp a
   // column (256 requests: 100 us a call against 106 with a block a column).
   const int splits = (int)grid.y;
   e = p.requests * 4 <= splits

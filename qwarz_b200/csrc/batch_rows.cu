@@ -27,17 +27,26 @@
 // What bounds it: a tile's MMAs take 8 D cycles, its 128 x 128 exponentials 1,024
 // (16 a cycle and SM).  At D 256 shared memory carries 320 KB a tile (128 of QK
 // operands, 64 of V, 128 of dequantised stores: 2,560 cycles) and the four warps
-// that dequantise K are busy for about 5,400 cycles a tile (3,000 converting and
-// storing, 2,400 issuing loads), which is the period measured; a second K buffer
-// does not fit.  At D 128 the period is about 2,500 cycles, the softmax's chain
-// from S(j) to P(j).  Converting once a tile for all 128 rows is why this kernel
-// starts at 9 columns (17 where a group has more than 8 heads): batch_few.cu
-// converts for every eight.
+// that dequantise K are busy for about 5,400 cycles a tile whose codes come from
+// HBM (3,000 converting and storing, 2,400 issuing loads); a second K buffer does
+// not fit.  At D 128 the period is about 2,500 cycles, the softmax's chain from
+// S(j) to P(j).  The rest is changes of item: the first QK waits for the old item's
+// last PV, and the softmax warps stage Q and write O before the next P.  A chunk
+// of 4,096 rows onto 61,440 tokens, with few of them, takes 2.5 us a tile (6,685 us,
+// 58 % of the measured bf16 rate); of the 299,000 cycles that the windows below
+// take, 46 tiles of 5,400 are 248,000, and of the 775,000 of the prompts 106 are
+// 572,000.
+//
+// batch_few.cu, which converts for every eight columns, has an item's first eight
+// (sixteen where a group has 9 to 16 heads).  On 16 requests of 4,096 to 32,768
+// tokens, 24/4/256, it takes 63 us with 6 columns where this kernel takes 172; with
+// 12 columns this one takes 176, and two groups of eight there would take 109, but
+// their launch takes 108 with 6 columns (capi_batch.cu).
 //
 // Measured, 24/4/256: 16 requests of 4,096 to 32,768 tokens, 7 rows each, 174 us
 // (22 % of the HBM rate, 13 % of the measured bf16 rate in useful rows, two thirds
 // of the tile's rows being empty); a step of prompt chunks, windows and decode
-// rows, 466 us (32 % of the measured bf16 rate).  16 x 7 rows at 32,768 tokens of
+// rows, 467 us (32 % of the measured bf16 rate).  16 x 7 rows at 32,768 tokens of
 // 32/8/128: 376 us.
 #include "attn_common.cuh"
 #include "batch_common.cuh"

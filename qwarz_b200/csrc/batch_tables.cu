@@ -106,7 +106,9 @@ __global__ void __launch_bounds__(kTabThreads) batch_tables_kernel(const __grid_
   auto denied = [&](const TabReq& t, int first) {
     return t.n > 0 && (!state_ok || t.wide || (t.grow > 0 && t.grow > count - first));
   };
-  auto kept = [&](const TabReq& t, int freed) { return t.ends && t.held > 0 && (!state_ok || t.held > F - count - freed); };
+  auto kept = [&](const TabReq& t, int freed) {
+    return t.ends && t.held > 0 && (!state_ok || t.held > F - count - freed);
+  };
 
   // the requests: CTA 0 writes the per-request words; the table entries and the
   // ring are shared out by request, a warp copies one request's pages at a time

@@ -181,7 +181,10 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
   // 8 requests of 32,768 tokens, 48/4/256: 124 us against 193 in batch_rows.cu; 512 of
   // 512 tokens, 96/8/64: 124 against 316.  What has more columns goes to batch_rows.cu.
   // The group of heads alone decides, so that a request's result does not depend on
-  // max_rows.
+  // max_rows.  With fewer heads a launch for two groups would gain on windows of 9 to
+  // 16 columns and lose on decode rows, whose CTAs it halves: 16 requests of 4,096 to
+  // 32,768 tokens, 24/4/256, 2 rows 109 us against 176, 1 row 108 against 63; 32/8/128,
+  // 3 rows 122 against 201, 1 row 120 against 71.
   p.col_groups = p.group > qwz::kBatchFewCols && p.group <= 2 * qwz::kBatchFewCols ? 2 : 1;
   p.few_cols = p.col_groups * qwz::kBatchFewCols;
   p.sm_scale_log2 = sm_scale * kLog2e;

@@ -26,8 +26,8 @@
 // take 39, the search for the top 20 another 12, a part's beginning and end being
 // half of that.  2, 3, 5, 6 or 8 CTAs an SM are 1 to 15 us slower than 4.
 // Measured: 448 rows of 151,000 BF16 logits, top 20, 51 us (2.6 TB/s, 41 % of
-// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 8.5 us and 7 rows
-// of 131,072 BF16, top 8, 8.7 us: the latency of two launches and of one part's
+// the measured copy bandwidth); 33 rows of 50,257 FP32, top 5, 8.7 us and 7 rows
+// of 131,072 BF16, top 8, 8.8 us: the latency of two launches and of one part's
 // ranking.  A CTA a row took 203 us for the first of these.
 #include "qwz_common.cuh"
 #include "batch_kernels.h"
