@@ -472,6 +472,66 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
                      int64_t out_stride, float sm_scale, int32_t dtype, void* stream);
 
 /*
+ * Requests that share a prefix.  A prefix is a request of the batch that holds
+ * its tokens like any other; prefix_of [R] names the prefix of each request (< 0:
+ * none).  A request's own lengths, rows, pages and positions do not count its
+ * prefix's tokens, which come before its own.
+ *
+ * qwz_batch_share_prefixes sorts the step's rows by the prefix they read, from
+ * what qwz_batch_tables wrote.  plan (int32, 3 R + 1 + rows words):
+ *   cu_shared [R + 1]   shared_rows[cu_shared[g] .. cu_shared[g + 1]] are the rows
+ *                       that read request g, in ascending order
+ *   reads [R]           the prefix that each request reads (-1: none)
+ *   alone [R]           the only request with rows that reads this one (-1: none,
+ *                       or several do)
+ *   shared_rows [rows]  (-1 behind the last one)
+ * positions_out [rows]: positions plus the tokens of the row's prefix (may be
+ * positions itself; no other output may share storage with an input).  A prefix
+ * that does not exist, is the request itself or has a prefix of its own sets
+ * QWZ_DEVERR_TABLE_RANGE and counts as none; so do, with their request's rows,
+ * row offsets outside [0, rows].  R is at most 2^14.
+ */
+int qwz_batch_share_prefixes(const int32_t* prefix_of, const int32_t* kv_lens, const int32_t* cu_rows,
+                             const int32_t* positions, const int32_t* request_of, int32_t* plan, int32_t* positions_out,
+                             int32_t requests, int32_t rows, void* stream);
+
+/*
+ * qwz_batch_attend behind shared prefixes: a row sees all kv_lens[g] tokens of the
+ * prefix g that its request reads, and of its own those that it sees there.  A
+ * prefix's tokens are read once for the rows of all its requests.  plan: as
+ * qwz_batch_share_prefixes wrote it for this step; entries outside the step's
+ * requests and rows set QWZ_DEVERR_TABLE_RANGE and are skipped.  workspace:
+ * qwz_batch_shared_workspace_bytes (0: bad sizes), for one call at a time.
+ */
+int64_t qwz_batch_shared_workspace_bytes(int32_t head_dim, int32_t rows, int32_t num_q_heads);
+int qwz_batch_attend_shared(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
+                            const void* v_scales, const int32_t* block_table, const int32_t* cu_rows,
+                            const int32_t* kv_lens, const int32_t* plan, void* out, void* workspace,
+                            int64_t workspace_bytes, int32_t rows, int32_t requests, int32_t max_rows,
+                            int32_t table_width, int32_t num_pages, int32_t num_q_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int64_t q_stride, int64_t out_stride, float sm_scale, int32_t dtype,
+                            void* stream);
+
+/*
+ * qwz_batch_append of rows whose Q and K are normed and rotated on the way:
+ *   x' = x * weight / sqrt(mean(x^2) + eps) over a head (weight NULL: x' = x)
+ *   (y_i, y_j) = (x'_i cos a - x'_j sin a, x'_j cos a + x'_i sin a),
+ *   a = positions[row] * inv_freq[i], i < num_freqs, j = i + num_freqs
+ *   (neighbours != 0: of the pairs (2i, 2i + 1)); dims from 2 num_freqs on are x'
+ * q_out [rows, q_heads, dim] is y of q, rounded once (it may be q itself); k is
+ * quantised from y without a rounding in between, v as it is.  Row strides in
+ * elements, multiples of 8; num_freqs a multiple of 8, at most head_dim / 2 (0: no
+ * rotation); inv_freq, q_weight and k_weight [head_dim] are FP32.
+ */
+int qwz_batch_append_rotated(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
+                             void* k_scales, void* v_scales, const int32_t* slots, const int32_t* positions,
+                             const float* inv_freq, const float* q_weight, const float* k_weight, void* k_held,
+                             void* v_held, int64_t rows, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                             int64_t q_out_stride, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t num_freqs, int32_t neighbours, float eps, int32_t num_pages, int32_t dtype,
+                             void* stream);
+
+/*
  * Of each row of logits [rows, vocab] (FP16/BF16/FP32, any row stride): the
  * log probability of ids[row] (int32, or int64 when ids64 != 0), the entropy
  * in nats, and the `top` (0..32) most likely tokens with their log

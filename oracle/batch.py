@@ -100,6 +100,111 @@ def attend(q, k_cache, v_cache, k_scales, v_scales, table, cu_rows, kv_lens, out
     return ref, mag
 
 
+def share_prefixes(prefix_of, kv_lens, cu_rows, positions, request_of):
+    """(cu_shared, reads, alone, shared_rows, positions_out) request by request,
+    and whether a prefix or a row range was not to be."""
+    R, T = len(kv_lens), len(positions)
+    bad, reads, alone = False, [], []
+    for b, g in enumerate(prefix_of):
+        fits = 0 <= g < R and g != b and prefix_of[g] < 0
+        bad |= g >= 0 and not fits
+        reads.append(g if fits else -1)
+    ranges = []
+    for b in range(R):
+        lo, hi = cu_rows[b], cu_rows[b + 1]
+        fits = 0 <= lo <= hi <= T
+        bad |= not fits
+        ranges.append(range(lo, hi) if fits else range(0))
+    cu, rows = [0], []
+    for g in range(R):
+        behind = [b for b in range(R) if reads[b] == g and len(ranges[b])]
+        alone.append(behind[0] if len(behind) == 1 else -1)
+        for b in behind:
+            rows += ranges[b]
+        cu.append(len(rows))
+    rows += [-1] * (T - len(rows))
+    out = [p + (max(kv_lens[reads[b]], 0) if b >= 0 and reads[b] >= 0 else 0) for p, b in zip(positions, request_of)]
+    return (cu, reads, alone, rows, out), bad
+
+
+def rotate(x, positions, inv_freq, neighbours, weight=None, eps=1e-6):
+    """FP64 norm and rotation of rows [T, heads, D]; returns (y, |a| + |b| of every
+    element's two terms)."""
+    x = x.double()
+    if weight is not None:
+        x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
+    h = inv_freq.numel()
+    angle = positions.double()[:, None] * inv_freq.double()
+    c, s = angle.cos()[:, None], angle.sin()[:, None]
+    i = torch.arange(h, device=x.device)
+    lo, hi = (2 * i, 2 * i + 1) if neighbours else (i, i + h)
+    y, mag = x.clone(), x.abs()
+    y[..., lo] = x[..., lo] * c - x[..., hi] * s
+    y[..., hi] = x[..., hi] * c + x[..., lo] * s
+    mag[..., lo] = mag[..., hi] = x[..., lo].abs() + x[..., hi].abs()
+    return y, mag
+
+
+def quantise(y):
+    """(packed E2M1 codes, E4M3 bytes) of FP64 rows [..., D], by distance to the
+    grids, ties to the even code."""
+    def nearest(v, grid):
+        up = torch.searchsorted(grid, v).clamp(1, len(grid) - 1)
+        lo, hi = v - grid[up - 1], grid[up] - v
+        return torch.where((hi < lo) | ((hi == lo) & (up % 2 == 0)), up, up - 1)
+
+    e4m3 = torch.arange(127, dtype=torch.uint8, device=y.device).view(torch.float8_e4m3fn).double()
+    e2m1 = torch.tensor(nvfp4.E2M1_VALUE[:8], dtype=torch.float64, device=y.device)
+    b = y.reshape(*y.shape[:-1], -1, 16)
+    scale = nearest((b.abs().amax(-1) / 6).clamp(max=448), e4m3)
+    s = e4m3[scale][..., None]
+    q = torch.where(s > 0, b / torch.where(s > 0, s, 1.0), 0.0)
+    m = nearest(q.abs().clamp(max=6), e2m1)
+    code = (m + 8 * ((m > 0) & (q < 0))).view(y.shape).to(torch.uint8)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scale.to(torch.uint8)
+
+
+def attend_shared(q, k_cache, v_cache, k_scales, v_scales, table, cu_rows, kv_lens, reads, out, sm_scale):
+    """`attend` where request b sees all tokens of request reads[b] (-1: none) first."""
+    ref, mag = out.double().clone(), torch.zeros_like(out, dtype=torch.float64)
+    P, H = k_cache.shape[0], k_cache.shape[2]
+    G = q.shape[1] // H
+
+    def tokens(b):
+        kv = max(int(kv_lens[b]), 0)
+        ids = table[b, :-(-kv // PAGE)].long()
+        good = ((ids >= 0) & (ids < P)).repeat_interleave(PAGE)[:kv]
+        ids = torch.where((ids >= 0) & (ids < P), ids, 0)
+        k, v = (dequant(c[ids].flatten(0, 1)[:kv], s[ids].flatten(0, 1)[:kv]).repeat_interleave(G, 1)
+                for c, s in ((k_cache, k_scales), (v_cache, v_scales)))
+        return k, v, good
+
+    for b in range(len(kv_lens)):
+        lo, hi = int(cu_rows[b]), int(cu_rows[b + 1])
+        n = hi - lo
+        if n <= 0:
+            continue
+        k, v, good = tokens(b)
+        kv = k.shape[0]
+        j = torch.arange(kv, device=q.device)
+        seen = (j[None] < kv - n + torch.arange(n, device=q.device)[:, None] + 1) & good[None]
+        if reads[b] >= 0:
+            pk, pv, pgood = tokens(reads[b])
+            k, v = torch.cat([pk, k]), torch.cat([pv, v])
+            seen = torch.cat([pgood[None].expand(n, -1), seen], 1)
+        if not k.shape[0]:
+            ref[lo:hi] = 0
+            continue
+        s = torch.einsum("nhd,thd->hnt", q[lo:hi].double(), k) * sm_scale
+        s = s.masked_fill(~seen, -torch.inf)
+        m = s.amax(-1, keepdim=True)
+        p = torch.exp(s - torch.where(m.isinf(), 0.0, m))
+        p = p / torch.where(m.isinf(), 1.0, p.sum(-1, keepdim=True))
+        ref[lo:hi] = torch.einsum("hnt,thd->nhd", p, v)
+        mag[lo:hi] = torch.einsum("hnt,thd->nhd", p, v.abs())
+    return ref, mag
+
+
 def token_logprobs(logits, ids, top):
     """FP64 log probabilities of ids, entropy, top log probabilities and their
     indices (equal values by lowest index, NaN last)."""

@@ -65,12 +65,17 @@ SIGNATURES = {
     "qwz_batch_append": [c_void_p] * 9 + [c_int64] * 3 + [c_int32] * 4 + [c_void_p],
     "qwz_batch_attend_workspace_bytes": [c_int32],
     "qwz_batch_attend": [c_void_p] * 10 + [c_int64] + [c_int32] * 8 + [c_int64] * 2 + [c_float, c_int32, c_void_p],
+    "qwz_batch_share_prefixes": [c_void_p] * 7 + [c_int32] * 2 + [c_void_p],
+    "qwz_batch_shared_workspace_bytes": [c_int32] * 3,
+    "qwz_batch_attend_shared": [c_void_p] * 11 + [c_int64] + [c_int32] * 8 + [c_int64] * 2 + [c_float, c_int32, c_void_p],
+    "qwz_batch_append_rotated": [c_void_p] * 15 + [c_int64] * 5 + [c_int32] * 5 + [c_float] + [c_int32] * 2 + [c_void_p],
     "qwz_token_logprobs_workspace_bytes": [c_int32] * 4,
     "qwz_token_logprobs": [c_void_p, c_void_p, c_int32] + [c_void_p] * 5 + [c_int64] + [c_int32] * 3
                           + [c_int64, c_int32, c_void_p],
 }
 _RESTYPE = {"qwz_version": c_char_p, "qwz_last_error": c_char_p, "qwz_peer_buffer_bytes": c_int64,
-            "qwz_batch_attend_workspace_bytes": c_int64, "qwz_token_logprobs_workspace_bytes": c_int64}
+            "qwz_batch_attend_workspace_bytes": c_int64, "qwz_batch_shared_workspace_bytes": c_int64,
+            "qwz_token_logprobs_workspace_bytes": c_int64}
 
 _LIB = None
 

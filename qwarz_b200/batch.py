@@ -9,6 +9,13 @@ prompt chunks is
                batch.attend(...)     attention of all rows over their pages
     scoring.token_logprobs(...)      what the logits say of the drafted tokens
 
+Where requests share a prompt prefix, and where Q and K are still to be rotated:
+
+    batch.build_tables(...)
+    batch.share_prefixes(...)        rows by prefix, positions behind it
+    per layer: batch.append_rotated(...)  Q and K normed and rotated, K/V into their slots
+               batch.attend_shared(...)   a prefix read once for all of its requests
+
 All lengths stay on the device, so a step can be captured into a CUDA graph.
 As in `ops`: launches go to the current stream of the tensors' device, nothing
 synchronises or allocates (except `attend_workspace`), a CPU tensor raises.
@@ -161,15 +168,10 @@ def attend_workspace(device, head_dim: int) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def attend(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace, max_rows: int,
-           sm_scale: float | None = None) -> None:
-    """Attention of the rows q [T, q_heads, dim] of all requests over their
-    pages, into out (same shape and type; row strides any multiple of 8).
-    Row s of a request's n rows sees its first kv - n + s + 1 tokens; a row
-    that sees none is 0, one with a NaN or +inf score NaN.  `max_rows` is a
-    host bound of the rows a request has (1 for a decode step).  q_heads is 1
-    to 64 times kv_heads."""
-    dev = _device(q, (k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace))
+def _attend_args(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace, max_rows,
+                 sm_scale, plan=None):
+    """Checks of `attend` and `attend_shared`; returns (device, the C arguments)."""
+    dev = _device(q, (k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace, plan))
     P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)
     q_heads = q.shape[1] if q.dim() == 3 else 0
     if q_heads == 0 or q_heads % heads != 0:
@@ -185,9 +187,131 @@ def attend(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_len
         raise ValueError("block_table must be [requests, width], cu_rows [requests + 1], kv_lens [requests]")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
+    shared = ()
+    if plan is not None:
+        _int32(("plan",), (plan,))
+        if plan.numel() < 3 * R + 1 + T:
+            raise ValueError(f"plan must have 3 * requests + 1 + rows = {3 * R + 1 + T} words (prefix_plan)")
+        shared = (plan.data_ptr(),)
+    return dev, (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                 block_table.data_ptr(), cu_rows.data_ptr(), kv_lens.data_ptr(), *shared, out.data_ptr(),
+                 workspace.data_ptr(), workspace.nbytes, T, R, max_rows, width, P, q_heads, heads, dim, q_stride,
+                 out_stride, dim ** -0.5 if sm_scale is None else float(sm_scale), _dtype_code(dtype))
+
+
+def attend(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace, max_rows: int,
+           sm_scale: float | None = None) -> None:
+    """Attention of the rows q [T, q_heads, dim] of all requests over their
+    pages, into out (same shape and type; row strides any multiple of 8).
+    Row s of a request's n rows sees its first kv - n + s + 1 tokens; a row
+    that sees none is 0, one with a NaN or +inf score NaN.  `max_rows` is a
+    host bound of the rows a request has (1 for a decode step).  q_heads is 1
+    to 64 times kv_heads."""
+    dev, args = _attend_args(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace,
+                             max_rows, sm_scale)
+    _launch(dev, "qwz_batch_attend", *args)
+
+
+def prefix_plan(device, requests: int, rows: int) -> torch.Tensor:
+    """The tensor that `share_prefixes` fills and `attend_shared` reads, for
+    steps of that many requests and up to that many rows (allocate before capture)."""
+    return torch.empty(3 * requests + 1 + rows, dtype=_I32, device=device)
+
+
+def share_prefixes(prefix_of, kv_lens, cu_rows, positions, request_of, plan, positions_out) -> None:
+    """Rows of a step by the shared prefix they read, once a step for all layers.
+
+    A prefix is a request of the batch that holds its tokens, usually idle;
+    `prefix_of[b]` [R] names the one whose tokens come before request b's own
+    (-1: none).  What `build_tables` counts (lengths, rows, pages, positions) are
+    a request's own.  `kv_lens`, `cu_rows`, `positions` [T] and `request_of` [T]
+    are its outputs; `plan` (`prefix_plan`) receives the rows by prefix and
+    `positions_out` [T] the positions from the prefix's start (may be
+    `positions`).  A prefix that does not exist, is the request itself or has one
+    itself counts as none (device error word).  All tensors int32, at most 2^14
+    requests; the plan's layout is in include/qwz_b200.h."""
+    dev = _device(prefix_of, (kv_lens, cu_rows, positions, request_of, plan, positions_out))
+    _int32(("prefix_of", "kv_lens", "cu_rows", "positions", "request_of", "plan", "positions_out"),
+           (prefix_of, kv_lens, cu_rows, positions, request_of, plan, positions_out))
+    R, T = kv_lens.numel(), positions.numel()
+    if prefix_of.numel() != R or cu_rows.numel() != R + 1:
+        raise ValueError("prefix_of and kv_lens have one entry per request, cu_rows requests + 1")
+    if request_of.numel() != T or positions_out.numel() != T:
+        raise ValueError("positions, request_of and positions_out must have the same length")
+    if plan.numel() < 3 * R + 1 + T:
+        raise ValueError(f"plan must have 3 * requests + 1 + rows = {3 * R + 1 + T} words (prefix_plan)")
     _launch(
-        dev, "qwz_batch_attend",
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-        block_table.data_ptr(), cu_rows.data_ptr(), kv_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-        workspace.nbytes, T, R, max_rows, width, P, q_heads, heads, dim, q_stride, out_stride,
-        dim ** -0.5 if sm_scale is None else float(sm_scale), _dtype_code(dtype))
+        dev, "qwz_batch_share_prefixes",
+        prefix_of.data_ptr(), kv_lens.data_ptr(), cu_rows.data_ptr(), positions.data_ptr(), request_of.data_ptr(),
+        plan.data_ptr(), positions_out.data_ptr(), R, T)
+
+
+def append_rotated(q, k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq,
+                   neighbours: bool = False, q_weight=None, k_weight=None, eps: float = 1e-6, k_held=None,
+                   v_held=None) -> None:
+    """`append` of rows whose Q and K are normed and rotated on the way.
+
+    q [T, q_heads, dim], k and v [T, kv_heads, dim] (one of FP16/BF16, row
+    strides multiples of 8, parts of a packed projection for instance); q_out
+    receives the rotated q (it may be q).  `positions` [T] int32; `inv_freq`
+    (FP32, a multiple of 8 long, at most dim / 2) is the angle of each pair of
+    dims at position 1: pairs (i, i + len(inv_freq)), or (2i, 2i + 1) with
+    `neighbours`; dims behind them are not rotated.  With `q_weight`,
+    `k_weight` (FP32 [dim]) a head is first divided by the root of its mean
+    square (plus eps) and multiplied by the weight.  K is quantised from the
+    rotated values without a rounding in between.  slots, k_held and v_held: as
+    in `append`."""
+    dev = _device(q, (k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq, q_weight,
+                      k_weight, k_held, v_held))
+    P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)
+    q_heads = q.shape[1] if q.dim() == 3 else 0
+    T, q_stride = _rows("q", q, q_heads, dim)
+    dtype = q.dtype
+    strides = [q_stride]
+    for name, t, n in (("k", k, heads), ("v", v, heads), ("q_out", q_out, q_heads)):
+        Tt, stride = _rows(name, t, n, dim)
+        if Tt != T or t.dtype is not dtype:
+            raise ValueError("q, k, v and q_out must have the same rows and dtype")
+        strides.append(stride)
+    _int32(("slots", "positions"), (slots, positions))
+    if slots.numel() != T or positions.numel() != T:
+        raise ValueError("slots and positions must have one entry per row")
+    f32 = torch.float32
+    if inv_freq.dtype is not f32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 vector")
+    extra = []
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None and (t.dtype is not f32 or t.shape != (dim,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 [{dim}]")
+        extra.append(None if t is None else t.data_ptr())
+    for t in (k_held, v_held):
+        if t is not None:
+            if t.dtype is not dtype or t.shape != k.shape:
+                raise ValueError("k_held and v_held must have k's shape and dtype")
+            _contig("k_held and v_held", t)
+        extra.append(None if t is None else t.data_ptr())
+    _launch(
+        dev, "qwz_batch_append_rotated",
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scales.data_ptr(), v_scales.data_ptr(), slots.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), *extra,
+        T, *strides, q_heads, heads, dim, inv_freq.numel(), int(neighbours), eps, P, _dtype_code(dtype))
+
+
+def shared_workspace(device, head_dim: int, rows: int, q_heads: int) -> torch.Tensor:
+    """Workspace of `attend_shared` for steps of up to that many rows, for one
+    call at a time (allocate before capture)."""
+    n = _lib.load().qwz_batch_shared_workspace_bytes(head_dim, rows, q_heads)
+    if n == 0:
+        raise ValueError("head_dim must be 64, 128 or 256, rows >= 0, q_heads in 1..16384")
+    return torch.empty(n, dtype=_U8, device=device)
+
+
+def attend_shared(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, plan, out, workspace,
+                  max_rows: int, sm_scale: float | None = None) -> None:
+    """`attend` behind shared prefixes: a row sees every token of the prefix
+    that its request reads and then its own as in `attend`.  The prefix's pages
+    are read once for the rows of all its requests together.  `plan` is what
+    `share_prefixes` wrote for the step, `workspace` a `shared_workspace`."""
+    dev, args = _attend_args(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace,
+                             max_rows, sm_scale, plan)
+    _launch(dev, "qwz_batch_attend_shared", *args)

@@ -32,7 +32,19 @@ struct BatchAttnParams {
   int few_cols;                  // most (row, head) columns a KV head of batch_few.cu has
   int col_groups;                // groups of eight of them
   float sm_scale_log2;           // sm_scale * log2(e)
+  // attention behind shared prefixes (the plan of batch_prefix.cu)
+  const int32_t* cu_shared;      // [requests + 1] request g is the prefix of the rows shared_rows[cu_shared[g] ..]
+  const int32_t* reads;          // [requests] the prefix a request reads (-1: none)
+  const int32_t* alone;          // [requests] the only request that reads this one (-1: none, or several do)
+  const int32_t* shared_rows;    // [rows] rows by prefix
+  float* prefix_ml;              // [rows, q_heads, 2] the prefix's part of a row: reference maximum and sum
+  float* prefix_o;               // [rows, q_heads, dim] unnormalised
 };
+// What a launch of batch_few.cu and batch_rows.cu does: all of a request's tokens
+// (kBatchPlain); the tokens of prefixes, for all rows that read them, into
+// prefix_ml and prefix_o (kBatchPrefix); a request's own tokens, joined with
+// that (kBatchOwn).
+enum BatchMode : int { kBatchPlain = 0, kBatchPrefix = 1, kBatchOwn = 2 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA
 constexpr int kBatchMaxSms = 256;
 constexpr int kBatchMaxCtas = 4 * kBatchMaxSms;  // batch_few.cu has up to 4 CTAs an SM
@@ -81,6 +93,36 @@ struct BatchAppendParams {
   int kv_heads, dim, num_pages;
 };
 
+// The step's rows by the prefix they read (batch_prefix.cu).
+struct BatchShareParams {
+  const int32_t* prefix_of;      // [requests]
+  const int32_t* kv_lens;        // [requests]
+  const int32_t* cu_rows;        // [requests + 1]
+  const int32_t* positions;      // [rows]
+  const int32_t* request_of;     // [rows]
+  int32_t* cu_shared;            // [requests + 1]
+  int32_t* reads;                // [requests]
+  int32_t* alone;                // [requests]
+  int32_t* shared_rows;          // [rows]
+  int32_t* positions_out;        // [rows]
+  int requests, rows;
+};
+constexpr int kShareMaxRequests = 1 << 14;
+
+// Q and K normed and rotated, K and V quantised into their slots (batch_prefix.cu).
+struct BatchRotateParams {
+  BatchAppendParams kv;          // k before the norm and the rotation
+  const void* q;                 // [rows, q_heads, dim]
+  void* q_out;
+  const int32_t* positions;      // [rows]
+  const float* inv_freq;         // [freqs] radians a position
+  const float* q_weight;         // [dim] of the head norm, or null
+  const float* k_weight;
+  long long q_stride, q_out_stride;
+  int q_heads, freqs, neighbours;  // neighbours: pairs (2i, 2i + 1), otherwise (i, i + freqs)
+  float eps;
+};
+
 // Token log probabilities (token_logprobs.cu).
 struct LogprobParams {
   const void* logits;            // [rows, vocab], row stride `stride` elements
@@ -104,5 +146,9 @@ cudaError_t launch_batch_tables(const BatchTablesParams& p, int sms, cudaStream_
 cudaError_t launch_batch_append(const BatchAppendParams& p, int dtype, cudaStream_t stream);
 cudaError_t launch_batch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
                                 cudaStream_t stream);
+cudaError_t launch_batch_attend_shared(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
+                                       cudaStream_t stream);
+cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t stream);
+cudaError_t launch_batch_rotate(const BatchRotateParams& p, int dtype, cudaStream_t stream);
 
 }  // namespace qwz
