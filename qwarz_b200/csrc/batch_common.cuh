@@ -59,49 +59,39 @@ QWZ_DEVINL float part_weight(float m, float l, float M) {
   return m == -CUDART_INF_F ? 0.f * l : exp2_approx(m - M);
 }
 
+// Tokens of request b, clipped to its table row.
+QWZ_DEVINL int tokens_of(const BatchAttnParams& p, int b) {
+  const int kv = __ldg(p.kv_lens + b);
+  if (kv > p.table_width * kPage) flag_error(kErrTableRange);
+  return max(0, min(kv, p.table_width * kPage));
+}
+
 // The rows that have request b for their prefix, as a request whose rows are
-// places of shared_rows.  A request alone behind it whose columns batch_few.cu
-// takes reads the prefix there in front of its own tokens, which saves the records
-// of the row and the 128-row tile.
+// places of shared_rows.
 QWZ_DEVINL Req load_prefix(const BatchAttnParams& p, int b) {
   Req r;
   const int lo = __ldg(p.cu_shared + b), hi = __ldg(p.cu_shared + b + 1);
   r.row0 = lo;
   r.n = hi - lo;
-  r.kv = __ldg(p.kv_lens + b);
+  r.kv = tokens_of(p, b);
   if (lo < 0 || hi < lo || hi > p.rows) {
     flag_error(kErrTableRange);
     r.row0 = 0;
     r.n = 0;
   }
-  if (r.kv > p.table_width * kPage) {
-    flag_error(kErrTableRange);
-    r.kv = p.table_width * kPage;
-  }
-  if (r.kv < 0) r.kv = 0;
-  if (r.n * p.group <= p.few_cols && __ldg(p.alone + b) >= 0) r.n = 0;
   return r;
 }
 
 // The prefix that request b reads (-1: none).
 QWZ_DEVINL int prefix_of(const BatchAttnParams& p, int b) {
   const int g = __ldg(p.reads + b);
-  return g < p.requests ? g : -1;
+  if (g < p.requests) return g;
+  flag_error(kErrTableRange);
+  return -1;
 }
 
-// A row's weights when its own tokens (reference m, sum l) meet its prefix's part.
-struct Join {
-  float own, pre, inv;
-};
-QWZ_DEVINL Join join_of(const BatchAttnParams& p, size_t row_head, float m, float l) {
-  const float2 v = __ldcg(reinterpret_cast<const float2*>(p.prefix_ml) + row_head);
-  const float M = fmaxf(m, v.x);
-  Join j;
-  j.own = part_weight(m, l, M);
-  j.pre = part_weight(v.x, v.y, M);
-  const float L = j.own * l + j.pre * v.y;
-  j.inv = L > 0.f ? 1.f / L : 0.f;
-  return j;
+QWZ_DEVINL uint32_t where_word(uint32_t what, int first, int parts, int row) {
+  return what | ((uint32_t)first << 2) | ((uint32_t)(parts - 1) << 12) | ((uint32_t)row << 22);
 }
 
 // Exclusive scan of one value a thread over the CTA (blockDim.x <= 1024, a

@@ -114,7 +114,7 @@ QWZ_DEVINL void cp_async_small(uint32_t dst, const void* src) {
 // weighs its units and kOver more for what its item costs beside them (its Q,
 // the merge and the store), so that CTAs with many short items get fewer.
 //
-// With M kBatchOwn a request that is alone behind its prefix has the prefix's
+// With M kBatchShared a request whose prefix is marked direct has the prefix's
 // units in front of its own.
 template <int U, int M>
 struct FewWalk {
@@ -124,7 +124,7 @@ struct FewWalk {
   long long base;          // weighed units before the request
   batch::Req r;
   // the prefix that the request reads here: its units, request and tokens (0: none)
-  int pre = 0, pre_b = 0, pre_kv = 0;
+  int pre = 0, pre_b = -1, pre_kv = 0;
 
   // whether request r has columns of the group that begins at c0 (those with more
   // than few_cols are batch_rows.cu's)
@@ -132,23 +132,18 @@ struct FewWalk {
     const int cols = r.n * p.group;
     return cols > c0 && cols <= p.few_cols;
   }
-  // Request b's prefix where it reads it by itself (-1: none, or the prefix's part is a record).
+  // Request b's prefix where it reads it by itself (-1: none, or it is a part of its own).
   static QWZ_DEVINL int direct(const BatchAttnParams& p, int b) {
-    if constexpr (M != kBatchOwn) return -1;
+    if constexpr (M == kBatchPlain) return -1;
     const int g = batch::prefix_of(p, b);
-    return g >= 0 && __ldg(p.alone + g) == b ? g : -1;
-  }
-  static QWZ_DEVINL int tokens_of(const BatchAttnParams& p, int g) {
-    const int kv = __ldg(p.kv_lens + g);
-    if (kv > p.table_width * kPage) flag_error(kErrTableRange);
-    return max(0, min(kv, p.table_width * kPage));
+    return g >= 0 && __ldcg(p.direct + g) != 0 ? g : -1;
   }
   // a request without tokens still has rows to write
   static QWZ_DEVINL int units_of(const BatchAttnParams& p, const batch::Req& r, int b) {
     int units = max(1, (r.kv + U - 1) / U);
-    if constexpr (M == kBatchOwn) {
+    if constexpr (M == kBatchShared) {
       const int g = direct(p, b);
-      if (g >= 0) units += (tokens_of(p, g) + U - 1) / U;
+      if (g >= 0) units += (batch::tokens_of(p, g) + U - 1) / U;
     }
     return units;
   }
@@ -160,9 +155,9 @@ struct FewWalk {
     b = bb;
     r = batch::load_req(p, b);
     units = units_of(p, r, b);
-    if constexpr (M == kBatchOwn) {
+    if constexpr (M == kBatchShared) {
       pre_b = direct(p, b);
-      pre_kv = pre_b >= 0 ? tokens_of(p, pre_b) : 0;
+      pre_kv = pre_b >= 0 ? batch::tokens_of(p, pre_b) : 0;
       pre = (pre_kv + U - 1) / U;
     }
   }
@@ -309,18 +304,6 @@ QWZ_DEVINL void few_qk(uint32_t codes, uint32_t scales, int r0, int qd, const ui
   for (int i = 0; i < 4; ++i) s[i] = sa[i] + sb[i];
 }
 
-// Whether request b's rows still have to meet their prefix's part.
-QWZ_DEVINL bool few_joins(const BatchAttnParams& p, int b) {
-  const int g = batch::prefix_of(p, b);
-  return g >= 0 && __ldg(p.alone + g) != b;
-}
-QWZ_DEVINL void few_join(const batch::Join& j, const float4& pre, float4& own) {
-  own.x = j.own * own.x + j.pre * pre.x;
-  own.y = j.own * own.y + j.pre * pre.y;
-  own.z = j.own * own.z + j.pre * pre.z;
-  own.w = j.own * own.w + j.pre * pre.w;
-}
-
 }  // namespace
 
 template <typename T, int D, int M>
@@ -384,6 +367,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   __syncthreads();
   int32_t* meta = p.meta + cta * kBatchMeta;
   if (tid == 0) meta[0] = 0;
+  if (M == kBatchShared && tid == 0 && split == 0) p.busy[1 + blockIdx.x] = (int)min(total, splits);
   if (none) {
     griddep_launch_dependents();
     return;
@@ -393,7 +377,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   int pre_b = cur.b, pre_unit = cur.unit, pre_left = cur.left(end_b, end_unit), pre_kv = cur.r.kv;
   const int32_t* pre_row = p.block_table + (size_t)pre_b * p.table_width;
   int pre_in = 0;  // units left of the prefix, in front of the request's own
-  if constexpr (M == kBatchOwn) {
+  if constexpr (M == kBatchShared) {
     pre_in = max(cur.pre - cur.unit, 0);
     if (pre_in > 0) {
       pre_row = p.block_table + (size_t)cur.pre_b * p.table_width;
@@ -440,11 +424,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         }
       }
       ++pre_unit;
-      if (M == kBatchOwn && pre_in > 0 && --pre_in == 0) {  // on to the request's own tokens
+      if (M == kBatchShared && pre_in > 0 && --pre_in == 0) {  // on to the request's own tokens
         pre_unit = 0;
         pre_row = p.block_table + (size_t)pre_b * p.table_width;
-        pre_kv = __ldg(p.kv_lens + pre_b);
-        pre_kv = max(0, min(pre_kv, p.table_width * kPage));
+        pre_kv = batch::tokens_of(p, pre_b);
       }
       if (--pre_left == 0 && pre_b != end_b) {  // on to the next request
         batch::Req r = {0, 0, 0};
@@ -457,9 +440,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
           pre_left = pre_b == end_b ? end_unit : Walk::units_of(p, r, pre_b);
           pre_kv = r.kv;
           pre_row = p.block_table + (size_t)pre_b * p.table_width;
-          if constexpr (M == kBatchOwn) {
+          if constexpr (M == kBatchShared) {
             const int g = Walk::direct(p, pre_b);
-            const int kv = g >= 0 ? Walk::tokens_of(p, g) : 0;
+            const int kv = g >= 0 ? batch::tokens_of(p, g) : 0;
             pre_in = (kv + F::kUnit - 1) / F::kUnit;
             if (pre_in > 0) {
               pre_row = p.block_table + (size_t)g * p.table_width;
@@ -531,7 +514,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
     int lim1 = 2 * qd + 1 < cols ? lim_base + (c0 + 2 * qd + 1) / p.group : 0;
     int kv = cur.r.kv, in_prefix = 0;  // units left of the prefix, whose tokens all rows see
     bool crossing = false;             // out of which the item goes into the request's own tokens
-    if constexpr (M == kBatchOwn) {
+    if constexpr (M == kBatchShared) {
       in_prefix = max(cur.pre - cur.unit, 0);
       crossing = in_prefix > 0;
       if (crossing) {
@@ -547,9 +530,9 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
     for (int j = 0; j < MT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
     int tw = cur.unit * F::kUnit + warp * F::kTok;
-    if (M == kBatchOwn && in_prefix == 0) tw -= cur.pre * F::kUnit;
+    if (M == kBatchShared && !crossing) tw -= cur.pre * F::kUnit;
     for (int n = cur.left(end_b, end_unit); n > 0; --n, tw += F::kUnit) {
-      if constexpr (M == kBatchOwn) {
+      if constexpr (M == kBatchShared) {
         if (in_prefix > 0) {
           --in_prefix;
         } else if (crossing) {  // the first unit of the request's own tokens
@@ -697,22 +680,23 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         L0 += w0[w] * ml_of(w)[2 * qd].y;
         L1 += w1[w] * ml_of(w)[2 * qd + 1].y;
       }
-      float i0 = L0 > 0.f ? 1.f / L0 : 0.f, i1 = L1 > 0.f ? 1.f / L1 : 0.f;
-      bool joins = false;  // with the prefix's part of the row
-      size_t rh[2] = {0, 0};
-      batch::Join jn[2] = {{1.f, 0.f, 0.f}, {1.f, 0.f, 0.f}};
-      if constexpr (M == kBatchOwn) {
-        joins = whole && few_joins(p, cur.b);
-        if (joins) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = min(c0 + 2 * qd + e, c0 + cols - 1);
-            rh[e] = (size_t)(cur.r.row0 + c / p.group) * (p.kv_heads * p.group) + hd * p.group + c % p.group;
-            jn[e] = batch::join_of(p, rh[e], e ? M1 : M0, e ? L1 : L0);
-          }
-          i0 = jn[0].inv;
-          i1 = jn[1].inv;
-        }
+      const float i0 = L0 > 0.f ? 1.f / L0 : 0.f, i1 = L1 > 0.f ? 1.f / L1 : 0.f;
+      // the lane's two columns as parts of rows (kind 1: own tokens)
+      const bool joins = M == kBatchShared && cur.pre_b < 0 && batch::prefix_of(p, cur.b) >= 0;
+      auto part_of = [&](int c) {
+        return ((size_t)p.rows + cur.r.row0 + (c0 + c) / p.group) * (p.kv_heads * p.group) +
+               hd * p.group + (c0 + c) % p.group;
+      };
+      if (M == kBatchShared && starts_here && tid < cols) {
+        const long long last = (cur.base + Walk::kOver + cur.units) * splits - 1;
+        p.where[part_of(tid)] = !ends_here ? batch::where_word(kWhereFew, split, (int)(last / total) - split + 1, tid)
+                                : joins    ? kWhereWhole
+                                           : kWhereDone;
+      }
+      if (M == kBatchShared && whole && joins && warp == 0 && g == 0) {
+        float2* ml = reinterpret_cast<float2*>(p.part_ml);
+        if (2 * qd < cols) ml[part_of(2 * qd)] = make_float2(M0, L0);
+        if (2 * qd + 1 < cols) ml[part_of(2 * qd + 1)] = make_float2(M1, L1);
       }
       if (!whole && warp == 0 && g == 0) {
         float2* ml = reinterpret_cast<float2*>(rec + kFewCols * D);
@@ -737,14 +721,10 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         for (int e = 0; e < 2; ++e) {
           const int c = 2 * qd + e;
           if (c >= cols) continue;
-          float x = e ? a.y : a.x, y = e ? a.w : a.z;
-          const float inv = e ? i1 : i0;
-          if (M == kBatchOwn && joins) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(p.prefix_o + rh[e] * D + d));
-            x = jn[e].own * x + jn[e].pre * v.x;
-            y = jn[e].own * y + jn[e].pre * v.y;
-          }
-          if (whole) {
+          const float x = e ? a.y : a.x, y = e ? a.w : a.z, inv = e ? i1 : i0;
+          if (M == kBatchShared && whole && joins) {
+            *reinterpret_cast<float2*>(p.part_o + part_of(c) * D + d) = make_float2(x, y);
+          } else if (whole) {
             T* dst = reinterpret_cast<T*>(p.out) + (cur.r.row0 + (c0 + c) / p.group) * p.out_stride +
                      (hd * p.group + (c0 + c) % p.group) * D + d;
             const T h[2] = {InTraits<T>::from_float(x * inv), InTraits<T>::from_float(y * inv)};
@@ -758,7 +738,6 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         const long long last_unit = cur.base + Walk::kOver + cur.units - 1;
         meta[0] = cols;
         meta[1] = cur.r.row0;
-        meta[2] = cur.b;
         meta[4] = (int)(((last_unit + 1) * splits - 1) / total);
         meta[5] = (int)min(total, splits);  // fewer units than splits leave some without a record
       }
@@ -779,7 +758,7 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
 // Merges the records of the items that more than one CTA worked on, in the
 // order of the splits: block (head, split, y) takes columns y, y + gridDim.z,
 // ... of the item that this split began and did not finish.
-template <typename T, int D, int Mode>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ float w[kBatchMaxCtas], sums[kBatchMaxCtas];
@@ -854,18 +833,9 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
         a.z += v.z;
         a.w += v.w;
       }
-      float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L > 0.f ? 1.f / L : 0.f;
       const int cc = hd % p.col_groups * kFewCols + c;  // column of the KV head
       const int s = cc / p.group, h = hd / p.col_groups * p.group + cc % p.group;
-      if constexpr (Mode == kBatchOwn) {
-        if (few_joins(p, __ldcg(meta + 2))) {
-          const size_t rh = (size_t)(row0 + s) * (p.kv_heads * p.group) + h;
-          const batch::Join jn = batch::join_of(p, rh, M, L);
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(p.prefix_o + rh * D) + tid);
-          few_join(jn, v, a);
-          inv = jn.inv;
-        }
-      }
       T* dst = reinterpret_cast<T*>(p.out) + (row0 + s) * p.out_stride + h * D + tid * 4;
       dst[0] = InTraits<T>::from_float(a.x * inv);
       dst[1] = InTraits<T>::from_float(a.y * inv);
@@ -880,7 +850,7 @@ __global__ void __launch_bounds__(256) batch_combine_kernel(const __grid_constan
 // items have a few parts each.
 constexpr int kCombineThreads = kFewCols * 32;
 
-template <typename T, int D, int Mode>
+template <typename T, int D>
 __global__ void __launch_bounds__(kCombineThreads)
     batch_combine_short_kernel(const __grid_constant__ BatchAttnParams p, int splits) {
   constexpr int kVecs = (D + 127) / 128;  // float4s of a lane (D 64: half the lanes)
@@ -901,7 +871,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   float4 a[kVecs];
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  float L = 0.f, M = -CUDART_INF_F;
+  float L = 0.f;
   const bool mine = lane * 4 < D;
   if (c < cols) {
     auto stat = [&](int j) {
@@ -909,6 +879,7 @@ __global__ void __launch_bounds__(kCombineThreads)
       if (i * busy / splits == (i + 1) * busy / splits) return make_float2(-CUDART_INF_F, 0.f);  // a split without units
       return __ldcg(reinterpret_cast<const float2*>(record(j) + kFewCols * D + 2 * c));
     };
+    float M = -CUDART_INF_F;
     for (int j = lane; j < parts; j += 32) M = fmaxf(M, stat(j).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -939,18 +910,8 @@ __global__ void __launch_bounds__(kCombineThreads)
     }
   }
   if (c >= cols || !mine) return;
-  float inv = L > 0.f ? 1.f / L : 0.f;
+  const float inv = L > 0.f ? 1.f / L : 0.f;
   const int cc = hd % p.col_groups * kFewCols + c;  // column of the KV head
-  if constexpr (Mode == kBatchOwn) {
-    if (few_joins(p, __ldcg(meta + 2))) {
-      const size_t rh = (size_t)(row0 + cc / p.group) * (p.kv_heads * p.group) + hd / p.col_groups * p.group + cc % p.group;
-      const batch::Join jn = batch::join_of(p, rh, M, L);
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v)
-        few_join(jn, __ldcg(reinterpret_cast<const float4*>(p.prefix_o + rh * D) + lane + 32 * v), a[v]);
-      inv = jn.inv;
-    }
-  }
   T* dst = reinterpret_cast<T*>(p.out) + (row0 + cc / p.group) * p.out_stride +
            (hd / p.col_groups * p.group + cc % p.group) * D;
 #pragma unroll
@@ -963,50 +924,43 @@ __global__ void __launch_bounds__(kCombineThreads)
 
 namespace {
 
+// CTAs that share a KV head's (and group of columns') units.
+template <int D>
+int few_splits(const BatchAttnParams& p, int sms) {
+  return max(1, sms * Few<D>::kCtas / (p.kv_heads * p.col_groups));
+}
+
 template <typename T, int D, int M>
 cudaError_t launch_few(const BatchAttnParams& p, const BatchPoolMaps& maps, int sms, cudaStream_t stream) {
   using F = Few<D>;
   // the heads of a token range run side by side: their slices of a token row
   // share DRAM pages and sectors
-  const int heads = p.kv_heads * p.col_groups;
-  const dim3 grid(heads, max(1, sms * F::kCtas / heads));
+  const dim3 grid(p.kv_heads * p.col_groups, few_splits<D>(p, sms));
   auto kernel = batch_few_kernel<T, D, M>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, grid, dim3(F::kThreads), F::kSmem, stream, p, maps);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || M == kBatchShared) return e;
   // Few requests have items of many parts: a block a column (one request of 4,000
   // tokens: 14 us a call against 17 with a warp a column); otherwise a warp a
   // column (256 requests: 100 us a call against 106 with a block a column).
   const int splits = (int)grid.y;
   e = p.requests * 4 <= splits
-          ? launch_pdl(batch_combine_kernel<T, D, M>, dim3(grid.x, grid.y, kFewCols), dim3(256), 0, stream, p)
-          : launch_pdl(batch_combine_short_kernel<T, D, M>, grid, dim3(kCombineThreads), kFewCols * splits * sizeof(float),
+          ? launch_pdl(batch_combine_kernel<T, D>, dim3(grid.x, grid.y, kFewCols), dim3(256), 0, stream, p)
+          : launch_pdl(batch_combine_short_kernel<T, D>, grid, dim3(kCombineThreads), kFewCols * splits * sizeof(float),
                        stream, p, splits);
   if (e != cudaSuccess || (long long)p.max_rows * p.group <= p.few_cols) return e;
-  return launch_rows<T, D, M>(p, sms, stream);
+  return launch_rows<T, D>(p, sms, stream);
 }
 
-template <typename T, int M>
+template <typename T>
 cudaError_t launch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int sms, cudaStream_t stream) {
   switch (dim) {
-    case 64: return launch_few<T, 64, M>(p, maps, sms, stream);
-    case 128: return launch_few<T, 128, M>(p, maps, sms, stream);
-    case 256: return launch_few<T, 256, M>(p, maps, sms, stream);
+    case 64: return launch_few<T, 64, kBatchPlain>(p, maps, sms, stream);
+    case 128: return launch_few<T, 128, kBatchPlain>(p, maps, sms, stream);
+    case 256: return launch_few<T, 256, kBatchPlain>(p, maps, sms, stream);
   }
   return cudaErrorInvalidValue;
-}
-
-// The prefixes' part of all rows, then every row's own tokens and the join.
-template <typename T>
-cudaError_t launch_shared(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int sms, cudaStream_t stream) {
-  cudaError_t e = cudaErrorInvalidValue;
-  switch (dim) {
-    case 64: e = launch_rows<T, 64, kBatchPrefix>(p, sms, stream); break;
-    case 128: e = launch_rows<T, 128, kBatchPrefix>(p, sms, stream); break;
-    case 256: e = launch_rows<T, 256, kBatchPrefix>(p, sms, stream); break;
-  }
-  return e != cudaSuccess ? e : launch_attend<T, kBatchOwn>(p, maps, dim, sms, stream);
 }
 
 }  // namespace
@@ -1019,14 +973,8 @@ int batch_few_box_rows(int dim) { return dim == 256 ? Few<256>::kTok : dim == 12
 
 cudaError_t launch_batch_attend(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
                                 cudaStream_t stream) {
-  return dtype == kDtypeBF16 ? launch_attend<__nv_bfloat16, kBatchPlain>(p, maps, dim, sms, stream)
-                             : launch_attend<__half, kBatchPlain>(p, maps, dim, sms, stream);
-}
-
-cudaError_t launch_batch_attend_shared(const BatchAttnParams& p, const BatchPoolMaps& maps, int dim, int dtype, int sms,
-                                       cudaStream_t stream) {
-  return dtype == kDtypeBF16 ? launch_shared<__nv_bfloat16>(p, maps, dim, sms, stream)
-                             : launch_shared<__half>(p, maps, dim, sms, stream);
+  return dtype == kDtypeBF16 ? launch_attend<__nv_bfloat16>(p, maps, dim, sms, stream)
+                             : launch_attend<__half>(p, maps, dim, sms, stream);
 }
 
 }  // namespace qwz

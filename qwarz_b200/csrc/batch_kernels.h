@@ -37,14 +37,19 @@ struct BatchAttnParams {
   const int32_t* reads;          // [requests] the prefix a request reads (-1: none)
   const int32_t* alone;          // [requests] the only request that reads this one (-1: none, or several do)
   const int32_t* shared_rows;    // [rows] rows by prefix
-  float* prefix_ml;              // [rows, q_heads, 2] the prefix's part of a row: reference maximum and sum
-  float* prefix_o;               // [rows, q_heads, dim] unnormalised
+  int32_t* direct;               // [requests] whether those that read this prefix do so by themselves
+  int32_t* busy;                 // [1 + kv_heads * col_groups] CTAs with work of batch_tiles.cu, of batch_few.cu's columns
+  // the parts of a row, of its prefix and of its own tokens: [2][rows, q_heads]
+  uint32_t* where;               // BatchWhere
+  float* part_ml;                // reference maximum and sum of a whole part
+  float* part_o;                 // and its unnormalised output [2][rows, q_heads, dim]
 };
 // What a launch of batch_few.cu and batch_rows.cu does: all of a request's tokens
-// (kBatchPlain); the tokens of prefixes, for all rows that read them, into
-// prefix_ml and prefix_o (kBatchPrefix); a request's own tokens, joined with
-// that (kBatchOwn).
-enum BatchMode : int { kBatchPlain = 0, kBatchPrefix = 1, kBatchOwn = 2 };
+// into out (kBatchPlain), or the parts that batch_join.cu merges (kBatchShared).
+enum BatchMode : int { kBatchPlain = 0, kBatchShared = 1 };
+// Where a part is: bits 0-1 what, 2-11 first CTA (split) of its records, 12-21 their
+// number less one, 22-29 its row in them.
+enum BatchWhere : uint32_t { kWhereDone = 0, kWhereWhole = 1, kWhereFew = 2, kWhereRows = 3 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA
 constexpr int kBatchMaxSms = 256;
 constexpr int kBatchMaxCtas = 4 * kBatchMaxSms;  // batch_few.cu has up to 4 CTAs an SM
@@ -59,6 +64,19 @@ constexpr int kBatchFewCols = 8;
 constexpr size_t kBatchMetaBytes = 2 * (size_t)kBatchMaxCtas * kBatchMeta * 4;
 size_t batch_few_record_bytes(int dim);  // all records of batch_few.cu
 size_t batch_workspace_bytes(int dim);
+// What attention behind shared prefixes adds to it.
+struct BatchSharedSpace {
+  int64_t direct, busy, where, ml, o, bytes;  // offsets
+  BatchSharedSpace(int dim, int64_t rows, int64_t q_heads) {
+    const int64_t pairs = 2 * rows * q_heads;
+    direct = 0;
+    busy = direct + 4 * (int64_t)(1 << 14);
+    where = busy + 4 * 1024;
+    ml = where + (4 * pairs + 15) / 16 * 16;
+    o = ml + 8 * pairs;
+    bytes = o + 4 * pairs * dim;
+  }
+};
 
 // Paging of many requests (batch_tables.cu).
 struct BatchTablesParams {

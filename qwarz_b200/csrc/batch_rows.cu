@@ -108,45 +108,30 @@ struct Rows {
   static constexpr size_t kRec = (size_t)kRwRows * (D + 2);  // floats of a record
 };
 
-// Walks the units (request, head, group of positions, tile) of the launch.  The
-// rows of a prefix all see all of it: their (position, head) pairs fill the items
-// without regard to positions, `per` pairs an item.
-template <int M>
+// Walks the units (request, head, group of positions, tile) of the launch.
 struct RowsWalk {
   int b, h, i, tile;
   int tiles, groups;
-  int per;                 // positions of an item (of a prefix: rows of an item)
+  int per;                 // positions of an item
   batch::Req r;
 
-  QWZ_DEVINL static batch::Req load(const BatchAttnParams& p, int b) {
-    if constexpr (M == kBatchPrefix) {
-      batch::Req r = batch::load_prefix(p, b);
-      r.n *= p.group;
-      return r;
-    } else {
-      return batch::load_req(p, b);
-    }
-  }
   QWZ_DEVINL static int tiles_of(const batch::Req& r, int per, int i) {
-    const int lim = M == kBatchPrefix ? r.kv : r.kv - r.n + min((i + 1) * per, r.n);
+    const int lim = r.kv - r.n + min((i + 1) * per, r.n);
     return max(1, (lim + kRwTok - 1) / kRwTok);
   }
   QWZ_DEVINL static long long head_cost(const batch::Req& r, int per) {
-    if constexpr (M == kBatchPrefix) return (long long)((r.n + per - 1) / per) * tiles_of(r, per, 0);
     long long c = 0;
     for (int i = 0; i * per < r.n; ++i) c += tiles_of(r, per, i);
     return c;
   }
-  QWZ_DEVINL static bool many(const BatchAttnParams& p, const batch::Req& r) {
-    return M == kBatchPrefix ? r.n > 0 : r.n * p.group > p.few_cols;
-  }
+  QWZ_DEVINL static bool many(const BatchAttnParams& p, const batch::Req& r) { return r.n * p.group > p.few_cols; }
   QWZ_DEVINL static long long cost(const BatchAttnParams& p, int b, int per) {
-    const batch::Req r = load(p, b);
+    const batch::Req r = batch::load_req(p, b);
     return many(p, r) ? p.kv_heads * head_cost(r, per) : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
-    r = load(p, b);
+    r = batch::load_req(p, b);
     groups = (r.n + per - 1) / per;
   }
   QWZ_DEVINL void seek(const BatchAttnParams& p, int b0, long long u) {
@@ -271,19 +256,9 @@ QWZ_DEVINL void rw_store(uint32_t tile, int row, int c, const RwChunks<D>& in) {
 
 }  // namespace
 
-// The row of q and out of place `at` of a prefix's rows (-1, and the error bit,
-// for an entry that is none).
-QWZ_DEVINL int rw_shared_row(const BatchAttnParams& p, int at) {
-  const int row = __ldg(p.shared_rows + at);
-  if (row >= 0 && row < p.rows) return row;
-  flag_error(kErrTableRange);
-  return -1;
-}
-
-template <typename T, int D, int M>
+template <typename T, int D>
 __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_constant__ BatchAttnParams p) {
   using R = Rows<D>;
-  using Walk = RowsWalk<M>;
   constexpr int NB = R::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sraw = smem_u32(smem);
@@ -326,11 +301,11 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
   griddep_wait();
 
   // ---------------------------------------------------- this CTA's share
-  const int per_pos = M == kBatchPrefix ? kRwRows : kRwRows / p.group;
+  const int per_pos = kRwRows / p.group;
   const int per = (p.requests + kRwScan - 1) / kRwScan;
   long long mine = 0, total;
   if (tid < kRwScan)
-    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, per_pos);
+    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += RowsWalk::cost(p, b, per_pos);
   const long long before = batch::block_scan(mine, sums, total);
   if (tid < kRwScan) starts[tid] = before;
   tc::fence_before();
@@ -341,7 +316,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
   const long long lo = (long long)blockIdx.x * total / n_cta, hi = ((long long)blockIdx.x + 1) * total / n_cta;
   const int units = (int)(hi - lo);
   int32_t* meta = p.meta + (kBatchMaxCtas + blockIdx.x) * kBatchMeta;
-  Walk cur;
+  RowsWalk cur;
   cur.per = per_pos;
   if (units > 0) {
     int at = 0;
@@ -490,7 +465,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
     bool ok = true;
     // 16 of the quadrant's Q rows of the walker's item -> K-major FP16 operand,
     // each row scaled by a power of two (exact for BF16 and FP16)
-    auto stage_q = [&](const Walk& w, int item) {
+    auto stage_q = [&](const RowsWalk& w, int item) {
       constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows a load
       const int sub = lane / LPR, ln = lane % LPR;
       const int pos0 = w.i * per_pos, npos = min(per_pos, w.r.n - pos0);
@@ -504,13 +479,7 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
           const int row = base + u * RPI + sub;
           const int pos = row / p.group;
           v[u] = make_uint4(0u, 0u, 0u, 0u);
-          if constexpr (M == kBatchPrefix) {
-            const int c = pos0 + row;
-            const int at = row < npos ? rw_shared_row(p, w.r.row0 + c / p.group) : -1;
-            if (at >= 0)
-              v[u] = __ldg(reinterpret_cast<const uint4*>(q + (long long)at * p.q_stride +
-                                                          (w.h * p.group + c % p.group) * D) + ln);
-          } else if (pos < npos)
+          if (pos < npos)
             v[u] = __ldg(reinterpret_cast<const uint4*>(q + (long long)(w.r.row0 + pos0 + pos) * p.q_stride +
                                                         (w.h * p.group + row % p.group) * D) + ln);
         }
@@ -551,12 +520,10 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       const int pos0 = cur.i * per_pos, npos = min(per_pos, cur.r.n - pos0);
       const int tile0 = cur.tile, n_tiles = min(cur.tiles - tile0, units - j), head = cur.h;
       const int row0 = cur.r.row0 + pos0;
-      const bool starts_here = tile0 == 0, ends_here = tile0 + n_tiles == cur.tiles;
-      const bool valid = M == kBatchPrefix ? r < npos : rpos < npos;
+      const bool starts_here = tile0 == 0, ends_here = tile0 + n_tiles == cur.tiles, valid = rpos < npos;
       const int all_tiles = cur.tiles;
       // keys below lim are visible; rows that do not exist are all zeros in Q
-      const int lim = !valid ? 0x7fffffff : M == kBatchPrefix ? cur.r.kv : cur.r.kv - cur.r.n + pos0 + rpos + 1;
-      const int first_place = cur.r.row0, request = cur.b;
+      const int lim = valid ? cur.r.kv - cur.r.n + pos0 + rpos + 1 : 0x7fffffff;
       const int last = j + n_tiles - 1;
       ok &= mbar_wait(bar(kRwQReady), item & 1);  // the other warps' row factors
       if (__any_sync(kFull, !ok || *abort_flag)) break;
@@ -680,50 +647,15 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
       if (__any_sync(kFull, !ok)) break;
       tc::fence_after();
       const float l = sums_of[r] + sums_of[kRwRows + r];
-      if (M == kBatchPrefix && starts_here && ends_here) {
-        const int at = valid ? rw_shared_row(p, first_place + (pos0 + r) / p.group) : -1;
-        const size_t rh = (size_t)max(at, 0) * (p.kv_heads * p.group) + head * p.group + (pos0 + r) % p.group;
-        float4* dst = reinterpret_cast<float4*>(p.prefix_o + rh * D);
-#pragma unroll 1
-        for (int c = grp * (D / 2); c < (grp + 1) * (D / 2); c += 32) {
-          float x[32];
-          rw_ld32(to + c, x);
-          if (at < 0) continue;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) dst[(c + e) / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-        }
-        if (at >= 0 && grp == 0) reinterpret_cast<float2*>(p.prefix_ml)[rh] = make_float2(m_fin, l);
-      } else if (starts_here && ends_here) {
+      if (starts_here && ends_here) {
         T* out = reinterpret_cast<T*>(p.out) + (long long)(row0 + (valid ? rpos : 0)) * p.out_stride +
                  (head * p.group + rhead) * D;
-        float inv = l > 0.f ? 1.f / l : 0.f;
-        bool joins = false;
-        batch::Join jn = {1.f, 0.f, 0.f};
-        const float4* pre = nullptr;
-        if constexpr (M == kBatchOwn) {
-          joins = valid && batch::prefix_of(p, request) >= 0;
-          if (joins) {
-            const size_t rh = (size_t)(row0 + rpos) * (p.kv_heads * p.group) + head * p.group + rhead;
-            jn = batch::join_of(p, rh, m_fin, l);
-            inv = jn.inv;
-            pre = reinterpret_cast<const float4*>(p.prefix_o + rh * D);
-          }
-        }
+        const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
         for (int c = grp * (D / 2); c < (grp + 1) * (D / 2); c += 32) {
           float x[32];
           rw_ld32(to + c, x);
           if (!valid) continue;
-          if (M == kBatchOwn && joins) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float4 v = __ldcg(pre + (c + e) / 4);
-              x[e] = jn.own * x[e] + jn.pre * v.x;
-              x[e + 1] = jn.own * x[e + 1] + jn.pre * v.y;
-              x[e + 2] = jn.own * x[e + 2] + jn.pre * v.z;
-              x[e + 3] = jn.own * x[e + 3] + jn.pre * v.w;
-            }
-          }
           uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
@@ -753,9 +685,8 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
         if (valid && grp == 0) *reinterpret_cast<float2*>(rec + kRwRows * D + 2 * r) = make_float2(m_fin, l);
         if (starts_here && tid == 0) {
           const long long last_unit = lo + (j - n_tiles) + all_tiles - 1;
-          meta[0] = M == kBatchPrefix ? npos : npos * p.group;
-          meta[1] = M == kBatchPrefix ? first_place : row0;
-          meta[2] = M == kBatchPrefix ? pos0 : request;
+          meta[0] = npos * p.group;
+          meta[1] = row0;
           meta[3] = head;
           meta[4] = (int)(((last_unit + 1) * n_cta - 1) / total);
           meta[5] = (int)min(total, n_cta);
@@ -782,11 +713,11 @@ __global__ void __launch_bounds__(kRwThreads, 1) batch_rows_kernel(const __grid_
 
 // Merges the records of items that more than one CTA worked on, in CTA order:
 // block (i, y) takes rows 8y .. 8y + 7 of the item that CTA i began.
-template <typename T, int D, int Mode>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_constant__ BatchAttnParams p) {
   using R = Rows<D>;
   __shared__ float w[8][kBatchMaxCtas];
-  __shared__ float inv_l[8], ref[8], sum[8];
+  __shared__ float inv_l[8];
   griddep_wait();
   griddep_launch_dependents();
   const int tid = threadIdx.x, i0 = blockIdx.x, n_cta = gridDim.x, y0 = blockIdx.y * 8;
@@ -818,30 +749,11 @@ __global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_co
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += shfl_xor(L, o);
-    if (lane == 0) {
-      inv_l[tid >> 5] = L > 0.f ? 1.f / L : 0.f;
-      ref[tid >> 5] = M;
-      sum[tid >> 5] = L;
-    }
+    if (lane == 0) inv_l[tid >> 5] = L > 0.f ? 1.f / L : 0.f;
   }
   __syncthreads();
   const int row = y0 + (tid & 7);
   if (row >= rows) return;
-  size_t rh = 0;  // (row, head) of the prefix's part
-  bool joins = false;
-  batch::Join jn = {1.f, 0.f, 0.f};
-  if constexpr (Mode == kBatchPrefix) {
-    const int c = __ldcg(meta + 2) + row, at = rw_shared_row(p, base + c / p.group);
-    if (at < 0) return;
-    rh = (size_t)at * (p.kv_heads * p.group) + hd * p.group + c % p.group;
-    if (tid < 8) reinterpret_cast<float2*>(p.prefix_ml)[rh] = make_float2(ref[tid], sum[tid]);
-  } else if constexpr (Mode == kBatchOwn) {
-    joins = batch::prefix_of(p, __ldcg(meta + 2)) >= 0;
-    if (joins) {
-      rh = (size_t)(base + row / p.group) * (p.kv_heads * p.group) + hd * p.group + row % p.group;
-      jn = batch::join_of(p, rh, ref[tid & 7], sum[tid & 7]);
-    }
-  }
   T* out = reinterpret_cast<T*>(p.out) + (long long)(base + row / p.group) * p.out_stride + (hd * p.group + row % p.group) * D;
   for (int d4 = tid >> 3; d4 < D / 4; d4 += 32) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -855,19 +767,7 @@ __global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_co
       a.z += wj * v.z;
       a.w += wj * v.w;
     }
-    if constexpr (Mode == kBatchPrefix) {
-      reinterpret_cast<float4*>(p.prefix_o + rh * D)[d4] = a;
-      continue;
-    }
-    float s = inv_l[tid & 7];
-    if (Mode == kBatchOwn && joins) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.prefix_o + rh * D) + d4);
-      a.x = jn.own * a.x + jn.pre * v.x;
-      a.y = jn.own * a.y + jn.pre * v.y;
-      a.z = jn.own * a.z + jn.pre * v.z;
-      a.w = jn.own * a.w + jn.pre * v.w;
-      s = jn.inv;
-    }
+    const float s = inv_l[tid & 7];
     T* dst = out + d4 * 4;
     dst[0] = InTraits<T>::from_float(a.x * s);
     dst[1] = InTraits<T>::from_float(a.y * s);
@@ -876,14 +776,14 @@ __global__ void __launch_bounds__(256) batch_rows_combine_kernel(const __grid_co
   }
 }
 
-template <typename T, int D, int M>
+template <typename T, int D>
 cudaError_t launch_rows(const BatchAttnParams& p, int ctas, cudaStream_t stream) {
-  auto kernel = batch_rows_kernel<T, D, M>;
+  auto kernel = batch_rows_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<D>::kSmem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(ctas), dim3(kRwThreads), Rows<D>::kSmem, stream, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(batch_rows_combine_kernel<T, D, M>, dim3(ctas, kRwRows / 8), dim3(256), 0, stream, p);
+  return launch_pdl(batch_rows_combine_kernel<T, D>, dim3(ctas, kRwRows / 8), dim3(256), 0, stream, p);
 }
 
 }  // namespace qwz

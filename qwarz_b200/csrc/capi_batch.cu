@@ -91,9 +91,6 @@ int append_checked(qwz::BatchAppendParams& p, const void* k, const void* v, void
   return QWZ_OK;
 }
 
-// Floats of the prefixes' (maximum, sum) of all rows and heads, whole 16-byte groups.
-int64_t shared_stats(int32_t rows, int32_t q_heads) { return (2 * (int64_t)rows * q_heads + 3) / 4 * 4; }
-
 // qwz_batch_attend, and with a plan qwz_batch_attend_shared.
 int attend_checked(const char* what, const int32_t* plan, bool shared, const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
                      const void* v_scales, const int32_t* block_table, const int32_t* cu_rows,
@@ -174,8 +171,13 @@ int attend_checked(const char* what, const int32_t* plan, bool shared, const voi
   p.reads = p.cu_shared + requests + 1;
   p.alone = p.reads + requests;
   p.shared_rows = p.alone + requests;
-  p.prefix_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + qwz::batch_workspace_bytes(head_dim));
-  p.prefix_o = p.prefix_ml + shared_stats(rows, num_q_heads);
+  uint8_t* space = static_cast<uint8_t*>(workspace) + qwz::batch_workspace_bytes(head_dim);
+  const qwz::BatchSharedSpace at(head_dim, rows, num_q_heads);
+  p.direct = reinterpret_cast<int32_t*>(space + at.direct);
+  p.busy = reinterpret_cast<int32_t*>(space + at.busy);
+  p.where = reinterpret_cast<uint32_t*>(space + at.where);
+  p.part_ml = reinterpret_cast<float*>(space + at.ml);
+  p.part_o = reinterpret_cast<float*>(space + at.o);
   return launched(qwz::launch_batch_attend_shared(p, maps, head_dim, dtype, sms, as_stream(stream)), what);
 }
 
@@ -295,8 +297,7 @@ int64_t qwz_batch_attend_workspace_bytes(int32_t head_dim) {
 int64_t qwz_batch_shared_workspace_bytes(int32_t head_dim, int32_t rows, int32_t num_q_heads) {
   if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || rows < 0 || num_q_heads < 1 || num_q_heads > 64 * 256)
     return 0;
-  return (int64_t)qwz::batch_workspace_bytes(head_dim) +
-         4 * (shared_stats(rows, num_q_heads) + (int64_t)rows * num_q_heads * head_dim);
+  return (int64_t)qwz::batch_workspace_bytes(head_dim) + qwz::BatchSharedSpace(head_dim, rows, num_q_heads).bytes;
 }
 
 int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,

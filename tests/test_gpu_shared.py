@@ -330,11 +330,14 @@ def test_attend_shared_large_scores():
 
 @pytest.mark.parametrize("rows", [[0, 1, 1, 1], [0, 9, 1, 30]])
 def test_attend_shared_without_prefixes(rows):
-    """Nothing shared: the bits of `attend`."""
+    """Nothing shared: what `attend` gives.  Either is within (2^-11 + 3e-5) of the sum of
+    p |v|, at most the largest |v| (6 x 1.1), of the same numbers (see `check`), and
+    rounded once."""
     head, plan, out, _ = run_shared([-1] * 4, rows, [500, 700, 64, 1000], 24, 4, 256, torch.float16)
     plain = torch.empty_like(out)
     batch.attend(*head, plain, batch.attend_workspace("cuda", 256), max_rows=max(rows))
-    assert torch.equal(out, plain)
+    tol = 2 * (2.0 ** -11 + 3e-5) * 6.6 + torch.finfo(out.dtype).eps * plain.double().abs() + 2.0 ** -24
+    assert bool(((out.double() - plain.double()).abs() <= tol).all())
 
 
 @pytest.mark.parametrize("rows", [1, 8])

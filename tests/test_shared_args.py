@@ -117,10 +117,12 @@ def test_without_work(lib, addr):
 
 def test_workspace_sizes(lib):
     plain = lib.qwz_batch_attend_workspace_bytes(128)
-    assert lib.qwz_batch_shared_workspace_bytes(128, 0, 8) == plain
-    assert lib.qwz_batch_shared_workspace_bytes(128, 3, 5) == plain + 4 * (32 + 15 * 128)
-    assert lib.qwz_batch_shared_workspace_bytes(256, 1 << 20, 64) == lib.qwz_batch_attend_workspace_bytes(256) + \
-        4 * (64 << 20) * 258
+    none = lib.qwz_batch_shared_workspace_bytes(128, 0, 8)
+    assert plain < none < plain + (1 << 20)
+    # two parts of a row and head: output, maximum and sum, a word
+    assert lib.qwz_batch_shared_workspace_bytes(128, 4, 6) == none + 2 * 24 * 4 * (128 + 3)
+    none = lib.qwz_batch_shared_workspace_bytes(256, 0, 64)
+    assert lib.qwz_batch_shared_workspace_bytes(256, 1 << 20, 64) == none + 2 * (64 << 20) * 4 * 259
     for bad in ((96, 1, 8), (128, -1, 8), (128, 1, 0), (128, 1, 1 << 15)):
         assert lib.qwz_batch_shared_workspace_bytes(*bad) == 0
     with pytest.raises(ValueError):
