@@ -344,7 +344,8 @@ QWZ_DEVINL void tl_fewer_regs() {
 
 // Columns [first, first + D / 2) of the warp's 32 tensor-memory rows to the places of
 // the lanes' rows (null: not stored), through shared memory so that four lanes write
-// 64 bytes of a row: as FP32, or as T times the row's factor.
+// 64 bytes of a row: as FP32, or as T times the row's factor.  (A lane writing its own
+// row 16 bytes at a time took 7 us an item instead of 5.)
 template <typename T, int D, bool FINAL>
 QWZ_DEVINL void tl_store_rows(uint32_t stage, uint32_t taddr, int first, void* dst, float factor) {
   constexpr int kPitch = Tiles<D>::kPitch, kCols = FINAL ? 32 : 16;
@@ -731,50 +732,54 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
     const uint32_t ts = tbase + lane_base + R::kTmS + 128u * grp, to = tbase + lane_base + R::kTmO;
     const uint32_t tp = tbase + lane_base + R::kTmP + R::kTmPStep * grp;
     bool ok = true;
-    // 16 of the quadrant's Q rows of an item -> K-major FP16 operand, each row scaled
-    // by a power of two (exact for BF16 and FP16): copied to its place as it is, then
-    // converted there.  (Rolled: code that runs once an item comes from L2.)
+    // 16 of the quadrant's Q rows of an item -> K-major FP16 operand, two lanes a row:
+    // copied to its place as it is; BF16 rows are then scaled there by a power of two that
+    // makes them exact in FP16.  (Rolled, and without sums over lanes in the loops: code
+    // that runs once an item comes from L2, and a chain of shuffles a row took 7 us.)
     auto stage_q = [&](const TlItem& it, int item) {
-      constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes a row, rows a step
-      const int sub = lane / LPR, ln = lane % LPR;
-      // lane l: the q row of (row, head) pair 16 grp + l of the quadrant
-      const int at = rank * kTlRows + 32 * wq + 16 * grp + (lane & 15), c = it.pair0 + at;
-      int mine_row = -1;
-      if (at < it.pairs) mine_row = it.pre ? tl_shared_row(p, it.row0 + c / p.group) : it.row0 + c / p.group;
-      const long long mine_at = mine_row < 0 ? -1 : mine_row * p.q_stride + (it.head * p.group + c % p.group) * D;
-      const int row0 = 32 * wq + 16 * grp;
-      auto place = [&](int row) {
-        return sb + R::kQ + (ln >> 3) * (kTlRows * 128) + row * 128 + (((ln & 7) ^ (row & 7)) << 4);
+      constexpr int N = D / 16;  // 16-byte chunks of a lane
+      const int row = 32 * wq + 16 * grp + (lane >> 1), at = rank * kTlRows + row, c = it.pair0 + at;
+      int q_row = -1;
+      if (at < it.pairs) q_row = it.pre ? tl_shared_row(p, it.row0 + c / p.group) : it.row0 + c / p.group;
+      const int first = (lane & 1) * N;
+      const T* from = reinterpret_cast<const T*>(p.q);
+      if (q_row >= 0) from += q_row * p.q_stride + (it.head * p.group + c % p.group) * D + first * 8;
+      auto place = [&](int n) {  // of the lane's chunk n
+        return sb + R::kQ + ((first + n) >> 3) * (kTlRows * 128) + row * 128 + ((((first + n) & 7) ^ (row & 7)) << 4);
       };
-#pragma unroll 1
-      for (int i = sub; i < 16; i += RPI) {
-        const long long from = __shfl_sync(kFull, mine_at, i);
-        cp_async16(place(row0 + i), reinterpret_cast<const T*>(p.q) + (from >= 0 ? from + ln * 8 : 0), from >= 0 ? 16u : 0u);
-      }
+#pragma unroll 4
+      for (int n = 0; n < N; ++n) cp_async16(place(n), from + (q_row >= 0 ? n * 8 : 0), q_row >= 0 ? 16u : 0u);
       cp_async_commit();
       cp_async_wait<0>();
-#pragma unroll 1
-      for (int i = sub; i < 16; i += RPI) {
-        const uint4 v = lds128(place(row0 + i));
-        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+      float s = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
         float amax = 0.f;
+#pragma unroll 2
+        for (int n = 0; n < N; ++n) {
+          const uint4 v = lds128(place(n));
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = InTraits<T>::to_float2(x[e]);
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = InTraits<T>::to_float2(x[e]);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
         }
+        amax = fmaxf(amax, shfl_xor(amax, 1));
+        s = pow2_row_scale(amax);
+#pragma unroll 2
+        for (int n = 0; n < N; ++n) {
+          const uint4 v = lds128(place(n));
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          uint32_t hh[4];
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, shfl_xor(amax, o));
-        const float s = pow2_row_scale(amax);
-        uint32_t hh[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = InTraits<T>::to_float2(x[e]);
-          hh[e] = pack_half2(f.x * s, f.y * s);
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = InTraits<T>::to_float2(x[e]);
+            hh[e] = pack_half2(f.x * s, f.y * s);
+          }
+          sts128(place(n), hh[0], hh[1], hh[2], hh[3]);
         }
-        sts128(place(row0 + i), hh[0], hh[1], hh[2], hh[3]);
-        if (ln == 0) sts32(sb + R::kRowfac + 4 * ((item & 1) * kTlRows + row0 + i), __float_as_uint(p.sm_scale_log2 / s));
       }
+      if ((lane & 1) == 0) sts32(sb + R::kRowfac + 4 * ((item & 1) * kTlRows + row), __float_as_uint(p.sm_scale_log2 / s));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -945,7 +950,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
       if (__any_sync(kFull, !ok)) break;
       tc::fence_after();
       const float l = lds_f(R::kSum, sums_of) + lds_f(R::kSum, sums_of + kTlRows);
-      const uint32_t stage = sb + R::kStage + warp * 32 * R::kPitch;
       TlItem it;
       take(item, it);  // (it is there)
       const int head = it.head, rhead = (it.pair0 + rr) % p.group, at_row = it.row0 + (it.pair0 + rr) / p.group;
@@ -954,6 +958,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
       // (-1: no such pair, or, of a prefix, for a bad entry, which has no output)
       const int row = rr >= it.pairs ? -1 : pre ? tl_shared_row(p, at_row) : at_row;
       const bool whole = starts_here && it.parts == 1;
+      const uint32_t stage = sb + R::kStage + warp * 32 * R::kPitch;
       // (kind, row, head) of the row's part
       const size_t part = ((size_t)(pre ? 0 : p.rows) + max(row, 0)) * (p.kv_heads * p.group) + head * p.group + rhead;
       if (starts_here && grp == 0 && row >= 0)
