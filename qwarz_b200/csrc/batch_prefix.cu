@@ -5,9 +5,10 @@
 // A prefix is a request that has none itself; e(b) is the one that request b
 // reads, n(b) the request's rows.  Rows are listed by prefix, then by row, so
 // the place of request b's first row is the sum of n(b') over the requests with
-// (e(b'), b') < (e(b), b).  With R requests a CTA compares its 32 with all of
-// them (R / 8 comparisons a thread); for 2^14 requests, the most a call takes,
-// that is still less than what a sort's passes would wait for one another.
+// (e(b'), b') < (e(b), b).  A warp has one request and compares it with all R (no
+// request waits for another's sums); a step's bytes are nothing beside the launch.
+// Measured: PLAN.  (Eight threads a request, whose
+// dependent loads and comparisons one after another bounded it: 28 us for 2,072.)
 #include "batch_common.cuh"
 #include "nvfp4_quant.cuh"
 
@@ -15,10 +16,9 @@ namespace qwz {
 
 namespace {
 
-constexpr int kShReq = 32;              // requests of a CTA
-constexpr int kShSub = 8;               // threads a request
-constexpr int kShThreads = kShReq * kShSub;
-constexpr int kShTile = 1024;           // requests in shared memory at a time
+constexpr int kShReq = 32;              // requests of a CTA, a warp each
+constexpr int kShThreads = kShReq * 32;
+constexpr int kShTile = 4096;           // requests in shared memory at a time
 
 // The prefix that request b reads: one that exists, is another and has none itself.
 QWZ_DEVINL int share_prefix(const BatchShareParams& p, int b) {
@@ -40,55 +40,13 @@ QWZ_DEVINL int share_rows(const BatchShareParams& p, int b, int& lo) {
 }  // namespace
 
 __global__ void __launch_bounds__(kShThreads) batch_share_kernel(const __grid_constant__ BatchShareParams p) {
-  __shared__ int2 tile[kShTile];        // (prefix, rows)
+  __shared__ int2 tile[kShTile];        // (prefix, rows; -1, 0: the request reads none or has no rows)
   griddep_wait();
-  const int tid = threadIdx.x, sub = tid % kShSub;
-  const int b = blockIdx.x * kShReq + tid / kShSub;
-  const int key = b < p.requests ? share_prefix(p, b) : -1;
-  int before = 0, of_lower = 0, readers = 0, reader = -1, total = 0;
-  for (int t0 = 0; t0 < p.requests; t0 += kShTile) {
-    const int n = min(kShTile, p.requests - t0);
-    __syncthreads();
-    for (int i = tid; i < n; i += kShThreads) {
-      int lo;
-      tile[i] = make_int2(share_prefix(p, t0 + i), share_rows(p, t0 + i, lo));
-    }
-    __syncthreads();
-    for (int i = sub; i < n; i += kShSub) {
-      const int2 o = tile[i];
-      if (o.x < 0 || o.y == 0) continue;
-      total += o.y;
-      if (o.x < key || (o.x == key && t0 + i < b)) before += o.y;
-      if (o.x < b) of_lower += o.y;
-      if (o.x == b) {
-        ++readers;
-        reader = t0 + i;
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 1; o < kShSub; o <<= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    of_lower += __shfl_xor_sync(0xffffffffu, of_lower, o);
-    readers += __shfl_xor_sync(0xffffffffu, readers, o);
-    reader = max(reader, __shfl_xor_sync(0xffffffffu, reader, o));
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  int lo = 0, n = 0;
-  if (b < p.requests) n = share_rows(p, b, lo);
-  if (sub == 0 && b < p.requests) {
-    p.reads[b] = key;
-    p.alone[b] = readers == 1 ? reader : -1;
-    p.cu_shared[b] = of_lower;
-    if (b == 0) p.cu_shared[p.requests] = total;
-  }
-  // the rows of the CTA's requests, by eight threads each
-  const int place = key >= 0 ? before : -1;
-  if (place >= 0)
-    for (int i = sub; i < n && place + i < p.rows; i += kShSub) p.shared_rows[place + i] = lo + i;
-  // positions from the prefix's start, and the places behind the last row
-  const int step = gridDim.x * kShThreads;
-  for (int t = blockIdx.x * kShThreads + tid; t < p.rows; t += step) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int b = blockIdx.x * kShReq + (tid >> 5);
+  const int step = gridDim.x * kShThreads, first = blockIdx.x * kShThreads + tid;
+  // positions from the prefix's start (their loads are on their way during the rest)
+  for (int t = first; t < p.rows; t += step) {
     const int r = __ldg(p.request_of + t);
     int pos = p.positions[t];
     if (r >= 0 && r < p.requests) {
@@ -96,8 +54,53 @@ __global__ void __launch_bounds__(kShThreads) batch_share_kernel(const __grid_co
       if (g >= 0) pos += max(__ldg(p.kv_lens + g), 0);
     }
     p.positions_out[t] = pos;
-    if (t >= total) p.shared_rows[t] = -1;
   }
+  if (blockIdx.x * kShReq >= p.requests && blockIdx.x > 0) return;
+  const int key = b < p.requests ? share_prefix(p, b) : -1;
+  int before = 0, of_lower = 0, readers = 0, reader = -1, total = 0;
+  for (int t0 = 0; t0 < p.requests; t0 += kShTile) {
+    const int n = min(kShTile, p.requests - t0);
+    __syncthreads();
+    for (int i = tid; i < n; i += kShThreads) {
+      int lo;
+      const int rows = share_rows(p, t0 + i, lo), g = share_prefix(p, t0 + i);
+      tile[i] = g >= 0 && rows > 0 ? make_int2(g, rows) : make_int2(0x7fffffff, 0);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = lane; i < n; i += 32) {
+      const int2 o = tile[i];
+      total += o.y;
+      before += o.x < key || (o.x == key && t0 + i < b) ? o.y : 0;
+      of_lower += o.x < b ? o.y : 0;
+      readers += o.x == b ? 1 : 0;
+      reader = o.x == b ? t0 + i : reader;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    of_lower += __shfl_xor_sync(0xffffffffu, of_lower, o);
+    readers += __shfl_xor_sync(0xffffffffu, readers, o);
+    reader = max(reader, __shfl_xor_sync(0xffffffffu, reader, o));
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if (b < p.requests) {
+    if (lane == 0) {
+      p.reads[b] = key;
+      p.alone[b] = readers == 1 ? reader : -1;
+      p.cu_shared[b] = of_lower;
+      if (b == 0) p.cu_shared[p.requests] = total;
+    }
+    if (key >= 0) {
+      int lo;
+      const int n = share_rows(p, b, lo);
+      for (int i = lane; i < n && (unsigned)(before + i) < (unsigned)p.rows; i += 32) p.shared_rows[before + i] = lo + i;
+    }
+  }
+  // the places behind the last row
+  const int ctas = (p.requests + kShReq - 1) / kShReq;
+  for (long long t = max(total, 0) + blockIdx.x * kShThreads + tid; t < p.rows; t += ctas * kShThreads) p.shared_rows[t] = -1;
   griddep_launch_dependents();
 }
 
@@ -114,11 +117,15 @@ cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t 
 //   (y_i, y_j) = (x'_i cos a - x'_j sin a, x'_j cos a + x'_i sin a),  a = position * inv_freq_i
 // with j = i + freqs, or the pairs (2i, 2i + 1); dims from 2 freqs on keep x'.
 // q_out is y rounded once.  K's y goes to the quantiser without a rounding in
-// between: E4M3 scales and E2M1 codes are those of the exact y, up to the
-// error of 64 bits, so they do not depend on how 32 bits round next to a border.
-// 64-bit arithmetic is half as fast as 32-bit here and only K's rotated dims need
-// it; angles of far positions need it anyway (a position of 10^6 leaves 32 bits
-// 0.06 radians).
+// between: E4M3 scales and E2M1 codes are those of the exact y, up to the error of
+// 64 bits, so they do not depend on how 32 bits round next to a border.  They are made
+// from 32 bits and an error bound, and again from 64 where a border is inside it (a few
+// heads in a hundred).  Angles are taken in 64 bits: 32 leave 0.06 radians of a position
+// of 10^6.
+//
+// Bytes bound it for long steps, as long as the instructions between them stay few: 400
+// a K or V head and 140 a Q head (one chunk of 8 dims a lane, the other dims of a pair by
+// shuffles, K in 64 bits) took 187 us for ROTATE_WAS.
 namespace {
 
 // Nearest float with an odd last bit unless y is a float itself: later roundings
@@ -136,15 +143,22 @@ QWZ_DEVINL float odd_of(float q, float rem) {
 
 // Eight elements of one 16-element block, whose other half the lane next to this
 // one has: code word and scale byte, with the rounding of nvfp4_quant.cuh for the
-// numbers that x stands for (exact, or rounded to odd).
+// numbers that x stands for: 16-bit ones, or (ODD) what was rounded to odd.  16-bit
+// numbers need no care: of 11 bits, they and their quotients are borders or keep 2^-12
+// away from them.
+template <bool ODD>
 QWZ_DEVINL void quantise8(const float (&x)[8], uint32_t& code, uint32_t& sbits) {
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  const float q6 = __fdiv_rn(amax, 6.f);
-  sbits = quant::e4m3_encode_nonneg(odd_of(q6, __fmaf_rn(-q6, 6.f, amax)));
-  const float s = quant::e4m3_decode(sbits);
+  float q6 = __fdiv_rn(amax, 6.f);
+  if constexpr (ODD) q6 = odd_of(q6, __fmaf_rn(-q6, 6.f, amax));
+  uint32_t pair, s2, unused;
+  asm("{\n .reg .b16 t;\n cvt.rn.satfinite.e4m3x2.f32 t, %2, %1;\n cvt.u32.u16 %0, t;\n}\n" : "=r"(pair) : "f"(q6), "f"(0.f));
+  sbits = pair;  // (the high one is 0)
+  e4m3x4_to_f16x2x2(pair, s2, unused);
+  const float s = InTraits<__half>::to_float2(s2).x;
   code = 0u;
   if (s > 0.f) {
     const float r = __frcp_rn(s), cut = 8.f * s;
@@ -155,10 +169,9 @@ QWZ_DEVINL void quantise8(const float (&x)[8], uint32_t& code, uint32_t& sbits) 
       for (int e = 0; e < 2; ++e) {
         const float c = fmaxf(fminf(x[i + e], cut), -cut);
         const float q = __fmul_rn(c, r);
-        const float d = __fmaf_rn(__fmaf_rn(-q, s, c), r, q);  // c / s, correctly rounded
-        y[e] = odd_of(d, __fmaf_rn(-d, s, c));
+        y[e] = __fmaf_rn(__fmaf_rn(-q, s, c), r, q);  // c / s, correctly rounded
+        if constexpr (ODD) y[e] = odd_of(y[e], __fmaf_rn(-y[e], s, c));
       }
-      uint32_t pair;
       asm("{\n .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n cvt.u32.u8 %0, t;\n}\n"
           : "=r"(pair)
           : "f"(y[0]), "f"(y[1]));
@@ -199,25 +212,123 @@ QWZ_DEVINL void to_floats(const uint4& v, F (&x)[8]) {
   }
 }
 
-template <typename F>
-QWZ_DEVINL void scale8(F (&x)[8], const float* weight, F r) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(weight)), b = __ldg(reinterpret_cast<const float4*>(weight) + 1);
-  const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+// (x0, x1) * (a0, a1) + (c0, c1) in one instruction.
+QWZ_DEVINL void fma_pair(float& d0, float& d1, float x0, float x1, float a0, float a1, float c0, float c1) {
+  asm("{\n .reg .b64 x, a, c;\n mov.b64 x, {%2, %3};\n mov.b64 a, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, a, c;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(x0), "f"(x1), "f"(a0), "f"(a1), "f"(c0), "f"(c1));
 }
-
 QWZ_DEVINL float rsqrt_of(float x) { return rsqrtf(x); }
 QWZ_DEVINL double rsqrt_of(double x) { return rsqrt(x); }
 QWZ_DEVINL float shfl_xor_any(float x, int o) { return __shfl_xor_sync(0xffffffffu, x, o); }
 QWZ_DEVINL double shfl_xor_any(double x, int o) { return __shfl_xor_sync(0xffffffffu, x, o); }
 
-// Norm and rotation of one head, eight dims a lane (chunk c of D / 8), in F's
-// precision.  cos_sin: the row's table.
-template <typename T, int D, typename F, typename F2>
-QWZ_DEVINL void turn8(const uint4& raw, int c, const float* weight, float eps, int freqs, bool neighbours,
-                      const F2* cos_sin, F (&x)[8]) {
-  constexpr int kLanes = D / 8;
+// A lane's two chunks of eight dims of a Q head, D / 16 lanes a head.  Where the pairs
+// are (i, i + freqs) a turning lane has both of a pair, so no lane needs another's dims.
+// y0 = x0 a0 + p0 b0, y1 = x1 a1 + p1 b1 with the pairs' other dims p, the cosines, sines
+// and weights in a and b, made once for all heads of a row.
+struct TurnQ {
+  float a[2][8], b[2][8];
+  int chunk[2];
+  bool turns[2];
+
+  QWZ_DEVINL void set(int l, const float* weight, int freqs, bool neighbours, const float2* cos_sin) {
+    const int half = freqs / 8;
+    const bool both = !neighbours && l < half;
+    chunk[0] = both ? l : 2 * l;
+    chunk[1] = both ? l + half : 2 * l + 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      turns[k] = neighbours ? chunk[k] < freqs / 4 : both;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[k][i] = weight != nullptr ? __ldg(weight + 8 * chunk[k] + i) : 1.f;
+        b[k][i] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w0 = a[0][i], w1 = a[1][i];
+      if (both) {
+        const float2 t = cos_sin[8 * l + i];
+        a[0][i] = t.x * w0;
+        a[1][i] = t.x * w1;
+        b[0][i] = -t.y * w1;
+        b[1][i] = t.y * w0;
+      }
+    }
+    if (neighbours) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (turns[k]) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float2 t = cos_sin[4 * chunk[k] + i / 2];
+            const float w0 = a[k][i], w1 = a[k][i + 1];
+            a[k][i] = t.x * w0;
+            a[k][i + 1] = t.x * w1;
+            b[k][i] = -t.y * w1;
+            b[k][i + 1] = t.y * w0;
+          }
+        }
+    }
+  }
+
+  template <typename T, int LANES, bool NEIGHBOURS>
+  QWZ_DEVINL void apply(uint4 (&raw)[2], bool norm, float eps) const {
+    float x[2][8], y[2][8];
+    to_floats<T>(raw[0], x[0]);
+    to_floats<T>(raw[1], x[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        if (turns[k]) {
+          const float p0 = NEIGHBOURS ? x[k][i + 1] : x[1 - k][i], p1 = NEIGHBOURS ? x[k][i] : x[1 - k][i + 1];
+          fma_pair(y[k][i], y[k][i + 1], p0, p1, b[k][i], b[k][i + 1], 0.f, 0.f);
+          fma_pair(y[k][i], y[k][i + 1], x[k][i], x[k][i + 1], a[k][i], a[k][i + 1], y[k][i], y[k][i + 1]);
+        } else {  // (0 times an infinity is no 0)
+          y[k][i] = x[k][i] * a[k][i];
+          y[k][i + 1] = x[k][i + 1] * a[k][i + 1];
+        }
+      }
+    float r = 1.f;
+    if (norm) {
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) fma_pair(s0, s1, x[k][i], x[k][i + 1], x[k][i], x[k][i + 1], s0, s1);
+      float sum = s0 + s1;
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      r = rsqrtf(sum / (16 * LANES) + eps);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      T h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = InTraits<T>::from_float(norm ? y[k][i] * r : y[k][i]);
+      raw[k] = *reinterpret_cast<const uint4*>(h);
+    }
+  }
+};
+
+// The eight dims `c` of a K head in F's precision, D / 8 lanes a head (all lanes of the
+// warp take part).
+template <typename T, int LANES, typename F, typename F2>
+QWZ_DEVINL void turn_k(const uint4& raw, int c, const float* weight, float eps, int freqs, bool neighbours,
+                       const F2* cos_sin, F (&y)[8]) {
+  const int half = freqs / 8, lane = threadIdx.x & 31;
+  const bool turns = c < 2 * half, low = c < half;
+  const int other = turns && !neighbours ? (low ? c + half : c - half) : c, from = lane - c + other;
+  uint4 w;
+  w.x = __shfl_sync(0xffffffffu, raw.x, from);
+  w.y = __shfl_sync(0xffffffffu, raw.y, from);
+  w.z = __shfl_sync(0xffffffffu, raw.z, from);
+  w.w = __shfl_sync(0xffffffffu, raw.w, from);
+  F x[8];
   to_floats<T>(raw, x);
   F r = 1;
   if (weight != nullptr) {
@@ -225,65 +336,131 @@ QWZ_DEVINL void turn8(const uint4& raw, int c, const float* weight, float eps, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) sum += shfl_xor_any(sum, o);
-    r = rsqrt_of(sum / D + (F)eps);
-    scale8(x, weight + 8 * c, r);
-  }
-  if (neighbours) {
-    if (c < freqs / 4) {
+    for (int k = LANES / 2; k > 0; k >>= 1) sum += shfl_xor_any(sum, k);
+    r = rsqrt_of(sum / (8 * LANES) + (F)eps);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const F2 t = cos_sin[4 * c + i];
-        const F a = x[2 * i], b = x[2 * i + 1];
-        x[2 * i] = a * t.x - b * t.y;
-        x[2 * i + 1] = b * t.x + a * t.y;
-      }
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * __ldg(weight + 8 * c + i);
+  }
+  if (!turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+  } else if (neighbours) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const F2 t = cos_sin[4 * c + i / 2];
+      y[i] = x[i] * t.x - x[i + 1] * t.y;
+      y[i + 1] = x[i + 1] * t.x + x[i] * t.y;
     }
   } else {
-    // the chunk `half` chunks away has the pairs' other halves
-    const int half = freqs / 8, lane = threadIdx.x & 31;
-    const bool turns = c < 2 * half, low = c < half;
-    const int other = turns ? (low ? c + half : c - half) : c;
-    const int from = lane - c + other;
-    uint4 w;
-    w.x = __shfl_sync(0xffffffffu, raw.x, from);
-    w.y = __shfl_sync(0xffffffffu, raw.y, from);
-    w.z = __shfl_sync(0xffffffffu, raw.z, from);
-    w.w = __shfl_sync(0xffffffffu, raw.w, from);
-    if (turns) {
-      F y[8];
-      to_floats<T>(w, y);
-      if (weight != nullptr) scale8(y, weight + 8 * other, r);
-      const int f0 = 8 * (low ? c : c - half);
+    F o[8];
+    to_floats<T>(w, o);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const F2 t = cos_sin[f0 + i];
-        x[i] = low ? x[i] * t.x - y[i] * t.y : x[i] * t.x + y[i] * t.y;
-      }
+    for (int i = 0; i < 8; ++i) {
+      const F2 t = cos_sin[8 * (low ? c : c - half) + i];
+      if (weight != nullptr) o[i] = o[i] * r * __ldg(weight + 8 * other + i);
+      y[i] = low ? x[i] * t.x - o[i] * t.y : x[i] * t.x + o[i] * t.y;
     }
   }
 }
 
-constexpr int kRotThreads = 256;
+// Code word and scale byte of a K head's eight dims from 64 bits.
+template <typename T, int LANES>
+__device__ __noinline__ void k_from_64(const uint4 raw, int c, const float* weight, float eps, int freqs, bool neighbours,
+                                       const double2* cos_sin, uint32_t& code, uint32_t& sbits) {
+  double y[8];
+  turn_k<T, LANES, double, double2>(raw, c, weight, eps, freqs, neighbours, cos_sin, y);
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = float_odd(y[i]);
+  quantise8<true>(x, code, sbits);
+}
 
-template <int ROWS>
-struct RotTable {
-  double2 wide[ROWS][128];  // (cos, sin) of a row's angles
-  float2 narrow[ROWS][128];
-};
+// The same from 32 bits; false where a border lies inside the error bound.
+//
+// An error is at most 24 x 2^-24 of |a| + |b|, the two terms of a dim (products, sum,
+// cosine, sine, weight: 8; half of the sum of squares' 16; the root and two products: 8),
+// and |a| + |b| <= 2 max |x'| of the head: below 2^-18 max |x'|.  A head without norm has
+// its other dims exactly.
+template <typename T, int LANES>
+QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_max, float eps, int freqs,
+                          bool neighbours, const float2* cos_sin, uint32_t& code, uint32_t& sbits) {
+  float y[8];
+  turn_k<T, LANES, float, float2>(raw, c, weight, eps, freqs, neighbours, cos_sin, y);
+  float most = 0.f, sum = 0.f, amax = 0.f;
+  {
+    float x[8];
+    to_floats<T>(raw, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      most = fmaxf(most, fabsf(x[i]));
+      sum += x[i] * x[i];
+      amax = fmaxf(amax, fabsf(y[i]));
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  if (weight != nullptr) most *= w_max * rsqrtf(sum / (8 * LANES) + eps) * 1.0001f;
+  float err = weight != nullptr || c < freqs / 4 ? most * 3.8146973e-6f : 0.f;
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  const float err2 = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, 1));
+  // the scale of the least and of the largest that amax can be (equal where it is exact)
+  const float q6 = __fdiv_rn(amax, 6.f), slack = err2 > 0.f ? err2 + q6 * 2.4e-7f : 0.f;
+  uint32_t pair, s2, unused;
+  asm("{\n .reg .b16 t;\n cvt.rn.satfinite.e4m3x2.f32 t, %2, %1;\n cvt.u32.u16 %0, t;\n}\n"
+      : "=r"(pair)
+      : "f"(q6 - slack), "f"(q6 + slack));
+  sbits = pair & 0xffu;
+  bool fine = sbits == pair >> 8 && most < 1e30f;
+  e4m3x4_to_f16x2x2(sbits, s2, unused);
+  const float s = InTraits<__half>::to_float2(s2).x;
+  code = 0u;
+  uint32_t high = 0u;
+  if (s > 0.f) {
+    const float r = __frcp_rn(s), d = err > 0.f ? err * r * 1.0001f + 2e-6f : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      float z[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float q = __fmul_rn(y[i + e], r);
+        z[e] = __fmaf_rn(__fmaf_rn(-q, s, y[i + e]), r, q);  // correctly rounded
+      }
+      asm("{\n .reg .b8 t, u;\n cvt.rn.satfinite.e2m1x2.f32 t, %3, %2;\n cvt.rn.satfinite.e2m1x2.f32 u, %5, %4;\n"
+          " cvt.u32.u8 %0, t;\n cvt.u32.u8 %1, u;\n}\n"
+          : "=r"(pair), "=r"(unused)
+          : "f"(z[0] - d), "f"(z[1] - d), "f"(z[0] + d), "f"(z[1] + d));
+      code |= pair << (4 * i);
+      high |= unused << (4 * i);
+    }
+    const uint32_t m = code & 0x77777777u, some = (m | (m >> 1) | (m >> 2)) & 0x11111111u;
+    code = m | (code & (some << 3));  // a zero magnitude carries no sign
+    const uint32_t mh = high & 0x77777777u, someh = (mh | (mh >> 1) | (mh >> 2)) & 0x11111111u;
+    fine = fine && code == (mh | (high & (someh << 3)));
+  }
+  return fine;
+}
+
+constexpr int kRotThreads = 256;
 
 }  // namespace
 
-// A CTA has ROWS rows: their angles' cosines and sines first, then heads, D / 8
-// lanes each, the row's Q heads, K heads and V heads in turn.  grid.y CTAs share
-// the heads of the same rows.
+// A CTA has ROWS rows: their angles' cosines and sines first, then tasks of one warp
+// each: q_units warp loads of a row's Q heads, its K heads, its V heads.  grid.y CTAs
+// share the tasks of the same rows.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kRotThreads) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p) {
-  constexpr int kLanes = D / 8, kHeads = 32 / kLanes;  // lanes a head, heads a warp
-  __shared__ RotTable<ROWS> table;
+__global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p, int q_units) {
+  constexpr int kLanes = D / 8, kHeads = 32 / kLanes;     // K, V: lanes a head, heads a warp
+  constexpr int kQLanes = D / 16, kQHeads = 32 / kQLanes;  // Q
+  constexpr int kLoads = 2;                                // warp loads of Q that are under way together
+  __shared__ double2 table[ROWS][128];                     // (cos, sin) of a row's angles
+  __shared__ float2 narrow[ROWS][128];
   griddep_wait();
   const BatchAppendParams& a = p.kv;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane % kLanes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const bool neighbours = p.neighbours != 0;
   const long long row0 = (long long)blockIdx.x * ROWS;
   const int rows = (int)min((long long)ROWS, a.rows - row0);
   for (int i = tid; i < rows * p.freqs; i += kRotThreads) {
@@ -296,57 +473,85 @@ __global__ void __launch_bounds__(kRotThreads) batch_rotate_kernel(const __grid_
     const double low = __fma_rn(angle, kTurn, -turns) + angle * kTurnLow + rest * kTurn;
     double s, co;
     sincospi(2.0 * ((turns - rint(turns)) + low), &s, &co);
-    table.wide[r][f] = make_double2(co, s);
-    table.narrow[r][f] = make_float2((float)co, (float)s);
+    table[r][f] = make_double2(co, s);
+    narrow[r][f] = make_float2((float)co, (float)s);
   }
   __syncthreads();
-  const int qu = (p.q_heads + kHeads - 1) / kHeads, ku = (a.kv_heads + kHeads - 1) / kHeads;
-  const int per_row = qu + 2 * ku, step = gridDim.y * (kRotThreads / 32);
-  for (int u = blockIdx.y * (kRotThreads / 32) + warp; u < rows * per_row; u += step) {
-    const int r = u / per_row, v = u % per_row;
+  const int q_tasks = (p.q_heads + q_units * kQHeads - 1) / (q_units * kQHeads), per_row = q_tasks + 2;
+  const int kv_units = (a.kv_heads + kHeads - 1) / kHeads;
+  for (int task = blockIdx.y * (kRotThreads / 32) + warp; task < rows * per_row; task += gridDim.y * (kRotThreads / 32)) {
+    const int r = task / per_row, v = task % per_row;
     const long long row = row0 + r;
-    const int kind = v < qu ? 0 : v < qu + ku ? 1 : 2;  // Q, K, V
-    const int head = (kind == 0 ? v : kind == 1 ? v - qu : v - qu - ku) * kHeads + lane / kLanes;
-    const bool mine = head < (kind == 0 ? p.q_heads : a.kv_heads);
-    const T* src = reinterpret_cast<const T*>(kind == 0 ? p.q : kind == 1 ? a.k : a.v) +
-                   row * (kind == 0 ? p.q_stride : kind == 1 ? a.k_stride : a.v_stride) + head * D + 8 * c;
-    const uint4 raw = mine ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-    if (kind == 0) {
-      float x[8];
-      turn8<T, D, float, float2>(raw, c, p.q_weight, p.eps, p.freqs, p.neighbours != 0, table.narrow[r], x);
-      if (mine) {
-        T h[8];
+    if (v < q_tasks) {
+      const int l = lane % kQLanes, sub = lane / kQLanes;
+      const int first = v * q_units * kQHeads, end = min(p.q_heads, first + q_units * kQHeads);
+      TurnQ turn;
+      turn.set(l, p.q_weight, p.freqs, neighbours, narrow[r]);
+      const T* src = reinterpret_cast<const T*>(p.q) + row * p.q_stride;
+      T* dst = reinterpret_cast<T*>(p.q_out) + row * p.q_out_stride;
+#pragma unroll 1
+      for (int h0 = first; h0 < end; h0 += kLoads * kQHeads) {
+        uint4 raw[kLoads][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = InTraits<T>::from_float(x[i]);
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out) + row * p.q_out_stride + head * D + 8 * c) =
-            *reinterpret_cast<const uint4*>(h);
+        for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int head = h0 + u * kQHeads + sub;
+            raw[u][k] = make_uint4(0u, 0u, 0u, 0u);
+            if (head < end) raw[u][k] = *reinterpret_cast<const uint4*>(src + head * D + 8 * turn.chunk[k]);
+          }
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          if (neighbours) turn.template apply<T, kQLanes, true>(raw[u], p.q_weight != nullptr, p.eps);
+          else turn.template apply<T, kQLanes, false>(raw[u], p.q_weight != nullptr, p.eps);
+          const int head = h0 + u * kQHeads + sub;
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (head < end) *reinterpret_cast<uint4*>(dst + head * D + 8 * turn.chunk[k]) = raw[u][k];
+        }
       }
       continue;
     }
-    float x[8];
-    if (kind == 1) {
-      double y[8];
-      turn8<T, D, double, double2>(raw, c, p.k_weight, p.eps, p.freqs, p.neighbours != 0, table.wide[r], y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = float_odd(y[i]);
-    } else {
-      to_floats<T>(raw, x);
-    }
-    uint32_t code, sbits;
-    quantise8(x, code, sbits);
-    if (!mine) continue;
+    const int c = lane % kLanes, sub = lane / kLanes;
+    const bool is_k = v == q_tasks;
     const int slot = __ldg(a.slots + row);
-    if (slot >= 0 && (slot >> 8) < a.num_pages) {
-      const size_t at = (size_t)slot * a.kv_heads + head;
-      reinterpret_cast<uint32_t*>(kind == 1 ? a.k_cache : a.v_cache)[at * kLanes + c] = code;
-      if ((c & 1) == 0) (kind == 1 ? a.k_scales : a.v_scales)[at * (D / 16) + c / 2] = (uint8_t)sbits;
-    } else if (slot >= 0) {
-      flag_error(kErrSlotRange);
+    const bool stored = slot >= 0 && (slot >> 8) < a.num_pages;
+    if (slot >= 0 && !stored) flag_error(kErrSlotRange);
+    const T* src = reinterpret_cast<const T*>(is_k ? a.k : a.v) + row * (is_k ? a.k_stride : a.v_stride) + sub * D + 8 * c;
+    float w_max = 1.f;
+    if (is_k && p.k_weight != nullptr) {
+      w_max = 0.f;
+      for (int i = 0; i < 8; ++i) w_max = fmaxf(w_max, fabsf(__ldg(p.k_weight + 8 * c + i)));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, o));
     }
-    void* held = kind == 1 ? a.k_held : a.v_held;
-    if (held != nullptr)
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(held) + (row * a.kv_heads + head) * D + 8 * c) =
-          held8<T>(code, sbits);
+    uint4 next = sub < a.kv_heads ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+    for (int u = 0; u < kv_units; ++u) {
+      const int head = u * kHeads + sub;
+      const uint4 raw = next;
+      next = make_uint4(0u, 0u, 0u, 0u);
+      if (u + 1 < kv_units && head + kHeads < a.kv_heads) next = *reinterpret_cast<const uint4*>(src + (u + 1) * kHeads * D);
+      uint32_t code, sbits;
+      if (is_k) {
+        const bool fine = k_from_32<T, kLanes>(raw, c, p.k_weight, w_max, p.eps, p.freqs, neighbours, narrow[r], code, sbits);
+        if (!__all_sync(0xffffffffu, fine))
+          k_from_64<T, kLanes>(raw, c, p.k_weight, p.eps, p.freqs, neighbours, table[r], code, sbits);
+      } else {
+        float x[8];
+        to_floats<T>(raw, x);
+        quantise8<false>(x, code, sbits);
+      }
+      if (head >= a.kv_heads) continue;
+      if (stored) {
+        const size_t at = (size_t)slot * a.kv_heads + head;
+        reinterpret_cast<uint32_t*>(is_k ? a.k_cache : a.v_cache)[at * kLanes + c] = code;
+        if ((c & 1) == 0) (is_k ? a.k_scales : a.v_scales)[at * (D / 16) + c / 2] = (uint8_t)sbits;
+      }
+      void* held = is_k ? a.k_held : a.v_held;
+      if (held != nullptr)
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(held) + (row * a.kv_heads + head) * D + 8 * c) = held8<T>(code, sbits);
+    }
   }
   griddep_launch_dependents();
 }
@@ -355,15 +560,16 @@ namespace {
 
 template <typename T, int D>
 cudaError_t launch_rotate(const BatchRotateParams& p, cudaStream_t stream) {
-  constexpr int kHeads = 256 / D;
-  const int per_row = (p.q_heads + kHeads - 1) / kHeads + 2 * ((p.kv.kv_heads + kHeads - 1) / kHeads);
-  // few rows: a row's heads over several CTAs, each with the row's angles
-  if (p.kv.rows <= 256)
+  constexpr int kQHeads = 512 / D;
+  // few rows: a row's tasks by themselves, each CTA with the row's angles, and short ones
+  const int units = p.kv.rows <= 1024 ? 2 : 12;
+  const int per_row = (p.q_heads + units * kQHeads - 1) / (units * kQHeads) + 2;
+  if (p.kv.rows <= 1024)
     return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)p.kv.rows, (per_row + 7) / 8), dim3(kRotThreads), 0,
-                      stream, p);
-  constexpr int kRows = 4;
+                      stream, p, units);
+  constexpr int kRows = 8;
   return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((p.kv.rows + kRows - 1) / kRows)),
-                    dim3(kRotThreads), 0, stream, p);
+                    dim3(kRotThreads), 0, stream, p, units);
 }
 
 template <typename T>
