@@ -139,24 +139,22 @@ struct FewWalk {
     return g >= 0 && __ldcg(p.direct + g) != 0 ? g : -1;
   }
   // a request without tokens still has rows to write
-  static QWZ_DEVINL int units_of(const BatchAttnParams& p, const batch::Req& r, int b) {
+  // (g: its prefix where it reads it by itself)
+  static QWZ_DEVINL int units_of(const BatchAttnParams& p, const batch::Req& r, int g) {
     int units = max(1, (r.kv + U - 1) / U);
-    if constexpr (M == kBatchShared) {
-      const int g = direct(p, b);
-      if (g >= 0) units += (batch::tokens_of(p, g) + U - 1) / U;
-    }
+    if (M == kBatchShared && g >= 0) units += (batch::tokens_of(p, g) + U - 1) / U;
     return units;
   }
   static QWZ_DEVINL long long cost(const BatchAttnParams& p, int b, int c0) {
     const batch::Req r = batch::load_req(p, b);
-    return few(p, r, c0) ? units_of(p, r, b) + kOver : 0;
+    return few(p, r, c0) ? units_of(p, r, -1) + kOver : 0;
   }
   QWZ_DEVINL void enter(const BatchAttnParams& p, int bb) {
     b = bb;
     r = batch::load_req(p, b);
-    units = units_of(p, r, b);
+    if constexpr (M == kBatchShared) pre_b = direct(p, b);
+    units = units_of(p, r, pre_b);
     if constexpr (M == kBatchShared) {
-      pre_b = direct(p, b);
       pre_kv = pre_b >= 0 ? batch::tokens_of(p, pre_b) : 0;
       pre = (pre_kv + U - 1) / U;
     }
@@ -175,6 +173,23 @@ struct FewWalk {
     if (b == p.requests) return;
     enter(p, b);
     unit = max((int)u - kOver, 0);
+  }
+  // The same by the warp, from the units before each request: the last request that
+  // begins at or before unit u.
+  QWZ_DEVINL void find(const BatchAttnParams& p, const long long* starts, long long u) {
+    const int lane = threadIdx.x & 31;
+    b = 0;
+    for (int n = p.requests + 1; n > 1;) {
+      const int step = (n + 31) / 32;
+      const int count = __popc(__ballot_sync(kFull, lane * step < n && __ldcg(starts + b + lane * step) <= u));
+      b += (count - 1) * step;
+      n = min(step, n - (count - 1) * step);
+    }
+    base = __ldcg(starts + b);
+    unit = 0;
+    if (b == p.requests) return;
+    enter(p, b);
+    unit = max((int)(u - base) - kOver, 0);
   }
   // To the next request that has work here.
   QWZ_DEVINL void next_request(const BatchAttnParams& p, int c0) {
@@ -340,19 +355,28 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
   long long* starts = reinterpret_cast<long long*>(sgen);  // weighed units before each scanning thread's requests
   long long* warp_sums = starts + kFewScan;
   const int per = (p.requests + kFewScan - 1) / kFewScan;
-  long long mine = 0;
-  if (tid < kFewScan)
-    for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, c0);
+  const long long* known = M == kBatchShared ? p.few_starts + (size_t)(c0 / kFewCols) * (p.requests + 1) : nullptr;
   long long total;
-  const long long before = batch::block_scan(mine, warp_sums, total);
-  if (tid < kFewScan) starts[tid] = before;
-  __syncthreads();
+  if constexpr (M == kBatchShared) {
+    total = __ldcg(known + p.requests);
+  } else {
+    long long mine = 0;
+    if (tid < kFewScan)
+      for (int b = tid * per; b < min(p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, c0);
+    const long long before = batch::block_scan(mine, warp_sums, total);
+    if (tid < kFewScan) starts[tid] = before;
+    __syncthreads();
+  }
   auto seek = [&](long long u) {
-    int at = 0;
-    for (int step = kFewScan / 2; step > 0; step >>= 1)
-      if (starts[at + step] <= u) at += step;
     Walk w;
-    w.seek(p, c0, min(at * per, p.requests), starts[at], u);
+    if constexpr (M == kBatchShared) {
+      w.find(p, known, u);
+    } else {
+      int at = 0;
+      for (int step = kFewScan / 2; step > 0; step >>= 1)
+        if (starts[at + step] <= u) at += step;
+      w.seek(p, c0, min(at * per, p.requests), starts[at], u);
+    }
     return w;
   };
   Walk cur = seek(split * total / splits);
@@ -437,11 +461,11 @@ __global__ void __launch_bounds__(Few<D>::kThreads, Few<D>::kCtas)
         }
         if (pre_b < p.requests) {
           pre_unit = 0;
-          pre_left = pre_b == end_b ? end_unit : Walk::units_of(p, r, pre_b);
+          const int g = Walk::direct(p, pre_b);
+          pre_left = pre_b == end_b ? end_unit : Walk::units_of(p, r, g);
           pre_kv = r.kv;
           pre_row = p.block_table + (size_t)pre_b * p.table_width;
           if constexpr (M == kBatchShared) {
-            const int g = Walk::direct(p, pre_b);
             const int kv = g >= 0 ? batch::tokens_of(p, g) : 0;
             pre_in = (kv + F::kUnit - 1) / F::kUnit;
             if (pre_in > 0) {

@@ -38,13 +38,15 @@ struct BatchAttnParams {
   const int32_t* alone;          // [requests] the only request that reads this one (-1: none, or several do)
   const int32_t* shared_rows;    // [rows] rows by prefix
   int32_t* direct;               // [requests] whether those that read this prefix do so by themselves
+  long long* few_starts;         // [col_groups][requests + 1] weighed units of batch_few.cu before each request
   int32_t* busy;                 // [1 + kv_heads * col_groups] CTAs with work of batch_tiles.cu, of batch_few.cu's columns
   // the parts of a row, of its prefix and of its own tokens: [2][rows, q_heads]
   uint32_t* where;               // BatchWhere
   float* part_ml;                // reference maximum and sum of a whole part
   float* part_o;                 // and its unnormalised output [2][rows, q_heads, dim]
 };
-// What a launch of batch_few.cu and batch_rows.cu does: all of a request's tokens
+constexpr int kShareMaxRequests = 1 << 14;
+// What a launch of batch_few.cu does: all of a request's tokens
 // into out (kBatchPlain), or the parts that batch_join.cu merges (kBatchShared).
 enum BatchMode : int { kBatchPlain = 0, kBatchShared = 1 };
 // Where a part is: bits 0-1 what, 2-11 first CTA (split) of its records, 12-21 their
@@ -66,11 +68,12 @@ size_t batch_few_record_bytes(int dim);  // all records of batch_few.cu
 size_t batch_workspace_bytes(int dim);
 // What attention behind shared prefixes adds to it.
 struct BatchSharedSpace {
-  int64_t direct, busy, where, ml, o, bytes;  // offsets
+  int64_t starts, direct, busy, where, ml, o, bytes;  // offsets
   BatchSharedSpace(int dim, int64_t rows, int64_t q_heads) {
     const int64_t pairs = 2 * rows * q_heads;
-    direct = 0;
-    busy = direct + 4 * (int64_t)(1 << 14);
+    starts = 0;
+    direct = starts + 2 * 8 * ((int64_t)kShareMaxRequests + 1);
+    busy = direct + 4 * (int64_t)kShareMaxRequests;
     where = busy + 4 * 1024;
     ml = where + (4 * pairs + 15) / 16 * 16;
     o = ml + 8 * pairs;
@@ -125,7 +128,6 @@ struct BatchShareParams {
   int32_t* positions_out;        // [rows]
   int requests, rows;
 };
-constexpr int kShareMaxRequests = 1 << 14;
 
 // Q and K normed and rotated, K and V quantised into their slots (batch_prefix.cu).
 struct BatchRotateParams {

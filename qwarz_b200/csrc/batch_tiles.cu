@@ -229,21 +229,21 @@ QWZ_DEVINL int tl_shared_row(const BatchAttnParams& p, int at) {
 // prefixes by themselves (tokens x KV heads x head dims) costs less than the
 // records, the 128-row tiles and the first wait of this kernel.
 constexpr long long kTlSmall = 24 * 1024 * 1024;
-QWZ_DEVINL bool tl_small(const BatchAttnParams& p, int dim, long long* sums) {
+// Also: `any`, whether a request has more rows than batch_few.cu takes.
+QWZ_DEVINL bool tl_small(const BatchAttnParams& p, int dim, long long* sums, bool& any) {
   const int per = (p.requests + kTlScan - 1) / kTlScan;
   long long mine = 0, total;
-  bool wide = false;
+  int wide = 0;  // 1: a request with many rows, 2: one that reads a prefix
   if (threadIdx.x < kTlScan)
     for (int b = threadIdx.x * per; b < min(p.requests, (int)(threadIdx.x + 1) * per); ++b) {
-      const int g = batch::prefix_of(p, b);
-      if (g < 0) continue;
-      const int n = batch::load_req(p, b).n;
-      if (n > 0) mine += batch::tokens_of(p, g);
-      wide |= n * p.group > p.few_cols;
+      const int g = batch::prefix_of(p, b), n = batch::load_req(p, b).n;
+      if (g >= 0 && n > 0) mine += batch::tokens_of(p, g);
+      if (n * p.group > p.few_cols) wide |= g >= 0 ? 3 : 1;
     }
-  const bool any = __syncthreads_or(wide) != 0;
+  any = __syncthreads_or(wide) != 0;
+  const bool behind = __syncthreads_or(wide & 2) != 0;
   batch::block_scan(mine, sums, total);
-  return !any && total * p.kv_heads * dim <= kTlSmall;
+  return !behind && total * p.kv_heads * dim <= kTlSmall;
 }
 
 // BYTES (4 or 16) to shared memory; zeros without a read where there is nothing.
@@ -332,6 +332,33 @@ struct Pair {
           : "memory");
   }
 };
+
+// The weighed units of batch_few.cu before each request, by one CTA: each of its CTAs
+// would else scan all requests, five dependent loads each, before its first copy.
+template <int D>
+QWZ_DEVINL void tl_few_starts(const BatchAttnParams& p, bool small, long long* sums) {
+  using Walk = FewWalk<Few<D>::kUnit, kBatchShared>;
+  const int per = (p.requests + kTlThreads - 1) / kTlThreads, b0 = threadIdx.x * per, b1 = min(p.requests, b0 + per);
+  for (int c = 0; c < p.col_groups; ++c) {
+    long long* out = p.few_starts + (size_t)c * (p.requests + 1);
+    long long mine = 0, total;
+    for (int b = b0; b < b1; ++b) {
+      const batch::Req r = batch::load_req(p, b);
+      int g = batch::prefix_of(p, b);
+      if (g >= 0 && !TilesWalk<Tiles<D>::kRows>::direct(p, g, batch::load_prefix(p, g), small)) g = -1;
+      const long long cost = Walk::few(p, r, c * kFewCols) ? Walk::units_of(p, r, g) + Walk::kOver : 0;
+      out[b] = cost;  // (its own cost for now)
+      mine += cost;
+    }
+    long long at = batch::block_scan(mine, sums, total);
+    for (int b = b0; b < b1; ++b) {
+      const long long cost = out[b];
+      out[b] = at;
+      at += cost;
+    }
+    if (threadIdx.x == 0) out[p.requests] = total;
+  }
+}
 
 template <int REGS>
 QWZ_DEVINL void tl_more_regs() {
@@ -442,15 +469,19 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
   griddep_wait();
 
   // ---------------------------------------------------- this CTA's (cluster's) share
-  const bool small = tl_small(p, D, sums);
+  bool any;
+  const bool small = tl_small(p, D, sums, any);
   if (blockIdx.x == 0)
     for (int g = tid; g < p.requests; g += kTlThreads) p.direct[g] = Walk::direct(p, g, batch::load_prefix(p, g), small);
   const int per = (2 * p.requests + kTlScan - 1) / kTlScan;
-  long long mine = 0, total;
-  if (tid < kTlScan)
-    for (int b = tid * per; b < min(2 * p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, small);
-  const long long before = batch::block_scan(mine, sums, total);
-  if (tid < kTlScan) starts[tid] = before;
+  long long mine = 0, total = 0;
+  if (any || !small) {
+    if (tid < kTlScan)
+      for (int b = tid * per; b < min(2 * p.requests, (tid + 1) * per); ++b) mine += Walk::cost(p, b, small);
+    const long long before = batch::block_scan(mine, sums, total);
+    if (tid < kTlScan) starts[tid] = before;
+  }
+  if (blockIdx.x + 1 == gridDim.x) tl_few_starts<D>(p, small, sums);  // batch_few.cu's shares, for all of its CTAs
   const int cluster = blockIdx.x / C, clusters = gridDim.x / C;
   const long long lo = (long long)cluster * total / clusters, hi = ((long long)cluster + 1) * total / clusters;
   if (tid == 0 && blockIdx.x == 0) p.busy[0] = (int)min(total, (long long)clusters);

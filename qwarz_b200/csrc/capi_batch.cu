@@ -173,6 +173,7 @@ int attend_checked(const char* what, const int32_t* plan, bool shared, const voi
   p.shared_rows = p.alone + requests;
   uint8_t* space = static_cast<uint8_t*>(workspace) + qwz::batch_workspace_bytes(head_dim);
   const qwz::BatchSharedSpace at(head_dim, rows, num_q_heads);
+  p.few_starts = reinterpret_cast<long long*>(space + at.starts);
   p.direct = reinterpret_cast<int32_t*>(space + at.direct);
   p.busy = reinterpret_cast<int32_t*>(space + at.busy);
   p.where = reinterpret_cast<uint32_t*>(space + at.where);
