@@ -246,6 +246,19 @@ def share_prefixes(prefix_of, kv_lens, cu_rows, positions, request_of, plan, pos
         plan.data_ptr(), positions_out.data_ptr(), R, T)
 
 
+def _weight(name: str, t, dim: int) -> int:
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != dim or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 [{dim}]")
+    return t.data_ptr()
+
+
+def _held(t, k) -> int:
+    if t.dtype is not k.dtype or t.shape != k.shape:
+        raise ValueError("k_held and v_held must have k's shape and dtype")
+    _contig("k_held and v_held", t)
+    return t.data_ptr()
+
+
 def append_rotated(q, k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq,
                    neighbours: bool = False, q_weight=None, k_weight=None, eps: float = 1e-6, k_held=None,
                    v_held=None) -> None:
@@ -264,37 +277,34 @@ def append_rotated(q, k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, 
     dev = _device(q, (k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq, q_weight,
                       k_weight, k_held, v_held))
     P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)
-    q_heads = q.shape[1] if q.dim() == 3 else 0
-    T, q_stride = _rows("q", q, q_heads, dim)
+    T, q_heads, _ = shape = q.shape if q.dim() == 3 else (0, 0, 0)
     dtype = q.dtype
-    strides = [q_stride]
-    for name, t, n in (("k", k, heads), ("v", v, heads), ("q_out", q_out, q_heads)):
-        Tt, stride = _rows(name, t, n, dim)
-        if Tt != T or t.dtype is not dtype:
-            raise ValueError("q, k, v and q_out must have the same rows and dtype")
-        strides.append(stride)
+    if q_out.shape != shape or v.shape != k.shape or k.shape[0] != T \
+            or q_out.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError("q, k, v and q_out must have the same rows and dtype, q_out the shape of q, v that of k")
+    q_stride, out_stride = _rows("q", q, q_heads, dim)[1], _rows("q_out", q_out, q_heads, dim)[1]
+    k_stride, v_stride = _rows("k", k, heads, dim)[1], _rows("v", v, heads, dim)[1]
     _int32(("slots", "positions"), (slots, positions))
     if slots.numel() != T or positions.numel() != T:
         raise ValueError("slots and positions must have one entry per row")
     f32 = torch.float32
     if inv_freq.dtype is not f32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float32 vector")
-    extra = []
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None and (t.dtype is not f32 or t.shape != (dim,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous float32 [{dim}]")
-        extra.append(None if t is None else t.data_ptr())
-    for t in (k_held, v_held):
-        if t is not None:
-            if t.dtype is not dtype or t.shape != k.shape:
-                raise ValueError("k_held and v_held must have k's shape and dtype")
-            _contig("k_held and v_held", t)
-        extra.append(None if t is None else t.data_ptr())
+    qw = kw = kh = vh = None
+    if q_weight is not None:
+        qw = _weight("q_weight", q_weight, dim)
+    if k_weight is not None:
+        kw = _weight("k_weight", k_weight, dim)
+    if k_held is not None:
+        kh = _held(k_held, k)
+    if v_held is not None:
+        vh = _held(v_held, k)
     _launch(
         dev, "qwz_batch_append_rotated",
         q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scales.data_ptr(), v_scales.data_ptr(), slots.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), *extra,
-        T, *strides, q_heads, heads, dim, inv_freq.numel(), int(neighbours), eps, P, _dtype_code(dtype))
+        k_scales.data_ptr(), v_scales.data_ptr(), slots.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), qw, kw,
+        kh, vh, T, q_stride, k_stride, v_stride, out_stride, q_heads, heads, dim, inv_freq.numel(), bool(neighbours), eps,
+        P, _dtype_code(dtype))
 
 
 def shared_workspace(device, head_dim: int, rows: int, q_heads: int) -> torch.Tensor:

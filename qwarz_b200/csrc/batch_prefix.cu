@@ -377,10 +377,11 @@ __device__ __noinline__ void k_from_64(const uint4 raw, int c, const float* weig
 
 // The same from 32 bits; false where a border lies inside the error bound.
 //
-// An error is at most 24 x 2^-24 of |a| + |b|, the two terms of a dim (products, sum,
-// cosine, sine, weight: 8; half of the sum of squares' 16; the root and two products: 8),
-// and |a| + |b| <= 2 max |x'| of the head: below 2^-18 max |x'|.  A head without norm has
-// its other dims exactly.
+// Errors in parts of 2^-24 of |a| + |b|, the two terms of a dim, which is at most twice the
+// head's largest |x'|: cosine or sine, product and sum 3; with a norm also half of the sum of
+// squares' 14 and of eps' 1, the root's 4 (two places), two products: 16.5.  So 6 x 2^-24 =
+// 3.6e-7 of max |x'|, and 33 x 2^-24 = 2.0e-6.  A head without norm has its other dims
+// exactly.  The quotient adds 2^-24 of at most 6.
 template <typename T, int LANES>
 QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_max, float eps, int freqs,
                           bool neighbours, const float2* cos_sin, uint32_t& code, uint32_t& sbits) {
@@ -403,7 +404,7 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   if (weight != nullptr) most *= w_max * rsqrtf(sum / (8 * LANES) + eps) * 1.0001f;
-  float err = weight != nullptr || c < freqs / 4 ? most * 3.8146973e-6f : 0.f;
+  const float err = weight != nullptr ? most * 2.1e-6f : c < freqs / 4 ? most * 3.8e-7f : 0.f;
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   const float err2 = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, 1));
   // the scale of the least and of the largest that amax can be (equal where it is exact)
@@ -419,7 +420,7 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
   code = 0u;
   uint32_t high = 0u;
   if (s > 0.f) {
-    const float r = __frcp_rn(s), d = err > 0.f ? err * r * 1.0001f + 2e-6f : 0.f;
+    const float r = __frcp_rn(s), d = err > 0.f ? err * r * 1.0001f + 6e-7f : 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       float z[2];
@@ -448,10 +449,10 @@ constexpr int kRotThreads = 256;
 }  // namespace
 
 // A CTA has ROWS rows: their angles' cosines and sines first, then tasks of one warp
-// each: q_units warp loads of a row's Q heads, its K heads, its V heads.  grid.y CTAs
-// share the tasks of the same rows.
+// each: q_units warp loads of a row's Q heads, kv_units of its K heads, of its V heads.
+// grid.y CTAs share the tasks of the same rows.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p, int q_units) {
+__global__ void __launch_bounds__(kRotThreads, 3) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p, int q_units, int kv_units) {
   constexpr int kLanes = D / 8, kHeads = 32 / kLanes;     // K, V: lanes a head, heads a warp
   constexpr int kQLanes = D / 16, kQHeads = 32 / kQLanes;  // Q
   constexpr int kLoads = 2;                                // warp loads of Q that are under way together
@@ -477,8 +478,8 @@ __global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __gr
     narrow[r][f] = make_float2((float)co, (float)s);
   }
   __syncthreads();
-  const int q_tasks = (p.q_heads + q_units * kQHeads - 1) / (q_units * kQHeads), per_row = q_tasks + 2;
-  const int kv_units = (a.kv_heads + kHeads - 1) / kHeads;
+  const int q_tasks = (p.q_heads + q_units * kQHeads - 1) / (q_units * kQHeads);
+  const int kv_tasks = (a.kv_heads + kv_units * kHeads - 1) / (kv_units * kHeads), per_row = q_tasks + 2 * kv_tasks;
   for (int task = blockIdx.y * (kRotThreads / 32) + warp; task < rows * per_row; task += gridDim.y * (kRotThreads / 32)) {
     const int r = task / per_row, v = task % per_row;
     const long long row = row0 + r;
@@ -513,7 +514,8 @@ __global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __gr
       continue;
     }
     const int c = lane % kLanes, sub = lane / kLanes;
-    const bool is_k = v == q_tasks;
+    const bool is_k = v < q_tasks + kv_tasks;
+    const int first = (v - q_tasks - (is_k ? 0 : kv_tasks)) * kv_units * kHeads, end = min(a.kv_heads, first + kv_units * kHeads);
     const int slot = __ldg(a.slots + row);
     const bool stored = slot >= 0 && (slot >> 8) < a.num_pages;
     if (slot >= 0 && !stored) flag_error(kErrSlotRange);
@@ -525,13 +527,13 @@ __global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __gr
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, o));
     }
-    uint4 next = sub < a.kv_heads ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+    uint4 next = first + sub < end ? *reinterpret_cast<const uint4*>(src + first * D) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
-    for (int u = 0; u < kv_units; ++u) {
-      const int head = u * kHeads + sub;
+    for (int h0 = first; h0 < end; h0 += kHeads) {
+      const int head = h0 + sub;
       const uint4 raw = next;
       next = make_uint4(0u, 0u, 0u, 0u);
-      if (u + 1 < kv_units && head + kHeads < a.kv_heads) next = *reinterpret_cast<const uint4*>(src + (u + 1) * kHeads * D);
+      if (head + kHeads < end) next = *reinterpret_cast<const uint4*>(src + (h0 + kHeads) * D);
       uint32_t code, sbits;
       if (is_k) {
         const bool fine = k_from_32<T, kLanes>(raw, c, p.k_weight, w_max, p.eps, p.freqs, neighbours, narrow[r], code, sbits);
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(kRotThreads, 2) batch_rotate_kernel(const __gr
         to_floats<T>(raw, x);
         quantise8<false>(x, code, sbits);
       }
-      if (head >= a.kv_heads) continue;
+      if (head >= end) continue;
       if (stored) {
         const size_t at = (size_t)slot * a.kv_heads + head;
         reinterpret_cast<uint32_t*>(is_k ? a.k_cache : a.v_cache)[at * kLanes + c] = code;
@@ -560,16 +562,17 @@ namespace {
 
 template <typename T, int D>
 cudaError_t launch_rotate(const BatchRotateParams& p, cudaStream_t stream) {
-  constexpr int kQHeads = 512 / D;
-  // few rows: a row's tasks by themselves, each CTA with the row's angles, and short ones
-  const int units = p.kv.rows <= 1024 ? 2 : 12;
-  const int per_row = (p.q_heads + units * kQHeads - 1) / (units * kQHeads) + 2;
-  if (p.kv.rows <= 1024)
-    return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)p.kv.rows, (per_row + 7) / 8), dim3(kRotThreads), 0,
-                      stream, p, units);
+  constexpr int kQHeads = 512 / D, kHeads = 256 / D;  // a warp load's
+  const int rows = (int)p.kv.rows, kv_heads = p.kv.kv_heads;
+  if (rows <= 1024) {  // few rows: short tasks, a row's over several CTAs, each with the row's angles
+    const int tasks = (p.q_heads + kQHeads - 1) / kQHeads + 2 * ((kv_heads + kHeads - 1) / kHeads);
+    return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)rows, (tasks + 7) / 8), dim3(kRotThreads), 0, stream, p,
+                      1, 1);
+  }
+  // many: the factors of Q are made once for 12 loads (170 us with 4, 150 with 12, 16,384 rows of 24/4/256)
   constexpr int kRows = 8;
-  return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((p.kv.rows + kRows - 1) / kRows)),
-                    dim3(kRotThreads), 0, stream, p, units);
+  return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kRotThreads), 0,
+                    stream, p, 12, (kv_heads + kHeads - 1) / kHeads);
 }
 
 template <typename T>

@@ -54,7 +54,7 @@ constexpr int kTlScan = 256;                 // threads that scan the requests
 constexpr int kTlSlot = 16384;
 constexpr int kTlAhead = 2;                  // slots whose codes are on their way
 constexpr int kTlItems = 4;                  // items in flight
-constexpr int kTlOver = 3;                   // what an item costs beside its tiles, in tiles (Q, the first waits, the end)
+constexpr int kTlOver = 5;                   // what an item costs beside its tiles, in tiles (Q, the first waits, the end)
 // registers a thread: 640 x 96 at launch; 256 x 112 + 256 x 80 + 128 x 64 after the
 // split.  (Spills in these loops cost an L2 access each: there is no L1 left.)
 constexpr int kTlSoftRegs = 112, kTlDqRegs = 80, kTlRestRegs = 64;
