@@ -403,7 +403,12 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if (weight != nullptr) most *= w_max * rsqrtf(sum / (8 * LANES) + eps) * 1.0001f;
+  bool fine = true;
+  if (weight != nullptr) {
+    const float mean = sum / (8 * LANES) + eps;
+    fine = mean > 1e-30f && mean < 1e30f;  // (squares that 32 bits hold)
+    most *= w_max * rsqrtf(mean) * 1.0001f;
+  }
   const float err = weight != nullptr ? most * 2.1e-6f : c < freqs / 4 ? most * 3.8e-7f : 0.f;
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   const float err2 = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, 1));
@@ -414,7 +419,7 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
       : "=r"(pair)
       : "f"(q6 - slack), "f"(q6 + slack));
   sbits = pair & 0xffu;
-  bool fine = sbits == pair >> 8 && most < 1e30f;
+  fine = fine && sbits == pair >> 8 && most < 1e30f;
   e4m3x4_to_f16x2x2(sbits, s2, unused);
   const float s = InTraits<__half>::to_float2(s2).x;
   code = 0u;

@@ -223,6 +223,26 @@ def test_rotated_far_positions():
     assert torch.equal(held.double(), obatch.dequant(*obatch.quantise(y)))
 
 
+@pytest.mark.parametrize("norm,eps", [(True, 0.0), (True, 1e-6), (False, 1e-6)])
+def test_rotated_smallest_and_largest_k(norm, eps):
+    """K rows whose squares 32 bits do not hold, and rows of zeros."""
+    T = 8
+    q, k, v, _ = make_rows(T, 4, 2, 128, torch.bfloat16, 8)
+    k.mul_(torch.tensor([1.0, 2.0 ** -90, 2.0 ** -60, 2.0 ** -20, 2.0 ** 30, 2.0 ** 63, 2.0 ** 80, 2.0 ** -126],
+                        device="cuda").bfloat16()[:, None, None])
+    pool = [torch.zeros(1, PAGE, 2, w, dtype=torch.uint8, device="cuda") for w in (64, 64, 8, 8)]
+    held = torch.empty(T, 2, 128, dtype=torch.bfloat16, device="cuda")
+    kw, positions, inv = weight_of(128, 3) if norm else None, i32(range(5, 5 + T)), freqs_of(32)
+    batch.append_rotated(q, k, v, torch.empty_like(q.contiguous()), *pool, make_slots(T, 1, 4), positions, inv,
+                         k_weight=kw, eps=eps, k_held=held)
+    y, _ = obatch.rotate(k, positions, inv, False, kw, eps)
+    assert torch.equal(held.double(), obatch.dequant(*obatch.quantise(y)))
+    k.zero_()
+    batch.append_rotated(q, k, v, torch.empty_like(q.contiguous()), *pool, make_slots(T, 1, 4), positions, inv,
+                         k_weight=kw, eps=1e-6, k_held=held)
+    assert int(held.count_nonzero()) == 0
+
+
 def test_rotated_slot_outside_the_pool():
     x = torch.ones(3, 1, 64, device="cuda").half()
     pool = [torch.zeros(2, PAGE, 1, w, dtype=torch.uint8, device="cuda") for w in (32, 32, 4, 4)]
