@@ -6,8 +6,10 @@
 //
 // over the parts (m_i, l_i, o_i) in a fixed order: the prefix's by CTA, then the own
 // tokens' by CTA.  A warp has one (row, head), or G warps take every G-th part of
-// it.  It reads D + 2 floats a part, mostly from L2; the chain of loads from `where`
-// over the statistics to the outputs bounds it.
+// it (below 4,096 (row, head) pairs, whose items have many parts).  It reads D + 2 floats a
+// part, mostly from L2; the chain of loads from the row's request over `where` and the
+// statistics to the outputs bounds it.
+// Measured (cold, alone): 96 pairs 10 us, 1,536 of about 14 parts 19 us, 8,192 of three 19 us.
 #include "batch_common.cuh"
 
 namespace qwz {

@@ -1,14 +1,14 @@
 // Requests behind shared prefixes, sm_100a: the step's rows sorted by the prefix
 // they read, and the writer that norms and rotates Q and K on the way (the
-// attention is that of batch_rows.cu and batch_few.cu).
+// attention is that of batch_tiles.cu, batch_few.cu and batch_join.cu).
 //
 // A prefix is a request that has none itself; e(b) is the one that request b
 // reads, n(b) the request's rows.  Rows are listed by prefix, then by row, so
 // the place of request b's first row is the sum of n(b') over the requests with
 // (e(b'), b') < (e(b), b).  A warp has one request and compares it with all R (no
 // request waits for another's sums); a step's bytes are nothing beside the launch.
-// Measured: PLAN.  (Eight threads a request, whose
-// dependent loads and comparisons one after another bounded it: 28 us for 2,072.)
+// Measured: 3.6 us for 66 requests of 64 rows, 12.2 us for 2,072 of 21,130: the latency of
+// the loads that depend on one another.  (Eight threads a request: 28 us for the latter.)
 #include "batch_common.cuh"
 #include "nvfp4_quant.cuh"
 
@@ -120,12 +120,15 @@ cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t 
 // between: E4M3 scales and E2M1 codes are those of the exact y, up to the error of
 // 64 bits, so they do not depend on how 32 bits round next to a border.  They are made
 // from 32 bits and an error bound, and again from 64 where a border is inside it (a few
-// heads in a hundred).  Angles are taken in 64 bits: 32 leave 0.06 radians of a position
+// groups of heads in a hundred).  Angles are taken in 64 bits: 32 leave 0.06 radians of a position
 // of 10^6.
 //
-// Bytes bound it for long steps, as long as the instructions between them stay few: 400
-// a K or V head and 140 a Q head (one chunk of 8 dims a lane, the other dims of a pair by
-// shuffles, K in 64 bits) took 187 us for ROTATE_WAS.
+// Instructions bound it for long steps (issue slots 60 %, DRAM 41 %).  Measured, GPU times:
+// 16,384 rows of 24/4/256, a quarter of the dims turned, with norm and held values, 152 us
+// (56 % of the measured copy bandwidth); 5,001 rows of 14/2/64 13.4 us; 448 rows of 32/8/128
+// 8.6 us; 16 rows of 24/4/256 5.0 us, less than the call costs the host.  Forms that were
+// slower on the first: all of K in 64 bits with 8 dims a lane for Q, whose pairs' other dims
+// came by shuffles, 214 us; the same with factors made once a row, 187 us.
 namespace {
 
 // Nearest float with an odd last bit unless y is a float itself: later roundings

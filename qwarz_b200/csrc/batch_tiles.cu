@@ -32,6 +32,21 @@
 // The roles' loops stay rolled: together they have to fit the instruction cache.
 // (Codes held four slots ahead in registers, which unrolls the conversion by four, made
 // every conversion of a slot take 450 to 1,250 cycles instead of 300.)
+//
+// What bounds it.  At D 256 S and O fill the tensor memory, so P lies on its own S and
+// QK(j + 2) waits for PV(j): a tile's chain QK (1,300 cycles), softmax (3,100), PV (1,300)
+// and the waits between take 8,200 cycles, two tiles at a time, 4,100 a tile of 256 rows
+// where its MMAs need 2,048.  At D 128 a tile of 128 rows takes 3,200 (1,024): the MMAs of a
+// single CTA, whose operands take all of the shared memory's bandwidth, run at half rate
+// (two CTAs a unit there: 119 us against 90, since the items are not 256 rows wide).  An item
+// costs another 10 us (Q staged 4, the end 5, the first waits), which its weight in the
+// shares stands for: 12 requests with questions 206 us with five tiles, 266 with two, 211
+// with seven.
+// Measured, whole calls on the GPU, against the same rows in batch_rows.cu's form: 64 rows
+// behind 32,768 tokens, 24/4/256, 129 us (141); 256 of 32/8/128 163 (251); 24 x 7-row
+// windows 215 (278); questions of 12 requests 206 (306).
+// Not kept: Q staged by the V warps (219 us for the windows), the softmax's next chunk loaded
+// ahead (230), QK(1) of an item held back until P(0) so that the groups alternate (228).
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 #include "tc_common.cuh"
