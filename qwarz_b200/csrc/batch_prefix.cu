@@ -124,11 +124,12 @@ cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t 
 // of 10^6.
 //
 // Instructions bound it for long steps (issue slots 60 %, DRAM 41 %).  Measured, GPU times:
-// 16,384 rows of 24/4/256, a quarter of the dims turned, with norm and held values, 152 us
-// (56 % of the measured copy bandwidth); 5,001 rows of 14/2/64 13.4 us; 448 rows of 32/8/128
-// 8.6 us; 16 rows of 24/4/256 5.0 us, less than the call costs the host.  Forms that were
+// 16,384 rows of 24/4/256, a quarter of the dims turned, with norm and held values, 145 us
+// (59 % of the measured copy bandwidth); 5,001 rows of 14/2/64 12.4 us; 448 rows of 32/8/128
+// 8.3 us; 16 rows of 24/4/256 5.0 us, less than the call costs the host.  Forms that were
 // slower on the first: all of K in 64 bits with 8 dims a lane for Q, whose pairs' other dims
-// came by shuffles, 214 us; the same with factors made once a row, 187 us.
+// came by shuffles, 214 us; the same with factors made once a row, 187 us; CTAs of 256
+// threads, two an SM 160 us, three 151 us.
 namespace {
 
 // Nearest float with an odd last bit unless y is a float itself: later roundings
@@ -452,7 +453,7 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
   return fine;
 }
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 
 }  // namespace
 
@@ -460,7 +461,7 @@ constexpr int kRotThreads = 256;
 // each: q_units warp loads of a row's Q heads, kv_units of its K heads, of its V heads.
 // grid.y CTAs share the tasks of the same rows.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kRotThreads, 3) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p, int q_units, int kv_units) {
+__global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __grid_constant__ BatchRotateParams p, int q_units, int kv_units) {
   constexpr int kLanes = D / 8, kHeads = 32 / kLanes;     // K, V: lanes a head, heads a warp
   constexpr int kQLanes = D / 16, kQHeads = 32 / kQLanes;  // Q
   constexpr int kLoads = 2;                                // warp loads of Q that are under way together
@@ -574,11 +575,11 @@ cudaError_t launch_rotate(const BatchRotateParams& p, cudaStream_t stream) {
   const int rows = (int)p.kv.rows, kv_heads = p.kv.kv_heads;
   if (rows <= 1024) {  // few rows: short tasks, a row's over several CTAs, each with the row's angles
     const int tasks = (p.q_heads + kQHeads - 1) / kQHeads + 2 * ((kv_heads + kHeads - 1) / kHeads);
-    return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)rows, (tasks + 7) / 8), dim3(kRotThreads), 0, stream, p,
+    return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)rows, (tasks + 3) / 4), dim3(kRotThreads), 0, stream, p,
                       1, 1);
   }
-  // many: the factors of Q are made once for 12 loads (170 us with 4, 150 with 12, 16,384 rows of 24/4/256)
-  constexpr int kRows = 8;
+  // many: the factors of Q are made once for 12 loads (16,384 rows of 24/4/256: 170 us with 4, 151 with 12)
+  constexpr int kRows = 4;
   return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kRotThreads), 0,
                     stream, p, 12, (kv_heads + kHeads - 1) / kHeads);
 }

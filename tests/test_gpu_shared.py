@@ -170,6 +170,13 @@ def test_rotated(T, heads, kv_heads, dim, freqs, neighbours, norm, dtype):
         assert torch.equal(c, want_c) and torch.equal(s, want_s)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,freqs", [(24, 4, 256, 32), (32, 8, 128, 64), (14, 2, 64, 8), (40, 3, 128, 24)])
+@pytest.mark.parametrize("norm,dtype,neighbours", [(True, torch.bfloat16, False), (False, torch.float16, True)])
+def test_rotated_long_steps(heads, kv_heads, dim, freqs, norm, dtype, neighbours):
+    """More rows than are taken one by one (1,101 = 275 x 4 + 1)."""
+    test_rotated(1101, heads, kv_heads, dim, freqs, neighbours, norm, dtype)
+
+
 @pytest.mark.parametrize("neighbours", [False, True])
 def test_rotated_in_place(neighbours):
     """q rotated in the packed rows it lies in; K and V beside it stay as they were."""
