@@ -500,8 +500,9 @@ int qwz_batch_share_prefixes(const int32_t* prefix_of, const int32_t* kv_lens, c
  * prefix g that its request reads, and of its own those that it sees there.  A
  * prefix's tokens are read once for the rows of all its requests.  plan: as
  * qwz_batch_share_prefixes wrote it for this step; entries outside the step's
- * requests and rows set QWZ_DEVERR_TABLE_RANGE and are skipped.  workspace:
- * qwz_batch_shared_workspace_bytes (0: bad sizes), for one call at a time.
+ * requests and rows set QWZ_DEVERR_TABLE_RANGE and are skipped.  out shares no
+ * storage with q.  workspace: qwz_batch_shared_workspace_bytes (0: bad sizes),
+ * 16-byte aligned, for one call at a time.
  */
 int64_t qwz_batch_shared_workspace_bytes(int32_t head_dim, int32_t rows, int32_t num_q_heads);
 int qwz_batch_attend_shared(const void* q, const void* k_cache, const void* v_cache, const void* k_scales,
@@ -521,7 +522,9 @@ int qwz_batch_attend_shared(const void* q, const void* k_cache, const void* v_ca
  * q_out [rows, q_heads, dim] is y of q, rounded once (it may be q itself); k is
  * quantised from y without a rounding in between, v as it is.  Row strides in
  * elements, multiples of 8; num_freqs a multiple of 8, at most head_dim / 2 (0: no
- * rotation); inv_freq, q_weight and k_weight [head_dim] are FP32.
+ * rotation); inv_freq, q_weight and k_weight [head_dim] are FP32.  No output but
+ * q_out shares storage with an input or another output; rows of one slot would
+ * leave a mix of theirs there.
  */
 int qwz_batch_append_rotated(const void* q, const void* k, const void* v, void* q_out, void* k_cache, void* v_cache,
                              void* k_scales, void* v_scales, const int32_t* slots, const int32_t* positions,

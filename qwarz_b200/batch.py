@@ -272,8 +272,8 @@ def append_rotated(q, k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, 
     `neighbours`; dims behind them are not rotated.  With `q_weight`,
     `k_weight` (FP32 [dim]) a head is first divided by the root of its mean
     square (plus eps) and multiplied by the weight.  K is quantised from the
-    rotated values without a rounding in between.  slots, k_held and v_held: as
-    in `append`."""
+    rotated values without a rounding in between.  slots (each non-negative one
+    once), k_held and v_held: as in `append`."""
     dev = _device(q, (k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq, q_weight,
                       k_weight, k_held, v_held))
     P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)
@@ -321,7 +321,8 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows,
     """`attend` behind shared prefixes: a row sees every token of the prefix
     that its request reads and then its own as in `attend`.  The prefix's pages
     are read once for the rows of all its requests together.  `plan` is what
-    `share_prefixes` wrote for the step, `workspace` a `shared_workspace`."""
+    `share_prefixes` wrote for the step, `workspace` a `shared_workspace`; out
+    shares no storage with q."""
     dev, args = _attend_args(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace,
                              max_rows, sm_scale, plan)
     _launch(dev, "qwz_batch_attend_shared", *args)

@@ -121,6 +121,8 @@ int attend_checked(const char* what, const int32_t* plan, bool shared, const voi
     return fail(QWZ_EINVAL, "workspace smaller than qwz_batch_attend_workspace_bytes(head_dim)");
   if (shared && workspace_bytes < qwz_batch_shared_workspace_bytes(head_dim, rows, num_q_heads))
     return fail(QWZ_EINVAL, "workspace smaller than qwz_batch_shared_workspace_bytes(head_dim, rows, num_q_heads)");
+  if (shared && rows_meet(q, width, q_stride, out, width, out_stride, rows))
+    return fail(QWZ_EINVAL, "out must not share storage with q");
   const int sms = batch_sms();
   if (sms <= 0) return fail(QWZ_ELAUNCH, "no CUDA device");
   qwz::BatchPoolMaps maps;
@@ -275,6 +277,8 @@ int qwz_batch_append_rotated(const void* q, const void* k, const void* v, void* 
               rows_meet(h, kv_width, kv_width, q, width, q_stride, rows) ||
               rows_meet(h, kv_width, kv_width, q_out, width, q_out_stride, rows)))
       return fail(QWZ_EINVAL, "k_held and v_held must not share storage with q, k, v or q_out");
+  if (k_held && v_held && rows_meet(k_held, kv_width, kv_width, v_held, kv_width, kv_width, rows))
+    return fail(QWZ_EINVAL, "k_held and v_held must not share storage");
   p.q = q;
   p.q_out = q_out;
   p.positions = positions;

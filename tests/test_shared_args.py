@@ -81,6 +81,7 @@ def test_rotated(lib, addr, change, needle):
     # rows of one packed tensor: q_out reaches into k's columns
     ({"q_stride": 1536, "k": ("q", 2048), "k_stride": 1536, "q_out": ("q", 16), "q_out_stride": 1536}, "q_out must be q"),
     ({"k": ("q_out", 1024), "k_stride": 1536, "q_out_stride": 1536}, "k or v"),
+    ({"k_held": ("k_weight", 65536), "v_held": ("k_weight", 66000 // 16 * 16)}, "k_held and v_held must not share storage"),
 ])
 def test_rotated_shared_storage(lib, addr, change, needle):
     args = rotate_args(addr)
@@ -94,7 +95,7 @@ def test_rotated_shared_storage(lib, addr, change, needle):
     ({10: None}, "workspace"), ({11: 16}, "workspace smaller"), ({11: "plain"}, "workspace smaller"), ({12: -1}, "rows"),
     ({13: (1 << 14) + 1}, "requests"), ({14: 0}, "max_rows"), ({15: 0}, "table_width"), ({16: 0}, "num_pages"),
     ({17: 23}, "num_q_heads"), ({19: 80}, "head_dim"), ({20: 24 * 256 - 8}, "q: the row stride"), ({22: 0.0}, "sm_scale"),
-    ({23: 2}, "dtype"),
+    ({23: 2}, "dtype"), ({}, "out must not share"),
 ])
 def test_attend_shared(lib, addr, change, needle):
     size = lib.qwz_batch_shared_workspace_bytes(256, 4, 24)
