@@ -271,9 +271,9 @@ def append_rotated(q, k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, 
     dims at position 1: pairs (i, i + len(inv_freq)), or (2i, 2i + 1) with
     `neighbours`; dims behind them are not rotated.  With `q_weight`,
     `k_weight` (FP32 [dim]) a head is first divided by the root of its mean
-    square (plus eps) and multiplied by the weight.  K is quantised from the
-    rotated values without a rounding in between.  slots (each non-negative one
-    once), k_held and v_held: as in `append`."""
+    square plus eps (taken as FP32) and multiplied by the weight.  K is quantised
+    from the rotated values without a rounding in between.  slots (each
+    non-negative one once), k_held and v_held: as in `append`."""
     dev = _device(q, (k, v, q_out, k_cache, v_cache, k_scales, v_scales, slots, positions, inv_freq, q_weight,
                       k_weight, k_held, v_held))
     P, heads, dim = _pool(k_cache, v_cache, k_scales, v_scales)

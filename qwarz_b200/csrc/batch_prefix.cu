@@ -123,10 +123,10 @@ cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t 
 // groups of heads in a hundred).  Angles are taken in 64 bits: 32 leave 0.06 radians of a position
 // of 10^6.
 //
-// Instructions bound it for long steps (issue slots 60 %, DRAM 41 %).  Measured, GPU times:
+// Instructions bound it for long steps (issue slots 58 %, DRAM 42 %).  Measured, GPU times:
 // 16,384 rows of 24/4/256, a quarter of the dims turned, with norm and held values, 145 us
-// (59 % of the measured copy bandwidth); 5,001 rows of 14/2/64 12.4 us; 448 rows of 32/8/128
-// 8.3 us; 16 rows of 24/4/256 5.0 us, less than the call costs the host.  Forms that were
+// (59 % of the measured copy bandwidth); 5,001 rows of 14/2/64 12.6 us; 448 rows of 32/8/128
+// 8.5 us; 16 rows of 24/4/256 4.9 us, less than the call costs the host.  Forms that were
 // slower on the first: all of K in 64 bits with 8 dims a lane for Q, whose pairs' other dims
 // came by shuffles, 214 us; the same with factors made once a row, 187 us; CTAs of 256
 // threads, two an SM 160 us, three 151 us.
@@ -573,12 +573,16 @@ template <typename T, int D>
 cudaError_t launch_rotate(const BatchRotateParams& p, cudaStream_t stream) {
   constexpr int kQHeads = 512 / D, kHeads = 256 / D;  // a warp load's
   const int rows = (int)p.kv.rows, kv_heads = p.kv.kv_heads;
-  if (rows <= 1024) {  // few rows: short tasks, a row's over several CTAs, each with the row's angles
-    const int tasks = (p.q_heads + kQHeads - 1) / kQHeads + 2 * ((kv_heads + kHeads - 1) / kHeads);
+  const int tasks = (p.q_heads + kQHeads - 1) / kQHeads + 2 * ((kv_heads + kHeads - 1) / kHeads);
+  // Few rows: short tasks, a row's over several CTAs, each with the row's angles.  Against the form for many,
+  // us: 24/4/256 (20 tasks a row) 512 rows 12.5 and 15.6, 1,024 rows 23.4 and 19.4; 32/8/128 (16) 8.3 and 13.1,
+  // 14.8 and 13.9; 14/2/64 (4) 1,024 rows 5.2 and 6.0, 2,048 rows 8.6 and 7.1
+  if (rows <= 1024 && rows * tasks <= 14500) {
     return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)rows, (tasks + 3) / 4), dim3(kRotThreads), 0, stream, p,
                       1, 1);
   }
-  // many: the factors of Q are made once for 12 loads (16,384 rows of 24/4/256: 170 us with 4, 151 with 12)
+  // Many: the factors of Q are made once for 12 loads (2,048 and 16,384 rows of 24/4/256: 26.5 and 147 us with 4,
+  // 24.5 and 137 with 12); 4 rows a CTA (2 rows 30.4 and 147, 8 rows 39 and 140)
   constexpr int kRows = 4;
   return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kRotThreads), 0,
                     stream, p, 12, (kv_heads + kHeads - 1) / kHeads);

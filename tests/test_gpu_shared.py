@@ -177,6 +177,23 @@ def test_rotated_long_steps(heads, kv_heads, dim, freqs, norm, dtype, neighbours
     test_rotated(1101, heads, kv_heads, dim, freqs, neighbours, norm, dtype)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (14, 2, 64)])
+def test_rotated_rows_do_not_depend_on_the_step(heads, kv_heads, dim):
+    """The first rows of a step of 1,400 have the bytes that they have in steps of 725, 700 and 1."""
+    T, P = 1400, 6
+    q, k, v, _ = make_rows(T, heads, kv_heads, dim, torch.bfloat16, 9)
+    slots, positions, inv, w = make_slots(T, P, 9), i32(np.arange(T) * 37), freqs_of(dim // 8), weight_of(dim, 3)
+    got = []
+    for n in (T, 725, 700, 1):
+        pool = [torch.zeros(P * PAGE, kv_heads, x, dtype=torch.uint8, device="cuda").view(P, PAGE, kv_heads, x)
+                for x in (dim // 2, dim // 2, dim // 16, dim // 16)]
+        out = torch.empty(n, heads, dim, dtype=torch.bfloat16, device="cuda")
+        batch.append_rotated(q[:n], k[:n], v[:n], out, *pool, slots[:n], positions[:n], inv, False, w, w)
+        got.append([out] + [x.flatten(0, 1)[slots[:n].long()] for x in pool])
+    for other in got[1:]:
+        assert all(torch.equal(a[:len(b)], b) for a, b in zip(got[0], other))
+
+
 @pytest.mark.parametrize("neighbours", [False, True])
 def test_rotated_in_place(neighbours):
     """q rotated in the packed rows it lies in; K and V beside it stay as they were."""
