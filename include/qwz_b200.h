@@ -500,8 +500,9 @@ int qwz_batch_share_prefixes(const int32_t* prefix_of, const int32_t* kv_lens, c
  * prefix g that its request reads, and of its own those that it sees there.  A
  * prefix's tokens are read once for the rows of all its requests.  plan: as
  * qwz_batch_share_prefixes wrote it for this step; entries outside the step's
- * requests and rows set QWZ_DEVERR_TABLE_RANGE and are skipped.  out shares no
- * storage with q.  workspace: qwz_batch_shared_workspace_bytes (0: bad sizes),
+ * requests and rows set QWZ_DEVERR_TABLE_RANGE and are skipped, and a row that it
+ * does not list behind its request's prefix sees its own tokens alone and sets the
+ * same bit (rows listed twice are undefined).  out shares no storage with q.  workspace: qwz_batch_shared_workspace_bytes (0: bad sizes),
  * 16-byte aligned, for one call at a time.
  */
 int64_t qwz_batch_shared_workspace_bytes(int32_t head_dim, int32_t rows, int32_t num_q_heads);

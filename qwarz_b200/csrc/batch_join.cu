@@ -5,7 +5,10 @@
 //   out = sum_i w_i o_i / sum_i w_i l_i,  w_i = 2^(m_i - max m)
 //
 // over the parts (m_i, l_i, o_i) in a fixed order: the prefix's by CTA, then the own
-// tokens' by CTA.  A warp has one (row, head), or G warps take every G-th part of
+// tokens' by CTA.  A row that the plan does not list behind its prefix has no part there in
+// this call, and what the workspace holds is an earlier call's: the part counts only where
+// the place it was made for lies in the prefix's range and names the row.
+// A warp has one (row, head), or G warps take every G-th part of
 // it (below 4,096 (row, head) pairs, whose items have many parts).  It reads D + 2 floats a
 // part, mostly from L2; the chain of loads from the row's request over `where` and the
 // statistics to the outputs bounds it.
@@ -76,9 +79,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const int s = out_row - r.row0;
     bool work = at + warp / G < pairs && b >= 0 && s < r.n;
     bool joins = false;
+    batch::Req of_prefix = {0, 0, 0};
     if (work) {
       const int g = batch::prefix_of(p, b);
-      joins = g >= 0 && __ldcg(p.direct + g) == 0;
+      if (g >= 0) {
+        joins = __ldcg(p.direct + g) == 0;
+        if (joins) of_prefix = batch::load_prefix(p, g);
+        // many rows whose prefix was left to their request: the plan lists fewer
+        if (!joins && r.n * p.group > p.few_cols) flag_error(kErrTableRange);
+      }
     }
     JoinSide side[2];  // 0: the prefix, 1: own tokens
 #pragma unroll
@@ -88,6 +97,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
       const size_t part = (size_t)k * p.rows * q_heads + rh;
       const uint32_t w = __ldcg(p.where + part), what = w & 3u;
       const int first = (w >> 2) & 1023, parts = (int)((w >> 12) & 1023) + 1, row = (w >> 22) & 255;
+      if (k == 0) {
+        const long long place = what == kWhereWhole ? w >> 2 : __float_as_uint(__ldcg(p.part_ml + 2 * part));
+        const bool there = what != kWhereDone && what != kWhereFew && place >= of_prefix.row0 &&
+                           place < (long long)of_prefix.row0 + of_prefix.n && __ldg(p.shared_rows + place) == out_row;
+        if (!there) {
+          flag_error(kErrTableRange);
+          continue;
+        }
+      }
       if (what == kWhereDone) {  // out has it
         work = work && k == 0;
       } else if (what == kWhereWhole) {

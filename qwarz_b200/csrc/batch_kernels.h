@@ -50,7 +50,9 @@ constexpr int kShareMaxRequests = 1 << 14;
 // into out (kBatchPlain), or the parts that batch_join.cu merges (kBatchShared).
 enum BatchMode : int { kBatchPlain = 0, kBatchShared = 1 };
 // Where a part is: bits 0-1 what, 2-11 first CTA (split) of its records, 12-21 their
-// number less one, 22-29 its row in them.
+// number less one, 22-29 its row in them.  A whole part of a prefix has the row's place in
+// shared_rows from bit 2 on (2^30 rows have workspaces of 575 GB), one in records has it for
+// its reference maximum.
 enum BatchWhere : uint32_t { kWhereDone = 0, kWhereWhole = 1, kWhereFew = 2, kWhereRows = 3 };
 constexpr int kBatchMeta = 8;    // int32 words per CTA
 constexpr int kBatchMaxSms = 256;

@@ -1007,8 +1007,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
       const uint32_t stage = sb + R::kStage + warp * 32 * R::kPitch;
       // (kind, row, head) of the row's part
       const size_t part = ((size_t)(pre ? 0 : p.rows) + max(row, 0)) * (p.kv_heads * p.group) + head * p.group + rhead;
-      if (starts_here && grp == 0 && row >= 0)
-        p.where[part] = !whole ? batch::where_word(kWhereRows, cluster, it.parts, rr) : joins ? kWhereWhole : kWhereDone;
+      if (starts_here && grp == 0 && row >= 0) {
+        // (of a prefix with the row's place in shared_rows, by which batch_join.cu knows this call's parts)
+        const uint32_t place = pre ? (uint32_t)at_row : 0u;
+        p.where[part] = !whole ? batch::where_word(kWhereRows, cluster, it.parts, rr)
+                        : joins ? (uint32_t)kWhereWhole | place << 2
+                                : (uint32_t)kWhereDone;
+        if (pre && !whole) p.part_ml[2 * part] = __uint_as_float(place);
+      }
       if (whole && !joins) {
         T* out = reinterpret_cast<T*>(p.out) + (long long)max(row, 0) * p.out_stride + (head * p.group + rhead) * D;
         tl_store_rows<T, D, true>(stage, to, grp * (D / 2), row >= 0 ? out : nullptr, l > 0.f ? 1.f / l : 0.f);

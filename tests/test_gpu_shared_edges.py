@@ -1,0 +1,96 @@
+"""The operators for requests that share prefixes (qwarz_b200.batch) at their edges: plans
+that do not fit, denied prefixes, weights, the ends of the types' ranges, long steps."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import batch as obatch
+from qwarz_b200 import _lib, batch
+from tests import test_gpu_shared as shared
+from tests.test_gpu_batch import check, i32, make_pool, make_tables
+from tests.test_gpu_shared import freqs_of, make_plan, make_rows, make_slots, run_shared, weight_of
+
+pytestmark = pytest.mark.gpu
+PAGE = 256
+
+
+@pytest.fixture(autouse=True)
+def clean_errors(cuda):
+    _lib.device_error(clear=True)
+    yield
+    assert _lib.device_error(clear=True) == 0  # a test that expects a bit clears it itself
+
+
+# ------------------------------------------------------- plans that do not fit
+def bent_step(seed, many):
+    """A step with a wide request (so that no prefix is read directly): one prefix whose item is
+    shared by many CTAs, or forty whose items lie within one."""
+    if many:
+        prefix, rows, kv = [-1] * 40, [0] * 40, [600] * 40
+        for g in range(40):
+            prefix += [g, g]
+            rows += [10, 1 + g % 3]
+            kv += [200 + g, 40 + 9 * g]
+        layout = (8, 8, 64)
+    else:
+        prefix, rows, kv, layout = [-1, 0, 0, 0, -1], [0, 10, 1, 1, 2], [600, 300, 40, 300, 50], (24, 4, 256)
+    heads, kv_heads, dim = layout
+    pages = sum(-(-n // PAGE) for n in kv)
+    pool, table = make_pool(pages, kv_heads, dim, seed), make_tables(kv, 3, pages, seed)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    return prefix, rows, kv, layout, pool, table, cu, make_plan(prefix, kv, cu, int(cu[-1]))
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("how", ["outside", "emptied", "later", "range"])
+def test_rows_the_plan_does_not_list(how, many):
+    """Rows behind a prefix that the plan does not list (entries outside the step's rows, an
+    emptied range, one that begins a row late, one that is none) see their own tokens alone and
+    set an error bit, whatever an earlier call left in the workspace; the others are as ever."""
+    prefix, rows, kv, (heads, kv_heads, dim), pool, table, cu, plan = bent_step(3, many)
+    R, T = len(kv), int(cu[-1])
+    ws = batch.shared_workspace("cuda", dim, T, heads)
+    ws.fill_(0xFF)
+    q = [torch.randn(T, heads, dim, generator=torch.Generator(device="cuda").manual_seed(s), device="cuda").half() for s in (1, 2)]
+    args = (*pool, table, i32(cu), i32(kv))
+    batch.attend_shared(q[0], *args, plan, torch.empty_like(q[0]), ws, max_rows=10)
+    bent, listed = plan.clone(), plan[3 * R + 1:]
+    if how == "outside":
+        at = torch.tensor([0, 3, 10])
+        bent[3 * R + 1 + at] = i32([T, -1, 1 << 30])
+        gone = listed[at.cuda()]
+    elif how == "emptied":
+        bent[:R + 1] = 0
+        gone = listed[listed >= 0]
+    else:
+        bent[0] = 1 if how == "later" else -5
+        gone = listed[:1 if how == "later" else int(plan[1])]
+    missing = torch.zeros(T, dtype=torch.bool, device="cuda")
+    missing[gone.long()] = True
+    room = torch.full((T + 6, heads, dim), 7.0, dtype=torch.float16, device="cuda")
+    out = room[3:-3]
+    batch.attend_shared(q[1], *args, bent, out, ws, max_rows=10)
+    assert _lib.device_error(clear=True) == 1
+    both, mag = obatch.attend_shared(q[1], *args, prefix, out, dim ** -0.5)
+    alone, mag_alone = obatch.attend_shared(q[1], *args, [-1] * R, out, dim ** -0.5)
+    some = missing[:, None, None]
+    check(out, torch.where(some, alone, both), torch.where(some, mag_alone, mag), torch.float16)
+    assert bool((room[:3] == 7).all()) and bool((room[-3:] == 7).all())
+
+
+def test_a_wide_reader_of_an_emptied_prefix():
+    """The only reader has too many rows to read its prefix by itself, and the plan lists none."""
+    heads, kv_heads, dim, kv = 24, 4, 256, [600, 300]
+    pool, table, cu = make_pool(5, kv_heads, dim, 1), i32([[0, 1, 2], [3, 4, -1]]), np.array([0, 0, 10])
+    plan = make_plan([-1, 0], kv, cu, 10)
+    q = torch.randn(10, heads, dim, device="cuda").half()
+    out, ws = torch.empty_like(q), batch.shared_workspace("cuda", dim, 10, heads)
+    args = (q, *pool, table, i32(cu), i32(kv))
+    batch.attend_shared(*args, plan, out, ws, max_rows=10)
+    plan[:3] = 0
+    batch.attend_shared(*args, plan, out, ws, max_rows=10)
+    assert _lib.device_error(clear=True) == 1
+    want, mag = obatch.attend_shared(*args, [-1, -1], out, dim ** -0.5)
+    check(out, want, mag, torch.float16)
