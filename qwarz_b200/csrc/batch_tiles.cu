@@ -375,6 +375,16 @@ QWZ_DEVINL void tl_few_starts(const BatchAttnParams& p, bool small, long long* s
   }
 }
 
+// a and b plus the two weights of w.  The sums take the rounded weights, as in
+// batch_few.cu: a row's weights add up to one, and the rounding of a dominant weight
+// cancels.  (FP16 and FP32 in one addition; a conversion and an addition in pairs behind the
+// chunk's vote: 24 windows of 7 rows 233 us, 216 so; of the unrounded weights 212.)
+QWZ_DEVINL void tl_add_pair(float& a, float& b, uint32_t w) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.f32.f16 %0, l, %0;\n add.f32.f16 %1, h, %1;\n}\n"
+      : "+f"(a), "+f"(b)
+      : "r"(w));
+}
+
 template <int REGS>
 QWZ_DEVINL void tl_more_regs() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(REGS));
@@ -426,8 +436,9 @@ QWZ_DEVINL void tl_store_rows(uint32_t stage, uint32_t taddr, int first, void* d
 }
 
 // The warp's first n chunks (of 32 columns) of P times the row's factor, a power of two
-// (references are whole numbers), so that weights keep their bits; in two steps, since
-// FP16 has no powers below 2^-24.
+// (references are whole numbers), in two steps, since FP16 has no powers below 2^-24.  Weights
+// that stay above 2^-14 keep their bits; below it they lose up to 2^-25, of a largest weight
+// of 2^6 at least (the row's sum keeps them: 2^-31 of it a weight).
 __noinline__ __device__ void tl_scale_p(uint32_t tp, int n, float factor) {
   tc::wait_st();
   const float first = fmaxf(factor, 6.103515625e-5f), second = factor / first;  // 2^-14 at least, the rest
@@ -902,8 +913,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
               pf_ffma2(p0, p1, x[2 * e], x[2 * e + 1], fac, -mu);
               p0 = exp2_approx(p0);
               p1 = exp2_approx(p1);
-              pf_fadd2(sa, sb2, p0, p1);
               pw[e] = pack_half2(p0, p1);
+              tl_add_pair(sa, sb2, pw[e]);
               asm("max.u16x2 %0, %0, %1;\n" : "+r"(top) : "r"(pw[e]));
             }
             // FP16 2^15; infinities and NaN are above it

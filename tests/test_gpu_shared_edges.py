@@ -94,3 +94,26 @@ def test_a_wide_reader_of_an_emptied_prefix():
     assert _lib.device_error(clear=True) == 1
     want, mag = obatch.attend_shared(*args, [-1, -1], out, dim ** -0.5)
     check(out, want, mag, torch.float16)
+
+
+# --------------------------------------------------------------------- weights
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (32, 8, 128), (14, 2, 64)])
+@pytest.mark.parametrize("rows", [[0, 1, 1, 40], [0, 1, 1, 1], [0, 130, 7, 9]])
+def test_weights_add_up_to_one(heads, kv_heads, dim, rows):
+    """Where every V is 1 the output is exactly 1, with some keys that draw most of the weight.
+
+    The sum of the weights takes what is multiplied with V, so both are FP32 sums of the same
+    numbers: at most 3,000 additions of 2^-24 each on either side, and 2^-25 a weight against a
+    largest one of 2^6 where earlier weights were scaled down, 3,000 x (2^-23 + 2^-31) at the very
+    worst and, over chains of at most 750 weights, below 2^-12, half of FP16's step below 1."""
+    kv = [2000, 300, 7, 700]
+    pool = make_pool(14, kv_heads, dim, 3)
+    pool[1].fill_(0x22)
+    pool[3].view(torch.uint8).fill_(0x38)
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    T, prefix = int(cu[-1]), [-1, 0, 0, 0]
+    q = 2 * torch.randn(T, heads, dim, generator=torch.Generator(device="cuda").manual_seed(dim), device="cuda").half()
+    out = torch.empty_like(q)
+    batch.attend_shared(q, *pool, make_tables(kv, 8, 14, 3), i32(cu), i32(kv), make_plan(prefix, kv, cu, T), out,
+                        batch.shared_workspace("cuda", dim, T, heads), max_rows=max(rows))
+    assert bool((out == 1).all()), f"{float((out != 1).float().mean()):.2%}, {float(out.min())} to {float(out.max())}"
