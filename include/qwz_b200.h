@@ -488,8 +488,12 @@ int qwz_batch_attend(const void* q, const void* k_cache, const void* v_cache, co
  * positions_out [rows]: positions plus the tokens of the row's prefix (may be
  * positions itself; no other output may share storage with an input).  A prefix
  * that does not exist, is the request itself or has a prefix of its own sets
- * QWZ_DEVERR_TABLE_RANGE and counts as none; so do, with their request's rows,
- * row offsets outside [0, rows].  R is at most 2^14.
+ * QWZ_DEVERR_TABLE_RANGE and counts as none; so does one that has rows in the step
+ * and no tokens after it (they were denied): what its readers' rows give in that
+ * step is void (reads -1 where prefix_of is not), and their rows are run again with
+ * the prefix's.  A prefix that ends in a step has no tokens in it: it ends after its
+ * last reader's step.  Row offsets outside [0, rows] count as no rows, with the
+ * same bit.  R is at most 2^14.
  */
 int qwz_batch_share_prefixes(const int32_t* prefix_of, const int32_t* kv_lens, const int32_t* cu_rows,
                              const int32_t* positions, const int32_t* request_of, int32_t* plan, int32_t* positions_out,

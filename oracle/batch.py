@@ -106,7 +106,7 @@ def share_prefixes(prefix_of, kv_lens, cu_rows, positions, request_of):
     R, T = len(kv_lens), len(positions)
     bad, reads, alone = False, [], []
     for b, g in enumerate(prefix_of):
-        fits = 0 <= g < R and g != b and prefix_of[g] < 0
+        fits = 0 <= g < R and g != b and prefix_of[g] < 0 and (kv_lens[g] > 0 or cu_rows[g + 1] <= cu_rows[g])
         bad |= g >= 0 and not fits
         reads.append(g if fits else -1)
     ranges = []

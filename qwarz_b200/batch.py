@@ -228,8 +228,10 @@ def share_prefixes(prefix_of, kv_lens, cu_rows, positions, request_of, plan, pos
     are its outputs; `plan` (`prefix_plan`) receives the rows by prefix and
     `positions_out` [T] the positions from the prefix's start (may be
     `positions`).  A prefix that does not exist, is the request itself or has one
-    itself counts as none (device error word).  All tensors int32, at most 2^14
-    requests; the plan's layout is in include/qwz_b200.h."""
+    itself counts as none (device error word).  So does one whose rows of this
+    step were denied: drop its readers' rows with its own and run them again.  A
+    prefix is ended after the last step that reads it.  All tensors int32, at most
+    2^14 requests; the plan's layout is in include/qwz_b200.h."""
     dev = _device(prefix_of, (kv_lens, cu_rows, positions, request_of, plan, positions_out))
     _int32(("prefix_of", "kv_lens", "cu_rows", "positions", "request_of", "plan", "positions_out"),
            (prefix_of, kv_lens, cu_rows, positions, request_of, plan, positions_out))

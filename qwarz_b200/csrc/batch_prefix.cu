@@ -20,11 +20,14 @@ constexpr int kShReq = 32;              // requests of a CTA, a warp each
 constexpr int kShThreads = kShReq * 32;
 constexpr int kShTile = 4096;           // requests in shared memory at a time
 
-// The prefix that request b reads: one that exists, is another and has none itself.
+// The prefix that request b reads: one that exists, is another and has none itself, and
+// whose rows, if it has any in this step, were not denied (they would be its tokens).
 QWZ_DEVINL int share_prefix(const BatchShareParams& p, int b) {
   const int g = __ldg(p.prefix_of + b);
   if (g < 0) return -1;
-  if (g < p.requests && g != b && __ldg(p.prefix_of + g) < 0) return g;
+  if (g < p.requests && g != b && __ldg(p.prefix_of + g) < 0 &&
+      (__ldg(p.kv_lens + g) > 0 || __ldg(p.cu_rows + g + 1) <= __ldg(p.cu_rows + g)))
+    return g;
   flag_error(kErrTableRange);
   return -1;
 }

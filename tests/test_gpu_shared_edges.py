@@ -117,3 +117,29 @@ def test_weights_add_up_to_one(heads, kv_heads, dim, rows):
     batch.attend_shared(q, *pool, make_tables(kv, 8, 14, 3), i32(cu), i32(kv), make_plan(prefix, kv, cu, T), out,
                         batch.shared_workspace("cuda", dim, T, heads), max_rows=max(rows))
     assert bool((out == 1).all()), f"{float((out != 1).float().mean()):.2%}, {float(out.min())} to {float(out.max())}"
+
+
+# ------------------------------------------------------ prefixes without tokens
+def test_a_denied_prefix():
+    """A prefix whose rows get no page has no tokens in the step: its readers, which have pages
+    and are granted, would have wrong positions.  It counts as none and sets a bit."""
+    R, T, W = 4, 13, 4
+    e = lambda *s: torch.full(s, -7, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = i32([[0, -1, -1, -1], [1, -1, -1, -1], [2, 3, -1, -1], [4, -1, -1, -1]])
+    cu, kv, held, state, slots, pos, req, far = e(R + 1), e(R), e(R), e(2), e(T), e(T), e(T), e(T)
+    batch.build_tables(i32([250, 9, 300, 30]), i32([10, 1, 0, 2]), i32([1, 1, 2, 1]), i32([-1] * 8), i32([0, 0]), table, cu, kv,
+                       held, state, slots, pos, req)
+    assert kv.tolist() == [0, 10, 300, 32] and _lib.device_error(clear=True) == 16
+    plan = batch.prefix_plan("cuda", R, T)
+    batch.share_prefixes(i32([-1, 0, -1, 2]), kv, cu, pos, req, plan, far)
+    assert _lib.device_error(clear=True) == 1
+    want, why = obatch.share_prefixes([-1, 0, -1, 2], kv.tolist(), cu.tolist(), pos.tolist(), req.tolist())
+    assert why and plan.tolist() == sum(want[:4], []) and far.tolist() == want[4]
+    assert want[1] == [-1, -1, -1, 2] and far[10:].tolist() == [9, 330, 331]
+
+
+def test_an_empty_prefix_is_no_error():
+    """One without rows and tokens is a prefix all the same."""
+    plan, far = batch.prefix_plan("cuda", 2, 1), i32([-7])
+    batch.share_prefixes(i32([-1, 0]), i32([0, 6]), i32([0, 0, 1]), i32([5]), i32([1]), plan, far)
+    assert plan.tolist() == [0, 1, 1, -1, 0, 1, -1, 0] and far.tolist() == [5]
