@@ -47,9 +47,9 @@ __global__ void __launch_bounds__(kShThreads) batch_share_kernel(const __grid_co
   griddep_wait();
   const int tid = threadIdx.x, lane = tid & 31;
   const int b = blockIdx.x * kShReq + (tid >> 5);
-  const int step = gridDim.x * kShThreads, first = blockIdx.x * kShThreads + tid;
   // positions from the prefix's start (their loads are on their way during the rest)
-  for (int t = first; t < p.rows; t += step) {
+  // (64 bits: a step more than the last row may pass 32)
+  for (long long t = blockIdx.x * kShThreads + tid; t < p.rows; t += gridDim.x * kShThreads) {
     const int r = __ldg(p.request_of + t);
     int pos = p.positions[t];
     if (r >= 0 && r < p.requests) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kShThreads) batch_share_kernel(const __grid_co
     if (key >= 0) {
       int lo;
       const int n = share_rows(p, b, lo);
-      for (int i = lane; i < n && (unsigned)(before + i) < (unsigned)p.rows; i += 32) p.shared_rows[before + i] = lo + i;
+      for (long long i = lane; i < n && before + i >= 0 && before + i < p.rows; i += 32) p.shared_rows[before + i] = (int)(lo + i);
     }
   }
   // the places behind the last row
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kShThreads) batch_share_kernel(const __grid_co
 
 cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t stream) {
   const int by_request = (p.requests + kShReq - 1) / kShReq;
-  const int by_row = min((p.rows + kShThreads - 1) / kShThreads, sms);
+  const int by_row = (int)min((p.rows + kShThreads - 1LL) / kShThreads, (long long)sms);
   return launch_pdl(batch_share_kernel, dim3(max(max(by_request, by_row), 1)), dim3(kShThreads), 0, stream, p);
 }
 

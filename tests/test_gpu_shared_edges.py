@@ -143,3 +143,18 @@ def test_an_empty_prefix_is_no_error():
     plan, far = batch.prefix_plan("cuda", 2, 1), i32([-7])
     batch.share_prefixes(i32([-1, 0]), i32([0, 6]), i32([0, 0, 1]), i32([5]), i32([1]), plan, far)
     assert plan.tolist() == [0, 1, 1, -1, 0, 1, -1, 0] and far.tolist() == [5]
+
+
+# ------------------------------------------------------------------ most rows
+def test_share_most_rows():
+    """Arrays of 2^31 - 9 rows: the positions of the last ones are written, and nothing else is read."""
+    T = (1 << 31) - 9
+    req = torch.full((T,), -1, dtype=torch.int32, device="cuda")
+    pos = torch.full((T,), 5, dtype=torch.int32, device="cuda")
+    req[:6], req[-3:] = 1, 1
+    plan = batch.prefix_plan("cuda", 2, T)
+    plan.fill_(-7)
+    batch.share_prefixes(i32([-1, 0]), i32([40, 6]), i32([0, 0, 6]), pos, req, plan, pos)
+    assert plan[:14].tolist() == [0, 6, 6, -1, 0, 1, -1, 0, 1, 2, 3, 4, 5, -1] and plan[-2:].tolist() == [-1, -1]
+    assert pos[:7].tolist() == [45] * 6 + [5] and pos[-4:].tolist() == [5, 45, 45, 45]
+    assert int((plan[13:] != -1).sum()) == 0 and int((pos != 5).sum()) == 9
