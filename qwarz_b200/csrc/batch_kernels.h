@@ -131,6 +131,7 @@ struct BatchShareParams {
   int requests, rows;
 };
 
+constexpr int kRotMaxHeads = 64 * 256;  // of Q
 // Q and K normed and rotated, K and V quantised into their slots (batch_prefix.cu).
 struct BatchRotateParams {
   BatchAppendParams kv;          // k before the norm and the rotation

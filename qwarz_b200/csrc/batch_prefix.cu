@@ -226,6 +226,9 @@ QWZ_DEVINL void fma_pair(float& d0, float& d1, float x0, float x1, float a0, flo
       : "=f"(d0), "=f"(d1)
       : "f"(x0), "f"(x1), "f"(a0), "f"(a1), "f"(c0), "f"(c1));
 }
+// Whether squares of T's numbers need more than 32 bits' range.
+template <typename T>
+constexpr bool kWide = !std::is_same<T, __half>::value;
 QWZ_DEVINL float rsqrt_of(float x) { return rsqrtf(x); }
 QWZ_DEVINL double rsqrt_of(double x) { return rsqrt(x); }
 QWZ_DEVINL float shfl_xor_any(float x, int o) { return __shfl_xor_sync(0xffffffffu, x, o); }
@@ -238,16 +241,16 @@ QWZ_DEVINL double shfl_xor_any(double x, int o) { return __shfl_xor_sync(0xfffff
 struct TurnQ {
   float a[2][8], b[2][8];
   int chunk[2];
-  bool turns[2];
+  bool turns;  // (both chunks or neither: freqs is a multiple of 8)
 
   QWZ_DEVINL void set(int l, const float* weight, int freqs, bool neighbours, const float2* cos_sin) {
     const int half = freqs / 8;
     const bool both = !neighbours && l < half;
     chunk[0] = both ? l : 2 * l;
     chunk[1] = both ? l + half : 2 * l + 1;
+    turns = neighbours ? l < freqs / 8 : both;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      turns[k] = neighbours ? chunk[k] < freqs / 4 : both;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         a[k][i] = weight != nullptr ? __ldg(weight + 8 * chunk[k] + i) : 1.f;
@@ -265,25 +268,24 @@ struct TurnQ {
         b[1][i] = t.y * w0;
       }
     }
-    if (neighbours) {
+    if (neighbours && turns) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (turns[k]) {
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float2 t = cos_sin[4 * chunk[k] + i / 2];
-            const float w0 = a[k][i], w1 = a[k][i + 1];
-            a[k][i] = t.x * w0;
-            a[k][i + 1] = t.x * w1;
-            b[k][i] = -t.y * w1;
-            b[k][i + 1] = t.y * w0;
-          }
+        for (int i = 0; i < 8; i += 2) {
+          const float2 t = cos_sin[4 * chunk[k] + i / 2];
+          const float w0 = a[k][i], w1 = a[k][i + 1];
+          a[k][i] = t.x * w0;
+          a[k][i + 1] = t.x * w1;
+          b[k][i] = -t.y * w1;
+          b[k][i + 1] = t.y * w0;
         }
     }
   }
 
+  // False where 32 bits do not hold the head's squares (q_from_64; never in FP16).
   template <typename T, int LANES, bool NEIGHBOURS>
-  QWZ_DEVINL void apply(uint4 (&raw)[2], bool norm, float eps) const {
+  QWZ_DEVINL bool apply(uint4 (&raw)[2], bool norm, float eps) const {
     float x[2][8], y[2][8];
     to_floats<T>(raw[0], x[0]);
     to_floats<T>(raw[1], x[1]);
@@ -291,7 +293,7 @@ struct TurnQ {
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        if (turns[k]) {
+        if (turns) {
           const float p0 = NEIGHBOURS ? x[k][i + 1] : x[1 - k][i], p1 = NEIGHBOURS ? x[k][i] : x[1 - k][i + 1];
           fma_pair(y[k][i], y[k][i + 1], p0, p1, b[k][i], b[k][i + 1], 0.f, 0.f);
           fma_pair(y[k][i], y[k][i + 1], x[k][i], x[k][i + 1], a[k][i], a[k][i + 1], y[k][i], y[k][i + 1]);
@@ -316,11 +318,56 @@ struct TurnQ {
     for (int k = 0; k < 2; ++k) {
       T h[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = InTraits<T>::from_float(norm ? y[k][i] * r : y[k][i]);
+      for (int i = 0; i < 8; ++i) h[i] = InTraits<T>::from_float(y[k][i] * r);
       raw[k] = *reinterpret_cast<const uint4*>(h);
     }
+    return !kWide<T> || (r > 1e-15f && r < 1e15f);
   }
 };
+
+// One Q head (where `mine`) of a row from 64 bits, rounded once.
+template <typename T, int D>
+__device__ __noinline__ void q_from_64(const BatchRotateParams& p, long long row, int head, bool mine, const double2* cos_sin) {
+  constexpr int kLanes = D / 16;
+  const int l = threadIdx.x % kLanes, half = p.freqs / 8;
+  const bool neighbours = p.neighbours != 0, both = !neighbours && l < half;
+  const int c[2] = {both ? l : 2 * l, both ? l + half : 2 * l + 1};
+  double x[2][8], sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (mine) raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + row * p.q_stride + head * D + 8 * c[k]);
+    to_floats<T>(raw, x[k]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += x[k][i] * x[k][i];
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) sum += shfl_xor_any(sum, o);
+  const double r = rsqrt_of(sum / D + (double)p.eps);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[k][i] = x[k][i] * r * __ldg(p.q_weight + 8 * c[k] + i);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    T h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      double y = x[k][i];
+      if (both) {
+        const double2 t = cos_sin[8 * l + i];
+        y = y * t.x + x[1 - k][i] * (k == 0 ? -t.y : t.y);
+      } else if (neighbours && c[k] < p.freqs / 4) {
+        const double2 t = cos_sin[4 * c[k] + i / 2];
+        y = y * t.x + x[k][i ^ 1] * (i % 2 == 0 ? -t.y : t.y);
+      }
+      h[i] = InTraits<T>::from_float(float_odd(y));
+    }
+    if (mine)
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.q_out) + row * p.q_out_stride + head * D + 8 * c[k]) =
+          *reinterpret_cast<const uint4*>(h);
+  }
+}
 
 // The eight dims `c` of a K head in F's precision, D / 8 lanes a head (all lanes of the
 // warp take part).
@@ -470,6 +517,9 @@ __global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __gr
   constexpr int kLoads = 2;                                // warp loads of Q that are under way together
   __shared__ double2 table[ROWS][128];                     // (cos, sin) of a row's angles
   __shared__ float2 narrow[ROWS][128];
+  constexpr int kWords = kRotMaxHeads / 32;
+  __shared__ uint32_t late[kWide<T> ? ROWS * kWords : 1];  // a bit a Q head that q_from_64 does at the end
+  __shared__ int some_late;
   griddep_wait();
   const BatchAppendParams& a = p.kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -489,6 +539,9 @@ __global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __gr
     table[r][f] = make_double2(co, s);
     narrow[r][f] = make_float2((float)co, (float)s);
   }
+  if (tid == 0) some_late = 0;
+  if constexpr (kWide<T>)  // (the words of heads that there are)
+    for (int i = tid; i < ROWS * ((p.q_heads + 31) / 32); i += kRotThreads) late[i % ROWS * kWords + i / ROWS] = 0u;
   __syncthreads();
   const int q_tasks = (p.q_heads + q_units * kQHeads - 1) / (q_units * kQHeads);
   const int kv_tasks = (a.kv_heads + kv_units * kHeads - 1) / (kv_units * kHeads), per_row = q_tasks + 2 * kv_tasks;
@@ -505,6 +558,7 @@ __global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __gr
 #pragma unroll 1
       for (int h0 = first; h0 < end; h0 += kLoads * kQHeads) {
         uint4 raw[kLoads][2];
+        bool fine[kLoads];
 #pragma unroll
         for (int u = 0; u < kLoads; ++u)
 #pragma unroll
@@ -515,13 +569,24 @@ __global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __gr
           }
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-          if (neighbours) turn.template apply<T, kQLanes, true>(raw[u], p.q_weight != nullptr, p.eps);
-          else turn.template apply<T, kQLanes, false>(raw[u], p.q_weight != nullptr, p.eps);
+          fine[u] = neighbours ? turn.template apply<T, kQLanes, true>(raw[u], p.q_weight != nullptr, p.eps)
+                               : turn.template apply<T, kQLanes, false>(raw[u], p.q_weight != nullptr, p.eps);
           const int head = h0 + u * kQHeads + sub;
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            if (head < end) *reinterpret_cast<uint4*>(dst + head * D + 8 * turn.chunk[k]) = raw[u][k];
+            if (fine[u] && head < end) *reinterpret_cast<uint4*>(dst + head * D + 8 * turn.chunk[k]) = raw[u][k];
         }
+        if constexpr (kWide<T>)
+          if (!(fine[0] && fine[1])) {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+              const int head = h0 + u * kQHeads + sub;
+              if (!fine[u] && head < end) {
+                atomicOr(late + r * kWords + head / 32, 1u << head % 32);
+                some_late = 1;
+              }
+            }
+          }
       }
       continue;
     }
@@ -565,6 +630,19 @@ __global__ void __launch_bounds__(kRotThreads, 5) batch_rotate_kernel(const __gr
       void* held = is_k ? a.k_held : a.v_held;
       if (held != nullptr)
         *reinterpret_cast<uint4*>(reinterpret_cast<T*>(held) + (row * a.kv_heads + head) * D + 8 * c) = held8<T>(code, sbits);
+    }
+  }
+  if constexpr (kWide<T>) {
+    // (Here, where no task holds registers: in the loop, inlined or called, the path made them
+    // spill, 156 to 162 us for 16,384 rows of 24/4/256 against 149 so and 144 without it.)
+    __syncthreads();
+    if (some_late == 0) return;
+    const int steps = (p.q_heads + kQHeads - 1) / kQHeads;
+#pragma unroll 1
+    for (int i = warp; i < rows * steps; i += kRotThreads / 32) {
+      const int r = i / steps, head = i % steps * kQHeads + lane / kQLanes;
+      const bool mine = head < p.q_heads && (late[r * kWords + head / 32] >> head % 32 & 1u) != 0u;
+      if (__any_sync(0xffffffffu, mine)) q_from_64<T, D>(p, row0 + r, head, mine, table[r]);
     }
   }
   griddep_launch_dependents();

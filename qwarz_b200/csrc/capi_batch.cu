@@ -251,7 +251,7 @@ int qwz_batch_append_rotated(const void* q, const void* k, const void* v, void* 
   int rc = append_checked(p.kv, k, v, k_cache, v_cache, k_scales, v_scales, slots, k_held, v_held, rows, k_stride,
                           v_stride, num_kv_heads, head_dim, num_pages, dtype);
   if (rc) return rc;
-  if (num_q_heads < 1 || num_q_heads > 64 * 256) return fail(QWZ_EINVAL, "num_q_heads must be in 1..16384");
+  if (num_q_heads < 1 || num_q_heads > qwz::kRotMaxHeads) return fail(QWZ_EINVAL, "num_q_heads must be in 1..16384");
   if (num_freqs < 0 || num_freqs % 8 != 0 || 2 * num_freqs > head_dim)
     return fail(QWZ_EINVAL, "num_freqs must be a multiple of 8, at most head_dim / 2");
   if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(QWZ_EINVAL, "eps must be finite and >= 0");

@@ -158,3 +158,35 @@ def test_share_most_rows():
     assert plan[:14].tolist() == [0, 6, 6, -1, 0, 1, -1, 0, 1, 2, 3, 4, 5, -1] and plan[-2:].tolist() == [-1, -1]
     assert pos[:7].tolist() == [45] * 6 + [5] and pos[-4:].tolist() == [5, 45, 45, 45]
     assert int((plan[13:] != -1).sum()) == 0 and int((pos != 5).sum()) == 9
+
+
+# ------------------------------------------------------------- Q's whole range
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+@pytest.mark.parametrize("heads,dim,freqs", [(24, 256, 32), (5, 128, 64), (3, 64, 16), (70, 64, 24)])
+@pytest.mark.parametrize("rows", [1, 250])
+def test_rotated_smallest_and_largest_q(rows, heads, dim, freqs, eps, neighbours):
+    """Q heads whose squares 32 bits do not hold are normed as any other: 18 x 2^-24 of the two
+    terms (see `close`), the output's half step of 2^-8, and its half step below 2^-126."""
+    scales = [1.0, 2.0 ** -90, 2.0 ** -60, 2.0 ** -20, 2.0 ** 30, 2.0 ** 63, 2.0 ** 80, 2.0 ** 120, 2.0 ** -126]
+    T = len(scales) * rows
+    q, k, v, _ = make_rows(T, heads, 1, dim, torch.bfloat16, 8)
+    q.mul_(torch.tensor(scales * rows, device="cuda").bfloat16()[:, None, None])
+    q[2, 1] = 0.0
+    P = T // PAGE + 1
+    pool = [torch.zeros(P, PAGE, 1, w, dtype=torch.uint8, device="cuda") for w in (dim // 2, dim // 2, dim // 16, dim // 16)]
+    out = torch.empty_like(q.contiguous())
+    w, positions, inv = weight_of(dim, 3), i32(range(5, 5 + T)), freqs_of(freqs)
+    batch.append_rotated(q, k, v, out, *pool, make_slots(T, P, 4), positions, inv, neighbours, q_weight=w, eps=eps)
+    packed = q.contiguous()  # and in place
+    batch.append_rotated(packed, k, v, packed, *pool, make_slots(T, P, 4), positions, inv, neighbours, q_weight=w, eps=eps)
+    assert torch.equal(packed.view(torch.int16), out.view(torch.int16))
+    if eps == 0.0:  # 0 / 0, as the formula says
+        assert bool(out[2, 1].isnan().all())
+        out[2, 1] = q[2, 1] = 0.0
+    y, mag = obatch.rotate(q, positions, inv, neighbours, w, float(np.float32(eps)))
+    if eps == 0.0:
+        y[2, 1] = mag[2, 1] = 0.0
+    off = mag * 18 * 2.0 ** -24
+    tol = off + (y.abs() + off) * 2.0 ** -8 + 2.0 ** -134
+    assert bool(((out.double() - y).abs() <= tol).all()), float(((out.double() - y).abs() / tol).max())
