@@ -43,6 +43,14 @@ bool rows_meet(const void* a, int64_t width, int64_t stride, const void* b, int6
   return off < 2 * width || off + 2 * other > pitch;
 }
 
+// The same of such rows and bytes [b, b + n), which may lie between two rows.
+bool row_meets(const void* a, int64_t width, int64_t stride, int64_t rows, const void* b, int64_t n) {
+  if (!meet(a, 2 * ((rows - 1) * stride + width), b, n)) return false;
+  const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)), pitch = 2 * stride;
+  const int64_t row = off < 2 * width ? 0 : (off - 2 * width) / pitch + 1;  // the first that ends behind b
+  return row < rows && row * pitch < off + n;
+}
+
 // SMs of the current device (0: none).
 int batch_sms() {
   int dev = 0, sms = 0;
@@ -272,13 +280,33 @@ int qwz_batch_append_rotated(const void* q, const void* k, const void* v, void* 
     return fail(QWZ_EINVAL, "q_out must not share storage with k or v");
   const void* held[] = {k_held, v_held};
   for (const void* h : held)
-    if (h && (rows_meet(h, kv_width, kv_width, k, kv_width, k_stride, rows) ||
-              rows_meet(h, kv_width, kv_width, v, kv_width, v_stride, rows) ||
-              rows_meet(h, kv_width, kv_width, q, width, q_stride, rows) ||
-              rows_meet(h, kv_width, kv_width, q_out, width, q_out_stride, rows)))
+    if (row_meets(k, kv_width, k_stride, rows, h, 2 * rows * kv_width) ||
+        row_meets(v, kv_width, v_stride, rows, h, 2 * rows * kv_width) ||
+        row_meets(q, width, q_stride, rows, h, 2 * rows * kv_width) ||
+        row_meets(q_out, width, q_out_stride, rows, h, 2 * rows * kv_width))
       return fail(QWZ_EINVAL, "k_held and v_held must not share storage with q, k, v or q_out");
-  if (k_held && v_held && rows_meet(k_held, kv_width, kv_width, v_held, kv_width, kv_width, rows))
+  if (meet(k_held, 2 * rows * kv_width, v_held, 2 * rows * kv_width))
     return fail(QWZ_EINVAL, "k_held and v_held must not share storage");
+  const struct {
+    const void* at;
+    int64_t n;
+  } small[] = {{slots, 4 * rows}, {positions, 4 * rows}, {inv_freq, 4 * (int64_t)num_freqs}, {q_weight, 4 * (int64_t)head_dim},
+               {k_weight, 4 * (int64_t)head_dim}},
+    pool[] = {{k_cache, num_pages * qwz::kPage * kv_width / 2}, {v_cache, num_pages * qwz::kPage * kv_width / 2},
+              {k_scales, num_pages * qwz::kPage * kv_width / 16}, {v_scales, num_pages * qwz::kPage * kv_width / 16}};
+  bool clash = false;
+  for (const auto& in : small) {
+    clash |= row_meets(q_out, width, q_out_stride, rows, in.at, in.n);
+    for (const void* h : held) clash |= meet(h, 2 * rows * kv_width, in.at, in.n);
+    for (const auto& c : pool) clash |= meet(c.at, c.n, in.at, in.n);
+  }
+  for (const auto& c : pool) {
+    clash |= row_meets(q, width, q_stride, rows, c.at, c.n) || row_meets(q_out, width, q_out_stride, rows, c.at, c.n) ||
+             row_meets(k, kv_width, k_stride, rows, c.at, c.n) || row_meets(v, kv_width, v_stride, rows, c.at, c.n);
+    for (const void* h : held) clash |= meet(h, 2 * rows * kv_width, c.at, c.n);
+    for (const auto& d : pool) clash |= &c < &d && meet(c.at, c.n, d.at, d.n);
+  }
+  if (clash) return fail(QWZ_EINVAL, "outputs must not share storage with inputs or with each other");
   p.q = q;
   p.q_out = q_out;
   p.positions = positions;

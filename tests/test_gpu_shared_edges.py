@@ -190,3 +190,31 @@ def test_rotated_smallest_and_largest_q(rows, heads, dim, freqs, eps, neighbours
     off = mag * 18 * 2.0 ** -24
     tol = off + (y.abs() + off) * 2.0 ** -8 + 2.0 ** -134
     assert bool(((out.double() - y).abs() <= tol).all()), float(((out.double() - y).abs() / tol).max())
+
+
+# -------------------------------------------------------------------- storage
+def test_rotated_arrays_side_by_side():
+    """Outputs that touch inputs and each other, and arrays between two rows of q_out."""
+    T, heads, kv_heads, dim = 7, 6, 2, 64
+    q, k, v, _ = make_rows(T, heads, kv_heads, dim, torch.float16, 4)
+    slots, positions, inv = make_slots(T, 1, 4), i32(range(T)), freqs_of(16)
+    codes, scales = PAGE * kv_heads * dim // 2, PAGE * kv_heads * dim // 16
+    got = []
+    for packed in (False, True):
+        if packed:  # rows of q_out 4 MB apart, the first one with everything else behind it
+            room = torch.zeros(T, 1 << 21, dtype=torch.float16, device="cuda")
+            out = room[:, :heads * dim].view(T, heads, dim)
+            at = heads * dim
+            rest = []
+            for n in (T * kv_heads * dim * 2,) * 2 + (codes, codes, scales, scales):
+                rest.append(room[0, at:at + n // 2])
+                at += n // 2
+            kh, vh = (t.view(T, kv_heads, dim) for t in rest[:2])
+            pool = [t.view(torch.uint8).view(1, PAGE, kv_heads, -1) for t in rest[2:]]
+        else:
+            out = torch.zeros(T, heads, dim, dtype=torch.float16, device="cuda")
+            kh, vh = (torch.zeros(T, kv_heads, dim, dtype=torch.float16, device="cuda") for _ in range(2))
+            pool = [torch.zeros(1, PAGE, kv_heads, w, dtype=torch.uint8, device="cuda") for w in (32, 32, 4, 4)]
+        batch.append_rotated(q, k, v, out, *pool, slots, positions, inv, k_held=kh, v_held=vh)
+        got.append([out, kh, vh, *pool])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
