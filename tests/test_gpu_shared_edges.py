@@ -218,3 +218,33 @@ def test_rotated_arrays_side_by_side():
         batch.append_rotated(q, k, v, out, *pool, slots, positions, inv, k_held=kh, v_held=vh)
         got.append([out, kh, vh, *pool])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ------------------------------------------------------------------- more steps
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [[0, 1, 1], [0, 8, 8], [0, 1, 40]])
+def test_attend_shared_infinite_query(rows, dtype):
+    """A query element that is not finite makes its row and head NaN and nothing else."""
+    head, plan, out, ws = run_shared([-1, 0, 0], rows, [3000, 300, 200], 24, 4, 256, dtype)
+    for value in (float("inf"), float("nan")):
+        q = head[0].clone()
+        q[-1, 5, 100] = value
+        got = torch.empty_like(out)
+        batch.attend_shared(q, *head[1:], plan, got, ws, max_rows=max(rows))
+        assert bool(got[-1, 5].isnan().all())
+        got[-1, 5] = out[-1, 5]
+        assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (64, 8, 128), (14, 2, 64)])
+def test_attend_shared_long_chunks(heads, kv_heads, dim):
+    """Prompt chunks of 1,100 and 2,000 rows, decode rows and a window behind two prefixes."""
+    run_shared([-1, -1, 0, 1, 0, 0, 1], [0, 0, 1100, 2000, 1, 7, 1], [700, 257, 1100, 2300, 500, 40, 9], heads, kv_heads, dim,
+               torch.bfloat16)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,freqs", [(64, 8, 128, 64), (48, 8, 256, 32), (49, 7, 128, 16), (128, 4, 64, 32)])
+def test_rotated_wide_layouts(heads, kv_heads, dim, freqs):
+    """More Q heads than one warp's task holds, in long steps and short ones."""
+    for T in (1101, 5):
+        shared.test_rotated(T, heads, kv_heads, dim, freqs, False, True, torch.bfloat16)
