@@ -9,7 +9,7 @@
 // this call, and what the workspace holds is an earlier call's: the part counts only where
 // the place it was made for lies in the prefix's range and names the row.
 // A warp has one (row, head), or G warps take every G-th part of
-// it (below 4,096 (row, head) pairs, whose items have many parts).  It reads D + 2 floats a
+// it (up to eight (row, head) pairs an SM, which leave warps idle and have many parts each).  It reads D + 2 floats a
 // part, mostly from L2; the chain of loads from the row's request over `where` and the
 // statistics to the outputs bounds it.
 // Measured (cold, alone): 96 pairs 10 us, 1,536 of about 14 parts 19 us, 8,192 of three 19 us.
@@ -209,14 +209,18 @@ cudaError_t launch_shared(const BatchAttnParams& p, const BatchPoolMaps& maps, i
   cudaError_t e = launch_tiles<T, D>(p, clusters * Tiles<D>::kCtas, stream);
   if (e == cudaSuccess) e = launch_few<T, D, kBatchShared>(p, maps, sms, stream);
   if (e != cudaSuccess) return e;
-  // four warps a (row, head) where there are few of them (the parts are many then)
+  // Four warps a (row, head) where there are few of them (the parts are many then).  Calls with
+  // four and with one, decode rows behind 8,192 tokens: 24/4/256, 16 rows (384 pairs) 54.9 and
+  // 59.1 us, 43 (1,032) 64.1 and 65.4, 53 (1,272) 70.3 and 67.2, 64 (1,536) 76.8 and 73.1;
+  // 32/8/128, 32 rows (1,024) 51.9 and 53.6, 40 (1,280) 61.3 and 57.1; 14/2/64, 72 rows
+  // (1,008) 43.0 and 45.8, 96 (1,344) 51.4 and 47.7.
   const long long pairs = (long long)p.rows * p.kv_heads * p.group;
   const int splits = few_splits<D>(p, sms);
   auto launch = [&](auto kernel, int per_cta) {
     const dim3 grid((unsigned)min((pairs + per_cta - 1) / per_cta, 8LL * sms));
     return launch_pdl(kernel, grid, dim3(kJoinWarps * 32), 0, stream, p, splits, clusters);
   };
-  return pairs <= 4 * 1024 ? launch(batch_join_kernel<T, D, 4>, 2) : launch(batch_join_kernel<T, D, 1>, 8);
+  return pairs <= 8LL * sms ? launch(batch_join_kernel<T, D, 4>, 2) : launch(batch_join_kernel<T, D, 1>, 8);
 }
 
 template <typename T>

@@ -656,14 +656,18 @@ cudaError_t launch_rotate(const BatchRotateParams& p, cudaStream_t stream) {
   const int rows = (int)p.kv.rows, kv_heads = p.kv.kv_heads;
   const int tasks = (p.q_heads + kQHeads - 1) / kQHeads + 2 * ((kv_heads + kHeads - 1) / kHeads);
   // Few rows: short tasks, a row's over several CTAs, each with the row's angles.  Against the form for many,
-  // us: 24/4/256 (20 tasks a row) 512 rows 12.5 and 15.6, 1,024 rows 23.4 and 19.4; 32/8/128 (16) 8.3 and 13.1,
-  // 14.8 and 13.9; 14/2/64 (4) 1,024 rows 5.2 and 6.0, 2,048 rows 8.6 and 7.1
-  if (rows <= 1024 && rows * tasks <= 14500) {
+  // us: 24/4/256 with norm 512 rows 14.1 and 15.6, 700 17.6 and 17.4, 800 20.0 and 17.5, 1,024 24.6 and 17.9;
+  // 32/8/128 9.4 and 11.2, 12.1 and 12.4, 13.9 and 12.4, 16.6 and 12.5; 64/8/128 13.5 and 18.0, 17.2 and 19.2,
+  // 19.4 and 19.2, 24.0 and 19.3; 48/8/256 with norm 24.6 and 38.4, 32.6 and 41.9, 36.8 and 41.2, 46.8 and 41.2;
+  // 14/2/64 3.8 and 5.3, 4.1 and 5.7, 6.1 and 5.8, 7.1 and 6.4
+  if (rows <= 700) {
     return launch_pdl(batch_rotate_kernel<T, D, 1>, dim3((unsigned)rows, (tasks + 3) / 4), dim3(kRotThreads), 0, stream, p,
                       1, 1);
   }
-  // Many: the factors of Q are made once for 12 loads (2,048 and 16,384 rows of 24/4/256: 26.5 and 147 us with 4,
-  // 24.5 and 137 with 12); 4 rows a CTA (2 rows 30.4 and 147, 8 rows 39 and 140)
+  // Many: the factors of Q are made once for 12 loads (2,048 and 16,384 rows of 24/4/256 in BF16 with norm and
+  // held values: 25.4 and 159 us with 4, 29.8 and 171 with 6, 22.9 and 148 with 12); 4 rows a CTA (2 rows 29.4
+  // and 190, 8 rows 34.6 and 160).  More than 24 heads of 256, 48 of 128 or 96 of 64 are a second task of a row,
+  // which falls to the same warp for each of the four rows: 16,384 rows of 64/8/128 199 us, 156 with 6 loads.
   constexpr int kRows = 4;
   return launch_pdl(batch_rotate_kernel<T, D, kRows>, dim3((unsigned)((rows + kRows - 1) / kRows)), dim3(kRotThreads), 0,
                     stream, p, 12, (kv_heads + kHeads - 1) / kHeads);

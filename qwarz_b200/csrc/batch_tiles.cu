@@ -40,8 +40,11 @@
 // single CTA, whose operands take all of the shared memory's bandwidth, run at half rate
 // (two CTAs a unit there: 119 us against 90, since the items are not 256 rows wide).  An item
 // costs another 10 us (Q staged 4, the end 5, the first waits), which its weight in the
-// shares stands for: 12 requests with questions 206 us with five tiles, 266 with two, 211
-// with seven.
+// shares stands for, at every head dim.  With a weight of two, three, five and eight tiles: 12
+// requests with questions behind two prompts of 8,192 tokens, 24/4/256, 461, 402, 348 and
+// 359 us, 32/8/128 445, 385, 352 and 361, 14/2/64 165, 151, 142 and 144; 24 windows of 7
+// rows behind two of 16,384, 168, 157, 159 and 166, 166, 148, 146 and 154, 74, 66, 66 and
+// 67; decode rows differ by less than 3 %.
 // Measured, whole calls on the GPU, against the same rows in batch_rows.cu's form: 64 rows
 // behind 32,768 tokens, 24/4/256, 129 us (141); 256 of 32/8/128 163 (251); 24 x 7-row
 // windows 215 (278); questions of 12 requests 206 (306).
@@ -241,11 +244,16 @@ QWZ_DEVINL int tl_shared_row(const BatchAttnParams& p, int at) {
 }
 
 // Whether every row behind a prefix is one of few and what they would read of
-// prefixes by themselves (tokens x KV heads x head dims) costs less than the
-// records, the 128-row tiles and the first wait of this kernel.
-constexpr long long kTlSmall = 24 * 1024 * 1024;
+// prefixes by themselves (tokens x KV heads) costs less than the records, the 128-row
+// tiles and the first wait of this kernel.  Calls with decode rows of own lengths to 500,
+// read by themselves and in tiles: 24/4/256, 4 behind 4,096 (65,536) 27 and 48 us, 16
+// behind 4,096 (262,144) 39 and 50, 64 behind 2,048 (524,288) 64 and 66, 16 behind 10,240
+// (655,360) 60 and 57, 16 behind 16,384 81 and 63; 32/8/128, 64 behind 1,024 (524,288) 52
+// and 58, 64 behind 1,536 (786,432) 60 and 59; 14/2/64, 64 behind 4,096 (524,288) 35 and
+// 39, 64 behind 6,144 (786,432) 40 and 41, 64 behind 8,192 45 and 42.
+constexpr long long kTlSmall = 600 * 1024;
 // Also: `any`, whether a request has more rows than batch_few.cu takes.
-QWZ_DEVINL bool tl_small(const BatchAttnParams& p, int dim, long long* sums, bool& any) {
+QWZ_DEVINL bool tl_small(const BatchAttnParams& p, long long* sums, bool& any) {
   const int per = (p.requests + kTlScan - 1) / kTlScan;
   long long mine = 0, total;
   int wide = 0;  // 1: a request with many rows, 2: one that reads a prefix
@@ -258,7 +266,7 @@ QWZ_DEVINL bool tl_small(const BatchAttnParams& p, int dim, long long* sums, boo
   any = __syncthreads_or(wide) != 0;
   const bool behind = __syncthreads_or(wide & 2) != 0;
   batch::block_scan(mine, sums, total);
-  return !behind && total * p.kv_heads * dim <= kTlSmall;
+  return !behind && total * p.kv_heads <= kTlSmall;
 }
 
 // BYTES (4 or 16) to shared memory; zeros without a read where there is nothing.
@@ -496,7 +504,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) batch_tiles_kernel(const __grid
 
   // ---------------------------------------------------- this CTA's (cluster's) share
   bool any;
-  const bool small = tl_small(p, D, sums, any);
+  const bool small = tl_small(p, sums, any);
   if (blockIdx.x == 0)
     for (int g = tid; g < p.requests; g += kTlThreads) p.direct[g] = Walk::direct(p, g, batch::load_prefix(p, g), small);
   const int per = (2 * p.requests + kTlScan - 1) / kTlScan;

@@ -248,3 +248,17 @@ def test_rotated_wide_layouts(heads, kv_heads, dim, freqs):
     """More Q heads than one warp's task holds, in long steps and short ones."""
     for T in (1101, 5):
         shared.test_rotated(T, heads, kv_heads, dim, freqs, False, True, torch.bfloat16)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(24, 4, 256), (8, 8, 64)])
+def test_attend_shared_many_long_prefixes(heads, kv_heads, dim):
+    """As many prefixes as before, too long for their readers to read them by themselves."""
+    P = 150
+    kv = [400 + 13 * i % 1700 for i in range(P)] + [1 + 7 * i % 300 for i in range(P + 50)]
+    run_shared([-1] * P + list(range(P)) + list(range(50)), [0] * P + [1] * (P + 50), kv, heads, kv_heads, dim, torch.float16)
+
+
+@pytest.mark.parametrize("prefix", [3060, 3080])
+def test_attend_shared_on_either_side_of_a_rule(prefix):
+    """50 rows behind a prefix whose tokens x KV heads x rows are just below 600 K, and just above."""
+    run_shared([-1] + [0] * 50, [0] + [1] * 50, [prefix] + [1 + 31 * i % 290 for i in range(50)], 24, 4, 256, torch.bfloat16)
