@@ -324,7 +324,9 @@ def attend_shared(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows,
     that its request reads and then its own as in `attend`.  The prefix's pages
     are read once for the rows of all its requests together.  `plan` is what
     `share_prefixes` wrote for the step, `workspace` a `shared_workspace`; out
-    shares no storage with q."""
+    shares no storage with q.  It pays from about 1 M prefix tokens x KV heads
+    that all rows read together (2 M at head dim 64); below, `attend` over tables
+    that name the prefix's pages for every request takes fewer launches."""
     dev, args = _attend_args(q, k_cache, v_cache, k_scales, v_scales, block_table, cu_rows, kv_lens, out, workspace,
                              max_rows, sm_scale, plan)
     _launch(dev, "qwz_batch_attend_shared", *args)

@@ -12,7 +12,8 @@
 // it (up to eight (row, head) pairs an SM, which leave warps idle and have many parts each).  It reads D + 2 floats a
 // part, mostly from L2; the chain of loads from the row's request over `where` and the
 // statistics to the outputs bounds it.
-// Measured (cold, alone): 96 pairs 10 us, 1,536 of about 14 parts 19 us, 8,192 of three 19 us.
+// Measured, from the end of the launch before it: 96 pairs 7 us, 1,536 of about 14 parts 14 us,
+// 4,032 11 us, 8,192 of three 18 us.
 #include "batch_common.cuh"
 
 namespace qwz {

@@ -7,7 +7,7 @@
 // the place of request b's first row is the sum of n(b') over the requests with
 // (e(b'), b') < (e(b), b).  A warp has one request and compares it with all R (no
 // request waits for another's sums); a step's bytes are nothing beside the launch.
-// Measured: 3.6 us for 66 requests of 64 rows, 12.2 us for 2,072 of 21,130: the latency of
+// Measured: 3.6 us for 66 requests of 64 rows, 12.3 us for 2,072 of 21,130: the latency of
 // the loads that depend on one another.  (Eight threads a request: 28 us for the latter.)
 #include "batch_common.cuh"
 #include "nvfp4_quant.cuh"
@@ -126,13 +126,15 @@ cudaError_t launch_batch_share(const BatchShareParams& p, int sms, cudaStream_t 
 // groups of heads in a hundred).  Angles are taken in 64 bits: 32 leave 0.06 radians of a position
 // of 10^6.
 //
-// Instructions bound it for long steps (issue slots 58 %, DRAM 42 %).  Measured, GPU times:
-// 16,384 rows of 24/4/256, a quarter of the dims turned, with norm and held values, 145 us
-// (59 % of the measured copy bandwidth); 5,001 rows of 14/2/64 12.6 us; 448 rows of 32/8/128
-// 8.5 us; 16 rows of 24/4/256 4.9 us, less than the call costs the host.  Forms that were
-// slower on the first: all of K in 64 bits with 8 dims a lane for Q, whose pairs' other dims
-// came by shuffles, 214 us; the same with factors made once a row, 187 us; CTAs of 256
-// threads, two an SM 160 us, three 151 us.
+// Q's y is made in 32 bits; BF16 heads whose squares 32 bits do not hold are left for 64.
+//
+// Instructions bound it for long steps (issue slots 57 %, DRAM 41 %).  Measured, GPU times:
+// 16,384 rows of 24/4/256 in BF16, a quarter of the dims turned, with norm and held values,
+// 148 us (57 % of the measured copy bandwidth); 5,001 rows of 14/2/64 12.0 us; 448 rows of
+// 32/8/128 8.1 us; 16 rows of 24/4/256 4.5 us, less than the call costs the host.  Forms that
+// were slower on the first, while it took 145 us: all of K in 64 bits with 8 dims a lane for
+// Q, whose pairs' other dims came by shuffles, 214 us; the same with factors made once a row,
+// 187 us; CTAs of 256 threads, two an SM 160 us, three 151 us.
 namespace {
 
 // Nearest float with an odd last bit unless y is a float itself: later roundings
@@ -176,7 +178,7 @@ QWZ_DEVINL void quantise8(const float (&x)[8], uint32_t& code, uint32_t& sbits) 
       for (int e = 0; e < 2; ++e) {
         const float c = fmaxf(fminf(x[i + e], cut), -cut);
         const float q = __fmul_rn(c, r);
-        y[e] = __fmaf_rn(__fmaf_rn(-q, s, c), r, q);  // c / s, correctly rounded
+        y[e] = __fmaf_rn(__fmaf_rn(-q, s, c), r, q);  // c / s, correctly rounded (Markstein, as in batch_tables.cu)
         if constexpr (ODD) y[e] = odd_of(y[e], __fmaf_rn(-y[e], s, c));
       }
       asm("{\n .reg .b8 t;\n cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n cvt.u32.u8 %0, t;\n}\n"
@@ -486,7 +488,7 @@ QWZ_DEVINL bool k_from_32(const uint4& raw, int c, const float* weight, float w_
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float q = __fmul_rn(y[i + e], r);
-        z[e] = __fmaf_rn(__fmaf_rn(-q, s, y[i + e]), r, q);  // correctly rounded
+        z[e] = __fmaf_rn(__fmaf_rn(-q, s, y[i + e]), r, q);  // y / s, correctly rounded (Markstein)
       }
       asm("{\n .reg .b8 t, u;\n cvt.rn.satfinite.e2m1x2.f32 t, %3, %2;\n cvt.rn.satfinite.e2m1x2.f32 u, %5, %4;\n"
           " cvt.u32.u8 %0, t;\n cvt.u32.u8 %1, u;\n}\n"

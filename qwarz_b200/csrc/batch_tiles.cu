@@ -46,10 +46,11 @@
 // rows behind two of 16,384, 168, 157, 159 and 166, 166, 148, 146 and 154, 74, 66, 66 and
 // 67; decode rows differ by less than 3 %.
 // Measured, whole calls on the GPU, against the same rows in batch_rows.cu's form: 64 rows
-// behind 32,768 tokens, 24/4/256, 129 us (141); 256 of 32/8/128 163 (251); 24 x 7-row
-// windows 215 (278); questions of 12 requests 206 (306).
-// Not kept: Q staged by the V warps (219 us for the windows), the softmax's next chunk loaded
-// ahead (230), QK(1) of an item held back until P(0) so that the groups alternate (228).
+// behind 32,768 tokens, 24/4/256, 130 us (141); 256 of 32/8/128 167 (251); 24 x 7-row
+// windows 203 (278); questions of 12 requests 205 (306).
+// Not kept, while the windows took 215 us: Q staged by the V warps (219), the softmax's next
+// chunk loaded ahead (230), QK(1) of an item held back until P(0) so that the groups
+// alternate (228).
 #include "attn_common.cuh"
 #include "batch_common.cuh"
 #include "tc_common.cuh"
@@ -385,7 +386,7 @@ QWZ_DEVINL void tl_few_starts(const BatchAttnParams& p, bool small, long long* s
 
 // a and b plus the two weights of w.  The sums take the rounded weights, as in
 // batch_few.cu: a row's weights add up to one, and the rounding of a dominant weight
-// cancels.  (FP16 and FP32 in one addition; a conversion and an addition in pairs behind the
+// cancels (the error is then at most 2^-11 of the sum of p |v - out|).  (FP16 and FP32 in one addition; a conversion and an addition in pairs behind the
 // chunk's vote: 24 windows of 7 rows 233 us, 216 so; of the unrounded weights 212.)
 QWZ_DEVINL void tl_add_pair(float& a, float& b, uint32_t w) {
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n add.f32.f16 %0, l, %0;\n add.f32.f16 %1, h, %1;\n}\n"
